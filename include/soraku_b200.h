@@ -162,6 +162,72 @@ int skb_decode_attention_noalloc(const float *qkv, int rows, int n_heads, int n_
                                  int max_pages, int page_size, int n_pages, int splits, float *out,
                                  cudaStream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Cache operators for long and endless streams, over the same paged pool.
+ * They have no counterpart in the reference, whose cache is one utterance
+ * long.  A row's `cached` slots are filled and new tokens take the next ones;
+ * `pos` is the RoPE position of the row's first new token, apart from its slot
+ * (after an eviction positions run ahead of slots; cached keys keep the rotation
+ * they were written with).  The query at slot i sees slot j <= i if window is
+ * 0, or i - j < window, or j < sinks (sinks need a window).
+ * n_heads / n_kv_heads is 1 to 4; a page must not be mapped to two rows.
+ * Rows with cached < 0 are idle: zeros out, the cache untouched.  A row whose
+ * counts or positions lie outside the inputs, the cache or the RoPE tables
+ * returns NaN and leaves the cache untouched, and so does every query that
+ * sees a slot whose page-table entry names no page.  Slots that a query does
+ * not see cannot change its output, whatever they hold; a query head that sees
+ * a key or value that is not finite returns 128 numbers that are not all finite.
+ * `mass` (optional): device [rows, n_kv_heads, max_pages * page_size], the
+ * softmax weights a slot received, added up over the queries and the heads of
+ * the group; the slots of new tokens begin at zero.
+ * The workspace functions return the bytes `work` must hold (-1: bad sizes);
+ * work is 256-byte aligned and belongs to one call at a time.
+ * ---------------------------------------------------------------------- */
+
+/* Attention of a ragged chunk of new tokens per row.
+ *   qkv         device [tokens, (n_heads + 2 n_kv_heads) * 128]  (q | k | v)
+ *   chunk_start device int32 [rows + 1]: row r's tokens are chunk_start[r] ..
+ *               chunk_start[r + 1] - 1, at most max_chunk; tokens behind
+ *               chunk_start[rows] are neither read nor written
+ *   rope_cos/sin device [max_pos, 64];  cached, pos: device int32 [rows]
+ *   kv_pool, page_table as for skb_decode_attention
+ *   out         device [tokens, n_heads * 128] */
+int64_t skb_chunk_attention_workspace(int tokens, int rows, int max_chunk, int n_heads, int n_kv_heads,
+                                      int max_pages, int page_size, int with_mass);
+int skb_chunk_attention(const float *qkv, int tokens, int rows, int n_heads, int n_kv_heads, int head_dim,
+                        const float *q_norm, const float *k_norm, float eps, const float *rope_cos,
+                        const float *rope_sin, int max_pos, const int32_t *chunk_start, int max_chunk,
+                        const int32_t *cached, const int32_t *pos, float *kv_pool, const int32_t *page_table,
+                        int max_pages, int page_size, int n_pages, int window, int sinks, float *mass, void *work,
+                        int64_t work_bytes, float *out, cudaStream_t stream);
+
+/* The same for one new token per row: qkv [rows, ...], out [rows, n_heads * 128].
+ * `work` may be NULL without mass. */
+int64_t skb_window_decode_workspace(int rows, int n_heads, int max_pages, int page_size, int window, int sinks,
+                                    int with_mass);
+int skb_window_decode_attention(const float *qkv, int rows, int n_heads, int n_kv_heads, int head_dim,
+                                const float *q_norm, const float *k_norm, float eps, const float *rope_cos,
+                                const float *rope_sin, int max_pos, const int32_t *cached, const int32_t *pos,
+                                float *kv_pool, const int32_t *page_table, int max_pages, int page_size, int n_pages,
+                                int window, int sinks, float *mass, void *work, int64_t work_bytes, float *out,
+                                cudaStream_t stream);
+
+/* Eviction by accumulated attention weight.  Of a row with more than `budget`
+ * filled slots, each kv head keeps the first `sinks`, the last `recent` and, of
+ * those between, the heaviest (equal weights: the lower slot; NaN counts as
+ * heaviest), in slot order; their keys and values move to the front in place.
+ *   kept       device int32 [rows, n_kv_heads, budget]: where each kept slot
+ *              was; -1 behind the last
+ *   mass_out   device, like mass: the kept slots' weights, zeros behind them
+ *   cached_out device int32 [rows]: min(cached, budget); counts that are
+ *              negative or exceed the cache come back as they are, with
+ *              nothing kept and nothing moved */
+int64_t skb_evict_workspace(int rows, int n_kv_heads);
+int skb_evict_cache(const float *mass, const int32_t *cached, int rows, int n_kv_heads, int head_dim, float *kv_pool,
+                    const int32_t *page_table, int max_pages, int page_size, int n_pages, int budget, int sinks,
+                    int recent, int32_t *kept, float *mass_out, int32_t *cached_out, void *work, int64_t work_bytes,
+                    cudaStream_t stream);
+
 /* Test hooks: the device exp used by the sampler, and raw Philox4x32-10.
  * ctr_key: device uint32 [n, 6] = (c0, c1, c2, c3, k0, k1); out: [n, 4]. */
 int skb_test_exp(const float *x, float *y, int n, cudaStream_t stream);

@@ -39,6 +39,18 @@ SIGNATURES = {
     "skb_decode_attention_noalloc": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float,
                                              c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                              c_int, c_int, c_void_p, c_void_p]),
+    "skb_chunk_attention_workspace": (c_int64, [c_int] * 8),
+    "skb_chunk_attention": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p,
+                                    c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                    c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "skb_window_decode_workspace": (c_int64, [c_int] * 7),
+    "skb_window_decode_attention": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float,
+                                            c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                            c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p,
+                                            c_void_p]),
+    "skb_evict_workspace": (c_int64, [c_int, c_int]),
+    "skb_evict_cache": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
+                                c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "skb_test_exp": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
     "skb_test_philox": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
     "skb_test_wait_timeout": (c_int, [c_void_p, c_int, c_void_p]),

@@ -228,3 +228,146 @@ def decode_attention(qkv: torch.Tensor, *, n_heads: int, n_kv_heads: int, q_norm
               pos.data_ptr(), kv_pool.data_ptr(), page_table.data_ptr(), page_table.shape[1], page_size, n_pages,
               splits, part.data_ptr(), tickets.data_ptr(), out.data_ptr(), _stream())
     return out
+
+
+# ------------------------------------------------- cache operators for streams
+def _whole(x, name: str, low: int = 0) -> int:
+    if isinstance(x, bool) or not isinstance(x, int) or x < low or x > 2**31 - 1:
+        raise ValueError(f"{name}: must be an int of at least {low}, got {x!r}")
+    return x
+
+
+def _cache_shapes(kv_pool, page_table, page_size: int, n_kv_heads: int | None = None):
+    """(n_pages, kv heads, rows, max_pages) of a paged cache, checked."""
+    _whole(page_size, "page_size", 1)
+    if not isinstance(kv_pool, torch.Tensor) or kv_pool.dim() != 5:
+        raise ValueError("kv_pool: expected a tensor [n_pages, 2, n_kv_heads, page_size, 128]")
+    kvh = kv_pool.shape[2] if n_kv_heads is None else n_kv_heads
+    _check(kv_pool, "kv_pool", (kv_pool.shape[0], 2, kvh, page_size, 128))
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+        raise ValueError("page_table: expected a tensor [rows, max_pages]")
+    _check(page_table, "page_table", tuple(page_table.shape), torch.int32)
+    if kv_pool.shape[0] < 1 or page_table.shape[1] < 1:
+        raise ValueError("kv_pool and page_table must hold at least one page")
+    return kv_pool.shape[0], kvh, page_table.shape[0], page_table.shape[1]
+
+
+def _same_device(**tensors):
+    devices = {t.device for t in tensors.values() if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"{', '.join(tensors)}: must be on one device, got {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def _cache_attention(name, qkv, n_heads, n_kv_heads, q_norm, k_norm, eps, rope_cos, rope_sin, chunk_start, max_chunk,
+                     cached, pos, kv_pool, page_table, page_size, window, sinks, mass, out):
+    _whole(n_heads, "n_heads", 1)
+    _whole(n_kv_heads, "n_kv_heads", 1)
+    _whole(window, "window")
+    _whole(sinks, "sinks")
+    n_pages, _, rows, max_pages = _cache_shapes(kv_pool, page_table, page_size, n_kv_heads)
+    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 2:
+        raise ValueError("qkv: expected a tensor [tokens, (n_heads + 2 n_kv_heads) * 128]")
+    tokens = rows if chunk_start is None else qkv.shape[0]
+    _check(qkv, "qkv", (tokens, (n_heads + 2 * n_kv_heads) * 128))
+    _check(q_norm, "q_norm", (128,))
+    _check(k_norm, "k_norm", (128,))
+    if not isinstance(rope_cos, torch.Tensor) or rope_cos.dim() != 2:
+        raise ValueError("rope_cos: expected a tensor [positions, 64]")
+    for n, t in (("rope_cos", rope_cos), ("rope_sin", rope_sin)):
+        _check(t, n, (rope_cos.shape[0], 64))
+    _check(cached, "cached", (rows,), torch.int32)
+    _check(pos, "pos", (rows,), torch.int32)
+    if mass is not None:
+        _check(mass, "mass", (rows, n_kv_heads, max_pages * page_size))
+    if chunk_start is not None:
+        _whole(max_chunk, "max_chunk")
+        _check(chunk_start, "chunk_start", (rows + 1,), torch.int32)
+    if out is not None:
+        _check(out, "out", (tokens, n_heads * 128))
+    device = _same_device(qkv=qkv, q_norm=q_norm, k_norm=k_norm, rope_cos=rope_cos, rope_sin=rope_sin, cached=cached,
+                          pos=pos, kv_pool=kv_pool, page_table=page_table, mass=mass, chunk_start=chunk_start, out=out)
+    with torch.cuda.device(device):
+        if out is None:
+            out = torch.empty((tokens, n_heads * 128), dtype=torch.float32, device=device)
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        heads = (n_heads, n_kv_heads, 128, q_norm.data_ptr(), k_norm.data_ptr(), float(eps), rope_cos.data_ptr(),
+                 rope_sin.data_ptr(), rope_cos.shape[0])
+        cache = (cached.data_ptr(), pos.data_ptr(), kv_pool.data_ptr(), page_table.data_ptr(), max_pages, page_size,
+                 n_pages, window, sinks, ptr(mass))
+        if chunk_start is None:
+            need = _lib.lib().skb_window_decode_workspace(rows, n_heads, max_pages, page_size, window, sinks,
+                                                          int(mass is not None))
+        else:
+            need = _lib.lib().skb_chunk_attention_workspace(tokens, rows, max_chunk, n_heads, n_kv_heads, max_pages,
+                                                            page_size, int(mass is not None))
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+        if chunk_start is None:
+            _lib.call(name, qkv.data_ptr(), rows, *heads, *cache, ptr(work), max(need, 0), out.data_ptr(), _stream())
+        else:
+            _lib.call(name, qkv.data_ptr(), tokens, rows, *heads, chunk_start.data_ptr(), max_chunk, *cache, ptr(work),
+                      max(need, 0), out.data_ptr(), _stream())
+    return out
+
+
+def chunk_attention(qkv: torch.Tensor, *, n_heads: int, n_kv_heads: int, q_norm: torch.Tensor, k_norm: torch.Tensor,
+                    eps: float, rope_cos: torch.Tensor, rope_sin: torch.Tensor, chunk_start: torch.Tensor,
+                    max_chunk: int, cached: torch.Tensor, pos: torch.Tensor, kv_pool: torch.Tensor,
+                    page_table: torch.Tensor, page_size: int, window: int = 0, sinks: int = 0,
+                    mass: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a ragged chunk of new tokens per row over the paged FP32 KV
+    cache; see skb_chunk_attention in include/soraku_b200.h.
+
+    Row r's tokens are ``qkv[chunk_start[r]:chunk_start[r + 1]]`` (at most
+    ``max_chunk``); they take the slots behind its ``cached[r]`` filled ones (the
+    pool is updated in place, ``cached`` is not) at RoPE positions ``pos[r]``,
+    ``pos[r] + 1``, ....  The query at slot i sees slot j <= i when ``window`` is
+    0, or i - j < window, or j < ``sinks``.  ``mass`` [rows, n_kv_heads, slots] is
+    added to in place.  Returns [tokens, n_heads * 128] (``out`` if given; rows
+    of it behind the last sequence stay as they were)."""
+    if chunk_start is None:
+        raise ValueError("chunk_start: expected a tensor")
+    return _cache_attention("skb_chunk_attention", qkv, n_heads, n_kv_heads, q_norm, k_norm, eps, rope_cos, rope_sin,
+                            chunk_start, max_chunk, cached, pos, kv_pool, page_table, page_size, window, sinks, mass, out)
+
+
+def window_decode_attention(qkv: torch.Tensor, *, n_heads: int, n_kv_heads: int, q_norm: torch.Tensor,
+                            k_norm: torch.Tensor, eps: float, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
+                            cached: torch.Tensor, pos: torch.Tensor, kv_pool: torch.Tensor, page_table: torch.Tensor,
+                            page_size: int, window: int = 0, sinks: int = 0, mass: torch.Tensor | None = None,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """``chunk_attention`` for one new token per row (``qkv`` [rows, ...]): the
+    decode step of a stream with a bounded window, or of a cache whose slots no
+    longer equal its positions; see skb_window_decode_attention in
+    include/soraku_b200.h.  Rows with ``cached`` < 0 are idle and return zeros."""
+    return _cache_attention("skb_window_decode_attention", qkv, n_heads, n_kv_heads, q_norm, k_norm, eps, rope_cos,
+                            rope_sin, None, 1, cached, pos, kv_pool, page_table, page_size, window, sinks, mass, out)
+
+
+def evict_cache(mass: torch.Tensor, *, cached: torch.Tensor, kv_pool: torch.Tensor, page_table: torch.Tensor,
+                page_size: int, budget: int, sinks: int = 0, recent: int = 0):
+    """Thins every row of more than ``budget`` filled slots to that many, per kv
+    head: the first ``sinks``, the last ``recent`` and the heaviest by ``mass``
+    of those between stay (equal weights: the lower slot) and move to the front in
+    slot order, in place; see skb_evict_cache in include/soraku_b200.h.  Returns
+    (kept int32 [rows, n_kv_heads, budget], the slots that were kept, -1 behind
+    the last; the weights moved alike, zeros behind them; the new ``cached``).
+    The pages behind ``ceil(cached / page_size)`` are then free."""
+    _whole(budget, "budget", 1)
+    _whole(sinks, "sinks")
+    _whole(recent, "recent")
+    n_pages, kvh, rows, max_pages = _cache_shapes(kv_pool, page_table, page_size)
+    _check(mass, "mass", (rows, kvh, max_pages * page_size))
+    _check(cached, "cached", (rows,), torch.int32)
+    device = _same_device(mass=mass, cached=cached, kv_pool=kv_pool, page_table=page_table)
+    with torch.cuda.device(device):
+        kept = torch.empty((rows, kvh, budget), dtype=torch.int32, device=device)
+        mass_out = torch.empty_like(mass)
+        cached_out = torch.empty_like(cached)
+        if rows > 0:
+            need = _lib.lib().skb_evict_workspace(rows, kvh)
+            work = torch.empty(need, dtype=torch.uint8, device=device)
+            _lib.call("skb_evict_cache", mass.data_ptr(), cached.data_ptr(), rows, kvh, 128, kv_pool.data_ptr(),
+                      page_table.data_ptr(), max_pages, page_size, n_pages, budget, sinks, recent, kept.data_ptr(),
+                      mass_out.data_ptr(), cached_out.data_ptr(), work.data_ptr(), need, _stream())
+    return kept, mass_out, cached_out

@@ -1,0 +1,638 @@
+"""The cache operators (chunk attention, windowed decode attention, eviction)
+against a plain restatement in 64 bits.
+
+Tolerances.  With norm weights near 1 a head of q or k has norm about
+sqrt(128) = 11.3, so a score q.k / sqrt(128) is a sum of 128 products whose
+absolute values add up to at most 11.3 w^2 < 25 for weights w < 1.5.  Each factor
+carries at most about 12 FP32 roundings of 2^-24 (norm, weight, rotation), the
+product another 4 of 2^-24 where it is formed from two 11-bit pieces each, the sum
+8: a score is off by at most 25 * 36 * 2^-24 = 5.4e-5, a weight by twice that
+relative, an output by 1.1e-4 of the largest value it mixes.  That is ATOL, the
+bound on any element.  The roundings are independent, so their mean square is
+far smaller: about sqrt(2) * 4 * 2^-24 = 3.4e-7 relative per product, the same for
+the sum of random terms, 2^-22 for a base-2 exponential, and outputs are sums of
+independent values weighted by them: 1e-6, three times that is REL, the bound
+on the norm of the difference over the norm."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+HD, EPS = 128, 1e-6
+ATOL, REL = 1.1e-4, 3e-6
+
+
+class Cache:
+    """A paged cache with rows of given lengths, its restatement in 64 bits, and
+    the tables the operators take."""
+
+    def __init__(self, cached, room, H=16, G=8, page=16, seed=0, spare=3, max_pos=4096, moved=0):
+        self.H, self.G, self.page, self.rows = H, G, page, len(cached)
+        g = self.gen = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        self.max_pages = max(1, -(-(max(max(cached), 0) + room) // page))
+        n_pages = self.rows * self.max_pages + spare
+        self.table = torch.randperm(n_pages, generator=g, device="cuda")[:self.rows * self.max_pages] \
+            .to(torch.int32).view(self.rows, self.max_pages)
+        self.pool = torch.randn(n_pages, 2, G, page, HD, generator=g, device="cuda")
+        self.qn = 1 + 0.1 * torch.randn(HD, generator=g, device="cuda")
+        self.kn = 1 + 0.1 * torch.randn(HD, generator=g, device="cuda")
+        ang = torch.arange(max_pos, dtype=torch.float64, device="cuda")[:, None] / \
+            1e6 ** (torch.arange(0, HD, 2, dtype=torch.float64, device="cuda") / HD)
+        self.cos, self.sin = ang.cos().float(), ang.sin().float()
+        self.cached = torch.tensor(cached, dtype=torch.int32, device="cuda")
+        self.pos = torch.clamp(self.cached, min=0) + moved
+        self.slots = self.max_pages * page
+        self.mass = torch.rand(self.rows, G, self.slots, generator=g, device="cuda")
+        self.mass64 = self.mass.double()
+        self.pool64 = self.pool.double()
+
+    def qkv(self, tokens):
+        return torch.randn(tokens, (self.H + 2 * self.G) * HD, generator=self.gen, device="cuda")
+
+    def args(self, **kw):
+        d = dict(n_heads=self.H, n_kv_heads=self.G, q_norm=self.qn, k_norm=self.kn, eps=EPS, rope_cos=self.cos,
+                 rope_sin=self.sin, cached=self.cached, pos=self.pos, kv_pool=self.pool, page_table=self.table,
+                 page_size=self.page)
+        d.update(kw)
+        return d
+
+    def row(self, r, n):
+        """[2, G, n, HD] of the first n slots of row r, in 64 bits."""
+        return self.pool64[self.table[r].long()].permute(1, 2, 0, 3, 4).reshape(2, self.G, -1, HD)[:, :, :n]
+
+    def put(self, r, slot, k, v):
+        page = int(self.table[r, slot // self.page])
+        self.pool64[page, 0, :, slot % self.page] = k
+        self.pool64[page, 1, :, slot % self.page] = v
+
+    def want(self, qkv, lengths, window=0, sinks=0, mass=False):
+        """Outputs of one call in 64 bits; appends to pool64, adds to mass64."""
+        H, G, rep = self.H, self.G, self.H // self.G
+        outs, at = [], 0
+        for r, n in enumerate(lengths):
+            x = qkv[at:at + n].double().view(n, H + 2 * G, HD)
+            at += n
+            c = int(self.cached[r])
+            if c < 0:
+                outs.append(torch.zeros(n, H * HD, dtype=torch.float64, device="cuda"))
+                continue
+            p = int(self.pos[r])
+            cs, sn = self.cos[p:p + n].double()[:, None], self.sin[p:p + n].double()[:, None]
+
+            def head(y, w):
+                y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + EPS) * w.double()
+                a, b = y[..., :64], y[..., 64:]
+                return torch.cat([a * cs - b * sn, b * cs + a * sn], -1)
+
+            q, k, v = head(x[:, :H], self.qn), head(x[:, H:H + G], self.kn), x[:, H + G:]
+            for t in range(n):
+                self.put(r, c + t, k[t], v[t])
+            K, V = self.row(r, c + n)
+            i = torch.arange(c, c + n, device="cuda")[:, None]
+            j = torch.arange(c + n, device="cuda")[None]
+            see = j <= i
+            if window:
+                see &= (i - j < window) | (j < sinks)
+            # what a query does not see cannot reach it, whatever it holds
+            s = torch.einsum("nghd,gjd->ghnj", q.view(n, G, rep, HD), torch.nan_to_num(K)) / math.sqrt(HD)
+            w = torch.softmax(s.masked_fill(~see, -math.inf), -1)
+            o = torch.einsum("ghnj,gjd->nghd", w, torch.nan_to_num(V))
+            for g in range(G):  # marks the heads of a query that see something not finite
+                sick = ~(torch.isfinite(K[g]).all(-1) & torch.isfinite(V[g]).all(-1))
+                o[(see & sick).any(-1), g] = math.nan
+            outs.append(o.reshape(n, H * HD))
+            if mass:
+                self.mass64[r, :, c:c + n] = 0
+                self.mass64[r, :, :c + n] += w.sum((1, 2))
+        return torch.cat(outs)
+
+    def check_cache(self):
+        torch.testing.assert_close(self.pool[:, 0].double(), self.pool64[:, 0], rtol=0, atol=5e-6, equal_nan=True)
+        assert torch.equal(torch.nan_to_num(self.pool[:, 1].double()), torch.nan_to_num(self.pool64[:, 1]))
+
+    def check_mass(self):
+        # sums of at most a few thousand weights, each off by at most 1.1e-4
+        # relative, and on average by REL
+        close(self.mass, self.mass64)
+
+
+def close(got, want):
+    """Within the bounds; a head that sees something not finite (all NaN in
+    ``want``) must show it, in at least one of its 128 numbers."""
+    fine = torch.isfinite(want)
+    heads = fine.view(-1, HD) if fine.shape[-1] % HD == 0 else fine.view(-1, 1)
+    assert torch.equal(heads.any(-1), heads.all(-1))
+    assert torch.equal(torch.isfinite(got).view(heads.shape).all(-1), heads.all(-1)), "finite in other places"
+    d = (got.double() - want)[fine]
+    if d.numel() == 0:
+        return
+    top = float(want[fine].abs().max())
+    assert float(d.abs().max()) <= ATOL * max(top, 1e-3), float(d.abs().max()) / max(top, 1e-30)
+    assert float(d.norm()) <= REL * float(want[fine].norm()) + 1e-12, float(d.norm() / want[fine].norm())
+
+
+def starts(lengths):
+    return torch.tensor([0] + list(lengths)).cumsum(0).to(torch.int32).cuda()
+
+
+def chunk(c, lengths, window=0, sinks=0, mass=False, extra=0, max_chunk=None, qkv=None, out=None):
+    from soraku_tts_b200 import kernels
+
+    qkv = c.qkv(sum(lengths) + extra) if qkv is None else qkv
+    got = kernels.chunk_attention(qkv, chunk_start=starts(lengths), max_chunk=max_chunk or max(lengths),
+                                  window=window, sinks=sinks, mass=c.mass if mass else None, out=out, **c.args())
+    return got, c.want(qkv, lengths, window, sinks, mass)
+
+
+HEADS = [(16, 8), (4, 4), (6, 2), (8, 2)]
+RAGGED = [((0,), (1,)), ((0, 7), (5, 0)), ((37, 300), (5, 5)), ((0, 0, 128), (127, 128, 129)), ((63, 64, 65, 1), (64, 1, 3, 200)),
+          ((511, 130, 257), (43, 70, 1))]
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("cached,lengths", RAGGED)
+def test_chunk_attention(heads, cached, lengths):
+    c = Cache(cached, max(lengths), *heads, seed=sum(cached) + heads[0])
+    got, want = chunk(c, lengths)
+    close(got, want)
+    c.check_cache()
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (5, 4), (64, 3), (100, 200), (128, 128), (1000, 4), (2**31 - 1, 2)])
+@pytest.mark.parametrize("page", [1, 16, 128])
+def test_chunk_attention_window(window, sinks, page):
+    c = Cache((0, 300, 517), 150, 4, 2, page=page, seed=window % 1000 + page, moved=900)
+    got, want = chunk(c, (33, 150, 2), window, sinks, mass=True)
+    close(got, want)
+    c.check_cache()
+    c.check_mass()
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("cached,lengths", RAGGED)
+def test_chunk_attention_mass(heads, cached, lengths):
+    c = Cache(cached, max(lengths), *heads, seed=sum(lengths) + heads[0])
+    got, want = chunk(c, lengths, mass=True)
+    close(got, want)
+    c.check_mass()
+
+
+def test_chunk_attention_long_rows():
+    c = Cache((4000, 3333), 300, 4, 2, page=64, seed=5, max_pos=5000)
+    got, want = chunk(c, (300, 211), mass=True)
+    close(got, want)
+    c.check_mass()
+
+
+def test_chunk_attention_leaves_other_memory_alone():
+    c = Cache((20, -1, 31, 7), 40, seed=3)
+    lengths, extra = (9, 4, 17, 0), 6
+    qkv = c.qkv(sum(lengths) + extra)
+    qkv[-extra:] = math.nan
+    out = torch.full((sum(lengths) + extra, c.H * HD), 7.0, device="cuda")
+    before, mass = c.pool.clone(), c.mass.clone()
+    got, want = chunk(c, lengths, mass=True, qkv=qkv, out=out, max_chunk=33)
+    assert got.data_ptr() == out.data_ptr()
+    close(got[:sum(lengths)], want)
+    assert torch.equal(got[sum(lengths):], torch.full_like(got[sum(lengths):], 7.0))
+    assert torch.equal(got[9:13], torch.zeros_like(got[9:13]))  # the idle row
+    c.check_cache()
+    touched = set()
+    for r, n in enumerate(lengths):
+        if int(c.cached[r]) >= 0:
+            touched |= {(int(c.table[r, s // c.page]), s % c.page) for s in range(int(c.cached[r]), int(c.cached[r]) + n)}
+    keep = torch.tensor([[(p, s) not in touched for s in range(c.page)] for p in range(c.pool.shape[0])], device="cuda")
+    assert torch.equal(c.pool.permute(0, 3, 1, 2, 4)[keep], before.permute(0, 3, 1, 2, 4)[keep])
+    for r, n in enumerate(lengths):
+        end = max(int(c.cached[r]), -1) + n if int(c.cached[r]) >= 0 else 0
+        assert torch.equal(c.mass[r, :, end:], mass[r, :, end:])
+
+
+# Garbage where no query looks: stale slots behind the row's end, slots that
+# fell out of the window, later tokens of the chunk for the earlier ones.
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3e38])
+def test_chunk_attention_masked_garbage(bad):
+    c = Cache((200, 64, 0), 70, 8, 4, seed=9)
+    lengths, window, sinks = (70, 5, 40), 50, 3
+    for r, n in enumerate(lengths):
+        filled = int(c.cached[r])
+        for s in list(range(filled + n, c.slots)) + list(range(sinks, filled - window - 1)):
+            page = int(c.table[r, s // c.page])
+            c.pool[page, :, :, s % c.page] = bad
+            c.pool64[page, :, :, s % c.page] = bad
+    qkv = c.qkv(sum(lengths))
+    v = qkv.view(-1, c.H + 2 * c.G, HD)
+    v[69, c.H + c.G:] = bad   # row 0's last token's values
+    v[74 + 30, c.H + c.G + 1, 5] = bad  # one number of row 2's 30th token, one head
+    got, want = chunk(c, lengths, window, sinks, qkv=qkv)
+    if abs(bad) == 3e38:  # finite: only its own readers mix it in
+        seen = torch.zeros(sum(lengths), dtype=torch.bool, device="cuda")
+        seen[69] = True
+        seen[74 + 30:] = True
+        close(got[~seen], want[~seen])
+        assert torch.isfinite(got[~seen]).all()
+    else:
+        close(got, want)
+
+
+def test_chunk_attention_nan_query_stays_alone():
+    c = Cache((10, 20), 12, seed=4)
+    qkv = c.qkv(24)
+    qkv.view(24, 32, HD)[5, 3, 9] = math.nan  # one query head of one token
+    got, want = chunk(c, (12, 12), qkv=qkv)
+    got, want = got.view(24, 16, HD), want.view(24, 16, HD)
+    assert torch.isnan(got[5, 3]).all()
+    got[5, 3] = want[5, 3] = 0
+    close(got, want)
+
+
+@pytest.mark.parametrize("scale", [1e-12, 1e-4, 1e4, 1e15])
+def test_chunk_attention_value_scales(scale):
+    """Values of any size, and sizes that change along the cache."""
+    c = Cache((400,), 20, 4, 2, seed=8)
+    ramp = torch.logspace(-3, 3, c.pool.shape[0], device="cuda")[:, None, None, None]
+    c.pool[:, 1] *= scale * ramp
+    c.pool64 = c.pool.double()
+    qkv = c.qkv(20)
+    qkv.view(20, 8, HD)[:, 6:] *= scale
+    got, want = chunk(c, (20,), qkv=qkv)
+    close(got.double() / scale, want / scale)
+
+
+def test_chunk_attention_sharp_and_flat_scores():
+    """Scores far apart (norm weights of 12: one slot takes all) and all alike."""
+    for w in (12.0, 1e-3):
+        c = Cache((300, 40), 30, 4, 2, seed=2)
+        c.qn.fill_(w)
+        got, want = chunk(c, (30, 30))
+        # scores are off in proportion to their size
+        d = (got.double() - want).abs().max()
+        assert float(d) <= ATOL * max(1.0, w) * float(c.pool.abs().max()), float(d)
+
+
+def test_bad_rows_return_nan_and_touch_nothing():
+    from soraku_tts_b200 import kernels
+
+    # too long for the cache; a position behind the tables; a negative one; sound
+    c = Cache((40, 10, 10, 10), 8, seed=6, max_pos=64)
+    c.cached[0] = c.slots - 3
+    c.pos[1], c.pos[2] = 60, -1
+    before = c.pool.clone()
+    lengths = (5, 5, 5, 5)
+    qkv = c.qkv(20)
+    got = kernels.chunk_attention(qkv, chunk_start=starts(lengths), max_chunk=5, **c.args())
+    assert torch.isnan(got[:15]).all()
+    c.cached[:3] = -1
+    want = c.want(qkv, lengths)
+    close(got[15:], want[15:])
+    pages = c.table[:3].long().flatten()
+    assert torch.equal(c.pool[pages], before[pages])
+    # more tokens than max_chunk says
+    got = kernels.chunk_attention(qkv, chunk_start=starts((0, 0, 0, 20)), max_chunk=5, **c.args())
+    assert torch.isnan(got).all()
+    # decode: the new slot behind the cache; positions
+    c.cached[:] = torch.tensor([c.slots, 10, 10, 10])
+    c.pos[3] = 10
+    q1 = c.qkv(4)
+    before = c.pool.clone()
+    got = kernels.window_decode_attention(q1, **c.args())
+    assert torch.isnan(got[[0, 2]]).all() and torch.isfinite(got[[1, 3]]).all()
+    pages = c.table[[0, 2]].long().flatten()
+    assert torch.equal(c.pool[pages], before[pages])
+
+
+def test_pages_outside_the_pool():
+    """A slot without a page poisons exactly the queries that see it."""
+    from soraku_tts_b200 import kernels
+
+    for bad in (-1, 10**6):
+        c = Cache((40, 40), 8, seed=6)
+        c.table[0, 1] = bad  # slots 16 .. 31 of row 0
+        qkv = c.qkv(16)
+        got = kernels.chunk_attention(qkv, chunk_start=starts((8, 8)), max_chunk=8, **c.args())
+        assert torch.isnan(got[:8]).all() and torch.isfinite(got[8:]).all()
+        # a window from slot 32 on does not see it
+        c.cached[:] = 46
+        got = kernels.window_decode_attention(c.qkv(2), window=14, **c.args())
+        assert torch.isfinite(got).all()
+        got = kernels.window_decode_attention(c.qkv(2), window=16, **c.args())
+        assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
+
+
+# ------------------------------------------------------------------- decode
+def decode(c, window=0, sinks=0, mass=False):
+    from soraku_tts_b200 import kernels
+
+    qkv = c.qkv(c.rows)
+    got = kernels.window_decode_attention(qkv, window=window, sinks=sinks, mass=c.mass if mass else None, **c.args())
+    return got, c.want(qkv, [1] * c.rows, window, sinks, mass)
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("cached", [(0,), (1, 0), (3, 4, 5), (31, 32, 33, 127, 128, 129, 700), (2500,)])
+@pytest.mark.parametrize("mass", [False, True])
+def test_window_decode_everything_visible(heads, cached, mass):
+    c = Cache(cached, 1, *heads, seed=sum(cached) + heads[1])
+    got, want = decode(c, mass=mass)
+    close(got, want)
+    c.check_cache()
+    c.check_mass()
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 7), (2, 0), (33, 4), (128, 300), (512, 16), (2**31 - 1, 0)])
+@pytest.mark.parametrize("page", [1, 16, 64])
+def test_window_decode_window(window, sinks, page):
+    c = Cache((0, 1, 32, 33, 34, 511, 900), 1, 4, 2, page=page, seed=window % 997, moved=77)
+    got, want = decode(c, window, sinks, mass=True)
+    close(got, want)
+    c.check_cache()
+    c.check_mass()
+
+
+@pytest.mark.parametrize("rows", [1, 9, 40, 150])
+def test_window_decode_ragged_batches(rows):
+    """Every cluster width, idle rows among them."""
+    g = torch.Generator().manual_seed(rows)
+    cached = [int(x) for x in torch.randint(0, 260, (rows,), generator=g)]
+    cached[rows // 2] = -1 if rows > 1 else cached[0]
+    c = Cache(cached, 1, seed=rows)
+    got, want = decode(c, 200, 2, mass=True)
+    close(got, want)
+    c.check_cache()
+    c.check_mass()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_window_decode_masked_garbage(bad):
+    c = Cache((200, 64, 5), 1, 8, 4, seed=9)
+    window, sinks = 50, 3
+    for r in range(3):
+        filled = int(c.cached[r])
+        for s in list(range(filled, c.slots)) + list(range(sinks, filled - window + 1)):
+            page = int(c.table[r, s // c.page])
+            c.pool[page, :, :, s % c.page] = bad
+            c.pool64[page, :, :, s % c.page] = bad
+    got, want = decode(c, window, sinks)
+    assert torch.isfinite(got).all()
+    close(got, want)
+
+
+def test_decode_agrees_with_chunks_of_one():
+    """The same token through both entry points."""
+    from soraku_tts_b200 import kernels
+
+    c = Cache((100, 7, 640), 1, seed=12)
+    qkv = c.qkv(3)
+    a = kernels.window_decode_attention(qkv, window=90, sinks=4, **c.args())
+    b = kernels.chunk_attention(qkv, chunk_start=starts((1, 1, 1)), max_chunk=1, window=90, sinks=4, **c.args())
+    close(a, b.double())
+
+
+# ----------------------------------------------------------------- eviction
+def plain_evict(c, budget, sinks, recent):
+    kept, mass = [], torch.zeros_like(c.mass)
+    pool = c.pool.clone()
+    for r in range(c.rows):
+        n = int(c.cached[r])
+        n = 0 if n < 0 or n > c.slots else n
+        for g in range(c.G):
+            keep = list(range(n))
+            if n > budget:
+                w = c.mass[r, g].tolist()
+                mid = sorted(range(sinks, n - recent), key=lambda j: (0 if w[j] != w[j] else 1, -w[j] if w[j] == w[j] else 0, j))
+                keep = sorted(list(range(sinks)) + mid[:budget - sinks - recent] + list(range(n - recent, n)))
+            kept.append(keep + [-1] * (budget - len(keep)))
+            for to, s in enumerate(keep):
+                mass[r, g, to] = c.mass[r, g, s]
+                pool[int(c.table[r, to // c.page]), :, g, to % c.page] = \
+                    c.pool[int(c.table[r, s // c.page]), :, g, s % c.page]
+    return torch.tensor(kept, dtype=torch.int32).view(c.rows, c.G, budget), mass, pool
+
+
+def check_evict(c, budget, sinks, recent):
+    from soraku_tts_b200 import kernels
+
+    want_kept, want_mass, want_pool = plain_evict(c, budget, sinks, recent)
+    before = c.mass.clone()
+    kept, mass, cached = kernels.evict_cache(c.mass, cached=c.cached, kv_pool=c.pool, page_table=c.table,
+                                             page_size=c.page, budget=budget, sinks=sinks, recent=recent)
+    assert torch.equal(kept.cpu(), want_kept)
+    assert torch.equal(torch.nan_to_num(mass, nan=-5.0), torch.nan_to_num(want_mass, nan=-5.0))
+    assert torch.equal(c.pool, want_pool)
+    assert torch.equal(torch.nan_to_num(c.mass, nan=-5.0), torch.nan_to_num(before, nan=-5.0))
+    ok = (c.cached >= 0) & (c.cached <= c.slots)
+    assert torch.equal(cached, torch.where(ok, torch.clamp(c.cached, max=budget), c.cached))
+    return kept, mass, cached
+
+
+@pytest.mark.parametrize("budget,sinks,recent", [(1, 0, 0), (1, 1, 0), (1, 0, 1), (7, 2, 3), (64, 4, 60), (100, 0, 0),
+                                                 (129, 4, 32), (400, 100, 200), (5000, 3, 9)])
+@pytest.mark.parametrize("page", [1, 16, 64])
+def test_evict(budget, sinks, recent, page):
+    check_evict(Cache((0, 1, 64, 130, 700), 3, 2, 2, page=page, seed=budget), budget, sinks, recent)
+
+
+@pytest.mark.parametrize("kind", ["all_equal", "few_values", "zeros_and_signs", "nan_inf", "descending", "ascending"])
+def test_evict_ties_and_odd_weights(kind):
+    c = Cache((300, 77, 50), 1, 4, 4, seed=1)
+    m = c.mass
+    if kind == "all_equal":
+        m.fill_(0.25)
+    elif kind == "few_values":
+        m.copy_((m * 4).floor())
+    elif kind == "zeros_and_signs":
+        m.copy_(((m - 0.5) * 3).round() * 0.5)
+        m[:, :, ::3] *= 0.0  # zeros of both signs rank alike
+    elif kind == "nan_inf":
+        m[:, :, 5::17], m[:, :, 7::19], m[:, :, 9::23] = math.nan, math.inf, -math.inf
+    else:
+        m.copy_(torch.arange(c.slots, device="cuda").float().expand_as(m) * (1 if kind == "ascending" else -1))
+    check_evict(c, 60, 2, 8)
+
+
+def test_evict_long_and_many_rows():
+    check_evict(Cache((9000,), 1, 2, 2, page=64, seed=2), 2049, 4, 100)
+    g = torch.Generator().manual_seed(3)
+    check_evict(Cache([int(x) for x in torch.randint(-1, 90, (70,), generator=g)], 1, 2, 1, seed=3), 33, 1, 5)
+
+
+def test_evict_counts_outside_the_cache():
+    c = Cache((30, 30, 30), 2, 2, 2, seed=4)
+    c.cached[0], c.cached[1] = c.slots + 1, -1
+    check_evict(c, 10, 1, 2)
+
+
+# ------------------------------------------------------------------ together
+def stream(c, window=0, sinks=2, budget=48, recent=8):
+    """Prompt in two pieces, frames, an eviction, more frames: the operators as
+    a long stream uses them.  Yields (output, what it should be)."""
+    from soraku_tts_b200 import kernels
+
+    def chunk_step(lengths):
+        qkv = c.qkv(sum(lengths))
+        got = kernels.chunk_attention(qkv, chunk_start=starts(lengths), max_chunk=max(lengths), window=window,
+                                      sinks=sinks if window else 0, mass=c.mass, **c.args())
+        want = c.want(qkv, lengths, window, sinks, True)
+        n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        c.cached, c.pos = c.cached + n, c.pos + n
+        return got, want
+
+    def frame():
+        qkv = c.qkv(c.rows)
+        got = kernels.window_decode_attention(qkv, window=window, sinks=sinks if window else 0, mass=c.mass, **c.args())
+        want = c.want(qkv, [1] * c.rows, window, sinks, True)
+        c.cached, c.pos = c.cached + 1, c.pos + 1
+        return got, want
+
+    yield chunk_step([40] * c.rows)
+    yield chunk_step([30 - r for r in range(c.rows)])
+    for _ in range(3):
+        yield frame()
+    for _ in range(2):
+        c.check_mass()
+        kept, mass, cached = kernels.evict_cache(c.mass, cached=c.cached, kv_pool=c.pool, page_table=c.table,
+                                                 page_size=c.page, budget=budget, sinks=sinks, recent=recent)
+        # the restatement keeps what the kernel chose (weights agree to
+        # rounding only), after checking that choice against its own weights
+        for r in range(c.rows):
+            n = int(c.cached[r])
+            for g in range(c.G):
+                k = kept[r, g][kept[r, g] >= 0].long()
+                w = c.mass64[r, g, :n].clone()
+                w[:sinks] = w[n - recent:] = math.inf
+                out = torch.ones(n, dtype=torch.bool, device="cuda")
+                out[k] = False
+                if n > budget:
+                    assert k.numel() == budget and float(w[k].min()) >= float(w[:n][out].max()) * (1 - 1e-5)
+                flat = c.pool64[c.table[r].long()][:, :, g].permute(1, 0, 2, 3).reshape(2, -1, HD)
+                flat[:, :k.numel()] = flat[:, k].clone()
+                c.pool64[c.table[r].long(), :, g] = flat.view(2, c.max_pages, c.page, HD).permute(1, 0, 2, 3)
+                m = torch.zeros_like(c.mass64[r, g])
+                m[:k.numel()] = c.mass64[r, g][k]
+                c.mass64[r, g] = m
+        c.mass, c.cached = mass, cached
+        yield frame()
+        yield chunk_step([5] * c.rows)
+
+
+@pytest.mark.parametrize("window", [0, 33])
+def test_stream(window):
+    c = Cache((0, 0, 0), 90, 8, 4, seed=21)
+    for got, want in stream(c, window):
+        close(got, want)
+    c.check_cache()
+    c.check_mass()
+
+
+def test_repeat_gives_the_same_bits():
+    from soraku_tts_b200 import kernels
+
+    res = []
+    for _ in range(2):
+        c = Cache((300, 1200), 140, seed=30)
+        a, _ = chunk(c, (140, 3), 500, 4, mass=True)
+        d, _ = decode(c, 300, 4, mass=True)
+        e = kernels.evict_cache(c.mass, cached=c.cached, kv_pool=c.pool, page_table=c.table, page_size=c.page, budget=200)
+        res.append([a, d, *e, c.pool, c.mass])
+    for x, y in zip(*res):
+        assert torch.equal(x, y)
+
+
+def test_on_another_stream_and_in_graphs():
+    """Two captured graphs of the same calls on different caches, replayed side
+    by side on two streams with new inputs: each keeps to its own memory."""
+    from soraku_tts_b200 import kernels
+
+    both = []
+    for seed in (40, 41):
+        c = Cache((100, 333), 50, seed=seed)
+        c.static = c.qkv(100)
+        c.frame = c.qkv(2)
+        c.start = starts((50, 50))
+        pool0, mass0 = c.pool.clone(), c.mass.clone()
+
+        def calls(c=c):
+            a = kernels.chunk_attention(c.static, chunk_start=c.start, max_chunk=50, mass=c.mass, **c.args())
+            d = kernels.window_decode_attention(c.frame, window=70, sinks=1, mass=c.mass, **c.args())
+            e = kernels.evict_cache(c.mass, cached=c.cached, kv_pool=c.pool, page_table=c.table, page_size=c.page, budget=80)
+            return [a, d, *e]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            calls()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = calls()
+        both.append((c, g, res, calls, pool0, mass0, side))
+    for c, *_ in both:
+        c.static.copy_(c.qkv(100))
+        c.frame.copy_(c.qkv(2))
+    want = []
+    for c, g, res, calls, pool0, mass0, side in both:
+        c.pool.copy_(pool0)
+        c.mass.copy_(mass0)
+        want.append([t.clone() for t in calls()] + [c.pool.clone(), c.mass.clone()])
+        c.pool.copy_(pool0)
+        c.mass.copy_(mass0)
+    torch.cuda.synchronize()
+    for c, g, res, calls, pool0, mass0, side in both:
+        with torch.cuda.stream(side):
+            g.replay()
+    torch.cuda.synchronize()
+    for (c, g, res, *_), w in zip(both, want):
+        for x, y in zip(res + [c.pool, c.mass], w):
+            assert torch.equal(x, y)
+
+
+def test_offsets_past_32_bits():
+    """Pages more than 2^31 floats into the pool."""
+    from soraku_tts_b200 import kernels
+
+    c = Cache((70, 40), 30, 4, 2, page=64, seed=50)
+    unit = 2 * c.G * c.page * HD
+    far = 2**32 // unit + 5
+    big = torch.zeros(far + c.pool.shape[0], 2, c.G, c.page, HD, device="cuda")
+    big[far:] = c.pool
+    qkv, frame = c.qkv(45), c.qkv(2)
+    kw = dict(chunk_start=starts((30, 15)), max_chunk=30)
+    a = kernels.chunk_attention(qkv, **kw, **c.args())
+    b = kernels.chunk_attention(qkv, **kw, **c.args(kv_pool=big, page_table=c.table + far))
+    assert torch.equal(a, b)
+    a = kernels.window_decode_attention(frame, **c.args())
+    b = kernels.window_decode_attention(frame, **c.args(kv_pool=big, page_table=c.table + far))
+    assert torch.equal(a, b)
+    for pool, table in ((c.pool, c.table), (big, c.table + far)):
+        kernels.evict_cache(c.mass, cached=c.cached, kv_pool=pool, page_table=table, page_size=c.page, budget=20)
+    assert torch.equal(big[far:], c.pool)
+
+
+def test_python_layer_refusals():
+    from soraku_tts_b200 import kernels
+
+    c = Cache((5, 5), 4, seed=60)
+    qkv = c.qkv(2)
+    for kw, match in ((dict(kv_pool=c.pool.transpose(1, 2)), "kv_pool"), (dict(page_size=32), "kv_pool"),
+                      (dict(cached=c.cached.long()), "cached"), (dict(pos=c.pos[:1]), "pos"),
+                      (dict(q_norm=c.qn[:64]), "q_norm"), (dict(mass=c.mass[:, :, 1:]), "mass"),
+                      (dict(out=torch.empty(2, 7, device="cuda")), "out"), (dict(sinks=2), "sinks"),
+                      (dict(rope_sin=c.sin[:5]), "rope_sin"), (dict(page_table=c.table.float()), "page_table")):
+        with pytest.raises(ValueError, match=match):
+            kernels.window_decode_attention(qkv, **c.args(**kw))
+    with pytest.raises(ValueError, match="qkv"):
+        kernels.window_decode_attention(qkv.double(), **c.args())
+    with pytest.raises(ValueError, match="chunk_start"):
+        kernels.chunk_attention(qkv, chunk_start=starts((2,)), max_chunk=2, **c.args())
+    with pytest.raises(ValueError, match="heads"):
+        kernels.chunk_attention(torch.empty(2, (40 + 16) * HD, device="cuda"), chunk_start=starts((1, 1)), max_chunk=1,
+                                **c.args(n_heads=40))
+    with pytest.raises(ValueError, match="budget"):
+        kernels.evict_cache(c.mass, cached=c.cached, kv_pool=c.pool, page_table=c.table, page_size=c.page, budget=3,
+                            sinks=2, recent=2)
