@@ -1,0 +1,234 @@
+// fp16 tensor-core pieces of the cache operators: FP32 operands as pairs of
+// fp16 tiles, the shared-memory and instruction descriptors of
+// tcgen05.mma kind::f16, tensor-memory loads and stores, bounded waits.
+//
+// An FP32 row x is scaled by a power of two to a largest magnitude in
+// [2^13, 2^14) and split into hi = fp16(x) and lo = fp16(x - hi): 22 bits,
+// and an absolute floor 2^-38 of the row's largest.  A product of two such
+// operands is hi.hi + hi.lo + lo.hi in FP32 (the dropped lo.lo is 2^-22
+// relative): three fp16 products at twice the rate of TF32 in half its shared
+// memory, where three TF32 products give the same bits.
+//
+// Tiles are [two halves of 64 columns][128 rows][128 bytes], each half in the
+// 128-byte swizzle (16-byte chunk c of row r at c ^ (r & 7)).  The same bytes
+// serve as a K-major operand whose rows are M or N (queries, keys) and as an
+// MN-major one whose rows are K (values).
+#pragma once
+
+#include "cache_ops.cuh"
+
+namespace skb {
+
+constexpr int UT_ROWS = 128;
+constexpr uint32_t UT_HALF = 128 * 128;       // bytes of 64 columns
+constexpr uint32_t UT_BYTES = 2 * UT_HALF;    // one fp16 tile
+constexpr float UT_POISON_E = -200.f;         // exponent of a row of zeros
+
+// ------------------------------------------------------------- descriptors
+// Shared-memory operand, 128-byte swizzle.  K-major: 8-row groups 1024 bytes
+// apart.  MN-major: 64-column halves `UT_HALF` apart (leading offset), 8-row
+// groups along K 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t ut_desc(uint32_t saddr, bool mn_major) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(mn_major ? (UT_HALF >> 4) : 1u) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+// kind::f16, D FP32, A and B fp16, M = N = 128.
+__host__ __device__ constexpr uint32_t ut_idesc(bool b_mn_major) {
+    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | (16u << 17) | (8u << 24);
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void ut_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// The accumulation in tensor memory cuts towards zero (measured: about 1e-8 of
+// the sum per step of 16 at full size, all of one sign), so the small
+// products come first, where the sum is still 2^-11 of its size, and no sum
+// runs on from tile to tile: that grew to 1.3e-5 over 8000 slots.
+
+// D[128 x 128] = A B^T over 128 columns, both operands as hi | lo tile pairs
+// (K-major) in shared memory.
+__device__ __forceinline__ void ut_mma_qk(uint32_t d, uint32_t a, uint32_t b) {
+    asm volatile("" : "+r"(a), "+r"(b));  // keeps 48 descriptors from being held across a caller's loop
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const uint64_t da = ut_desc(a + (p == 1 ? UT_BYTES : 0), false), db = ut_desc(b + (p == 0 ? UT_BYTES : 0), false);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint64_t off = ((k >> 2) * UT_HALF + (k & 3) * 32) >> 4;  // in the address field
+            umma_f16_ss(d, da + off, db + off, ut_idesc(false), p > 0 || k > 0);
+        }
+    }
+}
+// D[128 x 128] = P V: P as hi | lo (64 TMEM columns each), V as hi | lo tiles (MN-major).
+__device__ __forceinline__ void ut_mma_pv(uint32_t d, uint32_t p_tmem, uint32_t v) {
+    asm volatile("" : "+r"(p_tmem), "+r"(v));
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const uint32_t pa = p_tmem + (p == 1 ? 64 : 0);
+        const uint64_t dv = ut_desc(v + (p == 0 ? UT_BYTES : 0), true);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) umma_f16_ts(d, pa + k * 8, dv + (k * 2048 >> 4), ut_idesc(true), p > 0 || k > 0);
+    }
+}
+
+// ---------------------------------------------------------- tensor memory
+__device__ __forceinline__ void ut_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
+          "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
+          "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void ut_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void ut_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void ut_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ut_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ut_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ut_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ut_alloc(uint32_t* slot) {  // one warp, 512 columns
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void ut_free(uint32_t tmem) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// ----------------------------------------------------------------- waits
+__device__ __forceinline__ void ut_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Waits for phase `parity`, at most about 2 s and no longer than *abort stays
+// 0; false (and *abort set) when it gave up.  Every wait of a kernel goes
+// through here, so that one that runs out ends all the others.
+__device__ __forceinline__ bool ut_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    const uint32_t addr = smem_u32(bar);
+    uint64_t t0 = 0;
+    for (int it = 0;; ++it) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (it == 0) t0 = globaltimer_ns();
+        else if ((it & 63) == 0 && (*abort || globaltimer_ns() - t0 > SKB_WAIT_LIMIT_NS)) {
+            *abort = 1;
+            return false;
+        }
+    }
+}
+
+// ------------------------------------------------------- splitting a row
+// Pairs of FP32 in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+// The same on pairs that stay 64-bit registers.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t a) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2p(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+// hi = fp16 pair of x, lo = fp16 pair of what is left.
+__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
+    float2 f;
+    asm("{\n .reg .b16 p, q;\n cvt.rn.f16x2.f32 %0, %4, %3;\n mov.b32 {p, q}, %0;\n cvt.f32.f16 %1, p;\n cvt.f32.f16 %2, q;\n}"
+        : "=&r"(hi), "=f"(f.x), "=f"(f.y)
+        : "f"(x.x), "f"(x.y));
+    const float2 r = add2(x, make_float2(-f.x, -f.y));
+    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(lo) : "f"(r.x), "f"(r.y));
+}
+// Exponent floor(log2 max|x|) of a row held by a warp (4 numbers a lane), as
+// a whole number clamped to [-100, 127]; UT_POISON_E for a row of zeros, NaN
+// for one that holds something not finite.
+__device__ __forceinline__ float row_exponent(float4 x) {
+    const unsigned m = max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu),
+                           max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
+    const unsigned r = __reduce_max_sync(FULL, m);
+    const float e = (float)max((int)(r >> 23) - 127, -100);
+    return r >= 0x7f800000u ? __int_as_float(0x7fffffff) : (r == 0 ? UT_POISON_E : e);
+}
+// 2^e for whole e in [-126, 127].
+__device__ __forceinline__ float pow2_whole(float e) { return __int_as_float(((int)e + 127) << 23); }
+// Scales this lane's 4 numbers of row r by 2^(13 - e) and writes them to the
+// tile pair at `tile` (hi, then lo UT_BYTES further).  Rows that are not
+// finite become zeros.
+__device__ __forceinline__ void put_row(unsigned char* tile, int r, int lane, float4 x, float e) {
+    const bool ok = e == e;
+    const float s = ok ? pow2_whole(13.f - fmaxf(e, -100.f)) : 0.f;
+    if (!ok) x = make_float4(0.f, 0.f, 0.f, 0.f);
+    uint2 hi, lo;
+    const float2 s2 = make_float2(s, s);
+    split2(mul2(make_float2(x.x, x.y), s2), hi.x, lo.x);
+    split2(mul2(make_float2(x.z, x.w), s2), hi.y, lo.y);
+    const uint32_t at = (uint32_t)(lane >> 4) * UT_HALF + (uint32_t)r * 128u +
+                        ((((uint32_t)(lane & 15) >> 1) ^ (uint32_t)(r & 7)) * 16u) + (uint32_t)(lane & 1) * 8u;
+    *reinterpret_cast<uint2*>(tile + at) = hi;
+    *reinterpret_cast<uint2*>(tile + UT_BYTES + at) = lo;
+}
+
+}  // namespace skb
