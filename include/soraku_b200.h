@@ -191,9 +191,13 @@ int skb_decode_attention_noalloc(const float *qkv, int rows, int n_heads, int n_
  *               chunk_start[rows] are neither read nor written
  *   rope_cos/sin device [max_pos, 64];  cached, pos: device int32 [rows]
  *   kv_pool, page_table as for skb_decode_attention
- *   out         device [tokens, n_heads * 128] */
+ *   out         device [tokens, n_heads * 128]
+ * The workspace holds the queries and the seen keys and values in the form the
+ * tensor cores read: up to 1 KB per seen slot and kv head, at most the size of
+ * the pool and 128 KB per row and kv head, and 512 B per token and head. */
 int64_t skb_chunk_attention_workspace(int tokens, int rows, int max_chunk, int n_heads, int n_kv_heads,
-                                      int max_pages, int page_size, int with_mass);
+                                      int max_pages, int page_size, int n_pages, int window, int sinks,
+                                      int with_mass);
 int skb_chunk_attention(const float *qkv, int tokens, int rows, int n_heads, int n_kv_heads, int head_dim,
                         const float *q_norm, const float *k_norm, float eps, const float *rope_cos,
                         const float *rope_sin, int max_pos, const int32_t *chunk_start, int max_chunk,

@@ -39,7 +39,7 @@ SIGNATURES = {
     "skb_decode_attention_noalloc": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float,
                                              c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                              c_int, c_int, c_void_p, c_void_p]),
-    "skb_chunk_attention_workspace": (c_int64, [c_int] * 8),
+    "skb_chunk_attention_workspace": (c_int64, [c_int] * 11),
     "skb_chunk_attention": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p,
                                     c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                     c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),

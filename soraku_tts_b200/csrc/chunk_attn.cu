@@ -5,10 +5,17 @@
 //   o_ih = sum_j p_ihj v_j,  p_ihj = exp(q_ih.k_j / sqrt(128) - lse_ih) over the slots i sees
 //   mass[row][g][j] += sum_i sum over g's heads of p_ihj  (new slots begin at zero)
 //
-// Three launches: chunk_prep norms, rotates, appends k and v and writes the
-// queries as split fp16 tiles; chunk_attn; and, with `mass`, chunk_mass.
+// Three launches.  chunk_prep norms, rotates and appends the new keys and
+// values, and writes queries, and all keys and values that are seen, as split
+// fp16 tiles (umma.cuh) in the order in which the tensor cores read them;
+// chunk_attn; and, with `mass`, chunk_mass.  The tiles are written once for
+// all query tiles of a row: splitting them inside chunk_attn, per query tile,
+// kept its warps busy for two thirds of the time (8 queries tiles of 512 tokens
+// over 8192 slots: 160 us against 8.5 us of chunk_prep, measured).
 // A query tile is 128 (token, head) pairs of one kv head, P = 128 / n_rep
 // tokens, so a key or value tile that was loaded once serves all of them.
+#include <type_traits>
+
 #include "umma.cuh"
 
 namespace skb {
@@ -18,8 +25,12 @@ struct ChunkArgs {
     const int* chunk_start;  // [rows + 1]
     int tokens, max_chunk;
     int n_rep, P;           // heads per kv head, tokens per query tile
-    unsigned char* qtiles;  // workspace [tiles][KVH][2 UT_BYTES]: queries in log2 units, hi | lo
-    float* lse;             // workspace [tiles][KVH][128] (mass only), log2 units
+    // workspace
+    unsigned char* qtiles;  // [query tiles][KVH][2 UT_BYTES]: queries in log2 units, hi | lo
+    unsigned char* kvtiles; // [key tiles][KVH][2][2 UT_BYTES]: keys, values, hi | lo
+    float* meta;            // [key tiles][KVH][2][128]: factor of a key's scores; exponent of a value row
+    float* lse;             // [query tiles][KVH][128] (mass only), log2 units
+    long long key_tiles;
 };
 
 // What a row asks for: its tokens [b, b + n) and whether its numbers lie
@@ -47,6 +58,27 @@ __device__ __forceinline__ long long chunk_tile(const ChunkArgs& c, const ChunkR
     return x.b / c.P + r + t;
 }
 
+// The tiles of 128 slots that any query of a row sees: [0, a1) for the sinks,
+// [b0, end) for the windows.
+struct RowTiles {
+    int a1, b0, n, w0;
+    __device__ __forceinline__ RowTiles(const ChunkArgs& c, const ChunkRow& x) {
+        w0 = c.a.window > 0 ? max(0, x.cached - c.a.window + 1) : 0;  // first slot of the first query's window
+        a1 = (min(c.a.sinks, w0) + 127) >> 7;
+        b0 = max(w0 >> 7, a1);
+        n = x.idle || x.bad || x.n == 0 ? 0 : a1 + ((x.cached + x.n - 1) >> 7) + 1 - b0;
+    }
+    __device__ __forceinline__ int index(int tile) const { return tile < a1 ? tile : a1 + tile - b0; }
+    __device__ __forceinline__ int tile(int k) const { return k < a1 ? k : b0 + k - a1; }
+};
+// Where a row's key tiles begin in the workspace: behind those of the rows
+// before it.  By a whole warp.
+__device__ __forceinline__ long long row_base(const ChunkArgs& c, int r) {
+    int n = 0;
+    for (int p = threadIdx.x & 31; p < r; p += 32) n += RowTiles(c, chunk_row(c, p)).n;
+    return __reduce_add_sync(FULL, n);
+}
+
 // A whole number e with |q| < 2^e for every query in log2 units: a normed head
 // is at most sqrt(128) max|w| long per element, its rotation sqrt(2) times that.
 __device__ __forceinline__ float query_exponent(const float* qn, int lane) {
@@ -58,35 +90,110 @@ __device__ __forceinline__ float query_exponent(const float* qn, int lane) {
 
 constexpr float CH_QSCALE = 0.08838834764831845f * CO_LOG2E;  // 1 / sqrt(128), scores in log2 units
 
-// grid (min(max_chunk, 4096), rows, ceil((H + 2 KVH) / 8)), 256 threads: a warp per head vector
-__global__ void __launch_bounds__(256) chunk_prep_kernel(const ChunkArgs c) {
+constexpr int CP_TILES = 64;  // blocks side by side over a row's key tiles
+
+// Blocks [0, tokens): a new token each, 256 threads, a warp per head vector.
+// The others: cached slots, a block per (key tile, keys or values, kv head, row).
+__global__ void __launch_bounds__(256) chunk_prep_kernel(const ChunkArgs c, int tiles_x) {
     const CacheAttnArgs& a = c.a;
-    const int r = blockIdx.y, lane = threadIdx.x & 31, v = blockIdx.z * 8 + (threadIdx.x >> 5);
-    const ChunkRow x = chunk_row(c, r);
-    const int H = a.H, KVH = a.kv.KVH;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int H = a.H, KVH = a.kv.KVH, nv = H + 2 * KVH;
     pdl_trigger();
-    if (v >= H + 2 * KVH) return;
     const float eq = query_exponent(a.qn, lane);
-    for (int i = blockIdx.x; i < x.n; i += gridDim.x) {
-        const long long t = x.b + i;
+    const float qfac = pow2_whole(eq - 13.f);
+    if ((int)blockIdx.x < c.tokens) {
+        const int t = blockIdx.x;
+        int r = 0;  // rows that end at or before the token
+        for (int p = lane; p - lane < a.rows; p += 32)
+            r += __popc(__ballot_sync(FULL, p < a.rows && c.chunk_start[p + 1] <= t));
+        if (r >= a.rows) return;
+        ChunkRow x = chunk_row(c, r);
+        const int i = t - x.b;
+        if (i < 0 || i >= x.n) return;
+        const RowTiles rt(c, x);
+        const long long base = row_base(c, r);
+        if (base + rt.n > c.key_tiles) x.bad = true;  // pages mapped to several rows
         if (x.idle || x.bad) {
             const float o = x.idle ? 0.f : __int_as_float(0x7fffffff);
-            if (v < H) reinterpret_cast<float4*>(a.out)[(t * H + v) * 32 + lane] = make_float4(o, o, o, o);
-            continue;
+            for (int v = warp; v < H; v += 8)
+                reinterpret_cast<float4*>(a.out)[((long long)t * H + v) * 32 + lane] = make_float4(o, o, o, o);
+            return;
         }
         const int pos = a.pos[r] + i, slot = x.cached + i;
-        float4 y = reinterpret_cast<const float4*>(a.qkv)[(t * (H + 2 * KVH) + v) * 32 + lane];
-        if (v < H + KVH)
-            y = norm_rope_head(y, v < H ? a.qn : a.kn, a.eps, a.rope_cos + (long long)pos * 64,
-                               a.rope_sin + (long long)pos * 64, lane, true, true);
-        if (v < H) {
-            const int g = v / c.n_rep, m = (i % c.P) * c.n_rep + v % c.n_rep;
-            unsigned char* tile = c.qtiles + (chunk_tile(c, x, r, i / c.P) * KVH + g) * (2 * UT_BYTES);
-            put_row(tile, m, lane, make_float4(y.x * CH_QSCALE, y.y * CH_QSCALE, y.z * CH_QSCALE, y.w * CH_QSCALE), eq);
-        } else {
-            const bool value = v >= H + KVH;
-            const long long u = a.kv.key_unit(r, slot, v - H - (value ? KVH : 0));
-            if (u >= 0) reinterpret_cast<float4*>(a.kv.pool)[(u + (value ? a.kv.value_step() : 0)) * 32 + lane] = y;
+        const float4* row = reinterpret_cast<const float4*>(a.qkv) + (long long)t * nv * 32 + lane;
+        const float* cosr = a.rope_cos + (long long)pos * 64;
+        const float* sinr = a.rope_sin + (long long)pos * 64;
+        const long long tile = base + rt.index(slot >> 7);
+        for (int v0 = warp; v0 < nv; v0 += 32) {
+            float4 y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (v0 + 8 * j < nv) y[j] = row[(v0 + 8 * j) * 32];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int v = v0 + 8 * j;
+                if (v >= nv) break;
+                if (v < H + KVH) y[j] = norm_rope_head(y[j], v < H ? a.qn : a.kn, a.eps, cosr, sinr, lane, true, true);
+                if (v < H) {
+                    const int g = v / c.n_rep, m = (i % c.P) * c.n_rep + v % c.n_rep;
+                    unsigned char* q = c.qtiles + (chunk_tile(c, x, r, i / c.P) * KVH + g) * (2 * UT_BYTES);
+                    put4(q + ut_at(m, lane), y[j], CH_QSCALE * pow2_whole(13.f - eq));
+                    continue;
+                }
+                const int value = v >= H + KVH, g = v - H - (value ? KVH : 0);
+                const long long u = a.kv.key_unit(r, slot, g);
+                if (u >= 0) reinterpret_cast<float4*>(a.kv.pool)[(u + (value ? a.kv.value_step() : 0)) * 32 + lane] = y[j];
+                float top = max3_abs(max3_abs(y[j].x, y[j].y, y[j].z), y[j].w, 0.f);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = max3_abs(top, __shfl_xor_sync(FULL, top, o), 0.f);
+                const float e = u >= 0 ? top_exponent(top) : __int_as_float(0x7fffffff);
+                if (!(e >= -100.f)) y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                put4(c.kvtiles + ((tile * KVH + g) * 2 + value) * (2 * UT_BYTES) + ut_at(slot & 127, lane), y[j], row_scale(e));
+                if (lane == 0)
+                    c.meta[((tile * KVH + g) * 2 + value) * 128 + (slot & 127)] =
+                        value ? e : e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac : e;
+            }
+        }
+        return;
+    }
+    int b = blockIdx.x - c.tokens;
+    const int k0 = b % tiles_x;
+    b /= tiles_x;
+    const int value = b & 1, g = (b >> 1) % KVH, r = (b >> 1) / KVH;
+    const ChunkRow x = chunk_row(c, r);
+    const RowTiles rt(c, x);
+    if (k0 >= rt.n) return;
+    const long long base = row_base(c, r);
+    if (base + rt.n > c.key_tiles) return;
+    const float4* pool = reinterpret_cast<const float4*>(a.kv.pool) + (value ? a.kv.value_step() * 32 : 0);
+    const int row0 = warp * 16, i4 = lane >> 3, last = x.cached + x.n - 1;
+    for (int k = k0; k < rt.n; k += tiles_x) {
+        const int first = rt.tile(k) * 128 + row0;
+        if (first >= x.cached && first + 15 <= last) continue;  // new tokens only: theirs are written above
+        const long long at = ((base + k) * KVH + g) * 2 + value;
+        RowSet<4> d;
+        uint32_t unit[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int slot = first + 4 * q + i4;
+            unit[q] = UT_NONE;
+            if (slot < x.cached && (slot >= rt.w0 || slot < a.sinks)) {
+                const long long u = a.kv.key_unit(r, slot, g);
+                unit[q] = u < 0 ? UT_BAD : (uint32_t)u;
+            }
+        }
+        d.zero();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) d.load(q, pool, unit[q], lane);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float e = d.exponent(q, unit[q]);
+            const int slot = first + 4 * q + i4;
+            if (!(e >= -100.f)) d.zero(q);
+            if (slot >= x.cached && slot <= last) continue;
+            d.put(q, c.kvtiles + at * (2 * UT_BYTES), row0, row_scale(e), lane);
+            if ((lane & 7) == 0)
+                c.meta[at * 128 + row0 + 4 * q + i4] = value ? e : e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac : e;
         }
     }
 }
@@ -98,8 +205,10 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(const ChunkArgs c) {
 struct TileList {
     int n, full, full0;      // tiles; how many are whole; the first whole one
     int a1, b0, head;        // sink tiles [0, a1); window tiles from b0; of them `head` before the whole ones
+    int w0, last;            // first slot of any query's window; the last slot seen
     __device__ __forceinline__ TileList(int own_lo, int own_hi, int window, int sinks) {
-        const int w0 = window > 0 ? max(0, own_lo - window + 1) : 0;  // first slot of any query's window
+        w0 = window > 0 ? max(0, own_lo - window + 1) : 0;
+        last = own_hi;
         a1 = (min(sinks, w0) + 127) >> 7;
         b0 = max(w0 >> 7, a1);
         const int end = (own_hi >> 7) + 1;  // every tile before it holds a visible slot
@@ -122,49 +231,51 @@ struct TileList {
 };
 
 // -------------------------------------------------------------- chunk_attn
-constexpr int CA_SOFTMAX_WARPS = 4, CA_CONV_WARPS = 8;
-constexpr int CA_MMA_WARP = CA_SOFTMAX_WARPS + CA_CONV_WARPS;
-constexpr int CA_THREADS = 512;  // whole warpgroups: softmax, two of converters, one whose first warp issues products
-// Registers a thread: all are launched with 128.  The softmax threads hold a
-// whole output row, so they take from the others meanwhile; every sum over the
-// four warpgroups stays within the launch's 4 x 128.  Nobody takes registers
-// back before the softmax threads have given theirs up (a CTA-wide barrier
-// lies between): a warpgroup that is done early, or has nothing to do, would
-// otherwise take what they still wait for.
-constexpr int CA_REGS = 65536 / CA_THREADS, CA_REGS_SOFTMAX = 240, CA_REGS_CONV = 104, CA_REGS_MMA = 64;
-static_assert(CA_REGS_SOFTMAX + 2 * CA_REGS_CONV + CA_REGS_MMA <= 4 * CA_REGS, "register split");
-template <int N>
-__device__ __forceinline__ void regs_up() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_down() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-constexpr int CA_ROWS_PER_WARP = UT_ROWS / CA_CONV_WARPS;  // 16
-constexpr uint32_t CA_TM_O = 256, CA_TM_P = 384;           // TMEM columns: scores [0, 256), output, weights
-constexpr int CA_OUT_LD = 132;                              // floats of a staged output row
+// A CTA takes one query tile and a part of the key tiles it sees:
+//   warp P     asks for key and value tiles, 64 KB bulk copies into three
+//              stages, in the order K0 K1 V0 K2 V1 ...
+//   warp M     issues the products: S_i = Q K_i, then O = P_i V_i, S one tile ahead
+//   warp E     a tile's factors and exponents from the workspace, and the
+//              running exponent of the values
+//   softmax    CA_PARTS threads per query row, each with a part of a tile's
+//              keys and of the output's columns
+// Queries stay in tensor memory; weights overwrite their scores there; each
+// tile's output is added up in registers.
+constexpr int CA_PARTS = 4;
+constexpr int CA_W = 128 / CA_PARTS;  // a thread's keys, and its output columns
+constexpr int CA_SOFTMAX_WARPS = 4 * CA_PARTS, CA_WARP_M = CA_SOFTMAX_WARPS, CA_WARP_P = CA_WARP_M + 1,
+              CA_WARP_E = CA_WARP_M + 2;
+constexpr int CA_THREADS = 32 * (CA_SOFTMAX_WARPS + 4);
+constexpr int CA_STAGES = 3;
+// TMEM columns: two score tiles, a tile's output, the queries
+constexpr uint32_t CA_TM_O = 256, CA_TM_Q = 384;
+constexpr int CA_OUT_LD = 132;  // floats of a staged output row
 constexpr int CA_MAX_SPLITS = 8;
 
 struct CaSmem {
-    unsigned char q[2 * UT_BYTES];
-    unsigned char k[2 * UT_BYTES];
-    unsigned char v[2 * UT_BYTES];
-    float kc[3][128];                // factor of a key's scores: its scale undone
-    float ve[2][128];                // exponent of a value row
-    float vg[2][128];                // factor of its weights: 2^(exponent - the tile's running one + 6)
-    float vmax[2][CA_CONV_WARPS];    // largest exponent of a warp's rows
-    float m[128], l[128];            // this split's statistics
-    uint64_t q_full, k_full, k_empty, v_full, v_empty, p_full, s_full[2], ve_full[2], o_full;
+    unsigned char stage[CA_STAGES][2 * UT_BYTES];
+    float kc[2][128];                    // factor of a key's scores: its scale undone
+    float ve[2][128];                    // exponent of a value row
+    float vg[2][128];                    // factor of its weights: 2^(exponent - E + 6)
+    float mx[2][CA_PARTS][128], ex[2][CA_PARTS][128];  // a row part's largest score and value exponent
+    float m[128], l[CA_PARTS][128];      // this split's statistics (sums of row parts)
+    float E[2];                          // running exponent of the values
+    uint64_t q_full, full[CA_STAGES], empty[CA_STAGES], s_full[2], p_full, pv_done[2], meta_full[2], o_full;
+    // what the CTA works on
+    TileList list;
+    int k0, nt;          // its key tiles: list entries [k0, k0 + nt)
+    int live;            // rows that are queries
+    int own[128];        // a row's slot; -1: no query
+    int token0;          // token of the first query
+    long long tile_at;   // query tile in the workspace
     uint32_t tmem;
     int abort;
 };
 constexpr size_t CA_SMEM = sizeof(CaSmem) + 1024;
 static_assert(CA_SMEM <= 227 * 1024, "shared memory of one CTA");
-static_assert(128 * CA_OUT_LD * 4 <= 2 * 2 * UT_BYTES, "the staged output lies over the query and key tiles");
+static_assert(128 * CA_OUT_LD * 4 <= CA_STAGES * 2 * UT_BYTES, "the staged output lies over the tiles");
 
-// The four softmax warps.
-__device__ __forceinline__ void warpgroup_sync() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 2, %0;" ::"n"(32 * CA_SOFTMAX_WARPS) : "memory"); }
 
 __device__ __forceinline__ float4 ld_peer4(uint32_t local, uint32_t rank) {
     uint32_t ra;
@@ -184,11 +295,6 @@ __device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
     return v;
 }
 
-// Converter warps: where rows w*16 .. w*16+15 of a key tile lie.  Lane i < 16
-// holds row i's unit in the pool; CA_NONE: no query sees the slot (zeros),
-// CA_BAD: its page is outside the pool.
-constexpr uint32_t CA_NONE = 0xffffffffu, CA_BAD = 0xfffffffeu;
-
 // grid (splits * query tiles, KVH, rows), clusters of `splits` CTAs
 __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkArgs c, int splits) {
     extern __shared__ unsigned char ca_raw[];
@@ -200,171 +306,143 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     const int t = tiles_x - 1 - blockIdx.x / splits;  // the last query tile sees the most: first
     const ChunkRow x = chunk_row(c, r);
     const int i0 = t * c.P;
-    if (x.idle || x.bad || i0 >= x.n) {  // the same for a whole cluster
+    const RowTiles rt(c, x);
+    long long base = 0;
+    if (i0 < x.n && !x.idle && !x.bad) base = row_base(c, r);
+    if (x.idle || x.bad || i0 >= x.n || base + rt.n > c.key_tiles) {  // the same for a whole cluster
         pdl_wait();
         return;
     }
-    const int nq = min(c.P, x.n - i0);
-    const int own_lo = x.cached + i0, own_hi = own_lo + nq - 1;
-    const TileList list(own_lo, own_hi, a.window, a.sinks);
-    const int k0 = (int)((long long)z * list.n / splits), k1 = (int)((long long)(z + 1) * list.n / splits);
-    const int nt = k1 - k0;
-    const long long tile_at = chunk_tile(c, x, r, t) * a.kv.KVH + g;
-
     if (tid == 0) {
-        mbar_init(&sm.q_full, 1);
-        mbar_init(&sm.k_full, CA_CONV_WARPS);
-        mbar_init(&sm.k_empty, 1);
-        mbar_init(&sm.v_full, CA_CONV_WARPS);
-        mbar_init(&sm.v_empty, 1);
+        mbar_init(&sm.q_full, CA_SOFTMAX_WARPS);
         mbar_init(&sm.p_full, CA_SOFTMAX_WARPS);
         mbar_init(&sm.o_full, 1);
+        for (int b = 0; b < CA_STAGES; ++b) {
+            mbar_init(&sm.full[b], 1);
+            mbar_init(&sm.empty[b], 1);
+        }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&sm.s_full[b], 1);
-            mbar_init(&sm.ve_full[b], CA_CONV_WARPS);
+            mbar_init(&sm.pv_done[b], 1);
+            mbar_init(&sm.meta_full[b], 1);
         }
         mbar_fence_init();
         sm.abort = 0;
+        const int nq = min(c.P, x.n - i0);
+        const TileList list(x.cached + i0, x.cached + i0 + nq - 1, a.window, a.sinks);
+        sm.list = list;
+        sm.k0 = (int)((long long)z * list.n / splits);
+        sm.nt = (int)((long long)(z + 1) * list.n / splits) - sm.k0;
+        sm.live = nq * c.n_rep;
+        sm.token0 = x.b + i0;
+        sm.tile_at = chunk_tile(c, x, r, t) * a.kv.KVH + g;
     }
-    if (warp == CA_MMA_WARP) ut_alloc(&sm.tmem);
+    if (tid < 128) {
+        const int q = tid / c.n_rep;
+        sm.own[tid] = q < min(c.P, x.n - i0) ? x.cached + i0 + q : -1;
+    }
+    if (warp == CA_WARP_M) ut_alloc(&sm.tmem);
     ut_fence_before();
     __syncthreads();
     ut_fence_after();
     const uint32_t tmem = sm.tmem;
+    const int nt = sm.nt;
     volatile int* abort = &sm.abort;
     pdl_wait();
     if (c.lse) pdl_trigger();  // chunk_mass follows
 
-    if (warp >= CA_MMA_WARP) {
-        regs_down<CA_REGS_MMA>();
-        if (warp == CA_MMA_WARP && lane == 0 && nt > 0) {
-            mbar_expect_tx(&sm.q_full, 2 * UT_BYTES);
-            bulk_g2s(sm.q, c.qtiles + tile_at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.q_full);
-            const uint32_t q = smem_u32(sm.q), k = smem_u32(sm.k), v = smem_u32(sm.v);
+    if (warp == CA_WARP_P) {
+        if (lane == 0) {
+            int n = 0, landed = 0;  // copies asked for
+            auto fetch = [&](int i, int value) {
+                const int s = n % CA_STAGES;
+                if (n >= CA_STAGES && !ut_wait(&sm.empty[s], ((n - CA_STAGES) / CA_STAGES) & 1, abort)) return false;
+                const long long at = ((base + rt.index(sm.list.tile(sm.k0 + i))) * a.kv.KVH + g) * 2 + value;
+                mbar_expect_tx(&sm.full[s], 2 * UT_BYTES);
+                bulk_g2s(sm.stage[s], c.kvtiles + at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.full[s]);
+                ++n;
+                return true;
+            };
+            bool go = nt > 0 && fetch(0, 0);
+            for (int i = 0; i < nt && go; ++i) {
+                if (i + 1 < nt) go = fetch(i + 1, 0);
+                if (go) go = fetch(i, 1);
+            }
+            // no copy may be in flight when the CTA ends early
+            if (!go)
+                for (landed = max(0, n - CA_STAGES); landed < n; ++landed)
+                    mbar_wait(&sm.full[landed % CA_STAGES], (landed / CA_STAGES) & 1, nullptr);
+        }
+        __syncwarp();
+    } else if (warp == CA_WARP_M) {
+        if (lane == 0 && nt > 0) {
+            int n = 0;  // stages used
             bool go = ut_wait(&sm.q_full, 0, abort);
-            auto weigh = [&](int i) {  // O = P_i V_i
-                go = ut_wait(&sm.v_full, i & 1, abort) && ut_wait(&sm.p_full, i & 1, abort);
+            auto score = [&](int i) {  // S_i = Q K_i, over the weights of tile i - 2
+                const int s = n % CA_STAGES;
+                go = go && ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort) &&
+                     (i < 2 || ut_wait(&sm.pv_done[i & 1], ((i - 2) >> 1) & 1, abort));
                 if (!go) return;
                 ut_fence_after();
-                ut_mma_pv(tmem + CA_TM_O, tmem + CA_TM_P, v);
-                ut_commit(&sm.v_empty);
-            };
-            for (int i = 0; i < nt && go; ++i) {
-                go = ut_wait(&sm.k_full, i & 1, abort);
-                if (!go) break;
-                ut_fence_after();
-                ut_mma_qk(tmem + (i & 1) * 128, q, k);
-                ut_commit(&sm.k_empty);
+                ut_mma_qk_ts(tmem + (i & 1) * 128, tmem + CA_TM_Q, smem_u32(sm.stage[s]));
+                ut_commit(&sm.empty[s]);
                 ut_commit(&sm.s_full[i & 1]);
-                if (i > 0) weigh(i - 1);
+                ++n;
+            };
+            auto weigh = [&](int i) {  // O = P_i V_i
+                const int s = n % CA_STAGES;
+                go = go && ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort) && ut_wait(&sm.p_full, i & 1, abort);
+                if (!go) return;
+                ut_fence_after();
+                ut_mma_pv(tmem + CA_TM_O, tmem + (i & 1) * 128, smem_u32(sm.stage[s]));
+                ut_commit(&sm.empty[s]);
+                ut_commit(&sm.pv_done[i & 1]);
+                ++n;
+            };
+            score(0);
+            if (nt > 1) score(1);
+            for (int i = 0; i < nt; ++i) {
+                weigh(i);
+                if (i + 2 < nt) score(i + 2);
             }
-            if (go) weigh(nt - 1);
             ut_commit(&sm.o_full);  // every product issued so far
             ut_wait(&sm.o_full, 0, abort);
         }
         __syncwarp();
-    } else if (warp >= CA_SOFTMAX_WARPS) {
-        // ---- converters: FP32 rows of the pool -> split tiles
-        regs_down<CA_REGS_CONV>();
-        const int cw = warp - CA_SOFTMAX_WARPS, row0 = cw * CA_ROWS_PER_WARP;
-        const float4* pool4 = reinterpret_cast<const float4*>(a.kv.pool) + lane;
-        const uint32_t vstep = (uint32_t)a.kv.value_step();
-        const float qfac = pow2_whole(query_exponent(a.qn, lane) - 13.f);
-        const int w_lo = a.window > 0 ? max(0, own_lo - a.window + 1) : 0;
-        auto units = [&](int i) -> uint32_t {
-            const int slot = list.tile(k0 + i) * 128 + row0 + (lane & 15);
-            if (i >= nt || slot > own_hi || (slot < w_lo && slot >= a.sinks)) return CA_NONE;
-            const long long u = a.kv.key_unit(r, slot, g);
-            return u < 0 ? CA_BAD : (uint32_t)u;
-        };
-        float4 d[CA_ROWS_PER_WARP];
-        auto load = [&](int j, uint32_t us, uint32_t step) {
-            const uint32_t u = __shfl_sync(FULL, us, j);
-            d[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (u == CA_BAD) d[j].x = __int_as_float(0x7fffffff);
-            else if (u != CA_NONE) d[j] = __ldcg(pool4 + (long long)(u + step) * 32);
-        };
-        auto exponents = [&]() {  // lane j < 16: row j's
-            float e = UT_POISON_E;
-#pragma unroll
-            for (int j = 0; j < CA_ROWS_PER_WARP; ++j) {
-                const float x = row_exponent(d[j]);
-                if (lane == j) e = x;
-            }
-            return e;
-        };
-        // Writes the 16 rows and, behind each, asks for the row that takes
-        // its place in the registers.
-        auto put = [&](unsigned char* tile, float e, uint32_t us, uint32_t step) {
-#pragma unroll
-            for (int j = 0; j < CA_ROWS_PER_WARP; ++j) {
-                put_row(tile, row0 + j, lane, d[j], __shfl_sync(FULL, e, j));
-                load(j, us, step);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    } else if (warp == CA_WARP_E) {
+        float E = UT_POISON_E;
+        for (int i = 0; i < nt; ++i) {
+            const int b = i & 1;
+            const float* at = c.meta + ((base + rt.index(sm.list.tile(sm.k0 + i))) * a.kv.KVH + g) * 256;
+            const float4 k = reinterpret_cast<const float4*>(at)[lane], v = reinterpret_cast<const float4*>(at)[32 + lane];
+            const float top = warp_max(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));  // NaN aside
+            // the softmax of tile i - 2 is done with the buffers
+            if (i >= 2 && !ut_wait(&sm.pv_done[b], ((i - 2) >> 1) & 1, abort)) break;
+            if (sm.k0 + i < sm.list.full && top > E) E = top + 3.f;  // 3 bits to spare: it rarely moves
+            reinterpret_cast<float4*>(sm.kc[b])[lane] = k;
+            reinterpret_cast<float4*>(sm.ve[b])[lane] = v;
+            reinterpret_cast<float4*>(sm.vg[b])[lane] = make_float4(exp2_fast(v.x - E + 6.f), exp2_fast(v.y - E + 6.f),
+                                                                    exp2_fast(v.z - E + 6.f), exp2_fast(v.w - E + 6.f));
+            if (lane == 0) sm.E[b] = E;
             __syncwarp();
-        };
-        uint32_t u_cur = units(0), u_next = CA_NONE;
-        bool go = nt > 0;
-        if (go) {
-#pragma unroll
-            for (int j = 0; j < CA_ROWS_PER_WARP; ++j) load(j, u_cur, 0);
-        }
-        auto key_tile = [&](int i, uint32_t us, uint32_t step) {
-            const float e = exponents();
-            if (lane < 16) sm.kc[i % 3][row0 + lane] = e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac : e;
-            if (i > 0) go = ut_wait(&sm.k_empty, (i - 1) & 1, abort);
-            if (!go) return;
-            put(sm.k, e, us, step);
-            if (lane == 0) ut_arrive(&sm.k_full);
-        };
-        // order: K0, K1, V0, K2, V1, ...; d always holds the next one
-        if (go) {
-            u_next = units(1);
-            key_tile(0, nt > 1 ? u_next : u_cur, nt > 1 ? 0 : vstep);
-        }
-        for (int i = 0; i < nt && go; ++i) {
-            if (i + 1 < nt) {
-                key_tile(i + 1, u_cur, vstep);
-                if (!go) break;
-            }
-            const float e = exponents();
-            if (lane < 16) sm.ve[i & 1][row0 + lane] = e;
-            const float top = warp_max(e);
-            if (lane == 0) sm.vmax[i & 1][cw] = top;
-            __syncwarp();
-            if (lane == 0) ut_arrive(&sm.ve_full[i & 1]);
-            if (i > 0) go = ut_wait(&sm.v_empty, (i - 1) & 1, abort);
-            if (!go) break;
-            // behind V_i comes K_{i+2}, or V_{i+1} if there is none
-            const uint32_t u2 = units(i + 2);
-            const bool more = i + 2 < nt;
-            put(sm.v, e, more ? u2 : u_next, more ? 0 : vstep);
-            if (lane == 0) ut_arrive(&sm.v_full);
-            u_cur = u_next;
-            u_next = u2;
+            if (lane == 0) ut_arrive(&sm.meta_full[b]);
         }
         __syncwarp();
-    } else {
-        // ---- softmax: thread = query row
-        regs_up<CA_REGS_SOFTMAX>();
-        const int row = tid, own = own_lo + row / c.n_rep;
-        const bool live = row < nq * c.n_rep;
-        const int hi = live ? own : -1;                                       // sees slots <= hi
-        const int lo = a.window > 0 ? own - a.window : -1;                    // and > lo, or < sinks
-        const uint32_t lane_tm = tmem + ((uint32_t)(32 * warp) << 16);
+    } else if (warp < CA_SOFTMAX_WARPS) {
+        const int part = warp >> 2, row = tid & 127;
+        const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         float m = CO_LOW, l = 0.f, E = UT_POISON_E;
-        // The output row, over the tiles before the newest, in units
-        // 2^(E - 13 - 6) of that tile's E and m; f_o takes it there.
-        uint64_t acc[64];
+        // A part of the output row, over the tiles before the newest, in
+        // units 2^(E - 13 - 6) of that tile's E and m; f_o takes it there.
+        uint64_t acc[CA_W / 2];
 #pragma unroll
-        for (int q = 0; q < 64; ++q) acc[q] = 0;
+        for (int q = 0; q < CA_W / 2; ++q) acc[q] = 0;
         float f_o = 1.f;
         auto gather = [&]() {  // acc = acc f_o + the newest tile's product
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
+            for (int ch = 0; ch < CA_W / 32; ++ch) {
                 uint32_t o[32];
-                ut_ld32(lane_tm + CA_TM_O + ch * 32, o);
+                ut_ld32(lane_tm + CA_TM_O + part * CA_W + ch * 32, o);
                 ut_wait_ld();
 #pragma unroll
                 for (int q = 0; q < 16; ++q)
@@ -372,112 +450,131 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                                              pack2(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1])));
             }
         };
+        if (nt > 0 && part < 2) {  // the queries into tensor memory: this row of hi, or of lo
+            const unsigned char* q = c.qtiles + sm.tile_at * (2 * UT_BYTES) + part * UT_BYTES + row * 128;
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+                uint32_t w[32];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(q + ch * UT_HALF + ((j ^ (row & 7)) * 16));
+                    w[4 * j] = y.x;
+                    w[4 * j + 1] = y.y;
+                    w[4 * j + 2] = y.z;
+                    w[4 * j + 3] = y.w;
+                }
+                ut_st32(lane_tm + CA_TM_Q + part * 64 + ch * 32, w);
+            }
+            ut_wait_st();
+            ut_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) ut_arrive(&sm.q_full);
         // A wait that ran out ends every later one at once; the loop still runs
-        // through, because its barrier needs all four warps.
+        // through, because its barriers need all softmax warps.
         for (int i = 0; i < nt; ++i) {
-            const int b = i & 1, base = list.tile(k0 + i) * 128;
-            const bool whole = k0 + i < list.full;
-            const uint32_t st = lane_tm + b * 128;
-            const float4* kc = reinterpret_cast<const float4*>(sm.kc[i % 3]);
+            const int b = i & 1, base_slot = sm.list.tile(sm.k0 + i) * 128 + part * CA_W;
+            const bool whole = sm.k0 + i < sm.list.full;
+            const uint32_t st = lane_tm + b * 128 + part * CA_W;
+            const float4* kc = reinterpret_cast<const float4*>(sm.kc[b] + part * CA_W);
+            const float* ve = sm.ve[b] + part * CA_W;
+            // a row sees slots <= hi that are > lo, or < sinks
+            const int hi = sm.own[row], lo = a.window > 0 ? hi - a.window : -1;
+            ut_wait(&sm.meta_full[b], (i >> 1) & 1, abort);
             ut_wait(&sm.s_full[b], (i >> 1) & 1, abort);
             ut_fence_after();
-            // largest score (and, where queries differ in what they see, the
-            // largest exponent among the values this query sees)
+            // scores; the largest (and, where queries differ in what they
+            // see, the largest exponent among the values this query sees)
+            float2 s[CA_W / 2];
             float mx = CO_LOW, ex = UT_POISON_E;
-            if (!whole) ut_wait(&sm.ve_full[b], (i >> 1) & 1, abort);
-#pragma unroll 1
-            for (int ch = 0; ch < 4; ++ch) {
-                uint32_t s[32];
-                ut_ld32(st + ch * 32, s);
+            uint32_t seen[CA_W / 32];
+#pragma unroll
+            for (int ch = 0; ch < CA_W / 32; ++ch) {
+                uint32_t w[32];
+                ut_ld32(st + ch * 32, w);
                 ut_wait_ld();
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4 f = kc[ch * 8 + q];
+                    s[ch * 16 + 2 * q] = mul2(make_float2(__uint_as_float(w[4 * q]), __uint_as_float(w[4 * q + 1])),
+                                              make_float2(f.x, f.y));
+                    s[ch * 16 + 2 * q + 1] = mul2(make_float2(__uint_as_float(w[4 * q + 2]), __uint_as_float(w[4 * q + 3])),
+                                                  make_float2(f.z, f.w));
+                }
                 if (whole) {
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        const float4 f = kc[ch * 8 + q];
-                        const float2 u = mul2(make_float2(__uint_as_float(s[4 * q]), __uint_as_float(s[4 * q + 1])),
-                                              make_float2(f.x, f.y));
-                        const float2 v = mul2(make_float2(__uint_as_float(s[4 * q + 2]), __uint_as_float(s[4 * q + 3])),
-                                              make_float2(f.z, f.w));
-                        mx = fmaxf(fmaxf(mx, u.x), u.y);
-                        mx = fmaxf(fmaxf(mx, v.x), v.y);
-                    }
+                    for (int q = 0; q < 16; ++q) mx = fmaxf(fmaxf(mx, s[ch * 16 + q].x), s[ch * 16 + q].y);
                 } else {
+                    seen[ch] = 0;
 #pragma unroll
                     for (int q = 0; q < 32; ++q) {
-                        const int j = base + ch * 32 + q;
+                        const int j = base_slot + ch * 32 + q;
                         if (j <= hi && (j > lo || j < a.sinks)) {
-                            mx = fmaxf(mx, __uint_as_float(s[q]) * sm.kc[i % 3][ch * 32 + q]);
-                            ex = fmaxf(ex, sm.ve[b][ch * 32 + q]);
+                            seen[ch] |= 1u << q;
+                            mx = fmaxf(mx, (q & 1) ? s[ch * 16 + (q >> 1)].y : s[ch * 16 + (q >> 1)].x);
+                            ex = fmaxf(ex, ve[ch * 32 + q]);
                         }
                     }
                 }
             }
-            if (whole) {
-                ut_wait(&sm.ve_full[b], (i >> 1) & 1, abort);
-                const float4 e0 = reinterpret_cast<const float4*>(sm.vmax[b])[0];
-                const float4 e1 = reinterpret_cast<const float4*>(sm.vmax[b])[1];
-                ex = fmaxf(fmaxf(fmaxf(e0.x, e0.y), fmaxf(e0.z, e0.w)), fmaxf(fmaxf(e1.x, e1.y), fmaxf(e1.z, e1.w)));
-            }
-            if (!live) mx = CO_LOW;
+            sm.mx[b][part][row] = mx;
+            if (!whole) sm.ex[b][part][row] = ex;
+            softmax_sync();
             // The running maximum follows only when it is passed by 2^8, the
             // running exponent with 3 bits to spare: weights stay below 2^8,
-            // scaled ones below 2^14.
-            const float m_new = mx > m + 8.f ? mx : m;
-            const float E_new = ex > E ? ex + 3.f : E;
+            // scaled ones below 2^14.  In whole tiles the exponent is every row's.
+            float E_new = E;
+            if (whole) {
+                E_new = sm.E[b];
+            } else {
+#pragma unroll
+                for (int q = 0; q < CA_PARTS; ++q) ex = fmaxf(ex, sm.ex[b][q][row]);
+                if (ex > E) E_new = ex + 3.f;
+            }
+#pragma unroll
+            for (int q = 0; q < CA_PARTS; ++q) mx = fmaxf(mx, sm.mx[b][q][row]);
+            const float m_new = mx > m + 8.f && hi >= 0 ? mx : m;
             const float f_l = exp2_fast(m - m_new), f_new = f_l * exp2_fast(E - E_new);
             m = m_new;
             E = E_new;
-            l *= f_l;
-            if (whole) {  // E is the same for every row of the tile here
-                sm.vg[b][row] = exp2_fast(sm.ve[b][row] - E + 6.f);
-                warpgroup_sync();
-            }
-            if (i > 0) {  // P is free, and the product there, once P_{i-1} V_{i-1} is done
-                ut_wait(&sm.v_empty, (i - 1) & 1, abort);
+            // scores -> weights, scaled by their values' exponents, as hi | lo over the scores
+            float2 sum = make_float2(0.f, 0.f);
+            auto weigh = [&](auto whole_tile) {
+                const float2 mm = make_float2(-m, -m);
+#pragma unroll
+                for (int ch = 0; ch < CA_W / 16; ++ch) {
+                    uint32_t ph[8], pl[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        float2 p = add2(s[ch * 8 + q], mm);
+                        p = make_float2(exp2_fast(p.x), exp2_fast(p.y));
+                        if (decltype(whole_tile)::value) {
+                            sum = add2(sum, p);
+                            p = mul2(p, reinterpret_cast<const float2*>(sm.vg[b] + part * CA_W)[ch * 8 + q]);
+                        } else {
+                            const uint32_t bits = seen[ch >> 1] >> ((ch & 1) * 16 + 2 * q);
+                            const float2 v = reinterpret_cast<const float2*>(ve)[ch * 8 + q];
+                            if (!(bits & 1u)) p.x = 0.f;
+                            if (!(bits & 2u)) p.y = 0.f;
+                            sum = add2(sum, p);
+                            p.x = (bits & 1u) ? p.x * exp2_fast(v.x - E + 6.f) : 0.f;
+                            p.y = (bits & 2u) ? p.y * exp2_fast(v.y - E + 6.f) : 0.f;
+                        }
+                        split2(p, ph[q], pl[q]);
+                    }
+                    ut_st8(st + ch * 16, ph);
+                    ut_st8(st + ch * 16 + 8, pl);
+                }
+            };
+            if (whole) weigh(std::true_type{});
+            else weigh(std::false_type{});
+            l = fmaf(l, f_l, sum.x + sum.y);
+            if (i > 0) {  // the last tile's product, before this one's takes its place
+                ut_wait(&sm.pv_done[b ^ 1], ((i - 1) >> 1) & 1, abort);
                 ut_fence_after();
                 gather();
             }
             f_o = i == 0 ? 0.f : f_new;
-            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll 1
-            for (int ch = 0; ch < 8; ++ch) {
-                uint32_t s[16], ph[8], pl[8];
-                ut_ld16(st + ch * 16, s);
-                ut_wait_ld();
-                const float4* vg = reinterpret_cast<const float4*>(sm.vg[b]);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float4 f = kc[ch * 4 + q];
-                    float2 u = fma2(make_float2(__uint_as_float(s[4 * q]), __uint_as_float(s[4 * q + 1])),
-                                    make_float2(f.x, f.y), make_float2(-m, -m));
-                    float2 v = fma2(make_float2(__uint_as_float(s[4 * q + 2]), __uint_as_float(s[4 * q + 3])),
-                                    make_float2(f.z, f.w), make_float2(-m, -m));
-                    u = make_float2(exp2_fast(u.x), exp2_fast(u.y));
-                    v = make_float2(exp2_fast(v.x), exp2_fast(v.y));
-                    if (whole) {
-                        sum = add2(sum, add2(u, v));
-                        const float4 w = vg[ch * 4 + q];
-                        u = mul2(u, make_float2(w.x, w.y));
-                        v = mul2(v, make_float2(w.z, w.w));
-                    } else {
-                        float p[4] = {u.x, u.y, v.x, v.y};
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const int j = base + ch * 16 + 4 * q + y;
-                            const bool see = j <= hi && (j > lo || j < a.sinks);
-                            sum.x += see ? p[y] : 0.f;
-                            p[y] = see ? p[y] * exp2_fast(sm.ve[b][ch * 16 + 4 * q + y] - E + 6.f) : 0.f;
-                        }
-                        u = make_float2(p[0], p[1]);
-                        v = make_float2(p[2], p[3]);
-                    }
-                    split2(u, ph[2 * q], pl[2 * q]);
-                    split2(v, ph[2 * q + 1], pl[2 * q + 1]);
-                }
-                ut_st8(lane_tm + CA_TM_P + ch * 8, ph);
-                ut_st8(lane_tm + CA_TM_P + 64 + ch * 8, pl);
-            }
-            l += sum.x + sum.y;
             ut_wait_st();
             ut_fence_before();
             __syncwarp();
@@ -489,49 +586,51 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             ut_fence_after();
             gather();
         }
-        float* stage = reinterpret_cast<float*>(sm.q) + row * CA_OUT_LD;
-        // rows that saw nothing, and dead ones, give zeros
-        const float f = l == 0.f || !live ? 0.f : exp2_fast(E - 19.f) / l;
+        sm.l[part][row] = l;
+        softmax_sync();
+        l = 0.f;
 #pragma unroll
-        for (int q = 0; q < 32; ++q) {
+        for (int q = 0; q < CA_PARTS; ++q) l += sm.l[q][row];
+        float* stage = reinterpret_cast<float*>(sm.stage) + row * CA_OUT_LD + part * CA_W;
+        // rows that saw nothing, and dead ones, give zeros
+        const float f = l == 0.f || row >= sm.live ? 0.f : exp2_fast(E - 19.f) / l;
+#pragma unroll
+        for (int q = 0; q < CA_W / 4; ++q) {
             float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
             const float2 u = unpack2(acc[2 * q]), v = unpack2(acc[2 * q + 1]);
             if (f != 0.f) w = make_float4(u.x * f, u.y * f, v.x * f, v.y * f);
             *reinterpret_cast<float4*>(stage + 4 * q) = w;
         }
-        sm.m[row] = m;
-        sm.l[row] = *abort ? __int_as_float(0x7fffffff) : l;  // a wait that ran out shows as NaN
+        if (part == 0) sm.m[row] = m;
+        softmax_sync();  // all parts have read the sums
+        if (part == 0) sm.l[0][row] = *abort ? __int_as_float(0x7fffffff) : l;  // a wait that ran out shows as NaN
         ut_fence_before();
-        warpgroup_sync();
-        regs_down<CA_REGS>();
     }
     __syncthreads();
-    if (warp >= CA_SOFTMAX_WARPS) regs_up<CA_REGS>();  // what the softmax threads gave back
-    if (warp == CA_MMA_WARP) {
+    if (warp == CA_WARP_M) {
         ut_fence_after();
         ut_free(tmem);
     }
     // ---- join the splits: CTA z of the cluster takes a part of the rows
     if (splits > 1)
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    const int rows_used = nq * c.n_rep;
-    const int ra = z * rows_used / splits, rb = (z + 1) * rows_used / splits;
-    const uint32_t stage = smem_u32(sm.q);
+    const int ra = z * sm.live / splits, rb = (z + 1) * sm.live / splits;
+    const uint32_t stage = smem_u32(sm.stage);
     for (int q = warp; q < rb - ra; q += CA_THREADS / 32) {  // a warp per row
         const int row = ra + q;
         float4 o;
         float M = CO_LOW, L = 0.f;
         const uint32_t at = stage + (uint32_t)(row * CA_OUT_LD + 4 * lane) * 4u;
         if (splits == 1) {
-            o = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.q) + row * CA_OUT_LD + 4 * lane);
+            o = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.stage) + row * CA_OUT_LD + 4 * lane);
             M = sm.m[row];
-            L = sm.l[row];
+            L = sm.l[0][row];
             if (L != L) o.x = o.y = o.z = o.w = L;
         } else {
             o = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int p = 0; p < splits; ++p) M = fmaxf(M, ld_peer(&sm.m[row], p));
             for (int p = 0; p < splits; ++p) {
-                const float w = ld_peer(&sm.l[row], p) * exp2_fast(ld_peer(&sm.m[row], p) - M);
+                const float w = ld_peer(&sm.l[0][row], p) * exp2_fast(ld_peer(&sm.m[row], p) - M);
                 const float4 y = ld_peer4(at, p);
                 L += w;
                 o.x = fmaf(w, y.x, o.x);
@@ -542,17 +641,16 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             const float inv = 1.f / L;
             o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         }
-        const long long tok = x.b + i0 + row / c.n_rep;
+        const long long tok = sm.token0 + row / c.n_rep;
         reinterpret_cast<float4*>(a.out)[(tok * a.H + g * c.n_rep + row % c.n_rep) * 32 + lane] = o;
-        if (c.lse && lane == 0) c.lse[tile_at * 128 + row] = M + log2f(L);
+        if (c.lse && lane == 0) c.lse[sm.tile_at * 128 + row] = M + log2f(L);
     }
     if (splits > 1)  // peers still read this CTA's shared memory
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // -------------------------------------------------------------- chunk_mass
-// One CTA per (128 slots, kv head, row): its keys become one split tile, the
-// rows of the products; the query tiles that see any of them pass through
+// One CTA per (key tile, kv head, row): its keys are the rows of the products; the query tiles that see any of them pass through
 // as columns.  A thread owns a slot and half of the columns, so weights are added in
 // a fixed order without atomics:
 //   sum over columns of exp2(s - lse)
@@ -583,13 +681,11 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
     pdl_wait();
     if (x.idle || x.bad || x.n == 0) return;
     const int last = x.cached + x.n - 1;
-    // the blockIdx.x-th tile that any query sees
-    int tile;
-    {
-        const int w0 = a.window > 0 ? max(0, x.cached - a.window + 1) : 0;
-        const int a1 = (min(a.sinks, w0) + 127) >> 7, b0 = max(w0 >> 7, a1);
-        tile = (int)blockIdx.x < a1 ? blockIdx.x : b0 + (blockIdx.x - a1);
-    }
+    const RowTiles rt(c, x);
+    if ((int)blockIdx.x >= rt.n) return;
+    const long long row_at = row_base(c, r);
+    if (row_at + rt.n > c.key_tiles) return;
+    const int tile = rt.tile(blockIdx.x);
     const int base = tile * 128;
     if (base > last) return;
     // queries (slots) that may see a slot of the tile: from `from` to `to`
@@ -600,7 +696,7 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
     const int t0 = (from - x.cached) / c.P, nt = (to - x.cached) / c.P - t0 + 1;
 
     if (tid == 0) {
-        mbar_init(&sm.k_full, CM_SUM_WARPS);
+        mbar_init(&sm.k_full, 1);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&sm.q_full[b], 1);
             mbar_init(&sm.q_empty[b], 1);
@@ -626,6 +722,10 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
                 bulk_g2s(sm.q[i & 1], c.qtiles + at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.q_full[i & 1]);
                 bulk_g2s(sm.lse[i & 1], c.lse + at * 128, 512, &sm.q_full[i & 1]);
             };
+            const long long kat = ((row_at + blockIdx.x) * a.kv.KVH + g) * 2;
+            mbar_expect_tx(&sm.k_full, 2 * UT_BYTES + 512);
+            bulk_g2s(sm.k, c.kvtiles + kat * (2 * UT_BYTES), 2 * UT_BYTES, &sm.k_full);
+            bulk_g2s(sm.kc, c.meta + kat * 128, 512, &sm.k_full);
             int fetched = 0;
             for (; fetched < 2 && fetched < nt; ++fetched) fetch(fetched);
             bool go = ut_wait(&sm.k_full, 0, abort);
@@ -650,36 +750,13 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
                 }
             }
             // leave nothing in flight: the copies asked for, the products issued
+            if (i < nt) mbar_wait(&sm.k_full, 0, nullptr);
             if (i < nt)
                 for (int f = max(0, fetched - 2); f < fetched; ++f) mbar_wait(&sm.q_full[f & 1], (f >> 1) & 1, nullptr);
         }
         __syncwarp();
     } else {
-        {  // the keys, 16 rows a warp
-            const float4* pool4 = reinterpret_cast<const float4*>(a.kv.pool) + lane;
-            const float qfac = pow2_whole(query_exponent(a.qn, lane) - 13.f);
-            float4 d[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int slot = base + warp * 16 + j;
-                d[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (slot <= last) {
-                    const long long u = a.kv.key_unit(r, slot, g);
-                    if (u >= 0) d[j] = __ldcg(pool4 + u * 32);
-                    else d[j].x = __int_as_float(0x7fffffff);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float e = row_exponent(d[j]);
-                put_row(sm.k, warp * 16 + j, lane, d[j], e);
-                if (lane == 0) sm.kc[warp * 16 + j] = e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac : e;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) ut_arrive(&sm.k_full);
-            asm volatile("bar.sync 2, 256;" ::: "memory");
-        }
+        ut_wait(&sm.k_full, 0, abort);
         const int key = 32 * (warp & 3) + lane, half = warp >> 2, slot = base + key;
         const float kc = sm.kc[key];
         const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * 64;
@@ -742,20 +819,47 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
     }
 }
 
-static int64_t align256(int64_t n) { return (n + 255) & ~255ll; }
-static int64_t chunk_tiles(int tokens, int rows, int n_rep) { return tokens / (128 / n_rep) + rows + 1; }
+static long long chunk_query_tiles(int tokens, int rows, int n_rep) { return tokens / (128 / n_rep) + rows + 1; }
+
+// Key tiles of all rows together, at most: each row's by the cache's width and
+// by its window; all of them by the pool, whose pages belong to one row each.
+// A row's end, and the gap between sinks and window, cut one tile more each.
+static long long chunk_key_tiles(int rows, int max_chunk, int max_pages, int page_size, long long n_pages, int window, int sinks) {
+    const long long cap = (long long)max_pages * page_size;
+    long long n = (cap + 127) / 128;
+    if (window > 0) {
+        const long long w = ((long long)sinks + 127) / 128 + ((long long)window + max_chunk + 127) / 128 + 1;
+        if (w < n) n = w;
+    }
+    n *= rows;
+    const long long all = n_pages * page_size / 128 + 2ll * rows;
+    return all < n ? all : n;
+}
+
+struct ChunkWork {
+    long long q, kv, meta, lse, total;  // byte offsets
+    ChunkWork(long long qtiles, long long ktiles, int KVH, bool with_mass) {
+        q = 0;
+        kv = qtiles * KVH * (2 * (long long)UT_BYTES);
+        meta = kv + ktiles * KVH * (4 * (long long)UT_BYTES);
+        lse = meta + ktiles * KVH * 1024;
+        total = lse + (with_mass ? (qtiles * KVH * 512 + 255) / 256 * 256 : 0);
+    }
+};
 
 }  // namespace skb
 
 using namespace skb;
 
 extern "C" int64_t skb_chunk_attention_workspace(int tokens, int rows, int max_chunk, int n_heads, int n_kv_heads,
-                                                 int max_pages, int page_size, int with_mass) {
+                                                 int max_pages, int page_size, int n_pages, int window, int sinks,
+                                                 int with_mass) {
     if (tokens < 0 || rows < 0 || max_chunk < 0 || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 ||
-        n_heads / n_kv_heads > CO_MAX_REP || max_pages < 1 || page_size < 1)
+        n_heads / n_kv_heads > CO_MAX_REP || max_pages < 1 || page_size < 1 || n_pages < 1 || window < 0 || sinks < 0)
         return -1;
-    const int64_t tiles = chunk_tiles(tokens, rows, n_heads / n_kv_heads) * n_kv_heads;
-    return tiles * (2 * (int64_t)UT_BYTES) + (with_mass ? align256(tiles * 512) : 0);
+    return ChunkWork(chunk_query_tiles(tokens, rows, n_heads / n_kv_heads),
+                     chunk_key_tiles(rows, max_chunk, max_pages, page_size, n_pages, window, sinks), n_kv_heads, with_mass)
+        .total;
 }
 
 extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n_heads, int n_kv_heads, int head_dim,
@@ -777,7 +881,8 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     if (rows == 0 || tokens == 0) return SKB_OK;
     if (!qkv || !out) return fail(SKB_ERR_ARG, "%s: null pointer", what);
     if (!work || ((uintptr_t)work & 255u) ||
-        work_bytes < skb_chunk_attention_workspace(tokens, rows, max_chunk, n_heads, n_kv_heads, max_pages, page_size, mass != nullptr))
+        work_bytes < skb_chunk_attention_workspace(tokens, rows, max_chunk, n_heads, n_kv_heads, max_pages, page_size, n_pages,
+                                                   window, sinks, mass != nullptr))
         return fail(SKB_ERR_ARG, "%s: needs a workspace of skb_chunk_attention_workspace bytes, 256-byte aligned", what);
     ChunkArgs c = {};
     c.a.qkv = qkv;
@@ -801,31 +906,35 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     c.max_chunk = max_chunk;
     c.n_rep = n_heads / n_kv_heads;
     c.P = 128 / c.n_rep;
-    c.qtiles = static_cast<unsigned char*>(work);
-    const long long tiles = chunk_tiles(tokens, rows, c.n_rep);
-    c.lse = mass ? reinterpret_cast<float*>(c.qtiles + tiles * n_kv_heads * (2 * (long long)UT_BYTES)) : nullptr;
+    const long long tiles = chunk_query_tiles(tokens, rows, c.n_rep);
+    c.key_tiles = chunk_key_tiles(rows, max_chunk, max_pages, page_size, n_pages, window, sinks);
+    const ChunkWork at(tiles, c.key_tiles, n_kv_heads, mass != nullptr);
+    unsigned char* w = static_cast<unsigned char*>(work);
+    c.qtiles = w + at.q;
+    c.kvtiles = w + at.kv;
+    c.meta = reinterpret_cast<float*>(w + at.meta);
+    c.lse = mass ? reinterpret_cast<float*>(w + at.lse) : nullptr;
 
     // no more tokens than there are, whatever max_chunk says
     const int most = max_chunk < 1 ? 1 : (max_chunk < tokens ? max_chunk : tokens);
     const int tiles_x = (most + c.P - 1) / c.P;
-    const long long cap = (long long)max_pages * page_size;
+    // key tiles of one row, at most
+    const long long row_tiles = chunk_key_tiles(1, most, max_pages, page_size, n_pages, window, sinks);
     // CTAs that have work, at most; while they leave SMs idle, up to 8 share a
-    // query tile's key tiles.  A row's keys are not known here; the cache, or
-    // the window, bounds them.
+    // query tile's key tiles.
     long long ctas = (long long)rows * tiles_x;
     if (ctas > tiles) ctas = tiles;
     ctas *= n_kv_heads;
-    long long seen = cap;
-    if (window > 0 && (long long)window + sinks + c.P < cap) seen = (long long)window + sinks + c.P;
-    const long long key_tiles = seen / 128 + 1;
     int splits = 1;
-    while (splits < CA_MAX_SPLITS && ctas * splits * 2 <= 148 && splits * 2 <= key_tiles) splits *= 2;
+    while (splits < CA_MAX_SPLITS && ctas * splits * 2 <= 148 && splits * 2 <= row_tiles) splits *= 2;
+    const int prep_x = row_tiles < CP_TILES ? (int)row_tiles : CP_TILES;
+    const long long prep_blocks = tokens + (long long)prep_x * 2 * n_kv_heads * rows;
+    if (prep_blocks > 0x7fffffffll) return fail(SKB_ERR_ARG, "%s: too many tokens and rows", what);
 
     cudaError_t e = set_smem_attrs(chunk_attn_kernel, CA_SMEM);
     if (e == cudaSuccess && mass) e = set_smem_attrs(chunk_mass_kernel, CM_SMEM);
     if (e == cudaSuccess)
-        e = launch(chunk_prep_kernel, dim3(most < 4096 ? most : 4096, rows, (n_heads + 2 * n_kv_heads + 7) / 8), dim3(256),
-                   0, stream, false, c);
+        e = launch(chunk_prep_kernel, dim3((unsigned)prep_blocks), dim3(256), 0, stream, false, c, prep_x);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(splits * tiles_x, n_kv_heads, rows);
@@ -843,14 +952,7 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
         cfg.numAttrs = 2;
         e = cudaLaunchKernelEx(&cfg, chunk_attn_kernel, c, splits);
     }
-    if (e == cudaSuccess && mass) {
-        // tiles that the row's queries see: the sinks' and the window's, or all
-        long long n = (cap + 127) / 128;
-        if (window > 0) {
-            const long long w = ((long long)sinks + 127) / 128 + ((long long)window + most + 127) / 128 + 1;
-            if (w < n) n = w;
-        }
-        e = launch(chunk_mass_kernel, dim3((unsigned)n, n_kv_heads, rows), dim3(CM_THREADS), CM_SMEM, stream, true, c);
-    }
+    if (e == cudaSuccess && mass)
+        e = launch(chunk_mass_kernel, dim3((unsigned)row_tiles, n_kv_heads, rows), dim3(CM_THREADS), CM_SMEM, stream, true, c);
     return e == cudaSuccess ? SKB_OK : fail(SKB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }

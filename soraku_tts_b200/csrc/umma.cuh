@@ -23,19 +23,19 @@ constexpr int UT_ROWS = 128;
 constexpr uint32_t UT_HALF = 128 * 128;       // bytes of 64 columns
 constexpr uint32_t UT_BYTES = 2 * UT_HALF;    // one fp16 tile
 constexpr float UT_POISON_E = -200.f;         // exponent of a row of zeros
+// Units of rows that are not in the pool: no query sees the slot (zeros), or
+// its page is outside (not a number).
+constexpr uint32_t UT_NONE = 0xffffffffu, UT_BAD = 0xfffffffeu;
 
 // ------------------------------------------------------------- descriptors
 // Shared-memory operand, 128-byte swizzle.  K-major: 8-row groups 1024 bytes
 // apart.  MN-major: 64-column halves `UT_HALF` apart (leading offset), 8-row
 // groups along K 1024 bytes apart (stride offset).
-__device__ __forceinline__ uint64_t ut_desc(uint32_t saddr, bool mn_major) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)(mn_major ? (UT_HALF >> 4) : 1u) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= (uint64_t)1u << 46;
-    d |= (uint64_t)2u << 61;
-    return d;
+// `off`: bytes added to the address, known when compiled.
+__device__ __forceinline__ uint64_t ut_desc(uint32_t saddr, uint32_t off, bool mn_major) {
+    const uint32_t lo = ((saddr >> 4) & 0x3FFFu) + (off >> 4) + ((mn_major ? (UT_HALF >> 4) : 1u) << 16);
+    const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    return (uint64_t)hi << 32 | lo;
 }
 // kind::f16, D FP32, A and B fp16, M = N = 128.
 __host__ __device__ constexpr uint32_t ut_idesc(bool b_mn_major) {
@@ -43,16 +43,14 @@ __host__ __device__ constexpr uint32_t ut_idesc(bool b_mn_major) {
 }
 __device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
 __device__ __forceinline__ void ut_commit(uint64_t* bar) {
@@ -70,23 +68,37 @@ __device__ __forceinline__ void ut_mma_qk(uint32_t d, uint32_t a, uint32_t b) {
     asm volatile("" : "+r"(a), "+r"(b));  // keeps 48 descriptors from being held across a caller's loop
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
-        const uint64_t da = ut_desc(a + (p == 1 ? UT_BYTES : 0), false), db = ut_desc(b + (p == 0 ? UT_BYTES : 0), false);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const uint64_t off = ((k >> 2) * UT_HALF + (k & 3) * 32) >> 4;  // in the address field
-            umma_f16_ss(d, da + off, db + off, ut_idesc(false), p > 0 || k > 0);
+            const uint32_t off = (k >> 2) * UT_HALF + (k & 3) * 32;
+            umma_f16_ss(d, ut_desc(a, off + (p == 1 ? UT_BYTES : 0), false), ut_desc(b, off + (p == 0 ? UT_BYTES : 0), false),
+                        ut_idesc(false), p > 0 || k > 0);
         }
     }
 }
-// D[128 x 128] = P V: P as hi | lo (64 TMEM columns each), V as hi | lo tiles (MN-major).
+// The same with A in tensor memory (hi | lo, 64 columns each): it halves what
+// the products read from shared memory.
+__device__ __forceinline__ void ut_mma_qk_ts(uint32_t d, uint32_t a_tmem, uint32_t b) {
+    asm volatile("" : "+r"(a_tmem), "+r"(b));
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        const uint32_t pa = a_tmem + (p == 1 ? 64 : 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            umma_f16_ts(d, pa + k * 8, ut_desc(b, (p == 0 ? UT_BYTES : 0) + (k >> 2) * UT_HALF + (k & 3) * 32, false),
+                        ut_idesc(false), p > 0 || k > 0);
+    }
+}
+// D[128 x 128] = P V: P in tensor memory, for each 16 keys 8 columns of hi,
+// then 8 of lo; V as hi | lo tiles (MN-major).
 __device__ __forceinline__ void ut_mma_pv(uint32_t d, uint32_t p_tmem, uint32_t v) {
     asm volatile("" : "+r"(p_tmem), "+r"(v));
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
-        const uint32_t pa = p_tmem + (p == 1 ? 64 : 0);
-        const uint64_t dv = ut_desc(v + (p == 0 ? UT_BYTES : 0), true);
+        const uint32_t pa = p_tmem + (p == 1 ? 8 : 0);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) umma_f16_ts(d, pa + k * 8, dv + (k * 2048 >> 4), ut_idesc(true), p > 0 || k > 0);
+        for (int k = 0; k < 8; ++k)
+            umma_f16_ts(d, pa + k * 16, ut_desc(v, (p == 0 ? UT_BYTES : 0) + k * 2048, true), ut_idesc(true), p > 0 || k > 0);
     }
 }
 
@@ -114,6 +126,16 @@ __device__ __forceinline__ void ut_st8(uint32_t taddr, const uint32_t (&v)[8]) {
                  "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
+__device__ __forceinline__ void ut_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
+        "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
+        "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
 __device__ __forceinline__ void ut_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void ut_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void ut_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -133,20 +155,22 @@ __device__ __forceinline__ void ut_arrive(uint64_t* bar) {
 }
 // Waits for phase `parity`, at most about 2 s and no longer than *abort stays
 // 0; false (and *abort set) when it gave up.  Every wait of a kernel goes
-// through here, so that one that runs out ends all the others.
+// through here, so that one that runs out ends all the others.  A try sleeps
+// up to 1 ms in hardware, so a waiting warp takes no issue slots.
 __device__ __forceinline__ bool ut_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
     const uint32_t addr = smem_u32(bar);
     uint64_t t0 = 0;
-    for (int it = 0;; ++it) {
+    for (;;) {
         uint32_t done;
         asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
             : "=r"(done)
-            : "r"(addr), "r"(parity)
+            : "r"(addr), "r"(parity), "r"(1000000u)
             : "memory");
         if (done) return true;
-        if (it == 0) t0 = globaltimer_ns();
-        else if ((it & 63) == 0 && (*abort || globaltimer_ns() - t0 > SKB_WAIT_LIMIT_NS)) {
+        const uint64_t now = globaltimer_ns();
+        if (t0 == 0) t0 = now;
+        if (*abort || now - t0 > SKB_WAIT_LIMIT_NS) {
             *abort = 1;
             return false;
         }
@@ -195,40 +219,94 @@ __device__ __forceinline__ uint64_t fma2p(uint64_t a, uint64_t b, uint64_t c) {
 }
 // hi = fp16 pair of x, lo = fp16 pair of what is left.
 __device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
-    float2 f;
-    asm("{\n .reg .b16 p, q;\n cvt.rn.f16x2.f32 %0, %4, %3;\n mov.b32 {p, q}, %0;\n cvt.f32.f16 %1, p;\n cvt.f32.f16 %2, q;\n}"
-        : "=&r"(hi), "=f"(f.x), "=f"(f.y)
+    asm("{\n .reg .b16 p, q, m;\n .reg .f32 u, v;\n"
+        " cvt.rn.f16x2.f32 %0, %3, %2;\n mov.b32 {p, q}, %0;\n mov.b16 m, 0xBC00;\n"  // -1
+        " fma.rn.f32.f16 u, p, m, %2;\n fma.rn.f32.f16 v, q, m, %3;\n cvt.rn.f16x2.f32 %1, v, u;\n}"
+        : "=&r"(hi), "=r"(lo)
         : "f"(x.x), "f"(x.y));
-    const float2 r = add2(x, make_float2(-f.x, -f.y));
-    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(lo) : "f"(r.x), "f"(r.y));
 }
-// Exponent floor(log2 max|x|) of a row held by a warp (4 numbers a lane), as
-// a whole number clamped to [-100, 127]; UT_POISON_E for a row of zeros, NaN
-// for one that holds something not finite.
-__device__ __forceinline__ float row_exponent(float4 x) {
-    const unsigned m = max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu),
-                           max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
-    const unsigned r = __reduce_max_sync(FULL, m);
-    const float e = (float)max((int)(r >> 23) - 127, -100);
-    return r >= 0x7f800000u ? __int_as_float(0x7fffffff) : (r == 0 ? UT_POISON_E : e);
+// Largest of |a|, |b|, |c|; NaN if one of them is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Exponent floor(log2) of a row's largest magnitude as a whole number in
+// [-100, 127]; UT_POISON_E for a row of zeros, NaN for one that holds
+// something not finite.
+__device__ __forceinline__ float top_exponent(float top) {
+    const unsigned t = __float_as_uint(top);
+    const float e = (float)max((int)(t >> 23) - 127, -100);
+    return t >= 0x7f800000u ? __int_as_float(0x7fffffff) : (t == 0 ? UT_POISON_E : e);
 }
 // 2^e for whole e in [-126, 127].
 __device__ __forceinline__ float pow2_whole(float e) { return __int_as_float(((int)e + 127) << 23); }
-// Scales this lane's 4 numbers of row r by 2^(13 - e) and writes them to the
-// tile pair at `tile` (hi, then lo UT_BYTES further).  Rows that are not
-// finite become zeros.
-__device__ __forceinline__ void put_row(unsigned char* tile, int r, int lane, float4 x, float e) {
-    const bool ok = e == e;
-    const float s = ok ? pow2_whole(13.f - fmaxf(e, -100.f)) : 0.f;
-    if (!ok) x = make_float4(0.f, 0.f, 0.f, 0.f);
+// The scale 2^(13 - e) of a row with exponent e; 0 for rows that become zeros
+// (of zeros, or not finite).
+__device__ __forceinline__ float row_scale(float e) { return e >= -100.f ? pow2_whole(13.f - e) : 0.f; }
+// 8 bytes at row r, columns 4c .. 4c+3 of the tile pair at `tile` (hi, then lo
+// UT_BYTES further).
+__device__ __forceinline__ uint32_t ut_at(int r, int c) {
+    return (uint32_t)(c >> 4) * UT_HALF + (uint32_t)r * 128u + ((((uint32_t)(c & 15) >> 1) ^ (uint32_t)(r & 7)) * 16u) +
+           (uint32_t)(c & 1) * 8u;
+}
+__device__ __forceinline__ void put4(unsigned char* at, float4 x, float s) {
     uint2 hi, lo;
     const float2 s2 = make_float2(s, s);
     split2(mul2(make_float2(x.x, x.y), s2), hi.x, lo.x);
     split2(mul2(make_float2(x.z, x.w), s2), hi.y, lo.y);
-    const uint32_t at = (uint32_t)(lane >> 4) * UT_HALF + (uint32_t)r * 128u +
-                        ((((uint32_t)(lane & 15) >> 1) ^ (uint32_t)(r & 7)) * 16u) + (uint32_t)(lane & 1) * 8u;
-    *reinterpret_cast<uint2*>(tile + at) = hi;
-    *reinterpret_cast<uint2*>(tile + UT_BYTES + at) = lo;
+    *reinterpret_cast<uint2*>(at) = hi;
+    *reinterpret_cast<uint2*>(at + UT_BYTES) = lo;
 }
+
+// 4 NQ rows of a tile in the registers of a warp, on their way from the pool
+// to a tile pair.  Lane 8 i + t holds, of rows i, 4 + i, ..., float4 columns
+// t, t+8, t+16, t+24, each pair of them swapped for odd i: a load instruction
+// reads whole 128-byte lines of four rows, and a store instruction's four
+// rows fall into both halves of the banks.
+template <int NQ>
+struct RowSet {
+    float4 d[NQ][4];
+    // `unit`: where this lane's row 4 q + i lies in the pool, or UT_NONE / UT_BAD
+    __device__ __forceinline__ void load(int q, const float4* pool, uint32_t unit, int lane) {
+        const int x = lane & 8;
+        const float4* p[2] = {pool + (long long)unit * 32 + (lane & 7) + x, pool + (long long)unit * 32 + (lane & 7) + (8 - x)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            asm volatile("{\n .reg .pred p;\n setp.lt.u32 p, %4, 0xfffffffe;\n"
+                         " @p ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%5];\n}"
+                         : "+f"(d[q][j].x), "+f"(d[q][j].y), "+f"(d[q][j].z), "+f"(d[q][j].w)
+                         : "r"(unit), "l"(p[j & 1] + 16 * (j >> 1)));
+    }
+    // Exponent of this lane's row 4 q + i (the same in its 8 lanes).
+    __device__ __forceinline__ float exponent(int q, uint32_t unit) const {
+        float m = max3_abs(d[q][0].x, d[q][0].y, d[q][0].z), n = max3_abs(d[q][0].w, d[q][1].x, d[q][1].y);
+        m = max3_abs(m, d[q][1].z, d[q][1].w);
+        n = max3_abs(n, d[q][2].x, d[q][2].y);
+        m = max3_abs(m, d[q][2].z, d[q][2].w);
+        n = max3_abs(n, d[q][3].x, d[q][3].y);
+        m = max3_abs(m, d[q][3].z, d[q][3].w);
+        m = max3_abs(m, n, __shfl_xor_sync(FULL, max3_abs(m, n, 0.f), 1));
+        m = max3_abs(m, __shfl_xor_sync(FULL, m, 2), 0.f);
+        m = max3_abs(m, __shfl_xor_sync(FULL, m, 4), 0.f);
+        return unit == UT_NONE ? UT_POISON_E : unit == UT_BAD ? __int_as_float(0x7fffffff) : top_exponent(m);
+    }
+    // Rows 4 q + i, scaled, into the tile at its row `row0` (a multiple of 8).
+    __device__ __forceinline__ void put(int q, unsigned char* tile, int row0, float s, int lane) const {
+        const int i = lane >> 3, t = lane & 7, x = i & 1;
+        unsigned char* at = tile + (row0 + 4 * q + i) * 128 + (((t >> 1) ^ i) * 16) + (t & 1) * 8;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            put4(at + (j >> 1) * UT_HALF + 64 * ((j & 1) ^ x ^ (q & 1)), d[q][j], s);
+    }
+    __device__ __forceinline__ void zero(int q) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[q][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) zero(q);
+    }
+};
 
 }  // namespace skb

@@ -300,7 +300,7 @@ def _cache_attention(name, qkv, n_heads, n_kv_heads, q_norm, k_norm, eps, rope_c
                                                           int(mass is not None))
         else:
             need = _lib.lib().skb_chunk_attention_workspace(tokens, rows, max_chunk, n_heads, n_kv_heads, max_pages,
-                                                            page_size, int(mass is not None))
+                                                            page_size, n_pages, window, sinks, int(mass is not None))
         work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
         if chunk_start is None:
             _lib.call(name, qkv.data_ptr(), rows, *heads, *cache, ptr(work), max(need, 0), out.data_ptr(), _stream())

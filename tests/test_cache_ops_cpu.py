@@ -78,15 +78,21 @@ def test_no_rows_or_no_tokens_is_no_work(lib):
 
 def test_workspace_sizes(lib):
     L = lib.lib()
-    assert L.skb_chunk_attention_workspace(-1, 2, 4, 16, 8, 4, 16, 0) == -1
-    assert L.skb_chunk_attention_workspace(5, 2, 4, 16, 8, 0, 16, 0) == -1
+    assert L.skb_chunk_attention_workspace(-1, 2, 4, 16, 8, 4, 16, 9, 0, 0, 0) == -1
+    assert L.skb_chunk_attention_workspace(5, 2, 4, 16, 8, 0, 16, 9, 0, 0, 0) == -1
     assert L.skb_window_decode_workspace(2, 16, 4, 16, 0, 0, 0) == 0
     assert L.skb_window_decode_workspace(2, 16, 4, 16, 0, 0, 1) == 2 * 16 * 64 * 4
     assert L.skb_window_decode_workspace(2, 16, 4, 16, 8, 4, 1) == 2 * 16 * 12 * 4
     assert L.skb_window_decode_workspace(2, 16, 0, 16, 8, 4, 1) == -1
     assert L.skb_evict_workspace(-1, 8) == -1
     # sizes that pass 32 bits are counted in 64
-    assert L.skb_chunk_attention_workspace(1 << 20, 1, 1 << 20, 16, 8, 1 << 14, 64, 0) >= (1 << 20) * 16 * 512
+    big = L.skb_chunk_attention_workspace(1 << 20, 1, 1 << 20, 16, 8, 1 << 14, 64, 1 << 14, 0, 0, 0)
+    assert big >= (1 << 20) * 16 * 512 + (1 << 20) * 8 * 1024
+    # no more key tiles than the pool, or the windows, can fill
+    by_pool = L.skb_chunk_attention_workspace(8, 64, 1, 16, 8, 1 << 10, 64, 100, 0, 0, 0)
+    assert by_pool < 64 * (1 << 16) * 8 * 1024
+    by_window = L.skb_chunk_attention_workspace(8, 64, 1, 16, 8, 1 << 10, 64, 1 << 16, 200, 4, 0)
+    assert by_window < 64 * 1000 * 8 * 1024
 
 
 def test_python_layer_refuses_before_the_gpu():
