@@ -92,17 +92,21 @@ constexpr float CH_QSCALE = 0.08838834764831845f * CO_LOG2E;  // 1 / sqrt(128), 
 
 constexpr int CP_TILES = 64;  // blocks side by side over a row's key tiles
 
-// Blocks [0, tokens): a new token each, 256 threads, a warp per head vector.
+// The first `token_blocks` blocks: `per_block` new tokens each (1, 2 or 4), 8 /
+// per_block warps to a token, which take its head vectors in turn.  Few tokens
+// are spread over many warps, many share a warp's look at their row's numbers.
 // The others: cached slots, a block per (key tile, keys or values, kv head, row).
-__global__ void __launch_bounds__(256) chunk_prep_kernel(const ChunkArgs c, int tiles_x) {
+__global__ void __launch_bounds__(256, 3) chunk_prep_kernel(const ChunkArgs c, int token_blocks, int per_block, int tiles_x) {
     const CacheAttnArgs& a = c.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int H = a.H, KVH = a.kv.KVH, nv = H + 2 * KVH;
     pdl_trigger();
     const float eq = query_exponent(a.qn, lane);
     const float qfac = pow2_whole(eq - 13.f);
-    if ((int)blockIdx.x < c.tokens) {
-        const int t = blockIdx.x;
+    if ((int)blockIdx.x < token_blocks) {
+        const int wpt = 8 / per_block, w = warp % wpt;
+        const int t = blockIdx.x * per_block + warp / wpt;
+        if (t >= c.tokens) return;
         int r = 0;  // rows that end at or before the token
         for (int p = lane; p - lane < a.rows; p += 32)
             r += __popc(__ballot_sync(FULL, p < a.rows && c.chunk_start[p + 1] <= t));
@@ -115,7 +119,7 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(const ChunkArgs c, int 
         if (base + rt.n > c.key_tiles) x.bad = true;  // pages mapped to several rows
         if (x.idle || x.bad) {
             const float o = x.idle ? 0.f : __int_as_float(0x7fffffff);
-            for (int v = warp; v < H; v += 8)
+            for (int v = w; v < H; v += wpt)
                 reinterpret_cast<float4*>(a.out)[((long long)t * H + v) * 32 + lane] = make_float4(o, o, o, o);
             return;
         }
@@ -124,14 +128,14 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(const ChunkArgs c, int 
         const float* cosr = a.rope_cos + (long long)pos * 64;
         const float* sinr = a.rope_sin + (long long)pos * 64;
         const long long tile = base + rt.index(slot >> 7);
-        for (int v0 = warp; v0 < nv; v0 += 32) {
+        for (int v0 = w; v0 < nv; v0 += 4 * wpt) {
             float4 y[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (v0 + 8 * j < nv) y[j] = row[(v0 + 8 * j) * 32];
+                if (v0 + wpt * j < nv) y[j] = row[(v0 + wpt * j) * 32];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int v = v0 + 8 * j;
+                const int v = v0 + wpt * j;
                 if (v >= nv) break;
                 if (v < H + KVH) y[j] = norm_rope_head(y[j], v < H ? a.qn : a.kn, a.eps, cosr, sinr, lane, true, true);
                 if (v < H) {
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(const ChunkArgs c, int 
         }
         return;
     }
-    int b = blockIdx.x - c.tokens;
+    int b = blockIdx.x - token_blocks;
     const int k0 = b % tiles_x;
     b /= tiles_x;
     const int value = b & 1, g = (b >> 1) % KVH, r = (b >> 1) / KVH;
@@ -171,7 +175,7 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(const ChunkArgs c, int 
         const int first = rt.tile(k) * 128 + row0;
         if (first >= x.cached && first + 15 <= last) continue;  // new tokens only: theirs are written above
         const long long at = ((base + k) * KVH + g) * 2 + value;
-        RowSet<4> d;
+        RowSet<2> d[2];
         uint32_t unit[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -182,16 +186,18 @@ __global__ void __launch_bounds__(256) chunk_prep_kernel(const ChunkArgs c, int 
                 unit[q] = u < 0 ? UT_BAD : (uint32_t)u;
             }
         }
-        d.zero();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) d.load(q, pool, unit[q], lane);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float e = d.exponent(q, unit[q]);
+            d[q >> 1].zero(q & 1);
+            d[q >> 1].load(q & 1, pool, unit[q], lane);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float e = d[q >> 1].exponent(q & 1, unit[q]);
             const int slot = first + 4 * q + i4;
-            if (!(e >= -100.f)) d.zero(q);
+            if (!(e >= -100.f)) d[q >> 1].zero(q & 1);
             if (slot >= x.cached && slot <= last) continue;
-            d.put(q, c.kvtiles + at * (2 * UT_BYTES), row0, row_scale(e), lane);
+            d[q >> 1].put(q & 1, c.kvtiles + at * (2 * UT_BYTES), row0 + 8 * (q >> 1), row_scale(e), lane);
             if ((lane & 7) == 0)
                 c.meta[at * 128 + row0 + 4 * q + i4] = value ? e : e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac : e;
         }
@@ -234,7 +240,8 @@ struct TileList {
 // A CTA takes one query tile and a part of the key tiles it sees:
 //   warp P     asks for key and value tiles, 64 KB bulk copies into three
 //              stages, in the order K0 K1 V0 K2 V1 ...
-//   warp M     issues the products: S_i = Q K_i, then O = P_i V_i, S one tile ahead
+//   warp M, O  issue the products: S_i = Q K_i, a tile ahead, and O = P_i V_i.
+//              Two warps, so that neither product stands behind the other's waits
 //   warp E     a tile's factors and exponents from the workspace, and the
 //              running exponent of the values
 //   softmax    CA_PARTS threads per query row, each with a part of a tile's
@@ -244,7 +251,7 @@ struct TileList {
 constexpr int CA_PARTS = 4;
 constexpr int CA_W = 128 / CA_PARTS;  // a thread's keys, and its output columns
 constexpr int CA_SOFTMAX_WARPS = 4 * CA_PARTS, CA_WARP_M = CA_SOFTMAX_WARPS, CA_WARP_P = CA_WARP_M + 1,
-              CA_WARP_E = CA_WARP_M + 2;
+              CA_WARP_E = CA_WARP_M + 2, CA_WARP_O = CA_WARP_M + 3;
 constexpr int CA_THREADS = 32 * (CA_SOFTMAX_WARPS + 4);
 constexpr int CA_STAGES = 3;
 // TMEM columns: two score tiles, a tile's output, the queries
@@ -260,7 +267,7 @@ struct CaSmem {
     float mx[2][CA_PARTS][128], ex[2][CA_PARTS][128];  // a row part's largest score and value exponent
     float m[128], l[CA_PARTS][128];      // this split's statistics (sums of row parts)
     float E[2];                          // running exponent of the values
-    uint64_t q_full, full[CA_STAGES], empty[CA_STAGES], s_full[2], p_full, pv_done[2], meta_full[2], o_full;
+    uint64_t q_landed, q_full, full[CA_STAGES], empty[CA_STAGES], s_full[2], p_full, pv_done[2], meta_full[2], o_full;
     // what the CTA works on
     TileList list;
     int k0, nt;          // its key tiles: list entries [k0, k0 + nt)
@@ -314,6 +321,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         return;
     }
     if (tid == 0) {
+        mbar_init(&sm.q_landed, 1);
         mbar_init(&sm.q_full, CA_SOFTMAX_WARPS);
         mbar_init(&sm.p_full, CA_SOFTMAX_WARPS);
         mbar_init(&sm.o_full, 1);
@@ -356,6 +364,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             int n = 0, landed = 0;  // copies asked for
             auto fetch = [&](int i, int value) {
                 const int s = n % CA_STAGES;
+                if (n == CA_STAGES - 1 && !ut_wait(&sm.q_full, 0, abort)) return false;  // the queries were there
                 if (n >= CA_STAGES && !ut_wait(&sm.empty[s], ((n - CA_STAGES) / CA_STAGES) & 1, abort)) return false;
                 const long long at = ((base + rt.index(sm.list.tile(sm.k0 + i))) * a.kv.KVH + g) * 2 + value;
                 mbar_expect_tx(&sm.full[s], 2 * UT_BYTES);
@@ -363,12 +372,18 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                 ++n;
                 return true;
             };
-            bool go = nt > 0 && fetch(0, 0);
+            bool go = nt > 0;
+            if (go) {  // the queries by way of the last stage
+                mbar_expect_tx(&sm.q_landed, 2 * UT_BYTES);
+                bulk_g2s(sm.stage[CA_STAGES - 1], c.qtiles + sm.tile_at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.q_landed);
+                go = fetch(0, 0);
+            }
             for (int i = 0; i < nt && go; ++i) {
                 if (i + 1 < nt) go = fetch(i + 1, 0);
                 if (go) go = fetch(i, 1);
             }
             // no copy may be in flight when the CTA ends early
+            if (!go && nt > 0) mbar_wait(&sm.q_landed, 0, nullptr);
             if (!go)
                 for (landed = max(0, n - CA_STAGES); landed < n; ++landed)
                     mbar_wait(&sm.full[landed % CA_STAGES], (landed / CA_STAGES) & 1, nullptr);
@@ -376,36 +391,32 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         __syncwarp();
     } else if (warp == CA_WARP_M) {
         if (lane == 0 && nt > 0) {
-            int n = 0;  // stages used
             bool go = ut_wait(&sm.q_full, 0, abort);
-            auto score = [&](int i) {  // S_i = Q K_i, over the weights of tile i - 2
-                const int s = n % CA_STAGES;
-                go = go && ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort) &&
+            for (int i = 0; i < nt && go; ++i) {  // S_i = Q K_i, over the weights of tile i - 2
+                const int n = i == 0 ? 0 : 2 * i - 1, s = n % CA_STAGES;
+                go = ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort) &&
                      (i < 2 || ut_wait(&sm.pv_done[i & 1], ((i - 2) >> 1) & 1, abort));
-                if (!go) return;
+                if (!go) break;
                 ut_fence_after();
                 ut_mma_qk_ts(tmem + (i & 1) * 128, tmem + CA_TM_Q, smem_u32(sm.stage[s]));
                 ut_commit(&sm.empty[s]);
                 ut_commit(&sm.s_full[i & 1]);
-                ++n;
-            };
-            auto weigh = [&](int i) {  // O = P_i V_i
-                const int s = n % CA_STAGES;
-                go = go && ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort) && ut_wait(&sm.p_full, i & 1, abort);
-                if (!go) return;
+            }
+        }
+        __syncwarp();
+    } else if (warp == CA_WARP_O) {
+        if (lane == 0 && nt > 0) {
+            bool go = true;
+            for (int i = 0; i < nt && go; ++i) {  // O = P_i V_i
+                const int n = i + 1 < nt ? 2 * i + 2 : 2 * nt - 1, s = n % CA_STAGES;
+                go = ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort) && ut_wait(&sm.p_full, i & 1, abort);
+                if (!go) break;
                 ut_fence_after();
                 ut_mma_pv(tmem + CA_TM_O, tmem + (i & 1) * 128, smem_u32(sm.stage[s]));
                 ut_commit(&sm.empty[s]);
                 ut_commit(&sm.pv_done[i & 1]);
-                ++n;
-            };
-            score(0);
-            if (nt > 1) score(1);
-            for (int i = 0; i < nt; ++i) {
-                weigh(i);
-                if (i + 2 < nt) score(i + 2);
             }
-            ut_commit(&sm.o_full);  // every product issued so far
+            ut_commit(&sm.o_full);  // every P V issued so far, and so every S before them
             ut_wait(&sm.o_full, 0, abort);
         }
         __syncwarp();
@@ -451,7 +462,8 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             }
         };
         if (nt > 0 && part < 2) {  // the queries into tensor memory: this row of hi, or of lo
-            const unsigned char* q = c.qtiles + sm.tile_at * (2 * UT_BYTES) + part * UT_BYTES + row * 128;
+            const unsigned char* q = sm.stage[CA_STAGES - 1] + part * UT_BYTES + row * 128;
+            ut_wait(&sm.q_landed, 0, abort);
 #pragma unroll
             for (int ch = 0; ch < 2; ++ch) {
                 uint32_t w[32];
@@ -664,6 +676,7 @@ struct CmSmem {
     float lse[2][128];
     float kc[128];
     float part[2][128];
+    int own[CM_SUM_WARPS][64];  // slots of the queries in a warp's columns; -1: none
     uint64_t k_full, q_full[2], q_empty[2], s_full[2], s_empty[2];
     uint32_t tmem;
     int abort;
@@ -760,7 +773,8 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
         const int key = 32 * (warp & 3) + lane, half = warp >> 2, slot = base + key;
         const float kc = sm.kc[key];
         const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * 64;
-        const bool sink = slot < a.sinks;
+        // queries at slots >= this do not see the slot
+        const unsigned upto = a.window == 0 || slot < a.sinks ? 0x7fffffffu : (unsigned)slot + (unsigned)a.window;
         float2 sum = make_float2(0.f, 0.f);
         for (int i = 0; i < nt; ++i) {
             const int b = i & 1;
@@ -769,6 +783,13 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
             // seen whole: every column is a query, behind every slot, inside the window
             const bool whole = nq * c.n_rep == 128 && first >= base + 127 &&
                                (a.window == 0 || first + nq - 1 - base < a.window || base + 128 <= a.sinks);
+            if (!whole) {  // one division a column, not one a weight
+                for (int col = lane; col < 64; col += 32) {
+                    const int qi = (half * 64 + col) / c.n_rep;
+                    sm.own[warp][col] = qi < nq ? first + qi : -1;
+                }
+                __syncwarp();
+            }
             if (!ut_wait(&sm.s_full[b], (i >> 1) & 1, abort)) break;
             // also waited for: the lse that came with the tile
             if (!ut_wait(&sm.q_full[b], (i >> 1) & 1, abort)) break;
@@ -789,18 +810,17 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
                                     make_float2(-f.z, -f.w));
                     float p[4] = {exp2_fast(u.x), exp2_fast(u.y), exp2_fast(v.x), exp2_fast(v.y)};
                     if (!whole) {
+                        const int4 own = reinterpret_cast<const int4*>(sm.own[warp])[ch * 8 + q];
+                        const int w[4] = {own.x, own.y, own.z, own.w};
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const int col = half * 64 + ch * 32 + 4 * q + y, qi = col / c.n_rep, own = first + qi;
-                            const bool see = qi < nq && slot <= own && (a.window == 0 || own - slot < a.window || sink);
-                            if (!see) p[y] = 0.f;
-                        }
+                        for (int y = 0; y < 4; ++y)
+                            if (w[y] < slot || (unsigned)w[y] >= upto) p[y] = 0.f;
                     }
                     sum = add2(sum, add2(make_float2(p[0], p[1]), make_float2(p[2], p[3])));
                 }
             }
             ut_fence_before();
-            __syncwarp();
+            __syncwarp();  // also: the slots in sm.own are read
             if (lane == 0) ut_arrive(&sm.s_empty[b]);
         }
         sm.part[half][key] = sum.x + sum.y;
@@ -925,19 +945,24 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     long long ctas = (long long)rows * tiles_x;
     if (ctas > tiles) ctas = tiles;
     ctas *= n_kv_heads;
-    int splits = 1;
-    while (splits < CA_MAX_SPLITS && ctas * splits * 2 <= 148 && splits * 2 <= row_tiles) splits *= 2;
+    long long splits = 148 / ctas;
+    if (splits > row_tiles) splits = row_tiles;
+    if (splits > CA_MAX_SPLITS) splits = CA_MAX_SPLITS;
+    if (splits < 1) splits = 1;
     const int prep_x = row_tiles < CP_TILES ? (int)row_tiles : CP_TILES;
-    const long long prep_blocks = tokens + (long long)prep_x * 2 * n_kv_heads * rows;
+    const int per_block = tokens <= 1024 ? 1 : 4;
+    const int token_blocks = (tokens + per_block - 1) / per_block;
+    const long long prep_blocks = token_blocks + (long long)prep_x * 2 * n_kv_heads * rows;
     if (prep_blocks > 0x7fffffffll) return fail(SKB_ERR_ARG, "%s: too many tokens and rows", what);
 
     cudaError_t e = set_smem_attrs(chunk_attn_kernel, CA_SMEM);
     if (e == cudaSuccess && mass) e = set_smem_attrs(chunk_mass_kernel, CM_SMEM);
     if (e == cudaSuccess)
-        e = launch(chunk_prep_kernel, dim3((unsigned)prep_blocks), dim3(256), 0, stream, false, c, prep_x);
+        e = launch(chunk_prep_kernel, dim3((unsigned)prep_blocks), dim3(256), 0, stream, false, c, token_blocks, per_block,
+                   prep_x);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(splits * tiles_x, n_kv_heads, rows);
+        cfg.gridDim = dim3((unsigned)splits * tiles_x, n_kv_heads, rows);
         cfg.blockDim = dim3(CA_THREADS);
         cfg.dynamicSmemBytes = CA_SMEM;
         cfg.stream = stream;
@@ -945,12 +970,12 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = splits;
+        attr[1].val.clusterDim.x = (unsigned)splits;
         attr[1].val.clusterDim.y = 1;
         attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 2;
-        e = cudaLaunchKernelEx(&cfg, chunk_attn_kernel, c, splits);
+        e = cudaLaunchKernelEx(&cfg, chunk_attn_kernel, c, (int)splits);
     }
     if (e == cudaSuccess && mass)
         e = launch(chunk_mass_kernel, dim3((unsigned)row_tiles, n_kv_heads, rows), dim3(CM_THREADS), CM_SMEM, stream, true, c);

@@ -155,17 +155,28 @@ __device__ __forceinline__ void ut_arrive(uint64_t* bar) {
 }
 // Waits for phase `parity`, at most about 2 s and no longer than *abort stays
 // 0; false (and *abort set) when it gave up.  Every wait of a kernel goes
-// through here, so that one that runs out ends all the others.  A try sleeps
-// up to 1 ms in hardware, so a waiting warp takes no issue slots.
+// through here, so that one that runs out ends all the others.  A test first,
+// which costs least when the phase is over (a try with a time to sleep took
+// 230 cycles then); after a few of them tries that sleep up to 20 us in hardware,
+// so that a waiting warp takes no issue slots.
 __device__ __forceinline__ bool ut_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
     const uint32_t addr = smem_u32(bar);
+    uint32_t done;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
     uint64_t t0 = 0;
     for (;;) {
-        uint32_t done;
         asm volatile(
             "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
             : "=r"(done)
-            : "r"(addr), "r"(parity), "r"(1000000u)
+            : "r"(addr), "r"(parity), "r"(20000u)
             : "memory");
         if (done) return true;
         const uint64_t now = globaltimer_ns();
