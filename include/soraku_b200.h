@@ -226,11 +226,9 @@ int skb_window_decode_attention(const float *qkv, int rows, int n_heads, int n_k
  *   cached_out device int32 [rows]: min(cached, budget); counts that are
  *              negative or exceed the cache come back as they are, with
  *              nothing kept and nothing moved */
-int64_t skb_evict_workspace(int rows, int n_kv_heads);
 int skb_evict_cache(const float *mass, const int32_t *cached, int rows, int n_kv_heads, int head_dim, float *kv_pool,
                     const int32_t *page_table, int max_pages, int page_size, int n_pages, int budget, int sinks,
-                    int recent, int32_t *kept, float *mass_out, int32_t *cached_out, void *work, int64_t work_bytes,
-                    cudaStream_t stream);
+                    int recent, int32_t *kept, float *mass_out, int32_t *cached_out, cudaStream_t stream);
 
 /* Test hooks: the device exp used by the sampler, and raw Philox4x32-10.
  * ctr_key: device uint32 [n, 6] = (c0, c1, c2, c3, k0, k1); out: [n, 4]. */

@@ -48,9 +48,8 @@ SIGNATURES = {
                                             c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                             c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p,
                                             c_void_p]),
-    "skb_evict_workspace": (c_int64, [c_int, c_int]),
     "skb_evict_cache": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
-                                c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+                                c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "skb_test_exp": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
     "skb_test_philox": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
     "skb_test_wait_timeout": (c_int, [c_void_p, c_int, c_void_p]),
@@ -153,3 +152,10 @@ def stream_ptr(stream=None) -> int:
 
     s = torch.cuda.current_stream() if stream is None else stream
     return int(s.cuda_stream)
+
+
+def device_stream_ptr(device: int) -> int:
+    """Raw cudaStream_t of the current torch stream of a device."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device)

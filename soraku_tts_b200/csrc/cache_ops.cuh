@@ -9,12 +9,17 @@
 // j <= i if there is no window (window == 0), or i - j < window, or j < sinks.
 #pragma once
 
+#include <atomic>
+
 #include "ops.cuh"
 #include "trunk.cuh"
 
 namespace skb {
 
 constexpr int CO_MAX_REP = 4;  // query heads per kv head
+// 32-bit units of rows that are not in the pool: none is meant (zeros), or its
+// page is outside (not a number).
+constexpr uint32_t UT_NONE = 0xffffffffu, UT_BAD = 0xfffffffeu;
 
 struct CacheView {
     float* pool;
@@ -63,6 +68,21 @@ inline int log2_of(int v) {
     int lg = 0;
     while ((1 << lg) < v) ++lg;
     return lg;
+}
+
+// set_smem_attrs once per kernel and device: the call costs as much as a third
+// of a launch.  Like every address cached per device, what it set is gone after
+// cudaDeviceReset.
+template <typename K>
+inline cudaError_t smem_attrs_once(K* kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = set_smem_attrs(kernel, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // exp2 in one instruction (relative error 2^-22); the argument of a softmax

@@ -30,6 +30,7 @@ struct ChunkArgs {
     unsigned char* kvtiles; // [key tiles][KVH][2][2 UT_BYTES]: keys, values, hi | lo
     float* meta;            // [key tiles][KVH][2][128]: factor of a key's scores; exponent of a value row
     float* lse;             // [query tiles][KVH][128] (mass only), log2 units
+    int* order;             // [rows]: rows by the tiles they see, most first; null: as they are
     long long key_tiles;
 };
 
@@ -90,12 +91,14 @@ __device__ __forceinline__ float query_exponent(const float* qn, int lane) {
 
 constexpr float CH_QSCALE = 0.08838834764831845f * CO_LOG2E;  // 1 / sqrt(128), scores in log2 units
 
-constexpr int CP_TILES = 64;  // blocks side by side over a row's key tiles
+constexpr int CP_TILES = 64;     // blocks side by side over a row's key tiles
+constexpr int CP_SORTED = 512;   // rows that are put in order; more come as they are
 
 // The first `token_blocks` blocks: `per_block` new tokens each (1, 2 or 4), 8 /
 // per_block warps to a token, which take its head vectors in turn.  Few tokens
 // are spread over many warps, many share a warp's look at their row's numbers.
-// The others: cached slots, a block per (key tile, keys or values, kv head, row).
+// The next block puts the rows in order.  The others: cached slots, a block per
+// (key tile, keys or values, kv head, row).
 __global__ void __launch_bounds__(256, 3) chunk_prep_kernel(const ChunkArgs c, int token_blocks, int per_block, int tiles_x) {
     const CacheAttnArgs& a = c.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -161,6 +164,21 @@ __global__ void __launch_bounds__(256, 3) chunk_prep_kernel(const ChunkArgs c, i
         return;
     }
     int b = blockIdx.x - token_blocks;
+    if (b == 0 && c.order) {  // the order in which chunk_attn takes the rows
+        __shared__ int seen[CP_SORTED];
+        for (int p = threadIdx.x; p < a.rows; p += 256) {
+            if (a.rows <= CP_SORTED) seen[p] = RowTiles(c, chunk_row(c, p)).n;
+            else c.order[p] = p;
+        }
+        __syncthreads();
+        for (int p = threadIdx.x; p < a.rows && a.rows <= CP_SORTED; p += 256) {
+            int rank = 0;
+            for (int q = 0; q < a.rows; ++q) rank += seen[q] > seen[p] || (seen[q] == seen[p] && q < p);
+            c.order[rank] = p;
+        }
+        return;
+    }
+    if (c.order) --b;
     const int k0 = b % tiles_x;
     b /= tiles_x;
     const int value = b & 1, g = (b >> 1) % KVH, r = (b >> 1) / KVH;
@@ -169,13 +187,13 @@ __global__ void __launch_bounds__(256, 3) chunk_prep_kernel(const ChunkArgs c, i
     if (k0 >= rt.n) return;
     const long long base = row_base(c, r);
     if (base + rt.n > c.key_tiles) return;
-    const float4* pool = reinterpret_cast<const float4*>(a.kv.pool) + (value ? a.kv.value_step() * 32 : 0);
+    const float* pool = a.kv.pool + (value ? a.kv.value_step() * 128 : 0);
     const int row0 = warp * 16, i4 = lane >> 3, last = x.cached + x.n - 1;
     for (int k = k0; k < rt.n; k += tiles_x) {
         const int first = rt.tile(k) * 128 + row0;
         if (first >= x.cached && first + 15 <= last) continue;  // new tokens only: theirs are written above
         const long long at = ((base + k) * KVH + g) * 2 + value;
-        RowSet<2> d[2];
+        RowSet d;
         uint32_t unit[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -187,17 +205,13 @@ __global__ void __launch_bounds__(256, 3) chunk_prep_kernel(const ChunkArgs c, i
             }
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            d[q >> 1].zero(q & 1);
-            d[q >> 1].load(q & 1, pool, unit[q], lane);
-        }
+        for (int q = 0; q < 4; ++q) d.load(q, pool, unit[q], lane);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float e = d[q >> 1].exponent(q & 1, unit[q]);
+            const float e = d.exponent(q, unit[q]);
             const int slot = first + 4 * q + i4;
-            if (!(e >= -100.f)) d[q >> 1].zero(q & 1);
             if (slot >= x.cached && slot <= last) continue;
-            d[q >> 1].put(q & 1, c.kvtiles + at * (2 * UT_BYTES), row0 + 8 * (q >> 1), row_scale(e), lane);
+            d.put(q, c.kvtiles + at * (2 * UT_BYTES), row0, row_scale(e), lane);
             if ((lane & 7) == 0)
                 c.meta[at * 128 + row0 + 4 * q + i4] = value ? e : e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac : e;
         }
@@ -282,7 +296,10 @@ constexpr size_t CA_SMEM = sizeof(CaSmem) + 1024;
 static_assert(CA_SMEM <= 227 * 1024, "shared memory of one CTA");
 static_assert(128 * CA_OUT_LD * 4 <= CA_STAGES * 2 * UT_BYTES, "the staged output lies over the tiles");
 
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 2, %0;" ::"n"(32 * CA_SOFTMAX_WARPS) : "memory"); }
+// The warps that share a quadrant's 32 rows.
+__device__ __forceinline__ void softmax_sync() {
+    asm volatile("bar.sync %0, %1;" ::"r"(2 + ((threadIdx.x >> 5) & 3)), "n"(32 * CA_PARTS) : "memory");
+}
 
 __device__ __forceinline__ float4 ld_peer4(uint32_t local, uint32_t rank) {
     uint32_t ra;
@@ -308,9 +325,10 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     CaSmem& sm = *reinterpret_cast<CaSmem*>(ca_raw + ((1024u - (smem_u32(ca_raw) & 1023u)) & 1023u));
     const CacheAttnArgs& a = c.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = blockIdx.y, r = blockIdx.z, z = blockIdx.x % splits;
-    const int tiles_x = gridDim.x / splits;
-    const int t = tiles_x - 1 - blockIdx.x / splits;  // the last query tile sees the most: first
+    const int g = blockIdx.y, z = blockIdx.x % splits;
+    const int t = gridDim.x / splits - 1 - blockIdx.x / splits;  // the last query tile sees the most: first
+    if (c.order) pdl_wait();
+    const int r = c.order ? c.order[blockIdx.z] : blockIdx.z;
     const ChunkRow x = chunk_row(c, r);
     const int i0 = t * c.P;
     const RowTiles rt(c, x);
@@ -857,12 +875,13 @@ static long long chunk_key_tiles(int rows, int max_chunk, int max_pages, int pag
 }
 
 struct ChunkWork {
-    long long q, kv, meta, lse, total;  // byte offsets
-    ChunkWork(long long qtiles, long long ktiles, int KVH, bool with_mass) {
+    long long q, kv, meta, order, lse, total;  // byte offsets
+    ChunkWork(long long qtiles, long long ktiles, int KVH, int rows, bool with_mass) {
         q = 0;
         kv = qtiles * KVH * (2 * (long long)UT_BYTES);
         meta = kv + ktiles * KVH * (4 * (long long)UT_BYTES);
-        lse = meta + ktiles * KVH * 1024;
+        order = meta + ktiles * KVH * 1024;
+        lse = order + (rows * 4ll + 255) / 256 * 256;
         total = lse + (with_mass ? (qtiles * KVH * 512 + 255) / 256 * 256 : 0);
     }
 };
@@ -878,7 +897,8 @@ extern "C" int64_t skb_chunk_attention_workspace(int tokens, int rows, int max_c
         n_heads / n_kv_heads > CO_MAX_REP || max_pages < 1 || page_size < 1 || n_pages < 1 || window < 0 || sinks < 0)
         return -1;
     return ChunkWork(chunk_query_tiles(tokens, rows, n_heads / n_kv_heads),
-                     chunk_key_tiles(rows, max_chunk, max_pages, page_size, n_pages, window, sinks), n_kv_heads, with_mass)
+                     chunk_key_tiles(rows, max_chunk, max_pages, page_size, n_pages, window, sinks), n_kv_heads, rows,
+                     with_mass)
         .total;
 }
 
@@ -928,7 +948,7 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     c.P = 128 / c.n_rep;
     const long long tiles = chunk_query_tiles(tokens, rows, c.n_rep);
     c.key_tiles = chunk_key_tiles(rows, max_chunk, max_pages, page_size, n_pages, window, sinks);
-    const ChunkWork at(tiles, c.key_tiles, n_kv_heads, mass != nullptr);
+    const ChunkWork at(tiles, c.key_tiles, n_kv_heads, rows, mass != nullptr);
     unsigned char* w = static_cast<unsigned char*>(work);
     c.qtiles = w + at.q;
     c.kvtiles = w + at.kv;
@@ -945,6 +965,8 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     long long ctas = (long long)rows * tiles_x;
     if (ctas > tiles) ctas = tiles;
     ctas *= n_kv_heads;
+    // more than one wave of CTAs: the rows with most work first
+    c.order = ctas > 148 && rows > 1 ? reinterpret_cast<int*>(w + at.order) : nullptr;
     long long splits = 148 / ctas;
     if (splits > row_tiles) splits = row_tiles;
     if (splits > CA_MAX_SPLITS) splits = CA_MAX_SPLITS;
@@ -952,11 +974,12 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     const int prep_x = row_tiles < CP_TILES ? (int)row_tiles : CP_TILES;
     const int per_block = tokens <= 1024 ? 1 : 4;
     const int token_blocks = (tokens + per_block - 1) / per_block;
-    const long long prep_blocks = token_blocks + (long long)prep_x * 2 * n_kv_heads * rows;
+    const long long prep_blocks = token_blocks + (c.order ? 1 : 0) + (long long)prep_x * 2 * n_kv_heads * rows;
     if (prep_blocks > 0x7fffffffll) return fail(SKB_ERR_ARG, "%s: too many tokens and rows", what);
 
-    cudaError_t e = set_smem_attrs(chunk_attn_kernel, CA_SMEM);
-    if (e == cudaSuccess && mass) e = set_smem_attrs(chunk_mass_kernel, CM_SMEM);
+    static std::atomic<unsigned long long> attn_done, mass_done;
+    cudaError_t e = smem_attrs_once(chunk_attn_kernel, CA_SMEM, attn_done);
+    if (e == cudaSuccess && mass) e = smem_attrs_once(chunk_mass_kernel, CM_SMEM, mass_done);
     if (e == cudaSuccess)
         e = launch(chunk_prep_kernel, dim3((unsigned)prep_blocks), dim3(256), 0, stream, false, c, token_blocks, per_block,
                    prep_x);

@@ -23,9 +23,6 @@ constexpr int UT_ROWS = 128;
 constexpr uint32_t UT_HALF = 128 * 128;       // bytes of 64 columns
 constexpr uint32_t UT_BYTES = 2 * UT_HALF;    // one fp16 tile
 constexpr float UT_POISON_E = -200.f;         // exponent of a row of zeros
-// Units of rows that are not in the pool: no query sees the slot (zeros), or
-// its page is outside (not a number).
-constexpr uint32_t UT_NONE = 0xffffffffu, UT_BAD = 0xfffffffeu;
 
 // ------------------------------------------------------------- descriptors
 // Shared-memory operand, 128-byte swizzle.  K-major: 8-row groups 1024 bytes
@@ -270,53 +267,59 @@ __device__ __forceinline__ void put4(unsigned char* at, float4 x, float s) {
     *reinterpret_cast<uint2*>(at + UT_BYTES) = lo;
 }
 
-// 4 NQ rows of a tile in the registers of a warp, on their way from the pool
-// to a tile pair.  Lane 8 i + t holds, of rows i, 4 + i, ..., float4 columns
-// t, t+8, t+16, t+24, each pair of them swapped for odd i: a load instruction
-// reads whole 128-byte lines of four rows, and a store instruction's four
-// rows fall into both halves of the banks.
-template <int NQ>
+// Sixteen rows of a tile in the registers of a warp, on their way from the
+// pool to a tile pair.  Lane 8 i + t holds, of rows i, 4 + i, 8 + i, 12 + i,
+// columns 8 t .. 8 t + 7 of either half: 32 bytes a load, and 16 bytes of hi or
+// lo a store, whose four rows are whole 128-byte lines.
 struct RowSet {
-    float4 d[NQ][4];
-    // `unit`: where this lane's row 4 q + i lies in the pool, or UT_NONE / UT_BAD
-    __device__ __forceinline__ void load(int q, const float4* pool, uint32_t unit, int lane) {
-        const int x = lane & 8;
-        const float4* p[2] = {pool + (long long)unit * 32 + (lane & 7) + x, pool + (long long)unit * 32 + (lane & 7) + (8 - x)};
+    float d[4][2][8];
+    // `unit`: where this lane's row 4 q + i lies in the pool, or UT_NONE / UT_BAD: zeros
+    __device__ __forceinline__ void load(int q, const float* pool, uint32_t unit, int lane) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            asm volatile("{\n .reg .pred p;\n setp.lt.u32 p, %4, 0xfffffffe;\n"
-                         " @p ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%5];\n}"
-                         : "+f"(d[q][j].x), "+f"(d[q][j].y), "+f"(d[q][j].z), "+f"(d[q][j].w)
-                         : "r"(unit), "l"(p[j & 1] + 16 * (j >> 1)));
+        for (int h = 0; h < 2; ++h) {
+            float* x = d[q][h];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = 0.f;
+            asm volatile(
+                "{\n .reg .pred p;\n setp.lt.u32 p, %8, 0xfffffffe;\n"
+                " @p ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%9];\n}"
+                : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7])
+                : "r"(unit), "l"(pool + (long long)unit * 128 + 64 * h + 8 * (lane & 7)));
+        }
     }
     // Exponent of this lane's row 4 q + i (the same in its 8 lanes).
     __device__ __forceinline__ float exponent(int q, uint32_t unit) const {
-        float m = max3_abs(d[q][0].x, d[q][0].y, d[q][0].z), n = max3_abs(d[q][0].w, d[q][1].x, d[q][1].y);
-        m = max3_abs(m, d[q][1].z, d[q][1].w);
-        n = max3_abs(n, d[q][2].x, d[q][2].y);
-        m = max3_abs(m, d[q][2].z, d[q][2].w);
-        n = max3_abs(n, d[q][3].x, d[q][3].y);
-        m = max3_abs(m, d[q][3].z, d[q][3].w);
-        m = max3_abs(m, n, __shfl_xor_sync(FULL, max3_abs(m, n, 0.f), 1));
+        float m = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) m = max3_abs(m, d[q][h][k], d[q][h][k + 1]);
+        m = max3_abs(m, __shfl_xor_sync(FULL, m, 1), 0.f);
         m = max3_abs(m, __shfl_xor_sync(FULL, m, 2), 0.f);
         m = max3_abs(m, __shfl_xor_sync(FULL, m, 4), 0.f);
         return unit == UT_NONE ? UT_POISON_E : unit == UT_BAD ? __int_as_float(0x7fffffff) : top_exponent(m);
     }
-    // Rows 4 q + i, scaled, into the tile at its row `row0` (a multiple of 8).
-    __device__ __forceinline__ void put(int q, unsigned char* tile, int row0, float s, int lane) const {
-        const int i = lane >> 3, t = lane & 7, x = i & 1;
-        unsigned char* at = tile + (row0 + 4 * q + i) * 128 + (((t >> 1) ^ i) * 16) + (t & 1) * 8;
+    // Rows 4 q + i, scaled, into the tile at its row `row0` (a multiple of
+    // 16).  A scale of 0 makes zeros of anything.
+    __device__ __forceinline__ void put(int q, unsigned char* tile, int row0, float s, int lane) {
+        const int i = lane >> 3, row = row0 + 4 * q + i;
+        unsigned char* at = tile + row * 128 + (((lane & 7) ^ (row & 7)) * 16);
+        const float2 s2 = make_float2(s, s);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            put4(at + (j >> 1) * UT_HALF + 64 * ((j & 1) ^ x ^ (q & 1)), d[q][j], s);
-    }
-    __device__ __forceinline__ void zero(int q) {
+        for (int h = 0; h < 2; ++h) {
+            uint4 hi, lo;
+            float* x = d[q][h];
+            if (s == 0.f) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) d[q][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) zero(q);
+                for (int k = 0; k < 8; ++k) x[k] = 0.f;
+            }
+            split2(mul2(make_float2(x[0], x[1]), s2), hi.x, lo.x);
+            split2(mul2(make_float2(x[2], x[3]), s2), hi.y, lo.y);
+            split2(mul2(make_float2(x[4], x[5]), s2), hi.z, lo.z);
+            split2(mul2(make_float2(x[6], x[7]), s2), hi.w, lo.w);
+            *reinterpret_cast<uint4*>(at + h * UT_HALF) = hi;
+            *reinterpret_cast<uint4*>(at + h * UT_HALF + UT_BYTES) = lo;
+        }
     }
 };
 

@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(WD_THREADS, NR <= 2 ? 2 : 1) window_decode_ker
 template <int NR>
 static cudaError_t window_decode_launch(const WdArgs& w, cudaStream_t stream) {
     const size_t smem = (size_t)WdStages<NR>::value * WD_STAGE;
-    cudaError_t e = set_smem_attrs(window_decode_kernel<NR>, smem);
+    static std::atomic<unsigned long long> done;
+    cudaError_t e = smem_attrs_once(window_decode_kernel<NR>, smem, done);
     if (e != cudaSuccess) return e;
     // Enough CTAs to fill 148 SMs twice over while the cluster stays within
     // the portable 8.

@@ -231,82 +231,89 @@ def decode_attention(qkv: torch.Tensor, *, n_heads: int, n_kv_heads: int, q_norm
 
 
 # ------------------------------------------------- cache operators for streams
-def _whole(x, name: str, low: int = 0) -> int:
-    if isinstance(x, bool) or not isinstance(x, int) or x < low or x > 2**31 - 1:
+_F32, _I32 = torch.float32, torch.int32
+
+
+def _whole(x, name: str, low: int = 0) -> None:
+    if type(x) is not int or x < low or x > 2**31 - 1:
         raise ValueError(f"{name}: must be an int of at least {low}, got {x!r}")
-    return x
 
 
-def _cache_shapes(kv_pool, page_table, page_size: int, n_kv_heads: int | None = None):
-    """(n_pages, kv heads, rows, max_pages) of a paged cache, checked."""
-    _whole(page_size, "page_size", 1)
-    if not isinstance(kv_pool, torch.Tensor) or kv_pool.dim() != 5:
-        raise ValueError("kv_pool: expected a tensor [n_pages, 2, n_kv_heads, page_size, 128]")
-    kvh = kv_pool.shape[2] if n_kv_heads is None else n_kv_heads
-    _check(kv_pool, "kv_pool", (kv_pool.shape[0], 2, kvh, page_size, 128))
-    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
-        raise ValueError("page_table: expected a tensor [rows, max_pages]")
-    _check(page_table, "page_table", tuple(page_table.shape), torch.int32)
-    if kv_pool.shape[0] < 1 or page_table.shape[1] < 1:
-        raise ValueError("kv_pool and page_table must hold at least one page")
-    return kv_pool.shape[0], kvh, page_table.shape[0], page_table.shape[1]
+def _all(device: int, tensors) -> None:
+    """_check of (name, tensor, shape, dtype), and that all lie on one device:
+    a frame of decoding makes a few of these calls, so the usual case costs four
+    attribute reads a tensor."""
+    for name, t, shape, dtype in tensors:
+        try:
+            if t.shape == shape and t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+                continue
+        except AttributeError:
+            pass
+        _check(t, name, shape, dtype)
+        raise ValueError(f"{name}: must be on the device of the others (cuda:{device}), is on {t.device}")
 
 
-def _same_device(**tensors):
-    devices = {t.device for t in tensors.values() if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"{', '.join(tensors)}: must be on one device, got {sorted(map(str, devices))}")
-    return devices.pop()
+def _dims(t, name: str, n: int, what: str):
+    if not isinstance(t, torch.Tensor) or t.dim() != n:
+        raise ValueError(f"{name}: expected a tensor {what}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: must be a CUDA tensor (no CPU path)")
+    return t.shape
+
+
+def _on(device: int, fn, *args):
+    """fn(*args) with ``device`` current, as kernel launches need it."""
+    if torch.cuda.current_device() == device:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 def _cache_attention(name, qkv, n_heads, n_kv_heads, q_norm, k_norm, eps, rope_cos, rope_sin, chunk_start, max_chunk,
                      cached, pos, kv_pool, page_table, page_size, window, sinks, mass, out):
     _whole(n_heads, "n_heads", 1)
     _whole(n_kv_heads, "n_kv_heads", 1)
+    _whole(page_size, "page_size", 1)
     _whole(window, "window")
     _whole(sinks, "sinks")
-    n_pages, _, rows, max_pages = _cache_shapes(kv_pool, page_table, page_size, n_kv_heads)
-    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 2:
-        raise ValueError("qkv: expected a tensor [tokens, (n_heads + 2 n_kv_heads) * 128]")
-    tokens = rows if chunk_start is None else qkv.shape[0]
-    _check(qkv, "qkv", (tokens, (n_heads + 2 * n_kv_heads) * 128))
-    _check(q_norm, "q_norm", (128,))
-    _check(k_norm, "k_norm", (128,))
-    if not isinstance(rope_cos, torch.Tensor) or rope_cos.dim() != 2:
-        raise ValueError("rope_cos: expected a tensor [positions, 64]")
-    for n, t in (("rope_cos", rope_cos), ("rope_sin", rope_sin)):
-        _check(t, n, (rope_cos.shape[0], 64))
-    _check(cached, "cached", (rows,), torch.int32)
-    _check(pos, "pos", (rows,), torch.int32)
+    n_pages = _dims(kv_pool, "kv_pool", 5, "[n_pages, 2, n_kv_heads, page_size, 128]")[0]
+    rows, max_pages = _dims(page_table, "page_table", 2, "[rows, max_pages]")
+    tokens = _dims(qkv, "qkv", 2, "[tokens, (n_heads + 2 n_kv_heads) * 128]")[0]
+    positions = _dims(rope_cos, "rope_cos", 2, "[positions, 64]")[0]
+    device = qkv.get_device()
+    if chunk_start is None:
+        tokens = rows
+    tensors = [("qkv", qkv, (tokens, (n_heads + 2 * n_kv_heads) * 128), _F32),
+               ("kv_pool", kv_pool, (n_pages, 2, n_kv_heads, page_size, 128), _F32),
+               ("page_table", page_table, (rows, max_pages), _I32), ("q_norm", q_norm, (128,), _F32),
+               ("k_norm", k_norm, (128,), _F32), ("rope_cos", rope_cos, (positions, 64), _F32),
+               ("rope_sin", rope_sin, (positions, 64), _F32), ("cached", cached, (rows,), _I32), ("pos", pos, (rows,), _I32)]
     if mass is not None:
-        _check(mass, "mass", (rows, n_kv_heads, max_pages * page_size))
+        tensors.append(("mass", mass, (rows, n_kv_heads, max_pages * page_size), _F32))
     if chunk_start is not None:
         _whole(max_chunk, "max_chunk")
-        _check(chunk_start, "chunk_start", (rows + 1,), torch.int32)
+        tensors.append(("chunk_start", chunk_start, (rows + 1,), _I32))
     if out is not None:
-        _check(out, "out", (tokens, n_heads * 128))
-    device = _same_device(qkv=qkv, q_norm=q_norm, k_norm=k_norm, rope_cos=rope_cos, rope_sin=rope_sin, cached=cached,
-                          pos=pos, kv_pool=kv_pool, page_table=page_table, mass=mass, chunk_start=chunk_start, out=out)
-    with torch.cuda.device(device):
-        if out is None:
-            out = torch.empty((tokens, n_heads * 128), dtype=torch.float32, device=device)
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        heads = (n_heads, n_kv_heads, 128, q_norm.data_ptr(), k_norm.data_ptr(), float(eps), rope_cos.data_ptr(),
-                 rope_sin.data_ptr(), rope_cos.shape[0])
-        cache = (cached.data_ptr(), pos.data_ptr(), kv_pool.data_ptr(), page_table.data_ptr(), max_pages, page_size,
-                 n_pages, window, sinks, ptr(mass))
-        if chunk_start is None:
-            need = _lib.lib().skb_window_decode_workspace(rows, n_heads, max_pages, page_size, window, sinks,
-                                                          int(mass is not None))
-        else:
-            need = _lib.lib().skb_chunk_attention_workspace(tokens, rows, max_chunk, n_heads, n_kv_heads, max_pages,
-                                                            page_size, n_pages, window, sinks, int(mass is not None))
-        work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-        if chunk_start is None:
-            _lib.call(name, qkv.data_ptr(), rows, *heads, *cache, ptr(work), max(need, 0), out.data_ptr(), _stream())
-        else:
-            _lib.call(name, qkv.data_ptr(), tokens, rows, *heads, chunk_start.data_ptr(), max_chunk, *cache, ptr(work),
-                      max(need, 0), out.data_ptr(), _stream())
+        tensors.append(("out", out, (tokens, n_heads * 128), _F32))
+    _all(device, tensors)
+    if n_pages < 1 or max_pages < 1:
+        raise ValueError("kv_pool and page_table must hold at least one page")
+    if out is None:
+        out = qkv.new_empty((tokens, n_heads * 128))
+    with_mass = 0 if mass is None else 1
+    need = 0
+    if chunk_start is not None:
+        need = _lib.lib().skb_chunk_attention_workspace(tokens, rows, max_chunk, n_heads, n_kv_heads, max_pages, page_size,
+                                                        n_pages, window, sinks, with_mass)
+    elif with_mass:
+        need = _lib.lib().skb_window_decode_workspace(rows, n_heads, max_pages, page_size, window, sinks, 1)
+    work = torch.empty(need, dtype=torch.uint8, device=qkv.device) if need > 0 else None
+    chunk = () if chunk_start is None else (chunk_start.data_ptr(), max_chunk)
+    _on(device, _lib.call, name, qkv.data_ptr(), *(() if chunk_start is None else (tokens,)), rows, n_heads, n_kv_heads, 128,
+        q_norm.data_ptr(), k_norm.data_ptr(), float(eps), rope_cos.data_ptr(), rope_sin.data_ptr(), positions, *chunk,
+        cached.data_ptr(), pos.data_ptr(), kv_pool.data_ptr(), page_table.data_ptr(), max_pages, page_size, n_pages, window,
+        sinks, mass.data_ptr() if with_mass else None, None if work is None else work.data_ptr(), max(need, 0),
+        out.data_ptr(), _lib.device_stream_ptr(device))
     return out
 
 
@@ -356,18 +363,20 @@ def evict_cache(mass: torch.Tensor, *, cached: torch.Tensor, kv_pool: torch.Tens
     _whole(budget, "budget", 1)
     _whole(sinks, "sinks")
     _whole(recent, "recent")
-    n_pages, kvh, rows, max_pages = _cache_shapes(kv_pool, page_table, page_size)
-    _check(mass, "mass", (rows, kvh, max_pages * page_size))
-    _check(cached, "cached", (rows,), torch.int32)
-    device = _same_device(mass=mass, cached=cached, kv_pool=kv_pool, page_table=page_table)
-    with torch.cuda.device(device):
-        kept = torch.empty((rows, kvh, budget), dtype=torch.int32, device=device)
-        mass_out = torch.empty_like(mass)
-        cached_out = torch.empty_like(cached)
-        if rows > 0:
-            need = _lib.lib().skb_evict_workspace(rows, kvh)
-            work = torch.empty(need, dtype=torch.uint8, device=device)
-            _lib.call("skb_evict_cache", mass.data_ptr(), cached.data_ptr(), rows, kvh, 128, kv_pool.data_ptr(),
-                      page_table.data_ptr(), max_pages, page_size, n_pages, budget, sinks, recent, kept.data_ptr(),
-                      mass_out.data_ptr(), cached_out.data_ptr(), work.data_ptr(), need, _stream())
+    _whole(page_size, "page_size", 1)
+    n_pages, _, kvh = _dims(kv_pool, "kv_pool", 5, "[n_pages, 2, n_kv_heads, page_size, 128]")[:3]
+    rows, max_pages = _dims(page_table, "page_table", 2, "[rows, max_pages]")
+    device = kv_pool.get_device()
+    _all(device, (("kv_pool", kv_pool, (n_pages, 2, kvh, page_size, 128), _F32),
+                  ("page_table", page_table, (rows, max_pages), _I32), ("cached", cached, (rows,), _I32),
+                  ("mass", mass, (rows, kvh, max_pages * page_size), _F32)))
+    if n_pages < 1 or max_pages < 1:
+        raise ValueError("kv_pool and page_table must hold at least one page")
+    kept = cached.new_empty((rows, kvh, budget))
+    mass_out = torch.empty_like(mass)
+    cached_out = torch.empty_like(cached)
+    if rows > 0:
+        _on(device, _lib.call, "skb_evict_cache", mass.data_ptr(), cached.data_ptr(), rows, kvh, 128, kv_pool.data_ptr(),
+            page_table.data_ptr(), max_pages, page_size, n_pages, budget, sinks, recent, kept.data_ptr(),
+            mass_out.data_ptr(), cached_out.data_ptr(), _lib.device_stream_ptr(device))
     return kept, mass_out, cached_out

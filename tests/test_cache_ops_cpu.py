@@ -23,8 +23,7 @@ CHUNK = dict(qkv=A, tokens=5, rows=2, n_heads=16, n_kv_heads=8, head_dim=128, q_
              page_size=16, n_pages=9, window=0, sinks=0, mass=None, work=A, work_bytes=1 << 40, out=A, stream=None)
 DECODE = {k: v for k, v in CHUNK.items() if k not in ("tokens", "chunk_start", "max_chunk")}
 EVICT = dict(mass=A, cached=A, rows=2, n_kv_heads=8, head_dim=128, kv_pool=A, page_table=A, max_pages=4, page_size=16,
-             n_pages=9, budget=32, sinks=4, recent=8, kept=A, mass_out=2 * A, cached_out=2 * A, work=A, work_bytes=1 << 40,
-             stream=None)
+             n_pages=9, budget=32, sinks=4, recent=8, kept=A, mass_out=2 * A, cached_out=2 * A, stream=None)
 
 ATTN_BAD = [("q_norm", None), ("k_norm", None), ("rope_cos", None), ("rope_sin", None), ("cached", None), ("pos", None),
             ("kv_pool", None), ("page_table", None), ("qkv", None), ("out", None), ("head_dim", 64), ("n_heads", 0),
@@ -57,11 +56,11 @@ def test_window_decode_attention_with_mass_needs_its_workspace(lib, change):
 
 
 @pytest.mark.parametrize("change", [
-    {n: None} for n in ("mass", "cached", "kv_pool", "page_table", "kept", "mass_out", "cached_out", "work")] + [
+    {n: None} for n in ("mass", "cached", "kv_pool", "page_table", "kept", "mass_out", "cached_out")] + [
     dict(head_dim=64), dict(rows=-1), dict(rows=65536), dict(n_kv_heads=0), dict(max_pages=0), dict(max_pages=1 << 27),
     dict(page_size=24), dict(page_size=0), dict(n_pages=0), dict(budget=0), dict(sinks=-1), dict(recent=-1),
     dict(sinks=30, recent=3), dict(sinks=2**31 - 1, recent=2**31 - 1), dict(mass_out=A), dict(cached_out=A),
-    dict(kv_pool=A + 4), dict(work_bytes=4)])
+    dict(kv_pool=A + 4)])
 def test_evict_cache_refuses(lib, change):
     args = dict(EVICT, **change)
     assert lib.lib().skb_evict_cache(*args.values()) == lib.SKB_ERR_ARG
@@ -84,7 +83,6 @@ def test_workspace_sizes(lib):
     assert L.skb_window_decode_workspace(2, 16, 4, 16, 0, 0, 1) == 2 * 16 * 64 * 4
     assert L.skb_window_decode_workspace(2, 16, 4, 16, 8, 4, 1) == 2 * 16 * 12 * 4
     assert L.skb_window_decode_workspace(2, 16, 0, 16, 8, 4, 1) == -1
-    assert L.skb_evict_workspace(-1, 8) == -1
     # sizes that pass 32 bits are counted in 64
     big = L.skb_chunk_attention_workspace(1 << 20, 1, 1 << 20, 16, 8, 1 << 14, 64, 1 << 14, 0, 0, 0)
     assert big >= (1 << 20) * 16 * 512 + (1 << 20) * 8 * 1024
