@@ -331,12 +331,30 @@ __global__ void __launch_bounds__(WD_THREADS, NR <= 2 ? 2 : 1) window_decode_ker
     }
     float* mass = a.mass + ((long long)r * KVH + g) * cap;
     const int end = s == C - 1 ? nv + 1 : ie;
-    for (int i = ib + tid; i < end; i += WD_THREADS) {
-        float sum = 0.f;
+    // eight slots a thread at a time, all of a batch's loads before its stores:
+    // one after the other they cost 14 of 109 us at 2 x 32k slots
+    constexpr int U = 8;
+    for (int i0 = ib + tid; i0 < end; i0 += WD_THREADS * U) {
+        float sc[U][NR], old[U];
 #pragma unroll
-        for (int h = 0; h < NR; ++h) sum += exp2_fast(scores[(long long)i * NR + h] - fm[h]) * fi[h];
-        const int slot = i < ns ? i : w0 + i - ns;
-        mass[slot] = i == nv ? sum : mass[slot] + sum;
+        for (int k = 0; k < U; ++k) {
+            const int i = i0 + k * WD_THREADS;
+            old[k] = 0.f;
+            if (i < end) {
+#pragma unroll
+                for (int h = 0; h < NR; ++h) sc[k][h] = scores[(long long)i * NR + h];
+                if (i != nv) old[k] = mass[i < ns ? i : w0 + i - ns];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int i = i0 + k * WD_THREADS;
+            if (i >= end) continue;
+            float sum = 0.f;
+#pragma unroll
+            for (int h = 0; h < NR; ++h) sum += exp2_fast(sc[k][h] - fm[h]) * fi[h];
+            mass[i < ns ? i : w0 + i - ns] = old[k] + sum;
+        }
     }
 }
 
