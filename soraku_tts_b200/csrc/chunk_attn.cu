@@ -281,7 +281,7 @@ struct CaSmem {
     float mx[2][CA_PARTS][128], ex[2][CA_PARTS][128];  // a row part's largest score and value exponent
     float m[128], l[CA_PARTS][128];      // this split's statistics (sums of row parts)
     float E[2];                          // running exponent of the values
-    uint64_t q_landed, q_full, full[CA_STAGES], empty[CA_STAGES], s_full[2], p_full, pv_done[2], meta_full[2], o_full;
+    uint64_t q_landed, q_full, full[CA_STAGES], empty[CA_STAGES], s_full[2], p_full[2], pv_done[2], o_free, meta_full[2], o_full;
     // what the CTA works on
     TileList list;
     int k0, nt;          // its key tiles: list entries [k0, k0 + nt)
@@ -299,6 +299,17 @@ static_assert(128 * CA_OUT_LD * 4 <= CA_STAGES * 2 * UT_BYTES, "the staged outpu
 // The warps that share a quadrant's 32 rows.
 __device__ __forceinline__ void softmax_sync() {
     asm volatile("bar.sync %0, %1;" ::"r"(2 + ((threadIdx.x >> 5) & 3)), "n"(32 * CA_PARTS) : "memory");
+}
+
+// The same; whether any of their threads says so.
+__device__ __forceinline__ bool softmax_any(bool mine) {
+    uint32_t any;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.or.pred p, %2, %3, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(any)
+        : "r"((uint32_t)mine), "r"(2 + ((threadIdx.x >> 5) & 3)), "n"(32 * CA_PARTS)
+        : "memory");
+    return any != 0;
 }
 
 __device__ __forceinline__ float4 ld_peer4(uint32_t local, uint32_t rank) {
@@ -341,7 +352,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     if (tid == 0) {
         mbar_init(&sm.q_landed, 1);
         mbar_init(&sm.q_full, CA_SOFTMAX_WARPS);
-        mbar_init(&sm.p_full, CA_SOFTMAX_WARPS);
+        mbar_init(&sm.o_free, CA_SOFTMAX_WARPS);
         mbar_init(&sm.o_full, 1);
         for (int b = 0; b < CA_STAGES; ++b) {
             mbar_init(&sm.full[b], 1);
@@ -349,6 +360,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&sm.s_full[b], 1);
+            mbar_init(&sm.p_full[b], CA_SOFTMAX_WARPS);
             mbar_init(&sm.pv_done[b], 1);
             mbar_init(&sm.meta_full[b], 1);
         }
@@ -427,7 +439,8 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             bool go = true;
             for (int i = 0; i < nt && go; ++i) {  // O = P_i V_i
                 const int n = i + 1 < nt ? 2 * i + 2 : 2 * nt - 1, s = n % CA_STAGES;
-                go = ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort) && ut_wait(&sm.p_full, i & 1, abort);
+                go = ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort) && ut_wait(&sm.p_full[i & 1], (i >> 1) & 1, abort) &&
+                     (i == 0 || ut_wait(&sm.o_free, (i - 1) & 1, abort));
                 if (!go) break;
                 ut_fence_after();
                 ut_mma_pv(tmem + CA_TM_O, tmem + (i & 1) * 128, smem_u32(sm.stage[s]));
@@ -547,29 +560,11 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                     }
                 }
             }
-            sm.mx[b][part][row] = mx;
-            if (!whole) sm.ex[b][part][row] = ex;
-            softmax_sync();
-            // The running maximum follows only when it is passed by 2^8, the
-            // running exponent with 3 bits to spare: weights stay below 2^8,
-            // scaled ones below 2^14.  In whole tiles the exponent is every row's.
             float E_new = E;
-            if (whole) {
-                E_new = sm.E[b];
-            } else {
-#pragma unroll
-                for (int q = 0; q < CA_PARTS; ++q) ex = fmaxf(ex, sm.ex[b][q][row]);
-                if (ex > E) E_new = ex + 3.f;
-            }
-#pragma unroll
-            for (int q = 0; q < CA_PARTS; ++q) mx = fmaxf(mx, sm.mx[b][q][row]);
-            const float m_new = mx > m + 8.f && hi >= 0 ? mx : m;
-            const float f_l = exp2_fast(m - m_new), f_new = f_l * exp2_fast(E - E_new);
-            m = m_new;
-            E = E_new;
+            float2 sum;
             // scores -> weights, scaled by their values' exponents, as hi | lo over the scores
-            float2 sum = make_float2(0.f, 0.f);
             auto weigh = [&](auto whole_tile) {
+                sum = make_float2(0.f, 0.f);
                 const float2 mm = make_float2(-m, -m);
 #pragma unroll
                 for (int ch = 0; ch < CA_W / 16; ++ch) {
@@ -587,8 +582,8 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                             if (!(bits & 1u)) p.x = 0.f;
                             if (!(bits & 2u)) p.y = 0.f;
                             sum = add2(sum, p);
-                            p.x = (bits & 1u) ? p.x * exp2_fast(v.x - E + 6.f) : 0.f;
-                            p.y = (bits & 2u) ? p.y * exp2_fast(v.y - E + 6.f) : 0.f;
+                            p.x = (bits & 1u) ? p.x * exp2_fast(v.x - E_new + 6.f) : 0.f;
+                            p.y = (bits & 2u) ? p.y * exp2_fast(v.y - E_new + 6.f) : 0.f;
                         }
                         split2(p, ph[q], pl[q]);
                     }
@@ -596,19 +591,45 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                     ut_st8(st + ch * 16 + 8, pl);
                 }
             };
+            // The running maximum follows only when it is passed by 2^8, the
+            // running exponent with 3 bits to spare: weights stay below 2^8,
+            // scaled ones below 2^14.  In a whole tile the exponent is every
+            // row's, and where no thread passed its maximum the row's parts
+            // need not tell one another theirs.
+            float f_l = 1.f;
+            if (whole) E_new = sm.E[b];
+            if (!whole || i == 0 || softmax_any(mx > m + 8.f && hi >= 0)) {
+                sm.mx[b][part][row] = mx;
+                if (!whole) sm.ex[b][part][row] = ex;
+                softmax_sync();
+                if (!whole) {
+#pragma unroll
+                    for (int q = 0; q < CA_PARTS; ++q) ex = fmaxf(ex, sm.ex[b][q][row]);
+                    if (ex > E) E_new = ex + 3.f;
+                }
+#pragma unroll
+                for (int q = 0; q < CA_PARTS; ++q) mx = fmaxf(mx, sm.mx[b][q][row]);
+                const float m_new = mx > m + 8.f && hi >= 0 ? mx : m;
+                f_l = exp2_fast(m - m_new);
+                m = m_new;
+            }
             if (whole) weigh(std::true_type{});
             else weigh(std::false_type{});
             l = fmaf(l, f_l, sum.x + sum.y);
+            ut_wait_st();
+            ut_fence_before();
+            __syncwarp();
+            if (lane == 0) ut_arrive(&sm.p_full[b]);
             if (i > 0) {  // the last tile's product, before this one's takes its place
                 ut_wait(&sm.pv_done[b ^ 1], ((i - 1) >> 1) & 1, abort);
                 ut_fence_after();
                 gather();
+                ut_fence_before();
+                __syncwarp();
+                if (lane == 0) ut_arrive(&sm.o_free);
             }
-            f_o = i == 0 ? 0.f : f_new;
-            ut_wait_st();
-            ut_fence_before();
-            __syncwarp();
-            if (lane == 0) ut_arrive(&sm.p_full);
+            f_o = i == 0 ? 0.f : f_l * exp2_fast(E - E_new);
+            E = E_new;
         }
         // ---- this split's output over its own sum, staged in shared memory
         if (nt > 0) {
