@@ -264,6 +264,7 @@ struct TileList {
 // tile's output is added up in registers.
 constexpr int CA_PARTS = 4;
 constexpr int CA_W = 128 / CA_PARTS;  // a thread's keys, and its output columns
+static_assert(CA_W == 32, "a part is a warp's width");
 constexpr int CA_SOFTMAX_WARPS = 4 * CA_PARTS, CA_WARP_M = CA_SOFTMAX_WARPS, CA_WARP_P = CA_WARP_M + 1,
               CA_WARP_E = CA_WARP_M + 2, CA_WARP_O = CA_WARP_M + 3;
 constexpr int CA_THREADS = 32 * (CA_SOFTMAX_WARPS + 4);
@@ -281,6 +282,8 @@ struct CaSmem {
     float mx[2][CA_PARTS][128], ex[2][CA_PARTS][128];  // a row part's largest score and value exponent
     float m[128], l[CA_PARTS][128];      // this split's statistics (sums of row parts)
     float E[2];                          // running exponent of the values
+    float vtop[2][CA_PARTS];             // largest exponent of a part's values
+    float own_vg[CA_SOFTMAX_WARPS][CA_W];  // a warp's factors in a tile that is not whole
     uint64_t q_landed, q_full, full[CA_STAGES], empty[CA_STAGES], s_full[2], p_full[2], pv_done[2], o_free, meta_full[2], o_full;
     // what the CTA works on
     TileList list;
@@ -289,6 +292,8 @@ struct CaSmem {
     int own[128];        // a row's slot; -1: no query
     int token0;          // token of the first query
     long long tile_at;   // query tile in the workspace
+    long long base;      // the row's key tiles there
+    int a1, b0;          // RowTiles of the row
     uint32_t tmem;
     int abort;
 };
@@ -374,6 +379,9 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         sm.live = nq * c.n_rep;
         sm.token0 = x.b + i0;
         sm.tile_at = chunk_tile(c, x, r, t) * a.kv.KVH + g;
+        sm.base = base;
+        sm.a1 = rt.a1;
+        sm.b0 = rt.b0;
     }
     if (tid < 128) {
         const int q = tid / c.n_rep;
@@ -386,6 +394,11 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     const uint32_t tmem = sm.tmem;
     const int nt = sm.nt;
     volatile int* abort = &sm.abort;
+    // where tile i of this CTA's list lies in the workspace
+    auto tile_of = [&](int i) {
+        const int tile = sm.list.tile(sm.k0 + i);
+        return (sm.base + (tile < sm.a1 ? tile : sm.a1 + tile - sm.b0)) * a.kv.KVH + blockIdx.y;
+    };
     pdl_wait();
     if (c.lse) pdl_trigger();  // chunk_mass follows
 
@@ -396,7 +409,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                 const int s = n % CA_STAGES;
                 if (n == CA_STAGES - 1 && !ut_wait(&sm.q_full, 0, abort)) return false;  // the queries were there
                 if (n >= CA_STAGES && !ut_wait(&sm.empty[s], ((n - CA_STAGES) / CA_STAGES) & 1, abort)) return false;
-                const long long at = ((base + rt.index(sm.list.tile(sm.k0 + i))) * a.kv.KVH + g) * 2 + value;
+                const long long at = tile_of(i) * 2 + value;
                 mbar_expect_tx(&sm.full[s], 2 * UT_BYTES);
                 bulk_g2s(sm.stage[s], c.kvtiles + at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.full[s]);
                 ++n;
@@ -455,9 +468,15 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         float E = UT_POISON_E;
         for (int i = 0; i < nt; ++i) {
             const int b = i & 1;
-            const float* at = c.meta + ((base + rt.index(sm.list.tile(sm.k0 + i))) * a.kv.KVH + g) * 256;
+            const float* at = c.meta + tile_of(i) * 256;
             const float4 k = reinterpret_cast<const float4*>(at)[lane], v = reinterpret_cast<const float4*>(at)[32 + lane];
-            const float top = warp_max(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));  // NaN aside
+            // largest exponents (NaN aside): of each 32 values, of all
+            float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+            top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+            top = fmaxf(top, __shfl_xor_sync(FULL, top, 4));
+            const float part_top = top;
+            top = warp_max(top);
             // the softmax of tile i - 2 is done with the buffers
             if (i >= 2 && !ut_wait(&sm.pv_done[b], ((i - 2) >> 1) & 1, abort)) break;
             if (sm.k0 + i < sm.list.full && top > E) E = top + 3.f;  // 3 bits to spare: it rarely moves
@@ -466,6 +485,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             reinterpret_cast<float4*>(sm.vg[b])[lane] = make_float4(exp2_fast(v.x - E + 6.f), exp2_fast(v.y - E + 6.f),
                                                                     exp2_fast(v.z - E + 6.f), exp2_fast(v.w - E + 6.f));
             if (lane == 0) sm.E[b] = E;
+            if ((lane & 7) == 0) sm.vtop[b][lane >> 3] = part_top;
             __syncwarp();
             if (lane == 0) ut_arrive(&sm.meta_full[b]);
         }
@@ -522,7 +542,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             const float4* kc = reinterpret_cast<const float4*>(sm.kc[b] + part * CA_W);
             const float* ve = sm.ve[b] + part * CA_W;
             // a row sees slots <= hi that are > lo, or < sinks
-            const int hi = sm.own[row], lo = a.window > 0 ? hi - a.window : -1;
+            const int hi = sm.own[row], lo = a.window > 0 ? max(-1, hi - a.window) : -1;
             ut_wait(&sm.meta_full[b], (i >> 1) & 1, abort);
             ut_wait(&sm.s_full[b], (i >> 1) & 1, abort);
             ut_fence_after();
@@ -530,40 +550,46 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             // see, the largest exponent among the values this query sees)
             float2 s[CA_W / 2];
             float mx = CO_LOW, ex = UT_POISON_E;
-            uint32_t seen[CA_W / 32];
-#pragma unroll
-            for (int ch = 0; ch < CA_W / 32; ++ch) {
+            uint32_t seen = FULL;  // bit per key of the part
+            if (!whole) {
+                const auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? FULL : (1u << n) - 1u; };
+                const int at = base_slot - 1;  // keys base_slot .. hi, less those <= lo that are no sinks
+                seen = below(hi - at) & (~below(lo - at) | below(a.sinks - base_slot));
+            }
+            {
                 uint32_t w[32];
-                ut_ld32(st + ch * 32, w);
+                ut_ld32(st, w);
                 ut_wait_ld();
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    const float4 f = kc[ch * 8 + q];
-                    s[ch * 16 + 2 * q] = mul2(make_float2(__uint_as_float(w[4 * q]), __uint_as_float(w[4 * q + 1])),
-                                              make_float2(f.x, f.y));
-                    s[ch * 16 + 2 * q + 1] = mul2(make_float2(__uint_as_float(w[4 * q + 2]), __uint_as_float(w[4 * q + 3])),
-                                                  make_float2(f.z, f.w));
+                    const float4 f = kc[q];
+                    s[2 * q] = mul2(make_float2(__uint_as_float(w[4 * q]), __uint_as_float(w[4 * q + 1])),
+                                    make_float2(f.x, f.y));
+                    s[2 * q + 1] = mul2(make_float2(__uint_as_float(w[4 * q + 2]), __uint_as_float(w[4 * q + 3])),
+                                        make_float2(f.z, f.w));
                 }
-                if (whole) {
+            }
+            if (__all_sync(FULL, seen == FULL)) {
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) mx = fmaxf(fmaxf(mx, s[ch * 16 + q].x), s[ch * 16 + q].y);
-                } else {
-                    seen[ch] = 0;
+                for (int q = 0; q < 16; ++q) mx = fmaxf(fmaxf(mx, s[q].x), s[q].y);
+                ex = sm.vtop[b][part];
+            } else {
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) {
-                        const int j = base_slot + ch * 32 + q;
-                        if (j <= hi && (j > lo || j < a.sinks)) {
-                            seen[ch] |= 1u << q;
-                            mx = fmaxf(mx, (q & 1) ? s[ch * 16 + (q >> 1)].y : s[ch * 16 + (q >> 1)].x);
-                            ex = fmaxf(ex, ve[ch * 32 + q]);
-                        }
-                    }
+                for (int q = 0; q < 16; ++q) {  // what is not seen weighs nothing from here on
+                    if (!(seen >> (2 * q) & 1u)) s[q].x = -INFINITY;
+                    if (!(seen >> (2 * q + 1) & 1u)) s[q].y = -INFINITY;
+                    mx = fmaxf(fmaxf(mx, s[q].x), s[q].y);
+                    if (seen >> (2 * q) & 1u) ex = fmaxf(ex, ve[2 * q]);
+                    if (seen >> (2 * q + 1) & 1u) ex = fmaxf(ex, ve[2 * q + 1]);
                 }
             }
             float E_new = E;
             float2 sum;
-            // scores -> weights, scaled by their values' exponents, as hi | lo over the scores
-            auto weigh = [&](auto whole_tile) {
+            // Scores -> weights, scaled by their values' exponents, as hi | lo
+            // over the scores.  `vg`: the factors 2^(exponent - E + 6), if one
+            // set holds for the warp; else (EACH) every thread forms its own.
+            // MASKED: some keys are not seen, whatever their factors are.
+            auto weigh = [&](const float2* vg, auto masked, auto each) {
                 sum = make_float2(0.f, 0.f);
                 const float2 mm = make_float2(-m, -m);
 #pragma unroll
@@ -573,17 +599,13 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                     for (int q = 0; q < 8; ++q) {
                         float2 p = add2(s[ch * 8 + q], mm);
                         p = make_float2(exp2_fast(p.x), exp2_fast(p.y));
-                        if (decltype(whole_tile)::value) {
-                            sum = add2(sum, p);
-                            p = mul2(p, reinterpret_cast<const float2*>(sm.vg[b] + part * CA_W)[ch * 8 + q]);
-                        } else {
-                            const uint32_t bits = seen[ch >> 1] >> ((ch & 1) * 16 + 2 * q);
-                            const float2 v = reinterpret_cast<const float2*>(ve)[ch * 8 + q];
-                            if (!(bits & 1u)) p.x = 0.f;
-                            if (!(bits & 2u)) p.y = 0.f;
-                            sum = add2(sum, p);
-                            p.x = (bits & 1u) ? p.x * exp2_fast(v.x - E_new + 6.f) : 0.f;
-                            p.y = (bits & 2u) ? p.y * exp2_fast(v.y - E_new + 6.f) : 0.f;
+                        sum = add2(sum, p);
+                        float2 f = vg[ch * 8 + q];
+                        if (decltype(each)::value) f = make_float2(exp2_fast(f.x - E_new + 6.f), exp2_fast(f.y - E_new + 6.f));
+                        p = mul2(p, f);
+                        if (decltype(masked)::value) {
+                            if (!(seen >> (ch * 16 + 2 * q) & 1u)) p.x = 0.f;
+                            if (!(seen >> (ch * 16 + 2 * q + 1) & 1u)) p.y = 0.f;
                         }
                         split2(p, ph[q], pl[q]);
                     }
@@ -613,8 +635,15 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                 f_l = exp2_fast(m - m_new);
                 m = m_new;
             }
-            if (whole) weigh(std::true_type{});
-            else weigh(std::false_type{});
+            if (whole) {
+                weigh(reinterpret_cast<const float2*>(sm.vg[b] + part * CA_W), std::false_type{}, std::false_type{});
+            } else if (__all_sync(FULL, E_new == __shfl_sync(FULL, E_new, 0))) {
+                sm.own_vg[warp][lane] = exp2_fast(ve[lane] - E_new + 6.f);
+                __syncwarp();
+                weigh(reinterpret_cast<const float2*>(sm.own_vg[warp]), std::true_type{}, std::false_type{});
+            } else {
+                weigh(reinterpret_cast<const float2*>(ve), std::true_type{}, std::true_type{});
+            }
             l = fmaf(l, f_l, sum.x + sum.y);
             ut_wait_st();
             ut_fence_before();
@@ -662,39 +691,46 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         ut_fence_after();
         ut_free(tmem);
     }
-    // ---- join the splits: CTA z of the cluster takes a part of the rows
+    // ---- join the splits: CTA z of the cluster takes a part of the rows.  The
+    // weights of all rows first, then all outputs: two trips to the peers' memory
+    // in all, where a warp that took row after row made two for each.
     if (splits > 1)
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    const int ra = z * sm.live / splits, rb = (z + 1) * sm.live / splits;
+    const int part = blockIdx.x % splits;
+    const int ra = part * sm.live / splits, rb = (part + 1) * sm.live / splits;
+    float (*weight)[128] = sm.mx[0];  // [split][row]; the maxima are done with
+    static_assert(2 * CA_PARTS >= CA_MAX_SPLITS, "weights fit the maxima's place");
+    for (int i = tid; i < (rb - ra) * splits; i += CA_THREADS) {
+        const int row = ra + i / splits, p = i % splits;
+        float M = CO_LOW, L = 0.f, mine = 0.f;
+#pragma unroll 4
+        for (int q = 0; q < splits; ++q) {
+            const float m = ld_peer(&sm.m[row], q), l = ld_peer(&sm.l[0][row], q);
+            const float up = fmaxf(M, m), f = exp2_fast(M - up), w = l * exp2_fast(m - up);
+            mine = q == p ? w : mine * f;
+            L = fmaf(L, f, w);
+            M = up;
+        }
+        weight[p][row] = mine / L;  // not a number where a wait ran out
+        if (c.lse && p == 0) c.lse[sm.tile_at * 128 + row] = M + log2f(L);
+    }
+    __syncthreads();
     const uint32_t stage = smem_u32(sm.stage);
-    for (int q = warp; q < rb - ra; q += CA_THREADS / 32) {  // a warp per row
-        const int row = ra + q;
-        float4 o;
-        float M = CO_LOW, L = 0.f;
-        const uint32_t at = stage + (uint32_t)(row * CA_OUT_LD + 4 * lane) * 4u;
-        if (splits == 1) {
-            o = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.stage) + row * CA_OUT_LD + 4 * lane);
-            M = sm.m[row];
-            L = sm.l[0][row];
-            if (L != L) o.x = o.y = o.z = o.w = L;
-        } else {
-            o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int p = 0; p < splits; ++p) M = fmaxf(M, ld_peer(&sm.m[row], p));
-            for (int p = 0; p < splits; ++p) {
-                const float w = ld_peer(&sm.l[0][row], p) * exp2_fast(ld_peer(&sm.m[row], p) - M);
-                const float4 y = ld_peer4(at, p);
-                L += w;
-                o.x = fmaf(w, y.x, o.x);
-                o.y = fmaf(w, y.y, o.y);
-                o.z = fmaf(w, y.z, o.z);
-                o.w = fmaf(w, y.w, o.w);
-            }
-            const float inv = 1.f / L;
-            o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    for (int i = tid; i < (rb - ra) * 32; i += CA_THREADS) {
+        const int row = ra + (i >> 5), col = i & 31;
+        const int at = row * CA_OUT_LD + 4 * col;
+        float4 o = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.stage) + at);
+        const float own = weight[part][row];
+        o = make_float4(o.x * own, o.y * own, o.z * own, o.w * own);
+#pragma unroll 2
+        for (int q = 1; q < splits; ++q) {
+            const int p = part + q < splits ? part + q : part + q - splits;
+            const float4 y = ld_peer4(stage + (uint32_t)at * 4u, p);
+            const float w = weight[p][row];
+            o = make_float4(fmaf(w, y.x, o.x), fmaf(w, y.y, o.y), fmaf(w, y.z, o.z), fmaf(w, y.w, o.w));
         }
         const long long tok = sm.token0 + row / c.n_rep;
-        reinterpret_cast<float4*>(a.out)[(tok * a.H + g * c.n_rep + row % c.n_rep) * 32 + lane] = o;
-        if (c.lse && lane == 0) c.lse[sm.tile_at * 128 + row] = M + log2f(L);
+        reinterpret_cast<float4*>(a.out)[(tok * a.H + blockIdx.y * c.n_rep + row % c.n_rep) * 32 + col] = o;
     }
     if (splits > 1)  // peers still read this CTA's shared memory
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
