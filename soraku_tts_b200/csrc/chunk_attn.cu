@@ -738,25 +738,29 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
 
 // -------------------------------------------------------------- chunk_mass
 // One CTA per (key tile, kv head, row): its keys are the rows of the products; the query tiles that see any of them pass through
-// as columns.  A thread owns a slot and half of the columns, so weights are added in
+// as columns.  A thread owns a slot and a quarter of the columns, so weights are added in
 // a fixed order without atomics:
 //   sum over columns of exp2(s - lse)
-constexpr int CM_SUM_WARPS = 8;                             // two per TMEM quadrant
+constexpr int CM_PARTS = 4;                                 // threads per slot
+constexpr int CM_SUM_WARPS = 4 * CM_PARTS;
+constexpr int CM_W = 128 / CM_PARTS;                        // a thread's columns
+constexpr int CM_LSE = 4;                                   // tiles' lse held
 constexpr int CM_THREADS = 32 * (CM_SUM_WARPS + 1);
 constexpr int CM_MMA_WARP = CM_SUM_WARPS;
 
 struct CmSmem {
     unsigned char k[2 * UT_BYTES];
     unsigned char q[2][2 * UT_BYTES];
-    float lse[2][128];
+    float lse[CM_LSE][128];
     float kc[128];
-    float part[2][128];
-    int own[CM_SUM_WARPS][64];  // slots of the queries in a warp's columns; -1: none
-    uint64_t k_full, q_full[2], q_empty[2], s_full[2], s_empty[2];
+    float part[CM_PARTS][128];
+    int own[CM_SUM_WARPS][CM_W];  // slots of the queries in a warp's columns; -1: none
+    uint64_t k_full, q_full[2], q_empty[2], s_full[2], s_empty[2], lse_full[CM_LSE];
     uint32_t tmem;
     int abort;
 };
 constexpr size_t CM_SMEM = sizeof(CmSmem) + 1024;
+static_assert(CM_W == 32, "a part is a warp's width");
 static_assert(CM_SMEM <= 227 * 1024, "shared memory of one CTA");
 
 __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkArgs c) {
@@ -791,6 +795,7 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
             mbar_init(&sm.s_full[b], 1);
             mbar_init(&sm.s_empty[b], CM_SUM_WARPS);
         }
+        for (int b = 0; b < CM_LSE; ++b) mbar_init(&sm.lse_full[b], 1);
         mbar_fence_init();
         sm.abort = 0;
     }
@@ -806,9 +811,10 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
             const long long at0 = chunk_tile(c, x, r, t0) * a.kv.KVH + g;
             auto fetch = [&](int i) {
                 const long long at = at0 + (long long)i * a.kv.KVH;
-                mbar_expect_tx(&sm.q_full[i & 1], 2 * UT_BYTES + 512);
+                mbar_expect_tx(&sm.q_full[i & 1], 2 * UT_BYTES);
                 bulk_g2s(sm.q[i & 1], c.qtiles + at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.q_full[i & 1]);
-                bulk_g2s(sm.lse[i & 1], c.lse + at * 128, 512, &sm.q_full[i & 1]);
+                mbar_expect_tx(&sm.lse_full[i % CM_LSE], 512);
+                bulk_g2s(sm.lse[i % CM_LSE], c.lse + at * 128, 512, &sm.lse_full[i % CM_LSE]);
             };
             const long long kat = ((row_at + blockIdx.x) * a.kv.KVH + g) * 2;
             mbar_expect_tx(&sm.k_full, 2 * UT_BYTES + 512);
@@ -826,11 +832,10 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
                 ut_mma_qk(tmem + (i & 1) * 128, smem_u32(sm.k), smem_u32(sm.q[i & 1]));
                 ut_commit(&sm.q_empty[i & 1]);
                 ut_commit(&sm.s_full[i & 1]);
-                // the other buffer's tile: its products are done and its
-                // sums read (they use the tile's lse) before it is refilled
+                // the other buffer's products are done; the lse that tile i - 3
+                // left is read, since its sums were waited for above
                 if (i >= 1 && i + 1 < nt) {
-                    go = ut_wait(&sm.q_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, abort) &&
-                         ut_wait(&sm.s_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, abort);
+                    go = ut_wait(&sm.q_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, abort);
                     if (go) {
                         fetch(i + 1);
                         ++fetched;
@@ -840,14 +845,17 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
             // leave nothing in flight: the copies asked for, the products issued
             if (i < nt) mbar_wait(&sm.k_full, 0, nullptr);
             if (i < nt)
-                for (int f = max(0, fetched - 2); f < fetched; ++f) mbar_wait(&sm.q_full[f & 1], (f >> 1) & 1, nullptr);
+                for (int f = max(0, fetched - 2); f < fetched; ++f) {
+                    mbar_wait(&sm.q_full[f & 1], (f >> 1) & 1, nullptr);
+                    mbar_wait(&sm.lse_full[f % CM_LSE], (f / CM_LSE) & 1, nullptr);
+                }
         }
         __syncwarp();
     } else {
         ut_wait(&sm.k_full, 0, abort);
-        const int key = 32 * (warp & 3) + lane, half = warp >> 2, slot = base + key;
+        const int key = 32 * (warp & 3) + lane, part = warp >> 2, slot = base + key;
         const float kc = sm.kc[key];
-        const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + half * 64;
+        const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + part * CM_W;
         // queries at slots >= this do not see the slot
         const unsigned upto = a.window == 0 || slot < a.sinks ? 0x7fffffffu : (unsigned)slot + (unsigned)a.window;
         float2 sum = make_float2(0.f, 0.f);
@@ -859,22 +867,18 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
             const bool whole = nq * c.n_rep == 128 && first >= base + 127 &&
                                (a.window == 0 || first + nq - 1 - base < a.window || base + 128 <= a.sinks);
             if (!whole) {  // one division a column, not one a weight
-                for (int col = lane; col < 64; col += 32) {
-                    const int qi = (half * 64 + col) / c.n_rep;
-                    sm.own[warp][col] = qi < nq ? first + qi : -1;
-                }
+                const int qi = (part * CM_W + lane) / c.n_rep;
+                sm.own[warp][lane] = qi < nq ? first + qi : -1;
                 __syncwarp();
             }
             if (!ut_wait(&sm.s_full[b], (i >> 1) & 1, abort)) break;
-            // also waited for: the lse that came with the tile
-            if (!ut_wait(&sm.q_full[b], (i >> 1) & 1, abort)) break;
+            if (!ut_wait(&sm.lse_full[i % CM_LSE], (i / CM_LSE) & 1, abort)) break;
             ut_fence_after();
-#pragma unroll 1
-            for (int ch = 0; ch < 2; ++ch) {
+            {
                 uint32_t s[32];
-                ut_ld32(lane_tm + b * 128 + ch * 32, s);
+                ut_ld32(lane_tm + b * 128, s);
                 ut_wait_ld();
-                const float4* lse = reinterpret_cast<const float4*>(sm.lse[b] + half * 64 + ch * 32);
+                const float4* lse = reinterpret_cast<const float4*>(sm.lse[i % CM_LSE] + part * CM_W);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const float4 f = lse[q];
@@ -885,7 +889,7 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
                                     make_float2(-f.z, -f.w));
                     float p[4] = {exp2_fast(u.x), exp2_fast(u.y), exp2_fast(v.x), exp2_fast(v.y)};
                     if (!whole) {
-                        const int4 own = reinterpret_cast<const int4*>(sm.own[warp])[ch * 8 + q];
+                        const int4 own = reinterpret_cast<const int4*>(sm.own[warp])[q];
                         const int w[4] = {own.x, own.y, own.z, own.w};
 #pragma unroll
                         for (int y = 0; y < 4; ++y)
@@ -898,7 +902,7 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
             __syncwarp();  // also: the slots in sm.own are read
             if (lane == 0) ut_arrive(&sm.s_empty[b]);
         }
-        sm.part[half][key] = sum.x + sum.y;
+        sm.part[part][key] = sum.x + sum.y;
     }
     __syncthreads();
     if (warp == CM_MMA_WARP) {
@@ -907,7 +911,9 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
     }
     const int slot = base + tid;
     if (tid < 128 && slot <= last) {
-        float s = sm.part[0][tid] + sm.part[1][tid];
+        float s = 0.f;
+#pragma unroll
+        for (int p = 0; p < CM_PARTS; ++p) s += sm.part[p][tid];
         if (*abort) s = __int_as_float(0x7fffffff);
         float* mass = a.mass + (((long long)r * a.kv.KVH + g) * a.kv.max_pages << a.kv.page_log2) + slot;
         *mass = slot >= x.cached ? s : *mass + s;
