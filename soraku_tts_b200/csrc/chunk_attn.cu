@@ -92,6 +92,7 @@ __device__ __forceinline__ float query_exponent(const float* qn, int lane) {
 constexpr float CH_QSCALE = 0.08838834764831845f * CO_LOG2E;  // 1 / sqrt(128), scores in log2 units
 
 constexpr int CP_TILES = 64;     // blocks side by side over a row's key tiles
+constexpr int CP_NQ = 2;         // groups of four rows a warp holds at once
 constexpr int CP_SORTED = 512;   // rows that are put in order; more come as they are
 
 // The first `token_blocks` blocks: `per_block` new tokens each (1, 2 or 4), 8 /
@@ -99,7 +100,7 @@ constexpr int CP_SORTED = 512;   // rows that are put in order; more come as the
 // are spread over many warps, many share a warp's look at their row's numbers.
 // The next block puts the rows in order.  The others: cached slots, a block per
 // (key tile, keys or values, kv head, row).
-__global__ void __launch_bounds__(256, 3) chunk_prep_kernel(const ChunkArgs c, int token_blocks, int per_block, int tiles_x) {
+__global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, int token_blocks, int per_block, int tiles_x) {
     const CacheAttnArgs& a = c.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int H = a.H, KVH = a.kv.KVH, nv = H + 2 * KVH;
@@ -193,27 +194,30 @@ __global__ void __launch_bounds__(256, 3) chunk_prep_kernel(const ChunkArgs c, i
         const int first = rt.tile(k) * 128 + row0;
         if (first >= x.cached && first + 15 <= last) continue;  // new tokens only: theirs are written above
         const long long at = ((base + k) * KVH + g) * 2 + value;
-        RowSet d;
-        uint32_t unit[4];
+#pragma unroll 1
+        for (int part = 0; part < 16; part += 4 * CP_NQ) {
+            RowSet<CP_NQ> d;
+            uint32_t unit[CP_NQ];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int slot = first + 4 * q + i4;
-            unit[q] = UT_NONE;
-            if (slot < x.cached && (slot >= rt.w0 || slot < a.sinks)) {
-                const long long u = a.kv.key_unit(r, slot, g);
-                unit[q] = u < 0 ? UT_BAD : (uint32_t)u;
+            for (int q = 0; q < CP_NQ; ++q) {
+                const int slot = first + part + 4 * q + i4;
+                unit[q] = UT_NONE;
+                if (slot < x.cached && (slot >= rt.w0 || slot < a.sinks)) {
+                    const long long u = a.kv.key_unit(r, slot, g);
+                    unit[q] = u < 0 ? UT_BAD : (uint32_t)u;
+                }
             }
-        }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) d.load(q, pool, unit[q], lane);
+            for (int q = 0; q < CP_NQ; ++q) d.load(q, pool, unit[q], lane);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float e = d.exponent(q, unit[q]);
-            const int slot = first + 4 * q + i4;
-            if (slot >= x.cached && slot <= last) continue;
-            d.put(q, c.kvtiles + at * (2 * UT_BYTES), row0, row_scale(e), lane);
-            if ((lane & 7) == 0)
-                c.meta[at * 128 + row0 + 4 * q + i4] = value ? e : e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac : e;
+            for (int q = 0; q < CP_NQ; ++q) {
+                const float e = d.exponent(q, unit[q]);
+                const int row = row0 + part + 4 * q + i4, slot = first - row0 + row;
+                if (slot >= x.cached && slot <= last) continue;
+                d.put(q, c.kvtiles + at * (2 * UT_BYTES), row0 + part, row_scale(e), lane);
+                if ((lane & 7) == 0)
+                    c.meta[at * 128 + row] = value ? e : e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac : e;
+            }
         }
     }
 }

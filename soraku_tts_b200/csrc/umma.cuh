@@ -267,12 +267,13 @@ __device__ __forceinline__ void put4(unsigned char* at, float4 x, float s) {
     *reinterpret_cast<uint2*>(at + UT_BYTES) = lo;
 }
 
-// Sixteen rows of a tile in the registers of a warp, on their way from the
-// pool to a tile pair.  Lane 8 i + t holds, of rows i, 4 + i, 8 + i, 12 + i,
-// columns 8 t .. 8 t + 7 of either half: 32 bytes a load, and 16 bytes of hi or
+// 4 NQ rows of a tile in the registers of a warp, on their way from the pool
+// to a tile pair.  Lane 8 i + t holds, of rows i, 4 + i, ..., columns
+// 8 t .. 8 t + 7 of either half: 32 bytes a load, and 16 bytes of hi or
 // lo a store, whose four rows are whole 128-byte lines.
+template <int NQ>
 struct RowSet {
-    float d[4][2][8];
+    float d[NQ][2][8];
     // `unit`: where this lane's row 4 q + i lies in the pool, or UT_NONE / UT_BAD: zeros
     __device__ __forceinline__ void load(int q, const float* pool, uint32_t unit, int lane) {
 #pragma unroll
