@@ -5,7 +5,7 @@
 // together to the front.  Keys keep the RoPE rotation of the position
 // they were written with.
 //
-// One launch, a thread-block cluster of 8 (or 4) CTAs per (row, kv head):
+// One launch, a thread-block cluster of 8 (or 2) CTAs per (row, kv head):
 //   select  the weight at the border by a radix search over order-preserving
 //           integer keys (8 bits a pass), then a scan that writes the kept slots
 //           and weights.  Up to EV_LOCAL slots every CTA does all of it for
@@ -15,8 +15,8 @@
 //   move    the copy, in place.  A kept slot never moves up, so a CTA that goes
 //           through the kept slots in order reads a round before it writes it
 //           and never overwrites what it still has to read.  Columns are
-//           independent, so the 512-byte rows are cut into parts of 128 (or
-//           256) bytes: the cluster's CTAs move keys or values, a part each,
+//           independent, so the 512-byte rows may be cut into parts of 128
+//           bytes: the cluster's CTAs move keys or values, a part each,
 //           without any order between them.  Where rows come from and go to is looked up
 //           for EV_BLOCK rows at once, so that a round waits for its data alone,
 //           and two rounds are on their way at a time.
@@ -40,7 +40,7 @@ struct EvictShape {
     static constexpr int ROUND = ROWS * EV_UNROLL;
 };
 constexpr int EV_BLOCK = 2048;   // rows whose places are looked up at once
-static_assert(EV_BLOCK % (2 * EvictShape<8>::ROUND) == 0 && EV_BLOCK % (2 * EvictShape<4>::ROUND) == 0, "whole rounds");
+static_assert(EV_BLOCK % (2 * EvictShape<8>::ROUND) == 0 && EV_BLOCK % (2 * EvictShape<2>::ROUND) == 0, "whole rounds");
 
 struct EvictArgs {
     const float* mass;  // [rows][KVH][slots]
@@ -369,10 +369,9 @@ extern "C" int skb_evict_cache(const float* mass, const int32_t* cached, int row
     a.mass_out = mass_out;
     a.cached_out = cached_out;
     // 8 CTAs a group while all of them fit the card at once (two on each of
-    // 148 SMs); more groups take whole memory pages better with wider parts:
-    // 32 groups of 32k slots to 8k 121 us against 140 with 4, 128 groups of 8k
-    // slots to 2k 160 against 126 (measured)
-    const int ctas = (long long)rows * n_kv_heads * 8 <= 296 ? 8 : 4;
+    // 148 SMs); more groups take whole rows, which memory likes better: 128
+    // groups of 8k slots to 2k 120 us, against 126 in halves and 160 in quarters
+    const int ctas = (long long)rows * n_kv_heads * 8 <= 296 ? 8 : 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, n_kv_heads, rows);
     cfg.blockDim = dim3(EV_THREADS);
@@ -384,6 +383,6 @@ extern "C" int skb_evict_cache(const float* mass, const int32_t* cached, int row
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, ctas == 8 ? evict_kernel<8> : evict_kernel<4>, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, ctas == 8 ? evict_kernel<8> : evict_kernel<2>, a);
     return e == cudaSuccess ? SKB_OK : fail(SKB_ERR_CUDA, "evict_cache: %s", cudaGetErrorString(e));
 }
