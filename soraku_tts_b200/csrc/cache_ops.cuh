@@ -95,7 +95,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 // A score below every real one: softmax statistics start from it instead of
 // -inf, so that -inf - -inf never arises.
-constexpr float CO_LOW = -1e30f;
+constexpr float CO_LOW = -3e38f;
 constexpr float CO_LOG2E = 1.4426950408889634f;
 
 }  // namespace skb

@@ -86,7 +86,7 @@ __device__ __forceinline__ float query_exponent(const float* qn, int lane) {
     const float4 w = __ldg(reinterpret_cast<const float4*>(qn) + lane);
     const float m = warp_max(fmaxf(fmaxf(fabsf(w.x), fabsf(w.y)), fmaxf(fabsf(w.z), fabsf(w.w))));
     const int e = (int)(__float_as_uint(m * 2.0405f) >> 23) - 126;
-    return (float)max(-100, min(100, e));
+    return (float)max(-100, min(127, e));
 }
 
 constexpr float CH_QSCALE = 0.08838834764831845f * CO_LOG2E;  // 1 / sqrt(128), scores in log2 units

@@ -275,6 +275,28 @@ def test_chunk_attention_sharp_and_flat_scores():
         assert float(d) <= ATOL * max(1.0, w) * float(c.pool.abs().max()), float(d)
 
 
+@pytest.mark.parametrize("w", [1e-18, 1e15, 1e18])
+def test_scores_of_any_size(w):
+    """A token that sees itself alone returns its own value, however far below
+    (or above) zero its score is: here -+ 11.3 w^2, as its query head is its key's."""
+    from soraku_tts_b200 import kernels
+
+    for sign in (1, -1):
+        for decode_form in (False, True):
+            c = Cache((20, 0, 7), 1 if decode_form else 9, 4, 4, seed=3)
+            c.qn.fill_(w)
+            c.kn.fill_(sign * w)
+            lengths = [1] * 3 if decode_form else [9, 1, 4]
+            qkv = c.qkv(sum(lengths))
+            heads = qkv.view(-1, 12, HD)
+            heads[:, 4:8] = heads[:, :4]
+            if decode_form:
+                got = kernels.window_decode_attention(qkv, window=1, **c.args())
+            else:
+                got = kernels.chunk_attention(qkv, chunk_start=starts(lengths), max_chunk=9, window=1, **c.args())
+            close(got, heads[:, 8:].reshape(-1, 4 * HD).double())
+
+
 def test_bad_rows_return_nan_and_touch_nothing():
     from soraku_tts_b200 import kernels
 
