@@ -187,8 +187,9 @@ int skb_decode_attention_noalloc(const float *qkv, int rows, int n_heads, int n_
 /* Attention of a ragged chunk of new tokens per row.
  *   qkv         device [tokens, (n_heads + 2 n_kv_heads) * 128]  (q | k | v)
  *   chunk_start device int32 [rows + 1]: row r's tokens are chunk_start[r] ..
- *               chunk_start[r + 1] - 1, at most max_chunk; tokens behind
- *               chunk_start[rows] are neither read nor written
+ *               chunk_start[r + 1] - 1, at most max_chunk; it never decreases;
+ *               tokens before chunk_start[0] and behind chunk_start[rows] are
+ *               neither read nor written
  *   rope_cos/sin device [max_pos, 64];  cached, pos: device int32 [rows]
  *   kv_pool, page_table as for skb_decode_attention
  *   out         device [tokens, n_heads * 128]

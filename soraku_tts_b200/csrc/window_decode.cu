@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(WD_THREADS, NR <= 2 ? 2 : 1) window_decode_ker
             sc[h] += __shfl_xor_sync(FULL, sc[h], 1);
             sc[h] += __shfl_xor_sync(FULL, sc[h], 2);
             sc[h] += __shfl_xor_sync(FULL, sc[h], 4);
-            if (poison) sc[h] = __int_as_float(0x7fffffff);
+            sc[h] = poison ? __int_as_float(0x7fffffff) : fmaf(0.f, sc[h], sc[h]);  // an infinite score is NaN too
             if (put != nullptr && real && t8 == 0) put[h] = sc[h];
             up |= real && sc[h] > m[h];
         }

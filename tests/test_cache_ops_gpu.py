@@ -240,6 +240,23 @@ def test_chunk_attention_masked_garbage(bad):
         close(got, want)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("value", [0, 1])
+def test_visible_garbage_shows(bad, value):
+    """One number of a key (or value) that is not finite: every head that sees it
+    says so, whatever sign its score takes, and no other does."""
+    for column in range(3):
+        c = Cache((40, 200, 9), 3, 8, 2, seed=50 + column)
+        for r, slot in ((0, 17), (1, 3), (1, 180)):
+            page = int(c.table[r, slot // c.page])
+            c.pool[page, value, 1, slot % c.page, 40 * column] = bad
+            c.pool64[page, value, 1, slot % c.page, 40 * column] = bad
+        saved = c.pool.clone(), c.pool64.clone()
+        close(*decode(c, 25, 5))
+        c.pool, c.pool64 = saved
+        close(*chunk(c, (3, 1, 2), 25, 5))
+
+
 def test_chunk_attention_nan_query_stays_alone():
     c = Cache((10, 20), 12, seed=4)
     qkv = c.qkv(24)
