@@ -456,8 +456,11 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             bool go = true;
             for (int i = 0; i < nt && go; ++i) {  // O = P_i V_i
                 const int n = i + 1 < nt ? 2 * i + 2 : 2 * nt - 1, s = n % CA_STAGES;
-                go = ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort) && ut_wait(&sm.p_full[i & 1], (i >> 1) & 1, abort) &&
-                     (i == 0 || ut_wait(&sm.o_free, (i - 1) & 1, abort));
+                // the weights first: with them the stage's copy before, K_i, is
+                // known to be over, so that `full` cannot be taken a phase early
+                go = ut_wait(&sm.p_full[i & 1], (i >> 1) & 1, abort) &&
+                     (i == 0 || ut_wait(&sm.o_free, (i - 1) & 1, abort)) &&
+                     ut_wait(&sm.full[s], (n / CA_STAGES) & 1, abort);
                 if (!go) break;
                 ut_fence_after();
                 ut_mma_pv(tmem + CA_TM_O, tmem + (i & 1) * 128, smem_u32(sm.stage[s]));

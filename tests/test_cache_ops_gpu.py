@@ -189,6 +189,24 @@ def test_chunk_attention_long_rows():
     c.check_mass()
 
 
+@pytest.mark.parametrize("heads", [(16, 8), (9, 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 3)])
+def test_chunk_attention_more_work_than_the_card_holds(heads, window, sinks):
+    """Several query tiles for every SM, with one key tile or several, idle and
+    empty rows between them."""
+    lengths = [(37 * r * r + 11 * r) % 330 for r in range(30)]
+    cached = [0 if r % 3 else (53 * r) % 400 for r in range(30)]
+    cached[4] = cached[17] = -1
+    c = Cache(cached, 330, *heads, seed=70)
+    got, want = chunk(c, lengths, window, sinks, mass=True)
+    close(got, want)
+    c.check_cache()
+    c.check_mass()
+    again = Cache(cached, 330, *heads, seed=70)
+    b, _ = chunk(again, lengths, window, sinks, mass=True)
+    assert torch.equal(got, b) and torch.equal(c.mass, again.mass)
+
+
 def test_chunk_attention_leaves_other_memory_alone():
     c = Cache((20, -1, 31, 7), 40, seed=3)
     lengths, extra = (9, 4, 17, 0), 6
