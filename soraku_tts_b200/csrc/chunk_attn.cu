@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         const int q = tid / c.n_rep;
         sm.own[tid] = q < min(c.P, x.n - i0) ? x.cached + i0 + q : -1;
     }
-    if (warp == CA_WARP_M) ut_alloc(&sm.tmem);
+    if (warp == CA_WARP_M) ut_alloc<512>(&sm.tmem);
     ut_fence_before();
     __syncthreads();
     ut_fence_after();
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                      (i < 2 || ut_wait(&sm.pv_done[i & 1], ((i - 2) >> 1) & 1, abort));
                 if (!go) break;
                 ut_fence_after();
-                ut_mma_qk_ts(tmem + (i & 1) * 128, tmem + CA_TM_Q, smem_u32(sm.stage[s]));
+                ut_mma_qk<128>(tmem + (i & 1) * 128, tmem + CA_TM_Q, smem_u32(sm.stage[s]));
                 ut_commit(&sm.empty[s]);
                 ut_commit(&sm.s_full[i & 1]);
             }
@@ -520,22 +520,8 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             }
         };
         if (nt > 0 && part < 2) {  // the queries into tensor memory: this row of hi, or of lo
-            const unsigned char* q = sm.stage[CA_STAGES - 1] + part * UT_BYTES + row * 128;
             ut_wait(&sm.q_landed, 0, abort);
-#pragma unroll
-            for (int ch = 0; ch < 2; ++ch) {
-                uint32_t w[32];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint4 y = *reinterpret_cast<const uint4*>(q + ch * UT_HALF + ((j ^ (row & 7)) * 16));
-                    w[4 * j] = y.x;
-                    w[4 * j + 1] = y.y;
-                    w[4 * j + 2] = y.z;
-                    w[4 * j + 3] = y.w;
-                }
-                ut_st32(lane_tm + CA_TM_Q + part * 64 + ch * 32, w);
-            }
-            ut_wait_st();
+            ut_row_to_tmem(sm.stage[CA_STAGES - 1] + part * UT_BYTES, row, lane_tm + CA_TM_Q + part * 64);
             ut_fence_before();
         }
         __syncwarp();
@@ -696,7 +682,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     __syncthreads();
     if (warp == CA_WARP_M) {
         ut_fence_after();
-        ut_free(tmem);
+        ut_free<512>(tmem);
     }
     // ---- join the splits: CTA z of the cluster takes a part of the rows.  The
     // weights of all rows first, then all outputs: two trips to the peers' memory
@@ -744,33 +730,42 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
 }
 
 // -------------------------------------------------------------- chunk_mass
-// One CTA per (key tile, kv head, row): its keys are the rows of the products; the query tiles that see any of them pass through
-// as columns.  A thread owns a slot and a quarter of the columns, so weights are added in
-// a fixed order without atomics:
+// One CTA per (key tile, kv head, row): its keys, in tensor memory, are the rows
+// of the products; the queries that see any of them pass through as columns, half
+// a query tile a step.  A thread owns a slot and half of a step's columns, so weights
+// are added in a fixed order without atomics:
 //   sum over columns of exp2(s - lse)
-constexpr int CM_PARTS = 4;                                 // threads per slot
+// Steps of half a tile let two CTAs share an SM: a CTA has few steps between its
+// start and its end, which then lie beside the other's work (4 windowed pieces of
+// 130 to 256 tokens with their weights: 88 us in whole tiles, one CTA an SM; 84 so).
+constexpr int CM_N = 64;                                    // columns of a step
+constexpr int CM_PARTS = 2;                                 // threads per slot
 constexpr int CM_SUM_WARPS = 4 * CM_PARTS;
-constexpr int CM_W = 128 / CM_PARTS;                        // a thread's columns
-constexpr int CM_LSE = 4;                                   // tiles' lse held
+constexpr int CM_W = CM_N / CM_PARTS;                       // a thread's columns
+constexpr int CM_STAGES = 3;
+constexpr int CM_LSE = 4;                                   // steps' lse held
 constexpr int CM_THREADS = 32 * (CM_SUM_WARPS + 1);
 constexpr int CM_MMA_WARP = CM_SUM_WARPS;
+constexpr uint32_t CM_TM_K = 2 * CM_N;                      // TMEM columns: two products, then the keys
+constexpr int CM_TM = 256;
+static_assert(CM_TM_K + 128 <= CM_TM && 2 * CM_TM <= 512, "tensor memory of two CTAs");
 
 struct CmSmem {
-    unsigned char k[2 * UT_BYTES];
-    unsigned char q[2][2 * UT_BYTES];
-    float lse[CM_LSE][128];
+    unsigned char stage[CM_STAGES][UT_BYTES];  // at first the keys in 0 and 1; step i's queries, hi | lo, in (i + 2) % 3
+    float lse[CM_LSE][CM_N];
     float kc[128];
     float part[CM_PARTS][128];
     int own[CM_SUM_WARPS][CM_W];  // slots of the queries in a warp's columns; -1: none
-    uint64_t k_full, q_full[2], q_empty[2], s_full[2], s_empty[2], lse_full[CM_LSE];
+    uint64_t k_full, k_copied, q_full[CM_STAGES], q_empty[CM_STAGES], s_full[2], s_empty[2], lse_full[CM_LSE], end;
     uint32_t tmem;
     int abort;
 };
 constexpr size_t CM_SMEM = sizeof(CmSmem) + 1024;
 static_assert(CM_W == 32, "a part is a warp's width");
-static_assert(CM_SMEM <= 227 * 1024, "shared memory of one CTA");
+static_assert(4 * CM_N * 128 == UT_BYTES, "a step's queries fill a stage");
+static_assert(2 * (CM_SMEM + 1024) <= 227 * 1024, "shared memory of two CTAs");
 
-__global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkArgs c) {
+__global__ void __launch_bounds__(CM_THREADS, 2) chunk_mass_kernel(const ChunkArgs c) {
     extern __shared__ unsigned char cm_raw[];
     CmSmem& sm = *reinterpret_cast<CmSmem*>(cm_raw + ((1024u - (smem_u32(cm_raw) & 1023u)) & 1023u));
     const CacheAttnArgs& a = c.a;
@@ -792,13 +787,22 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
     int to = last;
     if (a.window > 0 && base >= a.sinks) to = (int)min((long long)to, (long long)base + 127 + a.window - 1);
     if (from > to) return;
-    const int t0 = (from - x.cached) / c.P, nt = (to - x.cached) / c.P - t0 + 1;
+    // steps: halves of query tiles, numbered through the row
+    auto step_of = [&](int own, int head) {
+        const int t = (own - x.cached) / c.P, column = (own - x.cached - t * c.P) * c.n_rep + head;
+        return 2 * t + column / CM_N;
+    };
+    const int s0 = step_of(from, 0), ns = step_of(to, c.n_rep - 1) - s0 + 1;
 
     if (tid == 0) {
         mbar_init(&sm.k_full, 1);
-        for (int b = 0; b < 2; ++b) {
+        mbar_init(&sm.k_copied, CM_SUM_WARPS);
+        mbar_init(&sm.end, 1);
+        for (int b = 0; b < CM_STAGES; ++b) {
             mbar_init(&sm.q_full[b], 1);
             mbar_init(&sm.q_empty[b], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
             mbar_init(&sm.s_full[b], 1);
             mbar_init(&sm.s_empty[b], CM_SUM_WARPS);
         }
@@ -806,7 +810,7 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
         mbar_fence_init();
         sm.abort = 0;
     }
-    if (warp == CM_MMA_WARP) ut_alloc(&sm.tmem);
+    if (warp == CM_MMA_WARP) ut_alloc<CM_TM>(&sm.tmem);
     ut_fence_before();
     __syncthreads();
     ut_fence_after();
@@ -815,66 +819,77 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
 
     if (warp == CM_MMA_WARP) {
         if (lane == 0) {
-            const long long at0 = chunk_tile(c, x, r, t0) * a.kv.KVH + g;
             auto fetch = [&](int i) {
-                const long long at = at0 + (long long)i * a.kv.KVH;
-                mbar_expect_tx(&sm.q_full[i & 1], 2 * UT_BYTES);
-                bulk_g2s(sm.q[i & 1], c.qtiles + at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.q_full[i & 1]);
-                mbar_expect_tx(&sm.lse_full[i % CM_LSE], 512);
-                bulk_g2s(sm.lse[i % CM_LSE], c.lse + at * 128, 512, &sm.lse_full[i % CM_LSE]);
+                const int s = s0 + i, b = (i + 2) % CM_STAGES;
+                const long long at = chunk_tile(c, x, r, s >> 1) * a.kv.KVH + g;
+                const unsigned char* q = c.qtiles + at * (2 * UT_BYTES) + (s & 1) * (CM_N * 128);
+                mbar_expect_tx(&sm.q_full[b], UT_BYTES);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)  // hi and lo, two halves of 64 columns each
+                    bulk_g2s(sm.stage[b] + k * (CM_N * 128), q + k * UT_HALF, CM_N * 128, &sm.q_full[b]);
+                mbar_expect_tx(&sm.lse_full[i % CM_LSE], CM_N * 4);
+                bulk_g2s(sm.lse[i % CM_LSE], c.lse + at * 128 + (s & 1) * CM_N, CM_N * 4, &sm.lse_full[i % CM_LSE]);
             };
             const long long kat = ((row_at + blockIdx.x) * a.kv.KVH + g) * 2;
             mbar_expect_tx(&sm.k_full, 2 * UT_BYTES + 512);
-            bulk_g2s(sm.k, c.kvtiles + kat * (2 * UT_BYTES), 2 * UT_BYTES, &sm.k_full);
+            bulk_g2s(sm.stage[0], c.kvtiles + kat * (2 * UT_BYTES), 2 * UT_BYTES, &sm.k_full);
             bulk_g2s(sm.kc, c.meta + kat * 128, 512, &sm.k_full);
-            int fetched = 0;
-            for (; fetched < 2 && fetched < nt; ++fetched) fetch(fetched);
-            bool go = ut_wait(&sm.k_full, 0, abort);
-            int i = 0;
-            for (; i < nt && go; ++i) {
-                go = ut_wait(&sm.q_full[i & 1], (i >> 1) & 1, abort);
-                if (go && i >= 2) go = ut_wait(&sm.s_empty[i & 1], ((i - 2) >> 1) & 1, abort);
+            fetch(0);
+            int fetched = 1;
+            bool go = ut_wait(&sm.k_copied, 0, abort);
+            for (; go && fetched < CM_STAGES && fetched < ns; ++fetched) fetch(fetched);
+            for (int i = 0; i < ns && go; ++i) {
+                const int b = (i + 2) % CM_STAGES;
+                go = ut_wait(&sm.q_full[b], (i / CM_STAGES) & 1, abort) &&
+                     (i < 2 || ut_wait(&sm.s_empty[i & 1], ((i - 2) >> 1) & 1, abort));
                 if (!go) break;
                 ut_fence_after();
-                ut_mma_qk(tmem + (i & 1) * 128, smem_u32(sm.k), smem_u32(sm.q[i & 1]));
-                ut_commit(&sm.q_empty[i & 1]);
+                ut_mma_qk<CM_N>(tmem + (i & 1) * CM_N, tmem + CM_TM_K, smem_u32(sm.stage[b]));
+                ut_commit(&sm.q_empty[b]);
                 ut_commit(&sm.s_full[i & 1]);
-                // the other buffer's products are done; the lse that tile i - 3
-                // left is read, since its sums were waited for above
-                if (i >= 1 && i + 1 < nt) {
-                    go = ut_wait(&sm.q_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, abort);
+                // into the stage of step i - 1, when its products are done; the lse
+                // that step i - 2 left is read, since its sums were waited for above
+                if (i >= 1 && i + 2 < ns) {
+                    go = ut_wait(&sm.q_empty[(i + 1) % CM_STAGES], ((i - 1) / CM_STAGES) & 1, abort);
                     if (go) {
-                        fetch(i + 1);
+                        fetch(i + 2);
                         ++fetched;
                     }
                 }
             }
             // leave nothing in flight: the copies asked for, the products issued
-            if (i < nt) mbar_wait(&sm.k_full, 0, nullptr);
-            if (i < nt)
-                for (int f = max(0, fetched - 2); f < fetched; ++f) {
-                    mbar_wait(&sm.q_full[f & 1], (f >> 1) & 1, nullptr);
+            if (!go) {
+                mbar_wait(&sm.k_full, 0, nullptr);
+                for (int f = max(0, fetched - CM_STAGES); f < fetched; ++f) {
+                    mbar_wait(&sm.q_full[(f + 2) % CM_STAGES], (f / CM_STAGES) & 1, nullptr);
                     mbar_wait(&sm.lse_full[f % CM_LSE], (f / CM_LSE) & 1, nullptr);
                 }
+            }
+            ut_commit(&sm.end);
+            mbar_wait(&sm.end, 0, nullptr);
         }
         __syncwarp();
     } else {
-        ut_wait(&sm.k_full, 0, abort);
         const int key = 32 * (warp & 3) + lane, part = warp >> 2, slot = base + key;
+        const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        ut_wait(&sm.k_full, 0, abort);
+        ut_row_to_tmem(sm.stage[part], key, lane_tm + CM_TM_K + part * 64);  // hi, or lo
+        ut_fence_before();
+        __syncwarp();
+        if (lane == 0) ut_arrive(&sm.k_copied);
         const float kc = sm.kc[key];
-        const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + part * CM_W;
         // queries at slots >= this do not see the slot
         const unsigned upto = a.window == 0 || slot < a.sinks ? 0x7fffffffu : (unsigned)slot + (unsigned)a.window;
         float2 sum = make_float2(0.f, 0.f);
-        for (int i = 0; i < nt; ++i) {
-            const int b = i & 1;
-            const int first = x.cached + (t0 + i) * c.P;            // slot of the tile's first query
+        for (int i = 0; i < ns; ++i) {
+            const int b = i & 1, t = (s0 + i) >> 1, column = ((s0 + i) & 1) * CM_N;
+            const int first = x.cached + t * c.P;            // slot of the tile's first query
             const int nq = min(c.P, last + 1 - first);
             // seen whole: every column is a query, behind every slot, inside the window
-            const bool whole = nq * c.n_rep == 128 && first >= base + 127 &&
+            const bool whole = nq * c.n_rep >= column + CM_N && first >= base + 127 &&
                                (a.window == 0 || first + nq - 1 - base < a.window || base + 128 <= a.sinks);
             if (!whole) {  // one division a column, not one a weight
-                const int qi = (part * CM_W + lane) / c.n_rep;
+                const int qi = (column + part * CM_W + lane) / c.n_rep;
                 sm.own[warp][lane] = qi < nq ? first + qi : -1;
                 __syncwarp();
             }
@@ -883,7 +898,7 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
             ut_fence_after();
             {
                 uint32_t s[32];
-                ut_ld32(lane_tm + b * 128, s);
+                ut_ld32(lane_tm + b * CM_N + part * CM_W, s);
                 ut_wait_ld();
                 const float4* lse = reinterpret_cast<const float4*>(sm.lse[i % CM_LSE] + part * CM_W);
 #pragma unroll
@@ -914,7 +929,7 @@ __global__ void __launch_bounds__(CM_THREADS, 1) chunk_mass_kernel(const ChunkAr
     __syncthreads();
     if (warp == CM_MMA_WARP) {
         ut_fence_after();
-        ut_free(tmem);
+        ut_free<CM_TM>(tmem);
     }
     const int slot = base + tid;
     if (tid < 128 && slot <= last) {

@@ -33,15 +33,9 @@ __device__ __forceinline__ uint64_t ut_desc(uint32_t saddr, uint32_t off, bool m
     const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
     return (uint64_t)hi << 32 | lo;
 }
-// kind::f16, D FP32, A and B fp16, M = N = 128.
-__host__ __device__ constexpr uint32_t ut_idesc(bool b_mn_major) {
-    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | (16u << 17) | (8u << 24);
-}
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
-        : "memory");
+// kind::f16, D FP32, A and B fp16, M = 128.
+__host__ __device__ constexpr uint32_t ut_idesc(int n, bool b_mn_major) {
+    return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
@@ -58,31 +52,19 @@ __device__ __forceinline__ void ut_commit(uint64_t* bar) {
 // products come first, where the sum is still 2^-11 of its size, and no sum
 // runs on from tile to tile: that grew to 1.3e-5 over 8000 slots.
 
-// D[128 x 128] = A B^T over 128 columns, both operands as hi | lo tile pairs
-// (K-major) in shared memory.
-__device__ __forceinline__ void ut_mma_qk(uint32_t d, uint32_t a, uint32_t b) {
-    asm volatile("" : "+r"(a), "+r"(b));  // keeps 48 descriptors from being held across a caller's loop
-#pragma unroll
-    for (int p = 0; p < 3; ++p) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t off = (k >> 2) * UT_HALF + (k & 3) * 32;
-            umma_f16_ss(d, ut_desc(a, off + (p == 1 ? UT_BYTES : 0), false), ut_desc(b, off + (p == 0 ? UT_BYTES : 0), false),
-                        ut_idesc(false), p > 0 || k > 0);
-        }
-    }
-}
-// The same with A in tensor memory (hi | lo, 64 columns each): it halves what
-// the products read from shared memory.
-__device__ __forceinline__ void ut_mma_qk_ts(uint32_t d, uint32_t a_tmem, uint32_t b) {
-    asm volatile("" : "+r"(a_tmem), "+r"(b));
+// D[128 x N] = A B^T over 128 columns: A in tensor memory (hi | lo, 64 columns
+// each), which halves what the products read from shared memory; B as a hi | lo
+// pair of [two halves of 64 columns][N rows] tiles (K-major).
+template <int N>
+__device__ __forceinline__ void ut_mma_qk(uint32_t d, uint32_t a_tmem, uint32_t b) {
+    asm volatile("" : "+r"(a_tmem), "+r"(b));  // keeps 24 descriptors from being held across a caller's loop
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
         const uint32_t pa = a_tmem + (p == 1 ? 64 : 0);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            umma_f16_ts(d, pa + k * 8, ut_desc(b, (p == 0 ? UT_BYTES : 0) + (k >> 2) * UT_HALF + (k & 3) * 32, false),
-                        ut_idesc(false), p > 0 || k > 0);
+            umma_f16_ts(d, pa + k * 8, ut_desc(b, (p == 0 ? 256 * N : 0) + (k >> 2) * (128 * N) + (k & 3) * 32, false),
+                        ut_idesc(N, false), p > 0 || k > 0);
     }
 }
 // D[128 x 128] = P V: P in tensor memory, for each 16 keys 8 columns of hi,
@@ -94,7 +76,7 @@ __device__ __forceinline__ void ut_mma_pv(uint32_t d, uint32_t p_tmem, uint32_t 
         const uint32_t pa = p_tmem + (p == 1 ? 8 : 0);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            umma_f16_ts(d, pa + k * 16, ut_desc(v, (p == 0 ? UT_BYTES : 0) + k * 2048, true), ut_idesc(true), p > 0 || k > 0);
+            umma_f16_ts(d, pa + k * 16, ut_desc(v, (p == 0 ? UT_BYTES : 0) + k * 2048, true), ut_idesc(128, true), p > 0 || k > 0);
     }
 }
 
@@ -129,13 +111,33 @@ __device__ __forceinline__ void ut_wait_ld() { asm volatile("tcgen05.wait::ld.sy
 __device__ __forceinline__ void ut_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void ut_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ut_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void ut_alloc(uint32_t* slot) {  // one warp, 512 columns
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512u)
+template <int COLUMNS>
+__device__ __forceinline__ void ut_alloc(uint32_t* slot) {  // by one warp
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "n"(COLUMNS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
+template <int COLUMNS>
 __device__ __forceinline__ void ut_free(uint32_t tmem) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLUMNS) : "memory");
+}
+// Row `row` of one fp16 tile of 128 rows into 64 columns of tensor memory, a
+// lane its row.
+__device__ __forceinline__ void ut_row_to_tmem(const unsigned char* tile, int row, uint32_t taddr) {
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+        uint32_t w[32];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint4 y = *reinterpret_cast<const uint4*>(tile + ch * UT_HALF + row * 128 + ((j ^ (row & 7)) * 16));
+            w[4 * j] = y.x;
+            w[4 * j + 1] = y.y;
+            w[4 * j + 2] = y.z;
+            w[4 * j + 3] = y.w;
+        }
+        ut_st32(taddr + ch * 32, w);
+    }
+    ut_wait_st();
 }
 
 // ----------------------------------------------------------------- waits
