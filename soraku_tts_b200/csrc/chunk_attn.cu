@@ -30,7 +30,7 @@ struct ChunkArgs {
     unsigned char* kvtiles; // [key tiles][KVH][2][2 UT_BYTES]: keys, values, hi | lo
     float* meta;            // [key tiles][KVH][2][128]: factor of a key's scores; exponent of a value row
     float* lse;             // [query tiles][KVH][128] (mass only), log2 units
-    int* order;             // [rows]: rows by the tiles they see, most first; null: as they are
+    struct RowJob* jobs;    // [rows]: by the tiles they see, most first; null: rows as they are
     long long key_tiles;
 };
 
@@ -58,6 +58,12 @@ __device__ __forceinline__ ChunkRow chunk_row(const ChunkArgs& c, int r) {
 __device__ __forceinline__ long long chunk_tile(const ChunkArgs& c, const ChunkRow& x, int r, int t) {
     return x.b / c.P + r + t;
 }
+
+// A row as chunk_attn takes it: one read in place of a chain of three.
+struct __align__(32) RowJob {
+    int row, b, n, cached;  // no tokens: nothing to do
+    long long base, unused;
+};
 
 // The tiles of 128 slots that any query of a row sees: [0, a1) for the sinks,
 // [b0, end) for the windows.
@@ -93,7 +99,7 @@ constexpr float CH_QSCALE = 0.08838834764831845f * CO_LOG2E;  // 1 / sqrt(128), 
 
 constexpr int CP_TILES = 64;     // blocks side by side over a row's key tiles
 constexpr int CP_NQ = 2;         // groups of four rows a warp holds at once
-constexpr int CP_SORTED = 512;   // rows that are put in order; more come as they are
+constexpr int CP_SORTED = 512;   // more rows than that are taken as they come
 
 // The first `token_blocks` blocks: `per_block` new tokens each (1, 2 or 4), 8 /
 // per_block warps to a token, which take its head vectors in turn.  Few tokens
@@ -165,21 +171,24 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, i
         return;
     }
     int b = blockIdx.x - token_blocks;
-    if (b == 0 && c.order) {  // the order in which chunk_attn takes the rows
+    if (b == 0 && c.jobs) {  // the order in which chunk_attn takes the rows
         __shared__ int seen[CP_SORTED];
-        for (int p = threadIdx.x; p < a.rows; p += 256) {
-            if (a.rows <= CP_SORTED) seen[p] = RowTiles(c, chunk_row(c, p)).n;
-            else c.order[p] = p;
-        }
+        for (int p = threadIdx.x; p < a.rows; p += 256) seen[p] = RowTiles(c, chunk_row(c, p)).n;
         __syncthreads();
-        for (int p = threadIdx.x; p < a.rows && a.rows <= CP_SORTED; p += 256) {
+        for (int p = threadIdx.x; p < a.rows; p += 256) {
             int rank = 0;
-            for (int q = 0; q < a.rows; ++q) rank += seen[q] > seen[p] || (seen[q] == seen[p] && q < p);
-            c.order[rank] = p;
+            long long base = 0;
+            for (int q = 0; q < a.rows; ++q) {
+                rank += seen[q] > seen[p] || (seen[q] == seen[p] && q < p);
+                base += q < p ? seen[q] : 0;
+            }
+            const ChunkRow x = chunk_row(c, p);
+            const bool none = x.idle || x.bad || base + seen[p] > c.key_tiles;
+            c.jobs[rank] = RowJob{p, x.b, none ? 0 : x.n, x.cached, base, 0};
         }
         return;
     }
-    if (c.order) --b;
+    if (c.jobs) --b;
     const int k0 = b % tiles_x;
     b /= tiles_x;
     const int value = b & 1, g = (b >> 1) % KVH, r = (b >> 1) / KVH;
@@ -347,18 +356,39 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = blockIdx.y, z = blockIdx.x % splits;
     const int t = gridDim.x / splits - 1 - blockIdx.x / splits;  // the last query tile sees the most: first
-    if (c.order) pdl_wait();
-    const int r = c.order ? c.order[blockIdx.z] : blockIdx.z;
-    const ChunkRow x = chunk_row(c, r);
+    int r = blockIdx.z;
+    ChunkRow x;
+    long long base;
+    if (c.jobs) {
+        pdl_wait();
+        const int4 j = *reinterpret_cast<const int4*>(c.jobs + r);
+        base = c.jobs[r].base;
+        r = j.x;
+        x.b = j.y;
+        x.n = j.z;
+        x.cached = j.w;
+        x.idle = x.bad = false;
+    } else {
+        x = chunk_row(c, r);
+        base = row_base(c, r);
+    }
     const int i0 = t * c.P;
     const RowTiles rt(c, x);
-    long long base = 0;
-    if (i0 < x.n && !x.idle && !x.bad) base = row_base(c, r);
     if (x.idle || x.bad || i0 >= x.n || base + rt.n > c.key_tiles) {  // the same for a whole cluster
         pdl_wait();
         return;
     }
-    if (tid == 0) {
+    // where tile i of this CTA's list lies in the workspace
+    auto tile_of = [&](int i) {
+        const int tile = sm.list.tile(sm.k0 + i);
+        return (sm.base + (tile < sm.a1 ? tile : sm.a1 + tile - sm.b0)) * a.kv.KVH + blockIdx.y;
+    };
+    auto ask = [&](int n, int i, int value) {  // copy n: of tile i
+        const int s = n % CA_STAGES;
+        mbar_expect_tx(&sm.full[s], 2 * UT_BYTES);
+        bulk_g2s(sm.stage[s], c.kvtiles + (tile_of(i) * 2 + value) * (2 * UT_BYTES), 2 * UT_BYTES, &sm.full[s]);
+    };
+    if (tid == 32 * CA_WARP_P) {
         mbar_init(&sm.q_landed, 1);
         mbar_init(&sm.q_full, CA_SOFTMAX_WARPS);
         mbar_init(&sm.o_free, CA_SOFTMAX_WARPS);
@@ -386,6 +416,15 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         sm.base = base;
         sm.a1 = rt.a1;
         sm.b0 = rt.b0;
+        pdl_wait();
+        // the first copies are on their way while the CTA gets ready; the
+        // queries by way of the last stage
+        if (sm.nt > 0) {
+            mbar_expect_tx(&sm.q_landed, 2 * UT_BYTES);
+            bulk_g2s(sm.stage[CA_STAGES - 1], c.qtiles + sm.tile_at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.q_landed);
+            ask(0, 0, 0);
+            if (sm.nt > 1) ask(1, 1, 0);
+        }
     }
     if (tid < 128) {
         const int q = tid / c.n_rep;
@@ -398,41 +437,29 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     const uint32_t tmem = sm.tmem;
     const int nt = sm.nt;
     volatile int* abort = &sm.abort;
-    // where tile i of this CTA's list lies in the workspace
-    auto tile_of = [&](int i) {
-        const int tile = sm.list.tile(sm.k0 + i);
-        return (sm.base + (tile < sm.a1 ? tile : sm.a1 + tile - sm.b0)) * a.kv.KVH + blockIdx.y;
-    };
     pdl_wait();
     if (c.lse) pdl_trigger();  // chunk_mass follows
 
     if (warp == CA_WARP_P) {
         if (lane == 0) {
-            int n = 0, landed = 0;  // copies asked for
+            int n = min(nt, 2);  // copies asked for
             auto fetch = [&](int i, int value) {
-                const int s = n % CA_STAGES;
                 if (n == CA_STAGES - 1 && !ut_wait(&sm.q_full, 0, abort)) return false;  // the queries were there
-                if (n >= CA_STAGES && !ut_wait(&sm.empty[s], ((n - CA_STAGES) / CA_STAGES) & 1, abort)) return false;
-                const long long at = tile_of(i) * 2 + value;
-                mbar_expect_tx(&sm.full[s], 2 * UT_BYTES);
-                bulk_g2s(sm.stage[s], c.kvtiles + at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.full[s]);
+                if (n >= CA_STAGES && !ut_wait(&sm.empty[n % CA_STAGES], ((n - CA_STAGES) / CA_STAGES) & 1, abort))
+                    return false;
+                ask(n, i, value);
                 ++n;
                 return true;
             };
-            bool go = nt > 0;
-            if (go) {  // the queries by way of the last stage
-                mbar_expect_tx(&sm.q_landed, 2 * UT_BYTES);
-                bulk_g2s(sm.stage[CA_STAGES - 1], c.qtiles + sm.tile_at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.q_landed);
-                go = fetch(0, 0);
-            }
+            bool go = true;
             for (int i = 0; i < nt && go; ++i) {
-                if (i + 1 < nt) go = fetch(i + 1, 0);
+                if (i > 0 && i + 1 < nt) go = fetch(i + 1, 0);
                 if (go) go = fetch(i, 1);
             }
             // no copy may be in flight when the CTA ends early
             if (!go && nt > 0) mbar_wait(&sm.q_landed, 0, nullptr);
             if (!go)
-                for (landed = max(0, n - CA_STAGES); landed < n; ++landed)
+                for (int landed = max(0, n - CA_STAGES); landed < n; ++landed)
                     mbar_wait(&sm.full[landed % CA_STAGES], (landed / CA_STAGES) & 1, nullptr);
         }
         __syncwarp();
@@ -667,6 +694,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         float* stage = reinterpret_cast<float*>(sm.stage) + row * CA_OUT_LD + part * CA_W;
         // rows that saw nothing, and dead ones, give zeros
         const float f = l == 0.f || row >= sm.live ? 0.f : exp2_fast(E - 19.f) / l;
+        if (splits == 1 && c.lse && part == 0 && row < sm.live) c.lse[sm.tile_at * 128 + row] = m + log2f(l);
 #pragma unroll
         for (int q = 0; q < CA_W / 4; ++q) {
             float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -693,27 +721,30 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     const int ra = part * sm.live / splits, rb = (part + 1) * sm.live / splits;
     float (*weight)[128] = sm.mx[0];  // [split][row]; the maxima are done with
     static_assert(2 * CA_PARTS >= CA_MAX_SPLITS, "weights fit the maxima's place");
-    for (int i = tid; i < (rb - ra) * splits; i += CA_THREADS) {
-        const int row = ra + i / splits, p = i % splits;
-        float M = CO_LOW, L = 0.f, mine = 0.f;
+    if (splits > 1) {
+        for (int i = tid; i < (rb - ra) * splits; i += CA_THREADS) {
+            const int row = ra + i / splits, p = i % splits;
+            float M = CO_LOW, L = 0.f, mine = 0.f;
 #pragma unroll 4
-        for (int q = 0; q < splits; ++q) {
-            const float m = ld_peer(&sm.m[row], q), l = ld_peer(&sm.l[0][row], q);
-            const float up = fmaxf(M, m), f = exp2_fast(M - up), w = l * exp2_fast(m - up);
-            mine = q == p ? w : mine * f;
-            L = fmaf(L, f, w);
-            M = up;
+            for (int q = 0; q < splits; ++q) {
+                const float m = ld_peer(&sm.m[row], q), l = ld_peer(&sm.l[0][row], q);
+                const float up = fmaxf(M, m), f = exp2_fast(M - up), w = l * exp2_fast(m - up);
+                mine = q == p ? w : mine * f;
+                L = fmaf(L, f, w);
+                M = up;
+            }
+            weight[p][row] = mine / L;  // not a number where a wait ran out
+            if (c.lse && p == 0) c.lse[sm.tile_at * 128 + row] = M + log2f(L);
         }
-        weight[p][row] = mine / L;  // not a number where a wait ran out
-        if (c.lse && p == 0) c.lse[sm.tile_at * 128 + row] = M + log2f(L);
+        __syncthreads();
     }
-    __syncthreads();
     const uint32_t stage = smem_u32(sm.stage);
+    const float alone = *abort ? __int_as_float(0x7fffffff) : 1.f;  // not a number where a wait ran out
     for (int i = tid; i < (rb - ra) * 32; i += CA_THREADS) {
         const int row = ra + (i >> 5), col = i & 31;
         const int at = row * CA_OUT_LD + 4 * col;
         float4 o = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.stage) + at);
-        const float own = weight[part][row];
+        const float own = splits > 1 ? weight[part][row] : alone;
         o = make_float4(o.x * own, o.y * own, o.z * own, o.w * own);
 #pragma unroll 2
         for (int q = 1; q < splits; ++q) {
@@ -960,13 +991,13 @@ static long long chunk_key_tiles(int rows, int max_chunk, int max_pages, int pag
 }
 
 struct ChunkWork {
-    long long q, kv, meta, order, lse, total;  // byte offsets
+    long long q, kv, meta, jobs, lse, total;  // byte offsets
     ChunkWork(long long qtiles, long long ktiles, int KVH, int rows, bool with_mass) {
         q = 0;
         kv = qtiles * KVH * (2 * (long long)UT_BYTES);
         meta = kv + ktiles * KVH * (4 * (long long)UT_BYTES);
-        order = meta + ktiles * KVH * 1024;
-        lse = order + (rows * 4ll + 255) / 256 * 256;
+        jobs = meta + ktiles * KVH * 1024;
+        lse = jobs + (rows * (long long)sizeof(RowJob) + 255) / 256 * 256;
         total = lse + (with_mass ? (qtiles * KVH * 512 + 255) / 256 * 256 : 0);
     }
 };
@@ -1051,7 +1082,7 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     if (ctas > tiles) ctas = tiles;
     ctas *= n_kv_heads;
     // more than one wave of CTAs: the rows with most work first
-    c.order = ctas > 148 && rows > 1 ? reinterpret_cast<int*>(w + at.order) : nullptr;
+    c.jobs = ctas > 148 && rows <= CP_SORTED ? reinterpret_cast<RowJob*>(w + at.jobs) : nullptr;
     long long splits = 148 / ctas;
     if (splits > row_tiles) splits = row_tiles;
     if (splits > CA_MAX_SPLITS) splits = CA_MAX_SPLITS;
@@ -1059,7 +1090,7 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     const int prep_x = row_tiles < CP_TILES ? (int)row_tiles : CP_TILES;
     const int per_block = tokens <= 1024 ? 1 : 4;
     const int token_blocks = (tokens + per_block - 1) / per_block;
-    const long long prep_blocks = token_blocks + (c.order ? 1 : 0) + (long long)prep_x * 2 * n_kv_heads * rows;
+    const long long prep_blocks = token_blocks + (c.jobs ? 1 : 0) + (long long)prep_x * 2 * n_kv_heads * rows;
     if (prep_blocks > 0x7fffffffll) return fail(SKB_ERR_ARG, "%s: too many tokens and rows", what);
 
     static std::atomic<unsigned long long> attn_done, mass_done;
