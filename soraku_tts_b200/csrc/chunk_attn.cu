@@ -61,8 +61,9 @@ __device__ __forceinline__ long long chunk_tile(const ChunkArgs& c, const ChunkR
 
 // A row as chunk_attn takes it: one read in place of a chain of three.
 struct __align__(32) RowJob {
-    int row, b, n, cached;  // no tokens: nothing to do
-    long long base, unused;
+    int row, b, n, cached;
+    int first, tiles;  // its query tiles among those of all rows, in the order of the jobs
+    long long base;    // where its key tiles begin in the workspace
 };
 
 // The tiles of 128 slots that any query of a row sees: [0, a1) for the sinks,
@@ -172,19 +173,24 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, i
     }
     int b = blockIdx.x - token_blocks;
     if (b == 0 && c.jobs) {  // the order in which chunk_attn takes the rows
-        __shared__ int seen[CP_SORTED];
-        for (int p = threadIdx.x; p < a.rows; p += 256) seen[p] = RowTiles(c, chunk_row(c, p)).n;
+        __shared__ int seen[CP_SORTED], tiles[CP_SORTED];
+        for (int p = threadIdx.x; p < a.rows; p += 256) {
+            const ChunkRow x = chunk_row(c, p);
+            seen[p] = RowTiles(c, x).n;
+            tiles[p] = seen[p] == 0 ? 0 : (x.n + c.P - 1) / c.P;
+        }
         __syncthreads();
         for (int p = threadIdx.x; p < a.rows; p += 256) {
-            int rank = 0;
+            int rank = 0, first = 0;
             long long base = 0;
             for (int q = 0; q < a.rows; ++q) {
-                rank += seen[q] > seen[p] || (seen[q] == seen[p] && q < p);
+                const bool ahead = seen[q] > seen[p] || (seen[q] == seen[p] && q < p);
+                rank += ahead;
+                first += ahead ? tiles[q] : 0;
                 base += q < p ? seen[q] : 0;
             }
             const ChunkRow x = chunk_row(c, p);
-            const bool none = x.idle || x.bad || base + seen[p] > c.key_tiles;
-            c.jobs[rank] = RowJob{p, x.b, none ? 0 : x.n, x.cached, base, 0};
+            c.jobs[rank] = RowJob{p, x.b, x.n, x.cached, first, tiles[p], base};
         }
         return;
     }
@@ -348,27 +354,46 @@ __device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
     return v;
 }
 
-// grid (splits * query tiles, KVH, rows), clusters of `splits` CTAs
+// Clusters of `splits` CTAs, one per (query tile, kv head): with jobs in their
+// order, a row's last query tile, which sees the most, first; without, in a grid
+// (splits * query tiles, KVH, rows) in which rows may have fewer.
 __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkArgs c, int splits) {
     extern __shared__ unsigned char ca_raw[];
     CaSmem& sm = *reinterpret_cast<CaSmem*>(ca_raw + ((1024u - (smem_u32(ca_raw) & 1023u)) & 1023u));
     const CacheAttnArgs& a = c.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = blockIdx.y, z = blockIdx.x % splits;
-    const int t = gridDim.x / splits - 1 - blockIdx.x / splits;  // the last query tile sees the most: first
-    int r = blockIdx.z;
+    const int z = blockIdx.x % splits;
+    int g, t, r;
     ChunkRow x;
     long long base;
     if (c.jobs) {
+        const int unit = blockIdx.x / splits, tile = unit / a.kv.KVH;
+        g = unit % a.kv.KVH;
         pdl_wait();
-        const int4 j = *reinterpret_cast<const int4*>(c.jobs + r);
-        base = c.jobs[r].base;
-        r = j.x;
-        x.b = j.y;
-        x.n = j.z;
-        x.cached = j.w;
+        t = -1;
+        for (int p = lane; p - lane < a.rows && t < 0; p += 32) {  // the job that has this tile
+            int4 j = make_int4(0, 0, 0, 0), k = j;
+            if (p < a.rows) {
+                j = reinterpret_cast<const int4*>(c.jobs)[2 * p];
+                k = reinterpret_cast<const int4*>(c.jobs)[2 * p + 1];
+            }
+            const unsigned has = __ballot_sync(FULL, tile >= k.x && tile - k.x < k.y);
+            if (has == 0) continue;
+            const int src = __ffs(has) - 1;
+            r = __shfl_sync(FULL, j.x, src);
+            x.b = __shfl_sync(FULL, j.y, src);
+            x.n = __shfl_sync(FULL, j.z, src);
+            x.cached = __shfl_sync(FULL, j.w, src);
+            t = __shfl_sync(FULL, k.y - 1 - (tile - k.x), src);
+            base = (long long)(((unsigned long long)(unsigned)__shfl_sync(FULL, k.w, src) << 32) |
+                               (unsigned)__shfl_sync(FULL, k.z, src));
+        }
+        if (t < 0) return;  // the grid holds the most tiles that there could be
         x.idle = x.bad = false;
     } else {
+        g = blockIdx.y;
+        r = blockIdx.z;
+        t = gridDim.x / splits - 1 - blockIdx.x / splits;
         x = chunk_row(c, r);
         base = row_base(c, r);
     }
@@ -381,7 +406,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     // where tile i of this CTA's list lies in the workspace
     auto tile_of = [&](int i) {
         const int tile = sm.list.tile(sm.k0 + i);
-        return (sm.base + (tile < sm.a1 ? tile : sm.a1 + tile - sm.b0)) * a.kv.KVH + blockIdx.y;
+        return (sm.base + (tile < sm.a1 ? tile : sm.a1 + tile - sm.b0)) * a.kv.KVH + g;
     };
     auto ask = [&](int n, int i, int value) {  // copy n: of tile i
         const int s = n % CA_STAGES;
@@ -754,7 +779,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             o = make_float4(fmaf(w, y.x, o.x), fmaf(w, y.y, o.y), fmaf(w, y.z, o.z), fmaf(w, y.w, o.w));
         }
         const long long tok = sm.token0 + row / c.n_rep;
-        reinterpret_cast<float4*>(a.out)[(tok * a.H + blockIdx.y * c.n_rep + row % c.n_rep) * 32 + col] = o;
+        reinterpret_cast<float4*>(a.out)[(tok * a.H + g * c.n_rep + row % c.n_rep) * 32 + col] = o;
     }
     if (splits > 1)  // peers still read this CTA's shared memory
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -1081,12 +1106,17 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     long long ctas = (long long)rows * tiles_x;
     if (ctas > tiles) ctas = tiles;
     ctas *= n_kv_heads;
-    // more than one wave of CTAs: the rows with most work first
-    c.jobs = ctas > 148 && rows <= CP_SORTED ? reinterpret_cast<RowJob*>(w + at.jobs) : nullptr;
     long long splits = 148 / ctas;
     if (splits > row_tiles) splits = row_tiles;
     if (splits > CA_MAX_SPLITS) splits = CA_MAX_SPLITS;
     if (splits < 1) splits = 1;
+    // A grid over rows of unequal length starts CTAs that have nothing to do; where
+    // it is more than one wave, the CTAs go by a list of the rows, the longest
+    // first.  (One wave does without: a row's numbers are then read before
+    // chunk_prep is over.)
+    const long long grid = splits * tiles_x * n_kv_heads * rows;
+    c.jobs = grid > 148 && rows <= CP_SORTED ? reinterpret_cast<RowJob*>(w + at.jobs) : nullptr;
+    if (c.jobs && ctas * splits > 0x7fffffffll) return fail(SKB_ERR_ARG, "%s: too many tokens and rows", what);
     const int prep_x = row_tiles < CP_TILES ? (int)row_tiles : CP_TILES;
     const int per_block = tokens <= 1024 ? 1 : 4;
     const int token_blocks = (tokens + per_block - 1) / per_block;
@@ -1101,7 +1131,7 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
                    prep_x);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)splits * tiles_x, n_kv_heads, rows);
+        cfg.gridDim = c.jobs ? dim3((unsigned)(ctas * splits)) : dim3((unsigned)splits * tiles_x, n_kv_heads, rows);
         cfg.blockDim = dim3(CA_THREADS);
         cfg.dynamicSmemBytes = CA_SMEM;
         cfg.stream = stream;
