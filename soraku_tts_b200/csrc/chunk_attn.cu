@@ -25,6 +25,7 @@ struct ChunkArgs {
     const int* chunk_start;  // [rows + 1]
     int tokens, max_chunk;
     int n_rep, P;           // heads per kv head, tokens per query tile
+    int rep_inv;            // x * rep_inv >> 16 is x / n_rep for x < 128
     // workspace
     unsigned char* qtiles;  // [query tiles][KVH][2 UT_BYTES]: queries in log2 units, hi | lo
     unsigned char* kvtiles; // [key tiles][KVH][2][2 UT_BYTES]: keys, values, hi | lo
@@ -311,8 +312,6 @@ struct CaSmem {
     int own[128];        // a row's slot; -1: no query
     int token0;          // token of the first query
     long long tile_at;   // query tile in the workspace
-    long long base;      // the row's key tiles there
-    int a1, b0;          // RowTiles of the row
     uint32_t tmem;
     int abort;
 };
@@ -403,25 +402,42 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         pdl_wait();
         return;
     }
-    // where tile i of this CTA's list lies in the workspace
-    auto tile_of = [&](int i) {
-        const int tile = sm.list.tile(sm.k0 + i);
-        return (sm.base + (tile < sm.a1 ? tile : sm.a1 + tile - sm.b0)) * a.kv.KVH + g;
-    };
-    auto ask = [&](int n, int i, int value) {  // copy n: of tile i
+    // where a tile of the row's keys lies in the workspace
+    auto place = [&](int tile) { return (base + rt.index(tile)) * a.kv.KVH + g; };
+    auto ask = [&](int n, int tile, int value) {  // copy n
         const int s = n % CA_STAGES;
         mbar_expect_tx(&sm.full[s], 2 * UT_BYTES);
-        bulk_g2s(sm.stage[s], c.kvtiles + (tile_of(i) * 2 + value) * (2 * UT_BYTES), 2 * UT_BYTES, &sm.full[s]);
+        bulk_g2s(sm.stage[s], c.kvtiles + (place(tile) * 2 + value) * (2 * UT_BYTES), 2 * UT_BYTES, &sm.full[s]);
     };
     if (tid == 32 * CA_WARP_P) {
+        // the first copies are on their way while the CTA gets ready; the
+        // queries by way of the last stage
         mbar_init(&sm.q_landed, 1);
+        for (int b = 0; b < CA_STAGES; ++b) mbar_init(&sm.full[b], 1);
+        mbar_fence_init();
+        const int nq = min(c.P, x.n - i0);
+        const TileList list(x.cached + i0, x.cached + i0 + nq - 1, a.window, a.sinks);
+        const int k0 = (int)((unsigned)z * (unsigned)list.n / (unsigned)splits);  // z < 8, fewer than 2^23 tiles
+        const int k1 = (int)((unsigned)(z + 1) * (unsigned)list.n / (unsigned)splits);
+        const long long tile_at = chunk_tile(c, x, r, t) * a.kv.KVH + g;
+        pdl_wait();
+        if (k0 < k1) {
+            mbar_expect_tx(&sm.q_landed, 2 * UT_BYTES);
+            bulk_g2s(sm.stage[CA_STAGES - 1], c.qtiles + tile_at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.q_landed);
+            ask(0, list.tile(k0), 0);
+            if (k0 + 1 < k1) ask(1, list.tile(k0 + 1), 0);
+        }
+        sm.list = list;
+        sm.k0 = k0;
+        sm.nt = k1 - k0;
+        sm.live = nq * c.n_rep;
+        sm.token0 = x.b + i0;
+        sm.tile_at = tile_at;
+    } else if (tid == 0) {
         mbar_init(&sm.q_full, CA_SOFTMAX_WARPS);
         mbar_init(&sm.o_free, CA_SOFTMAX_WARPS);
         mbar_init(&sm.o_full, 1);
-        for (int b = 0; b < CA_STAGES; ++b) {
-            mbar_init(&sm.full[b], 1);
-            mbar_init(&sm.empty[b], 1);
-        }
+        for (int b = 0; b < CA_STAGES; ++b) mbar_init(&sm.empty[b], 1);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&sm.s_full[b], 1);
             mbar_init(&sm.p_full[b], CA_SOFTMAX_WARPS);
@@ -430,29 +446,9 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         }
         mbar_fence_init();
         sm.abort = 0;
-        const int nq = min(c.P, x.n - i0);
-        const TileList list(x.cached + i0, x.cached + i0 + nq - 1, a.window, a.sinks);
-        sm.list = list;
-        sm.k0 = (int)((long long)z * list.n / splits);
-        sm.nt = (int)((long long)(z + 1) * list.n / splits) - sm.k0;
-        sm.live = nq * c.n_rep;
-        sm.token0 = x.b + i0;
-        sm.tile_at = chunk_tile(c, x, r, t) * a.kv.KVH + g;
-        sm.base = base;
-        sm.a1 = rt.a1;
-        sm.b0 = rt.b0;
-        pdl_wait();
-        // the first copies are on their way while the CTA gets ready; the
-        // queries by way of the last stage
-        if (sm.nt > 0) {
-            mbar_expect_tx(&sm.q_landed, 2 * UT_BYTES);
-            bulk_g2s(sm.stage[CA_STAGES - 1], c.qtiles + sm.tile_at * (2 * UT_BYTES), 2 * UT_BYTES, &sm.q_landed);
-            ask(0, 0, 0);
-            if (sm.nt > 1) ask(1, 1, 0);
-        }
     }
     if (tid < 128) {
-        const int q = tid / c.n_rep;
+        const int q = tid * c.rep_inv >> 16;
         sm.own[tid] = q < min(c.P, x.n - i0) ? x.cached + i0 + q : -1;
     }
     if (warp == CA_WARP_M) ut_alloc<512>(&sm.tmem);
@@ -472,7 +468,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                 if (n == CA_STAGES - 1 && !ut_wait(&sm.q_full, 0, abort)) return false;  // the queries were there
                 if (n >= CA_STAGES && !ut_wait(&sm.empty[n % CA_STAGES], ((n - CA_STAGES) / CA_STAGES) & 1, abort))
                     return false;
-                ask(n, i, value);
+                ask(n, sm.list.tile(sm.k0 + i), value);
                 ++n;
                 return true;
             };
@@ -527,7 +523,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         float E = UT_POISON_E;
         for (int i = 0; i < nt; ++i) {
             const int b = i & 1;
-            const float* at = c.meta + tile_of(i) * 256;
+            const float* at = c.meta + place(sm.list.tile(sm.k0 + i)) * 256;
             const float4 k = reinterpret_cast<const float4*>(at)[lane], v = reinterpret_cast<const float4*>(at)[32 + lane];
             // largest exponents (NaN aside): of each 32 values, of all
             float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
@@ -716,6 +712,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         l = 0.f;
 #pragma unroll
         for (int q = 0; q < CA_PARTS; ++q) l += sm.l[q][row];
+        if (*abort) l = __int_as_float(0x7fffffff);  // a wait that ran out shows as NaN
         float* stage = reinterpret_cast<float*>(sm.stage) + row * CA_OUT_LD + part * CA_W;
         // rows that saw nothing, and dead ones, give zeros
         const float f = l == 0.f || row >= sm.live ? 0.f : exp2_fast(E - 19.f) / l;
@@ -729,7 +726,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         }
         if (part == 0) sm.m[row] = m;
         softmax_sync();  // all parts have read the sums
-        if (part == 0) sm.l[0][row] = *abort ? __int_as_float(0x7fffffff) : l;  // a wait that ran out shows as NaN
+        if (part == 0) sm.l[0][row] = l;
         ut_fence_before();
     }
     __syncthreads();
@@ -737,39 +734,44 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         ut_fence_after();
         ut_free<512>(tmem);
     }
+    auto place_out = [&](int row) {  // a row's output, in float4
+        const int q = row * c.rep_inv >> 16;  // row / n_rep
+        return reinterpret_cast<float4*>(a.out) + ((long long)(sm.token0 + q) * a.H + g * c.n_rep + row - q * c.n_rep) * 32;
+    };
+    if (splits == 1) {  // a CTA alone: its rows leave as they are, in whole lines
+        for (int row = warp; row < sm.live; row += CA_THREADS / 32)
+            place_out(row)[lane] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.stage) + row * CA_OUT_LD + 4 * lane);
+        return;
+    }
     // ---- join the splits: CTA z of the cluster takes a part of the rows.  The
     // weights of all rows first, then all outputs: two trips to the peers' memory
     // in all, where a warp that took row after row made two for each.
-    if (splits > 1)
-        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     const int part = blockIdx.x % splits;
     const int ra = part * sm.live / splits, rb = (part + 1) * sm.live / splits;
     float (*weight)[128] = sm.mx[0];  // [split][row]; the maxima are done with
     static_assert(2 * CA_PARTS >= CA_MAX_SPLITS, "weights fit the maxima's place");
-    if (splits > 1) {
-        for (int i = tid; i < (rb - ra) * splits; i += CA_THREADS) {
-            const int row = ra + i / splits, p = i % splits;
-            float M = CO_LOW, L = 0.f, mine = 0.f;
+    for (int i = tid; i < (rb - ra) * splits; i += CA_THREADS) {
+        const int row = ra + i / splits, p = i % splits;
+        float M = CO_LOW, L = 0.f, mine = 0.f;
 #pragma unroll 4
-            for (int q = 0; q < splits; ++q) {
-                const float m = ld_peer(&sm.m[row], q), l = ld_peer(&sm.l[0][row], q);
-                const float up = fmaxf(M, m), f = exp2_fast(M - up), w = l * exp2_fast(m - up);
-                mine = q == p ? w : mine * f;
-                L = fmaf(L, f, w);
-                M = up;
-            }
-            weight[p][row] = mine / L;  // not a number where a wait ran out
-            if (c.lse && p == 0) c.lse[sm.tile_at * 128 + row] = M + log2f(L);
+        for (int q = 0; q < splits; ++q) {
+            const float m = ld_peer(&sm.m[row], q), l = ld_peer(&sm.l[0][row], q);
+            const float up = fmaxf(M, m), f = exp2_fast(M - up), w = l * exp2_fast(m - up);
+            mine = q == p ? w : mine * f;
+            L = fmaf(L, f, w);
+            M = up;
         }
-        __syncthreads();
+        weight[p][row] = mine / L;
+        if (c.lse && p == 0) c.lse[sm.tile_at * 128 + row] = M + log2f(L);
     }
+    __syncthreads();
     const uint32_t stage = smem_u32(sm.stage);
-    const float alone = *abort ? __int_as_float(0x7fffffff) : 1.f;  // not a number where a wait ran out
     for (int i = tid; i < (rb - ra) * 32; i += CA_THREADS) {
         const int row = ra + (i >> 5), col = i & 31;
         const int at = row * CA_OUT_LD + 4 * col;
         float4 o = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.stage) + at);
-        const float own = splits > 1 ? weight[part][row] : alone;
+        const float own = weight[part][row];
         o = make_float4(o.x * own, o.y * own, o.z * own, o.w * own);
 #pragma unroll 2
         for (int q = 1; q < splits; ++q) {
@@ -778,11 +780,10 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
             const float w = weight[p][row];
             o = make_float4(fmaf(w, y.x, o.x), fmaf(w, y.y, o.y), fmaf(w, y.z, o.z), fmaf(w, y.w, o.w));
         }
-        const long long tok = sm.token0 + row / c.n_rep;
-        reinterpret_cast<float4*>(a.out)[(tok * a.H + g * c.n_rep + row % c.n_rep) * 32 + col] = o;
+        place_out(row)[col] = o;
     }
-    if (splits > 1)  // peers still read this CTA's shared memory
-        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // peers still read this CTA's shared memory
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // -------------------------------------------------------------- chunk_mass
@@ -1087,6 +1088,7 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     c.max_chunk = max_chunk;
     c.n_rep = n_heads / n_kv_heads;
     c.P = 128 / c.n_rep;
+    c.rep_inv = (65535 + c.n_rep) / c.n_rep;
     const long long tiles = chunk_query_tiles(tokens, rows, c.n_rep);
     c.key_tiles = chunk_key_tiles(rows, max_chunk, max_pages, page_size, n_pages, window, sinks);
     const ChunkWork at(tiles, c.key_tiles, n_kv_heads, rows, mass != nullptr);
