@@ -10,8 +10,13 @@
 // fp16 tiles (umma.cuh) in the order in which the tensor cores read them;
 // chunk_attn; and, with `mass`, chunk_mass.  The tiles are written once for
 // all query tiles of a row: splitting them inside chunk_attn, per query tile,
-// kept its warps busy for two thirds of the time (8 queries tiles of 512 tokens
-// over 8192 slots: 160 us against 8.5 us of chunk_prep, measured).
+// took its warps 7 to 11 thousand cycles a key tile, against 4 thousand now.
+// chunk_prep is bound by memory (8 prompts of 611 to 1024 tokens: 270 MB in 61
+// us, 4.4 TB/s), chunk_attn by the softmax of a tile (4 thousand cycles, beside
+// 3.1 thousand of products) and, in short rows, by the 9 thousand cycles in which a
+// CTA fills and drains its pipeline (the 8 prompts: 110 us; 512 tokens behind
+// 8192 slots: 90 us, 1.2 PFLOP/s of fp16 products, 70 % of what a library's
+// bf16 product reaches).
 // A query tile is 128 (token, head) pairs of one kv head, P = 128 / n_rep
 // tokens, so a key or value tile that was loaded once serves all of them.
 #include <type_traits>
@@ -740,7 +745,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     };
     if (splits == 1) {  // a CTA alone: its rows leave as they are, in whole lines
         for (int row = warp; row < sm.live; row += CA_THREADS / 32)
-            place_out(row)[lane] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.stage) + row * CA_OUT_LD + 4 * lane);
+            place_out(row)[lane] = reinterpret_cast<const float4*>(sm.stage)[row * (CA_OUT_LD / 4) + lane];
         return;
     }
     // ---- join the splits: CTA z of the cluster takes a part of the rows.  The
@@ -1104,7 +1109,9 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     // key tiles of one row, at most
     const long long row_tiles = chunk_key_tiles(1, most, max_pages, page_size, n_pages, window, sinks);
     // CTAs that have work, at most; while they leave SMs idle, up to 8 share a
-    // query tile's key tiles.
+    // query tile's key tiles.  (Sharing where they fill the card already makes
+    // clusters wait for SMs and adds the join: 8 prompts 199 us in pairs, 117 alone;
+    // two rows of five tokens 13.7 us alone, 12.5 in eights.)
     long long ctas = (long long)rows * tiles_x;
     if (ctas > tiles) ctas = tiles;
     ctas *= n_kv_heads;

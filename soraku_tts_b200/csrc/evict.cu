@@ -20,7 +20,10 @@
 //           without any order between them.  Where rows come from and go to is looked up
 //           for EV_BLOCK rows at once, so that a round waits for its data alone,
 //           and two rounds are on their way at a time.
-// Bound by memory: each kept slot that moves is 1 KB in and 1 KB out.
+// Bound by memory: each kept slot that moves is 1 KB in and 1 KB out (128 groups
+// of 5k to 8k slots to 2k: 119 us, 70 % of a plain copy's rate; two rounds are what
+// the registers hold, and a longer ring in shared memory, with fewer CTAs an SM,
+// took 122 us, and 142 instead of 120 at 32k slots).
 #include "cache_ops.cuh"
 
 namespace skb {
