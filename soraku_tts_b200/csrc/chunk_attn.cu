@@ -30,7 +30,7 @@ struct ChunkArgs {
     const int* chunk_start;  // [rows + 1]
     int tokens, max_chunk;
     int n_rep, P;           // heads per kv head, tokens per query tile
-    int rep_inv;            // x * rep_inv >> 16 is x / n_rep for x < 128
+    unsigned rep_inv;       // for over_rep
     // workspace
     unsigned char* qtiles;  // [query tiles][KVH][2 UT_BYTES]: queries in log2 units, hi | lo
     unsigned char* kvtiles; // [key tiles][KVH][2][2 UT_BYTES]: keys, values, hi | lo
@@ -39,6 +39,11 @@ struct ChunkArgs {
     struct RowJob* jobs;    // [rows]: by the tiles they see, most first; null: rows as they are
     long long key_tiles;
 };
+
+// x / n_rep without a division; right for x below 2^22 at least.
+__device__ __forceinline__ int over_rep(const ChunkArgs& c, int x) {
+    return (int)((unsigned long long)(unsigned)x * c.rep_inv >> 24);
+}
 
 // What a row asks for: its tokens [b, b + n) and whether its numbers lie
 // inside the inputs, the cache and the RoPE tables.
@@ -102,6 +107,20 @@ __device__ __forceinline__ float query_exponent(const float* qn, int lane) {
     return (float)max(-100, min(127, e));
 }
 
+// A head vector, a float4 per lane: RMSNorm with weight w, then rotated.
+__device__ __forceinline__ float4 norm_rope(float4 x, float4 w, float eps, float4 c, float4 s, int lane) {
+    const float inv = rsqrtf(warp_sum(x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w) / 128.0f + eps);
+    x = make_float4(w.x * (x.x * inv), w.y * (x.y * inv), w.z * (x.z * inv), w.w * (x.w * inv));
+    float4 o;  // the other half's: 64 elements away
+    o.x = __shfl_xor_sync(FULL, x.x, 16);
+    o.y = __shfl_xor_sync(FULL, x.y, 16);
+    o.z = __shfl_xor_sync(FULL, x.z, 16);
+    o.w = __shfl_xor_sync(FULL, x.w, 16);
+    const float t = lane < 16 ? -1.f : 1.f;
+    return make_float4(x.x * c.x + t * (o.x * s.x), x.y * c.y + t * (o.y * s.y), x.z * c.z + t * (o.z * s.z),
+                       x.w * c.w + t * (o.w * s.w));
+}
+
 constexpr float CH_QSCALE = 0.08838834764831845f * CO_LOG2E;  // 1 / sqrt(128), scores in log2 units
 
 constexpr int CP_TILES = 64;     // blocks side by side over a row's key tiles
@@ -142,9 +161,14 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, i
         }
         const int pos = a.pos[r] + i, slot = x.cached + i;
         const float4* row = reinterpret_cast<const float4*>(a.qkv) + (long long)t * nv * 32 + lane;
-        const float* cosr = a.rope_cos + (long long)pos * 64;
-        const float* sinr = a.rope_sin + (long long)pos * 64;
-        const long long tile = base + rt.index(slot >> 7);
+        // what all vectors of the token share, in registers
+        const float4 cs = reinterpret_cast<const float4*>(a.rope_cos + (long long)pos * 64)[lane & 15];
+        const float4 sn = reinterpret_cast<const float4*>(a.rope_sin + (long long)pos * 64)[lane & 15];
+        const float4 qw = __ldg(reinterpret_cast<const float4*>(a.qn) + lane);
+        const float4 kw = __ldg(reinterpret_cast<const float4*>(a.kn) + lane);
+        const long long tile = base + rt.index(slot >> 7), unit0 = a.kv.key_unit(r, slot, 0);
+        const int qrow = i % c.P * c.n_rep;
+        unsigned char* qtile = c.qtiles + chunk_tile(c, x, r, i / c.P) * KVH * (2 * UT_BYTES);
         for (int v0 = w; v0 < nv; v0 += 4 * wpt) {
             float4 y[4];
 #pragma unroll
@@ -154,15 +178,14 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, i
             for (int j = 0; j < 4; ++j) {
                 const int v = v0 + wpt * j;
                 if (v >= nv) break;
-                if (v < H + KVH) y[j] = norm_rope_head(y[j], v < H ? a.qn : a.kn, a.eps, cosr, sinr, lane, true, true);
+                if (v < H + KVH) y[j] = norm_rope(y[j], v < H ? qw : kw, a.eps, cs, sn, lane);
                 if (v < H) {
-                    const int g = v / c.n_rep, m = (i % c.P) * c.n_rep + v % c.n_rep;
-                    unsigned char* q = c.qtiles + (chunk_tile(c, x, r, i / c.P) * KVH + g) * (2 * UT_BYTES);
-                    put4(q + ut_at(m, lane), y[j], CH_QSCALE * pow2_whole(13.f - eq));
+                    const int g = over_rep(c, v), m = qrow + v - g * c.n_rep;
+                    put4(qtile + (long long)g * (2 * UT_BYTES) + ut_at(m, lane), y[j], CH_QSCALE * pow2_whole(13.f - eq));
                     continue;
                 }
                 const int value = v >= H + KVH, g = v - H - (value ? KVH : 0);
-                const long long u = a.kv.key_unit(r, slot, g);
+                const long long u = unit0 < 0 ? -1 : unit0 + ((long long)g << a.kv.page_log2);
                 if (u >= 0) reinterpret_cast<float4*>(a.kv.pool)[(u + (value ? a.kv.value_step() : 0)) * 32 + lane] = y[j];
                 float top = max3_abs(max3_abs(y[j].x, y[j].y, y[j].z), y[j].w, 0.f);
 #pragma unroll
@@ -453,7 +476,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         sm.abort = 0;
     }
     if (tid < 128) {
-        const int q = tid * c.rep_inv >> 16;
+        const int q = over_rep(c, tid);
         sm.own[tid] = q < min(c.P, x.n - i0) ? x.cached + i0 + q : -1;
     }
     if (warp == CA_WARP_M) ut_alloc<512>(&sm.tmem);
@@ -740,7 +763,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
         ut_free<512>(tmem);
     }
     auto place_out = [&](int row) {  // a row's output, in float4
-        const int q = row * c.rep_inv >> 16;  // row / n_rep
+        const int q = over_rep(c, row);
         return reinterpret_cast<float4*>(a.out) + ((long long)(sm.token0 + q) * a.H + g * c.n_rep + row - q * c.n_rep) * 32;
     };
     if (splits == 1) {  // a CTA alone: its rows leave as they are, in whole lines
@@ -950,8 +973,8 @@ __global__ void __launch_bounds__(CM_THREADS, 2) chunk_mass_kernel(const ChunkAr
             // seen whole: every column is a query, behind every slot, inside the window
             const bool whole = nq * c.n_rep >= column + CM_N && first >= base + 127 &&
                                (a.window == 0 || first + nq - 1 - base < a.window || base + 128 <= a.sinks);
-            if (!whole) {  // one division a column, not one a weight
-                const int qi = (column + part * CM_W + lane) / c.n_rep;
+            if (!whole) {  // once a column, not once a weight
+                const int qi = over_rep(c, column + part * CM_W + lane);
                 sm.own[warp][lane] = qi < nq ? first + qi : -1;
                 __syncwarp();
             }
@@ -1093,7 +1116,7 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     c.max_chunk = max_chunk;
     c.n_rep = n_heads / n_kv_heads;
     c.P = 128 / c.n_rep;
-    c.rep_inv = (65535 + c.n_rep) / c.n_rep;
+    c.rep_inv = ((1u << 24) + c.n_rep - 1) / c.n_rep;
     const long long tiles = chunk_query_tiles(tokens, rows, c.n_rep);
     c.key_tiles = chunk_key_tiles(rows, max_chunk, max_pages, page_size, n_pages, window, sinks);
     const ChunkWork at(tiles, c.key_tiles, n_kv_heads, rows, mass != nullptr);
