@@ -11,10 +11,10 @@
 // chunk_attn; and, with `mass`, chunk_mass.  The tiles are written once for
 // all query tiles of a row: splitting them inside chunk_attn, per query tile,
 // took its warps 7 to 11 thousand cycles a key tile, against 4 thousand now.
-// chunk_prep is bound by memory (8 prompts of 611 to 1024 tokens: 270 MB in 61
-// us, 4.4 TB/s), chunk_attn by the softmax of a tile (4 thousand cycles, beside
+// chunk_prep is bound by memory (8 prompts of 611 to 1024 tokens: 270 MB in 55
+// us, 4.9 TB/s), chunk_attn by the softmax of a tile (4 thousand cycles, beside
 // 3.1 thousand of products) and, in short rows, by the 9 thousand cycles in which a
-// CTA fills and drains its pipeline (the 8 prompts: 110 us; 512 tokens behind
+// CTA fills and drains its pipeline (the 8 prompts: 108 us; 512 tokens behind
 // 8192 slots: 90 us, 1.2 PFLOP/s of fp16 products, 70 % of what a library's
 // bf16 product reaches).
 // A query tile is 128 (token, head) pairs of one kv head, P = 128 / n_rep
@@ -228,29 +228,31 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, i
     b /= tiles_x;
     const int value = b & 1, g = (b >> 1) % KVH, r = (b >> 1) / KVH;
     const ChunkRow x = chunk_row(c, r);
+    const long long base = row_base(c, r);  // asked for beside the row's own numbers
     const RowTiles rt(c, x);
-    if (k0 >= rt.n) return;
-    const long long base = row_base(c, r);
-    if (base + rt.n > c.key_tiles) return;
+    if (k0 >= rt.n || base + rt.n > c.key_tiles) return;
     const float* pool = a.kv.pool + (value ? a.kv.value_step() * 128 : 0);
     const int row0 = warp * 16, i4 = lane >> 3, last = x.cached + x.n - 1;
     for (int k = k0; k < rt.n; k += tiles_x) {
         const int first = rt.tile(k) * 128 + row0;
         if (first >= x.cached && first + 15 <= last) continue;  // new tokens only: theirs are written above
         const long long at = ((base + k) * KVH + g) * 2 + value;
-#pragma unroll 1
+        uint32_t units[4];  // of this lane's rows i4, 4 + i4, ...: one look at the page table
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int slot = first + 4 * q + i4;
+            units[q] = UT_NONE;
+            if (slot < x.cached && (slot >= rt.w0 || slot < a.sinks)) {
+                const long long u = a.kv.key_unit(r, slot, g);
+                units[q] = u < 0 ? UT_BAD : (uint32_t)u;
+            }
+        }
+#pragma unroll
         for (int part = 0; part < 16; part += 4 * CP_NQ) {
             RowSet<CP_NQ> d;
             uint32_t unit[CP_NQ];
 #pragma unroll
-            for (int q = 0; q < CP_NQ; ++q) {
-                const int slot = first + part + 4 * q + i4;
-                unit[q] = UT_NONE;
-                if (slot < x.cached && (slot >= rt.w0 || slot < a.sinks)) {
-                    const long long u = a.kv.key_unit(r, slot, g);
-                    unit[q] = u < 0 ? UT_BAD : (uint32_t)u;
-                }
-            }
+            for (int q = 0; q < CP_NQ; ++q) unit[q] = units[part / 4 + q];
 #pragma unroll
             for (int q = 0; q < CP_NQ; ++q) d.load(q, pool, unit[q], lane);
 #pragma unroll
