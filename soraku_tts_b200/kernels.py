@@ -300,6 +300,8 @@ def _cache_attention(name, qkv, n_heads, n_kv_heads, q_norm, k_norm, eps, rope_c
         raise ValueError("kv_pool and page_table must hold at least one page")
     if out is None:
         out = qkv.new_empty((tokens, n_heads * 128))
+    if rows == 0 or tokens == 0:  # nothing to do, and empty tensors have no address
+        return out
     with_mass = 0 if mass is None else 1
     need = 0
     if chunk_start is not None:

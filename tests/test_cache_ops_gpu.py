@@ -649,6 +649,74 @@ def test_on_another_stream_and_in_graphs():
             assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("rows", [2, 40])
+def test_a_graph_serves_other_lengths(rows):
+    """Lengths, fill and positions are read on the device: a captured chunk call is
+    right for any others within its sizes, longer and shorter rows, empty and idle ones."""
+    from soraku_tts_b200 import kernels
+
+    most, tokens = 90, 60 * rows
+    c = Cache([70] * rows, 300, 4, 2, seed=44)
+    static, start = c.qkv(tokens), starts([60] * rows)
+    out = torch.empty(tokens, 4 * HD, device="cuda")
+
+    def call():
+        kernels.chunk_attention(static, chunk_start=start, max_chunk=most, mass=c.mass, window=120, sinks=5, out=out, **c.args())
+
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for step in range(3):
+        lengths = [(17 * r + 31 * step) % most for r in range(rows)]
+        while sum(lengths) > tokens:
+            lengths[lengths.index(max(lengths))] = 0
+        fill = torch.tensor([(r * 37 + 50 * step) % 200 for r in range(rows)], dtype=torch.int32, device="cuda")
+        fill[step % rows] = -1
+        c.cached.copy_(fill)
+        c.pos.copy_(torch.clamp(fill, min=0) + 3 * step)
+        start.copy_(starts(lengths))
+        static.copy_(c.qkv(tokens))
+        c.pool64, c.mass64 = c.pool.double(), c.mass.double()
+        out.fill_(5.0)
+        g.replay()
+        n = sum(lengths)
+        close(out[:n], c.want(static[:n], lengths, 120, 5, True))
+        assert torch.equal(out[n:], torch.full_like(out[n:], 5.0))
+        c.check_cache()
+        c.check_mass()
+
+
+def test_mass_may_start_undefined():
+    """New slots are set, not added to, and slots that no query sees are left."""
+    for form in ("chunk", "decode"):
+        c = Cache((100, 0, 33), 20, 4, 2, seed=45)
+        before = c.mass.clone()
+        for r, n in enumerate((100, 0, 33)):
+            c.mass[r, :, n:] = math.nan
+            c.mass64[r, :, n:] = 0
+        lengths = (20, 7, 1) if form == "chunk" else (1, 1, 1)
+        (chunk(c, lengths, 30, 2, mass=True) if form == "chunk" else decode(c, 30, 2, mass=True))
+        for r, (n, new) in enumerate(zip((100, 0, 33), lengths)):
+            assert torch.isnan(c.mass[r, :, n + new:]).all()
+            close(c.mass[r, :, :n + new].reshape(-1, 1), c.mass64[r, :, :n + new].reshape(-1, 1))
+        assert torch.equal(c.mass[0, :, 2:70], before[0, :, 2:70])
+
+
+def test_no_rows_and_no_tokens():
+    from soraku_tts_b200 import kernels
+
+    c = Cache((5, 9), 4, seed=61)
+    pool = c.pool.clone()
+    out = kernels.chunk_attention(c.qkv(0), chunk_start=starts((0, 0)), max_chunk=4, mass=c.mass, **c.args())
+    assert out.shape == (0, 16 * HD) and torch.equal(c.pool, pool)
+    none = dict(cached=c.cached[:0], pos=c.pos[:0], page_table=c.table[:0])
+    assert kernels.chunk_attention(c.qkv(0), chunk_start=starts(()), max_chunk=0, **c.args(**none)).shape == (0, 16 * HD)
+    assert kernels.window_decode_attention(c.qkv(0), **c.args(**none)).shape == (0, 16 * HD)
+    kept, mass, cached = kernels.evict_cache(c.mass[:0], cached=c.cached[:0], kv_pool=c.pool, page_table=c.table[:0],
+                                             page_size=c.page, budget=3)
+    assert kept.shape == (0, 8, 3) and mass.shape == c.mass[:0].shape and cached.shape == (0,)
+
+
 def test_offsets_past_32_bits():
     """Pages more than 2^31 floats into the pool."""
     from soraku_tts_b200 import kernels
