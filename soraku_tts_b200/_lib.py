@@ -152,10 +152,3 @@ def stream_ptr(stream=None) -> int:
 
     s = torch.cuda.current_stream() if stream is None else stream
     return int(s.cuda_stream)
-
-
-def device_stream_ptr(device: int) -> int:
-    """Raw cudaStream_t of the current torch stream of a device."""
-    import torch
-
-    return torch._C._cuda_getCurrentRawStream(device)

@@ -15,6 +15,8 @@ CUDA tensors (float32, codes int64), as the reference's packed ABI requires
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -263,10 +265,16 @@ def _dims(t, name: str, n: int, what: str):
 
 def _on(device: int, fn, *args):
     """fn(*args) with ``device`` current, as kernel launches need it."""
-    if torch.cuda.current_device() == device:
+    if torch._C._cuda_getDevice() == device:  # torch.cuda.current_device(), which costs three times as much
         return fn(*args)
     with torch.cuda.device(device):
         return fn(*args)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(name: str, *sizes: int) -> int:
+    """Bytes of workspace, a function of sizes alone; asking the library costs 1 us."""
+    return getattr(_lib.lib(), name)(*sizes)
 
 
 def _cache_attention(name, qkv, n_heads, n_kv_heads, q_norm, k_norm, eps, rope_cos, rope_sin, chunk_start, max_chunk,
@@ -305,17 +313,17 @@ def _cache_attention(name, qkv, n_heads, n_kv_heads, q_norm, k_norm, eps, rope_c
     with_mass = 0 if mass is None else 1
     need = 0
     if chunk_start is not None:
-        need = _lib.lib().skb_chunk_attention_workspace(tokens, rows, max_chunk, n_heads, n_kv_heads, max_pages, page_size,
-                                                        n_pages, window, sinks, with_mass)
+        need = _workspace("skb_chunk_attention_workspace", tokens, rows, max_chunk, n_heads, n_kv_heads, max_pages,
+                          page_size, n_pages, window, sinks, with_mass)
     elif with_mass:
-        need = _lib.lib().skb_window_decode_workspace(rows, n_heads, max_pages, page_size, window, sinks, 1)
+        need = _workspace("skb_window_decode_workspace", rows, n_heads, max_pages, page_size, window, sinks, 1)
     work = torch.empty(need, dtype=torch.uint8, device=qkv.device) if need > 0 else None
     chunk = () if chunk_start is None else (chunk_start.data_ptr(), max_chunk)
     _on(device, _lib.call, name, qkv.data_ptr(), *(() if chunk_start is None else (tokens,)), rows, n_heads, n_kv_heads, 128,
         q_norm.data_ptr(), k_norm.data_ptr(), float(eps), rope_cos.data_ptr(), rope_sin.data_ptr(), positions, *chunk,
         cached.data_ptr(), pos.data_ptr(), kv_pool.data_ptr(), page_table.data_ptr(), max_pages, page_size, n_pages, window,
         sinks, mass.data_ptr() if with_mass else None, None if work is None else work.data_ptr(), max(need, 0),
-        out.data_ptr(), _lib.device_stream_ptr(device))
+        out.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
     return out
 
 
@@ -380,5 +388,5 @@ def evict_cache(mass: torch.Tensor, *, cached: torch.Tensor, kv_pool: torch.Tens
     if rows > 0:
         _on(device, _lib.call, "skb_evict_cache", mass.data_ptr(), cached.data_ptr(), rows, kvh, 128, kv_pool.data_ptr(),
             page_table.data_ptr(), max_pages, page_size, n_pages, budget, sinks, recent, kept.data_ptr(),
-            mass_out.data_ptr(), cached_out.data_ptr(), _lib.device_stream_ptr(device))
+            mass_out.data_ptr(), cached_out.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
     return kept, mass_out, cached_out
