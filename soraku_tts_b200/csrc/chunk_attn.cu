@@ -334,7 +334,8 @@ struct CaSmem {
     float E[2];                          // running exponent of the values
     float vtop[2][CA_PARTS];             // largest exponent of a part's values
     float own_vg[CA_SOFTMAX_WARPS][CA_W];  // a warp's factors in a tile that is not whole
-    uint64_t q_landed, q_full, full[CA_STAGES], empty[CA_STAGES], s_full[2], p_full[2], pv_done[2], o_free, meta_full[2], o_full;
+    uint64_t q_landed, q_full, full[CA_STAGES], empty[CA_STAGES], s_full[2], p_full[2], pv_done[2], o_free, meta_full[2];
+    uint64_t s_end, o_full;  // every product of warp M, of warp O
     // what the CTA works on
     TileList list;
     int k0, nt;          // its key tiles: list entries [k0, k0 + nt)
@@ -466,6 +467,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     } else if (tid == 0) {
         mbar_init(&sm.q_full, CA_SOFTMAX_WARPS);
         mbar_init(&sm.o_free, CA_SOFTMAX_WARPS);
+        mbar_init(&sm.s_end, 1);
         mbar_init(&sm.o_full, 1);
         for (int b = 0; b < CA_STAGES; ++b) mbar_init(&sm.empty[b], 1);
         for (int b = 0; b < 2; ++b) {
@@ -527,6 +529,8 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                 ut_commit(&sm.empty[s]);
                 ut_commit(&sm.s_full[i & 1]);
             }
+            ut_commit(&sm.s_end);
+            mbar_wait(&sm.s_end, 0, nullptr);
         }
         __syncwarp();
     } else if (warp == CA_WARP_O) {
@@ -545,8 +549,8 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
                 ut_commit(&sm.empty[s]);
                 ut_commit(&sm.pv_done[i & 1]);
             }
-            ut_commit(&sm.o_full);  // every P V issued so far, and so every S before them
-            ut_wait(&sm.o_full, 0, abort);
+            ut_commit(&sm.o_full);
+            mbar_wait(&sm.o_full, 0, nullptr);  // tensor memory is not given back under a product
         }
         __syncwarp();
     } else if (warp == CA_WARP_E) {
