@@ -191,7 +191,8 @@ int skb_decode_attention_noalloc(const float *qkv, int rows, int n_heads, int n_
  *               tokens before chunk_start[0] and behind chunk_start[rows] are
  *               neither read nor written
  *   rope_cos/sin device [max_pos, 64];  cached, pos: device int32 [rows]
- *   kv_pool, page_table as for skb_decode_attention
+ *   kv_pool, page_table as for skb_decode_attention, but kv_pool is 32-byte
+ *               aligned (16 is enough for the two operators below)
  *   out         device [tokens, n_heads * 128]
  * The workspace holds the queries and the seen keys and values in the form the
  * tensor cores read: about 1 KB per kv head for each slot that max_pages (or the

@@ -1092,6 +1092,8 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     if (st != SKB_OK) return st;
     if (!chunk_start) return fail(SKB_ERR_ARG, "%s: null pointer", what);
     if (tokens < 0 || max_chunk < 0) return fail(SKB_ERR_ARG, "%s: bad sizes", what);
+    if ((uintptr_t)kv_pool & 31u)  // chunk_prep reads cached rows 32 bytes a lane
+        return fail(SKB_ERR_ARG, "%s: kv_pool must be 32-byte aligned", what);
     if ((long long)n_pages * 2 * n_kv_heads * page_size >= 0xfffffffell)
         return fail(SKB_ERR_ARG, "%s: the pool must hold fewer than 2^32 - 2 key and value rows", what);
     if (rows == 0 || tokens == 0) return SKB_OK;

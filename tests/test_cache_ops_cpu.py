@@ -67,6 +67,15 @@ def test_evict_cache_refuses(lib, change):
     assert "evict_cache" in lib.last_error()
 
 
+@pytest.mark.parametrize("offset", [4, 8, 16, 48])
+def test_chunk_attention_wants_a_pool_at_32_bytes(lib, offset):
+    """Its loads of cached rows are 32 bytes wide; even a call without work says so."""
+    for change in ({}, dict(tokens=0), dict(rows=0)):
+        args = dict(CHUNK, kv_pool=A + offset, **change)
+        assert lib.lib().skb_chunk_attention(*args.values()) == lib.SKB_ERR_ARG
+        assert "kv_pool" in lib.last_error()
+
+
 def test_no_rows_or_no_tokens_is_no_work(lib):
     L = lib.lib()
     assert L.skb_chunk_attention(*dict(CHUNK, rows=0, qkv=None, out=None).values()) == lib.SKB_OK

@@ -450,6 +450,25 @@ def test_decode_agrees_with_chunks_of_one():
     close(a, b.double())
 
 
+def test_pool_between_32_byte_borders():
+    """A pool 16 bytes behind such a border: refused by the chunk call, whose loads
+    are that wide, before a launch; right in decode and eviction."""
+    from soraku_tts_b200 import kernels
+
+    c = Cache((40, 90), 1, 4, 2, seed=13)
+    memory = torch.empty(c.pool.numel() + 4, device="cuda")
+    shifted = memory[4:].view(c.pool.shape)
+    assert shifted.data_ptr() % 32 == 16
+    shifted.copy_(c.pool)
+    c.pool = shifted
+    with pytest.raises(ValueError, match="kv_pool"):
+        chunk(c, (1, 1))
+    got, want = decode(c, 50, 3, mass=True)
+    close(got, want)
+    c.check_cache()
+    check_evict(c, 33, 2, 5)
+
+
 # ----------------------------------------------------------------- eviction
 def plain_evict(c, budget, sinks, recent):
     kept, mass = [], torch.zeros_like(c.mass)
