@@ -90,12 +90,19 @@ struct RowTiles {
     __device__ __forceinline__ int index(int tile) const { return tile < a1 ? tile : a1 + tile - b0; }
     __device__ __forceinline__ int tile(int k) const { return k < a1 ? k : b0 + k - a1; }
 };
+// Sum of a count over a warp.
+__device__ __forceinline__ long long warp_total(long long n) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
+    return n;
+}
 // Where a row's key tiles begin in the workspace: behind those of the rows
-// before it.  By a whole warp.
+// before it.  By a whole warp.  In 64 bits: a row's count is up to 2^23 tiles, so
+// 256 rows of counts that no pool holds pass 32.
 __device__ __forceinline__ long long row_base(const ChunkArgs& c, int r) {
-    int n = 0;
+    long long n = 0;
     for (int p = threadIdx.x & 31; p < r; p += 32) n += RowTiles(c, chunk_row(c, p)).n;
-    return __reduce_add_sync(FULL, n);
+    return warp_total(n);
 }
 
 // A whole number e with |q| < 2^e for every query in log2 units: a normed head

@@ -758,6 +758,29 @@ def test_offsets_past_32_bits():
     assert torch.equal(big[far:], c.pool)
 
 
+def test_row_counts_whose_sum_passes_32_bits():
+    """299 rows of 2^23 tiles' worth of slots that no page holds (their sum is
+    above 2^31) behind a sound row: NaN for them, nothing written, the sound row right."""
+    from soraku_tts_b200 import kernels
+
+    rows, page, filled = 300, 2**23, 5
+    c = Cache((filled,), 1, 2, 1, page=8, spare=0, seed=62)
+    qkv = c.qkv(rows)
+    pool = torch.zeros(1, 2, 1, page, HD, device="cuda")
+    pool[:, :, :, :8] = c.pool
+    table = torch.full((rows, 2**30 // page), -1, dtype=torch.int32, device="cuda")
+    table[0, 0] = 0
+    cached = torch.full((rows,), 2**30 - 2, dtype=torch.int32, device="cuda")
+    cached[0] = filled
+    got = kernels.chunk_attention(qkv, chunk_start=starts([1] * rows), max_chunk=1,
+                                  **c.args(kv_pool=pool, page_table=table, page_size=page, cached=cached,
+                                           pos=torch.full_like(cached, filled)))
+    assert torch.isnan(got[1:]).all()
+    close(got[:1], c.want(qkv[:1], (1,)))
+    torch.testing.assert_close(pool[:, :, :, :8].double(), c.pool64, rtol=0, atol=5e-6)
+    assert not pool[:, :, :, 8:].any()
+
+
 def test_python_layer_refusals():
     from soraku_tts_b200 import kernels
 
