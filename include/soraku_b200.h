@@ -198,7 +198,7 @@ int skb_decode_attention_noalloc(const float *qkv, int rows, int n_heads, int n_
  * tensor cores read: about 1 KB per kv head for each slot that max_pages (or the
  * window and max_chunk) lets a row see, and never more than the pool's size;
  * 512 B per token and head; and, as tiles are not shared by rows, up to 330 KB
- * per row and kv head. */
+ * per row and kv head, 460 KB with sinks. */
 int64_t skb_chunk_attention_workspace(int tokens, int rows, int max_chunk, int n_heads, int n_kv_heads,
                                       int max_pages, int page_size, int n_pages, int window, int sinks,
                                       int with_mass);

@@ -1044,7 +1044,10 @@ static long long chunk_query_tiles(int tokens, int rows, int n_rep) { return tok
 
 // Key tiles of all rows together, at most: each row's by the cache's width and
 // by its window; all of them by the pool, whose pages belong to one row each.
-// A row's end, and the gap between sinks and window, cut one tile more each.
+// Slots out of sight may have no page, so a row's tiles are counted against the
+// slots it sees: up to one tile more for its end, for the window's beginning and
+// for the sinks' end (a stretch of L slots lies in at most (L + 254) / 128
+// tiles, one that begins with a tile in (L + 127) / 128).
 static long long chunk_key_tiles(int rows, int max_chunk, int max_pages, int page_size, long long n_pages, int window, int sinks) {
     const long long cap = (long long)max_pages * page_size;
     long long n = (cap + 127) / 128;
@@ -1053,7 +1056,7 @@ static long long chunk_key_tiles(int rows, int max_chunk, int max_pages, int pag
         if (w < n) n = w;
     }
     n *= rows;
-    const long long all = n_pages * page_size / 128 + 2ll * rows;
+    const long long all = n_pages * page_size / 128 + (window > 0 && sinks > 0 ? 3ll : 2ll) * rows;
     return all < n ? all : n;
 }
 

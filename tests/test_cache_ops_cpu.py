@@ -102,6 +102,30 @@ def test_workspace_sizes(lib):
     assert by_window < 64 * 1000 * 8 * 1024
 
 
+def seen_tiles(cached, new, window, sinks):
+    """Tiles of 128 slots that a row's new tokens see."""
+    first = max(0, cached - window + 1) if window else 0
+    slots = list(range(min(sinks, first))) + list(range(first, cached + new))
+    return len({s // 128 for s in slots}), slots
+
+
+@pytest.mark.parametrize("page", [1, 16, 32, 64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (256, 0), (256, 4), (1024, 4), (1024, 200), (2, 1), (129, 128)])
+@pytest.mark.parametrize("rows", [1, 2, 9])
+def test_workspace_holds_every_seen_tile_when_unseen_slots_have_no_page(lib, page, window, sinks, rows):
+    """The pool holds the pages of the slots in sight and no other; all rows alike,
+    at every phase of the window against the tiles."""
+    size, kv_heads, new = lib.lib().skb_chunk_attention_workspace, 2, 3
+    tile = kv_heads * (2 * 2 * 128 * 128 * 2 + 1024)  # keys and values as pairs of 16 bits, two numbers a slot
+    for cached in range(1009, 1009 + 2 * 128, 3):
+        tiles, slots = seen_tiles(cached, new, window, sinks)
+        pages = rows * len({s // page for s in slots})
+        # what is not key tiles: a cache of one slot has one tile a row
+        rest = size(rows * new, rows, new, 4, kv_heads, 1, 1, rows, 0, 0, 0) - rows * tile
+        got = size(rows * new, rows, new, 4, kv_heads, -(-(cached + new) // page), page, pages, window, sinks, 0)
+        assert got >= rest + rows * tiles * tile, (cached, tiles)
+
+
 def test_python_layer_refuses_before_the_gpu():
     import torch
 

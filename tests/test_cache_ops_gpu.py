@@ -381,6 +381,51 @@ def test_pages_outside_the_pool():
         assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
 
 
+def seen_pages_only(c, lengths, window, sinks, spare=0):
+    """A pool that holds just the pages that some query sees; every other entry of
+    the table names none."""
+    used = torch.zeros_like(c.table, dtype=torch.bool)
+    for r, n in enumerate(lengths):
+        filled = int(c.cached[r])
+        first = max(0, filled - window + 1) if window else 0
+        slots = torch.cat([torch.arange(min(sinks, first)), torch.arange(first, filled + n)]).cuda()
+        if n:
+            used[r, slots // c.page] = True
+    pages = int(used.sum())
+    order = torch.randperm(pages + spare, generator=c.gen, device="cuda")[:pages]
+    pool = torch.full((pages + spare, *c.pool.shape[1:]), math.nan, device="cuda")
+    pool[order] = c.pool[c.table[used].long()]
+    table = torch.full_like(c.table, -1)
+    table[used] = order.to(torch.int32)
+    return pool, table
+
+
+@pytest.mark.parametrize("cached,lengths,page,window,sinks", [
+    ((1009,), (16,), 16, 256, 4), ((1009,) * 8, (16,) * 8, 16, 256, 4), ((1009,) * 8, (16,) * 8, 32, 256, 4),
+    ((1150, 1150), (3, 3), 16, 1024, 4), ((1010, 500, 0, 257), (1, 30, 5, 0), 1, 126, 1), ((1009, 880), (2, 40), 16, 3, 0),
+    ((1140,) * 30, (1,) * 30, 16, 2, 130)])
+def test_chunk_attention_with_pages_of_seen_slots_alone(cached, lengths, page, window, sinks):
+    """An endless stream gives back the pages behind its window."""
+    from soraku_tts_b200 import kernels
+
+    c = Cache(cached, max(lengths), 4, 2, page=page, seed=15 + page)
+    pool, table = seen_pages_only(c, lengths, window, sinks)
+    qkv = c.qkv(sum(lengths))
+    mass = c.mass.clone()
+    got = kernels.chunk_attention(qkv, chunk_start=starts(lengths), max_chunk=max(lengths), window=window, sinks=sinks,
+                                  mass=c.mass, **c.args(kv_pool=pool, page_table=table))
+    want = c.want(qkv, lengths, window, sinks, True)
+    close(got, want)
+    c.check_mass()
+    for r, n in enumerate(lengths):  # the new tokens are appended
+        for s in range(int(c.cached[r]), int(c.cached[r]) + n):
+            at, whole = (int(t[r, s // page]) for t in (table, c.table))
+            torch.testing.assert_close(pool[at, :, :, s % page].double(), c.pool64[whole, :, :, s % page], rtol=0, atol=5e-6)
+    for r in range(c.rows):
+        first = max(0, int(c.cached[r]) - window + 1)
+        assert torch.equal(c.mass[r, :, min(sinks, first):first], mass[r, :, min(sinks, first):first])
+
+
 # ------------------------------------------------------------------- decode
 def decode(c, window=0, sinks=0, mass=False):
     from soraku_tts_b200 import kernels
