@@ -37,7 +37,8 @@ struct ChunkArgs {
     float* meta;            // [key tiles][KVH][2][128]: factor of a key's scores; exponent of a value row
     float* lse;             // [query tiles][KVH][128] (mass only), log2 units
     struct RowJob* jobs;    // [rows]: by the tiles they see, most first; null: rows as they are
-    long long key_tiles;
+    int key_tiles;
+    bool roomy;             // they are enough for any rows, even ones that claim more than the pool has
 };
 
 // x / n_rep without a division; right for x below 2^22 at least.
@@ -90,19 +91,55 @@ struct RowTiles {
     __device__ __forceinline__ int index(int tile) const { return tile < a1 ? tile : a1 + tile - b0; }
     __device__ __forceinline__ int tile(int k) const { return k < a1 ? k : b0 + k - a1; }
 };
-// Sum of a count over a warp.
-__device__ __forceinline__ long long warp_total(long long n) {
+// Whether every slot in sight of a row has a page.  By a whole warp.
+__device__ __forceinline__ bool row_mapped(const ChunkArgs& c, int r, const ChunkRow& x, const RowTiles& rt) {
+    const int lane = threadIdx.x & 31, lg = c.a.kv.page_log2;
+    const int* table = c.a.kv.page_table + (long long)r * c.a.kv.max_pages;
+    bool all = true;
+    auto look = [&](int p0, int p1) {
+        for (; all && p0 <= p1; p0 += 128) {
+            bool bad = false;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
-    return n;
+            for (int j = 0; j < 4; ++j) {
+                const int p = p0 + 32 * j + lane;
+                if (p <= p1) bad |= (unsigned)__ldg(table + p) >= (unsigned)c.a.kv.n_pages;
+            }
+            all = !__any_sync(FULL, bad);
+        }
+    };
+    const int sinks = min(c.a.sinks, rt.w0);
+    if (sinks > 0) look(0, (sinks - 1) >> lg);
+    look(rt.w0 >> lg, (x.cached + x.n - 1) >> lg);
+    return all;
+}
+// row_base where the rows see more than the pool can hold, so that some see
+// slots without a page: room for the others alone.
+__device__ __forceinline__ int row_base_mapped(const ChunkArgs& c, int r) {
+    int base = 0;
+    for (int p = 0; p <= r; ++p) {
+        const ChunkRow x = chunk_row(c, p);
+        const RowTiles rt(c, x);
+        // the count first: a row that is longer than the pool is not looked through
+        const bool place = rt.n > 0 && base + rt.n <= c.key_tiles && row_mapped(c, p, x, rt);
+        if (p == r) return place ? base : -1;
+        if (place) base += rt.n;
+    }
+    return -1;
 }
 // Where a row's key tiles begin in the workspace: behind those of the rows
-// before it.  By a whole warp.  In 64 bits: a row's count is up to 2^23 tiles, so
-// 256 rows of counts that no pool holds pass 32.
-__device__ __forceinline__ long long row_base(const ChunkArgs& c, int r) {
-    long long n = 0;
-    for (int p = threadIdx.x & 31; p < r; p += 32) n += RowTiles(c, chunk_row(c, p)).n;
-    return warp_total(n);
+// before it; -1 if there is no room for them.  By a whole warp.  Rows may claim
+// 2^23 tiles each, so a lane's sum stops at CHUNK_TILES, which is more than any
+// workspace holds (and 32 such sums are less than 2^31).
+constexpr int CHUNK_TILES = 1 << 25;
+__device__ __forceinline__ int row_base(const ChunkArgs& c, int r) {
+    int before = 0, all = 0;
+    const int rows = c.roomy ? r : c.a.rows;
+    for (int p = threadIdx.x & 31; p < rows; p += 32) {
+        all = min(all + RowTiles(c, chunk_row(c, p)).n, CHUNK_TILES);
+        if (p < r) before = all;
+    }
+    if (!c.roomy && __reduce_add_sync(FULL, all) > c.key_tiles) return row_base_mapped(c, r);
+    return __reduce_add_sync(FULL, before);
 }
 
 // A whole number e with |q| < 2^e for every query in log2 units: a normed head
@@ -139,7 +176,7 @@ constexpr int CP_SORTED = 512;   // more rows than that are taken as they come
 // are spread over many warps, many share a warp's look at their row's numbers.
 // The next block puts the rows in order.  The others: cached slots, a block per
 // (key tile, keys or values, kv head, row).
-__global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, int token_blocks, int per_block, int tiles_x) {
+__global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const __grid_constant__ ChunkArgs c, int token_blocks, int per_block, int tiles_x) {
     const CacheAttnArgs& a = c.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int H = a.H, KVH = a.kv.KVH, nv = H + 2 * KVH;
@@ -150,16 +187,28 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, i
         const int wpt = 8 / per_block, w = warp % wpt;
         const int t = blockIdx.x * per_block + warp / wpt;
         if (t >= c.tokens) return;
-        int r = 0;  // rows that end at or before the token
-        for (int p = lane; p - lane < a.rows; p += 32)
-            r += __popc(__ballot_sync(FULL, p < a.rows && c.chunk_start[p + 1] <= t));
+        // r: rows that end at or before the token; with them row_base, in one
+        // look at the rows' numbers
+        int r = 0, before = 0, all = 0;
+        for (int p = lane; p - lane < a.rows; p += 32) {
+            bool ends = false;
+            if (p < a.rows) {
+                const int n = RowTiles(c, chunk_row(c, p)).n;
+                ends = c.chunk_start[p + 1] <= t;
+                all = min(all + n, CHUNK_TILES);
+                if (ends) before = all;
+            }
+            r += __popc(__ballot_sync(FULL, ends));
+        }
         if (r >= a.rows) return;
         ChunkRow x = chunk_row(c, r);
         const int i = t - x.b;
         if (i < 0 || i >= x.n) return;
         const RowTiles rt(c, x);
-        const long long base = row_base(c, r);
-        if (base + rt.n > c.key_tiles) x.bad = true;  // pages mapped to several rows
+        int base = __reduce_add_sync(FULL, before);
+        if (!c.roomy && __reduce_add_sync(FULL, all) > c.key_tiles) base = row_base_mapped(c, r);
+        // (rows that begin before the one ahead ends are counted otherwise elsewhere)
+        if (base < 0 || base + rt.n > c.key_tiles) x.bad = true;
         if (x.idle || x.bad) {
             const float o = x.idle ? 0.f : __int_as_float(0x7fffffff);
             for (int v = w; v < H; v += wpt)
@@ -210,12 +259,21 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, i
     int b = blockIdx.x - token_blocks;
     if (b == 0 && c.jobs) {  // the order in which chunk_attn takes the rows
         __shared__ int seen[CP_SORTED], tiles[CP_SORTED];
+        __shared__ unsigned long long all;  // 512 rows of up to 2^23 tiles
+        if (threadIdx.x == 0) all = 0;
+        __syncthreads();
         for (int p = threadIdx.x; p < a.rows; p += 256) {
             const ChunkRow x = chunk_row(c, p);
             seen[p] = RowTiles(c, x).n;
             tiles[p] = seen[p] == 0 ? 0 : (x.n + c.P - 1) / c.P;
+            atomicAdd(&all, (unsigned long long)seen[p]);
         }
         __syncthreads();
+        if (all > (unsigned long long)c.key_tiles) {  // rows without room are left out
+            for (int p = warp; p < a.rows; p += 8)
+                if (row_base_mapped(c, p) < 0 && lane == 0) seen[p] = tiles[p] = 0;
+            __syncthreads();
+        }
         for (int p = threadIdx.x; p < a.rows; p += 256) {
             int rank = 0, first = 0;
             long long base = 0;
@@ -235,15 +293,15 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const ChunkArgs c, i
     b /= tiles_x;
     const int value = b & 1, g = (b >> 1) % KVH, r = (b >> 1) / KVH;
     const ChunkRow x = chunk_row(c, r);
-    const long long base = row_base(c, r);  // asked for beside the row's own numbers
+    const int base = row_base(c, r);  // asked for beside the row's own numbers
     const RowTiles rt(c, x);
-    if (k0 >= rt.n || base + rt.n > c.key_tiles) return;
+    if (k0 >= rt.n || base < 0) return;
     const float* pool = a.kv.pool + (value ? a.kv.value_step() * 128 : 0);
     const int row0 = warp * 16, i4 = lane >> 3, last = x.cached + x.n - 1;
     for (int k = k0; k < rt.n; k += tiles_x) {
         const int first = rt.tile(k) * 128 + row0;
         if (first >= x.cached && first + 15 <= last) continue;  // new tokens only: theirs are written above
-        const long long at = ((base + k) * KVH + g) * 2 + value;
+        const long long at = ((long long)(base + k) * KVH + g) * 2 + value;
         uint32_t units[4];  // of this lane's rows i4, 4 + i4, ...: one look at the page table
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -394,7 +452,7 @@ __device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
 // Clusters of `splits` CTAs, one per (query tile, kv head): with jobs in their
 // order, a row's last query tile, which sees the most, first; without, in a grid
 // (splits * query tiles, KVH, rows) in which rows may have fewer.
-__global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkArgs c, int splits) {
+__global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_constant__ ChunkArgs c, int splits) {
     extern __shared__ unsigned char ca_raw[];
     CaSmem& sm = *reinterpret_cast<CaSmem*>(ca_raw + ((1024u - (smem_u32(ca_raw) & 1023u)) & 1023u));
     const CacheAttnArgs& a = c.a;
@@ -436,12 +494,12 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const ChunkAr
     }
     const int i0 = t * c.P;
     const RowTiles rt(c, x);
-    if (x.idle || x.bad || i0 >= x.n || base + rt.n > c.key_tiles) {  // the same for a whole cluster
+    if (x.idle || x.bad || i0 >= x.n || base < 0) {  // the same for a whole cluster
         pdl_wait();
         return;
     }
     // where a tile of the row's keys lies in the workspace
-    auto place = [&](int tile) { return (base + rt.index(tile)) * a.kv.KVH + g; };
+    auto place = [&](int tile) { return (long long)(base + rt.index(tile)) * a.kv.KVH + g; };
     auto ask = [&](int n, int tile, int value) {  // copy n
         const int s = n % CA_STAGES;
         mbar_expect_tx(&sm.full[s], 2 * UT_BYTES);
@@ -863,7 +921,7 @@ static_assert(CM_W == 32, "a part is a warp's width");
 static_assert(4 * CM_N * 128 == UT_BYTES, "a step's queries fill a stage");
 static_assert(2 * (CM_SMEM + 1024) <= 227 * 1024, "shared memory of two CTAs");
 
-__global__ void __launch_bounds__(CM_THREADS, 2) chunk_mass_kernel(const ChunkArgs c) {
+__global__ void __launch_bounds__(CM_THREADS, 2) chunk_mass_kernel(const __grid_constant__ ChunkArgs c) {
     extern __shared__ unsigned char cm_raw[];
     CmSmem& sm = *reinterpret_cast<CmSmem*>(cm_raw + ((1024u - (smem_u32(cm_raw) & 1023u)) & 1023u));
     const CacheAttnArgs& a = c.a;
@@ -875,8 +933,8 @@ __global__ void __launch_bounds__(CM_THREADS, 2) chunk_mass_kernel(const ChunkAr
     const int last = x.cached + x.n - 1;
     const RowTiles rt(c, x);
     if ((int)blockIdx.x >= rt.n) return;
-    const long long row_at = row_base(c, r);
-    if (row_at + rt.n > c.key_tiles) return;
+    const int row_at = row_base(c, r);
+    if (row_at < 0) return;
     const int tile = rt.tile(blockIdx.x);
     const int base = tile * 128;
     if (base > last) return;
@@ -928,7 +986,7 @@ __global__ void __launch_bounds__(CM_THREADS, 2) chunk_mass_kernel(const ChunkAr
                 mbar_expect_tx(&sm.lse_full[i % CM_LSE], CM_N * 4);
                 bulk_g2s(sm.lse[i % CM_LSE], c.lse + at * 128 + (s & 1) * CM_N, CM_N * 4, &sm.lse_full[i % CM_LSE]);
             };
-            const long long kat = ((row_at + blockIdx.x) * a.kv.KVH + g) * 2;
+            const long long kat = ((long long)(row_at + blockIdx.x) * a.kv.KVH + g) * 2;
             mbar_expect_tx(&sm.k_full, 2 * UT_BYTES + 512);
             bulk_g2s(sm.stage[0], c.kvtiles + kat * (2 * UT_BYTES), 2 * UT_BYTES, &sm.k_full);
             bulk_g2s(sm.kc, c.meta + kat * 128, 512, &sm.k_full);
@@ -1042,20 +1100,19 @@ __global__ void __launch_bounds__(CM_THREADS, 2) chunk_mass_kernel(const ChunkAr
 
 static long long chunk_query_tiles(int tokens, int rows, int n_rep) { return tokens / (128 / n_rep) + rows + 1; }
 
-// Key tiles of all rows together, at most: each row's by the cache's width and
-// by its window; all of them by the pool, whose pages belong to one row each.
+// Key tiles of one row, at most: by the cache's width and by its window.
+static long long chunk_row_tiles(int max_chunk, int max_pages, int page_size, int window, int sinks) {
+    const long long n = ((long long)max_pages * page_size + 127) / 128;
+    const long long w = ((long long)sinks + 127) / 128 + ((long long)window + max_chunk + 127) / 128 + 1;
+    return window > 0 && w < n ? w : n;
+}
+// Key tiles of all rows together, at most: each row's; all of them by the pool, whose pages belong to one row each.
 // Slots out of sight may have no page, so a row's tiles are counted against the
 // slots it sees: up to one tile more for its end, for the window's beginning and
 // for the sinks' end (a stretch of L slots lies in at most (L + 254) / 128
 // tiles, one that begins with a tile in (L + 127) / 128).
 static long long chunk_key_tiles(int rows, int max_chunk, int max_pages, int page_size, long long n_pages, int window, int sinks) {
-    const long long cap = (long long)max_pages * page_size;
-    long long n = (cap + 127) / 128;
-    if (window > 0) {
-        const long long w = ((long long)sinks + 127) / 128 + ((long long)window + max_chunk + 127) / 128 + 1;
-        if (w < n) n = w;
-    }
-    n *= rows;
+    const long long n = chunk_row_tiles(max_chunk, max_pages, page_size, window, sinks) * rows;
     const long long all = n_pages * page_size / 128 + (window > 0 && sinks > 0 ? 3ll : 2ll) * rows;
     return all < n ? all : n;
 }
@@ -1136,7 +1193,10 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     c.P = 128 / c.n_rep;
     c.rep_inv = ((1u << 24) + c.n_rep - 1) / c.n_rep;
     const long long tiles = chunk_query_tiles(tokens, rows, c.n_rep);
-    c.key_tiles = chunk_key_tiles(rows, max_chunk, max_pages, page_size, n_pages, window, sinks);
+    const long long key_tiles = chunk_key_tiles(rows, max_chunk, max_pages, page_size, n_pages, window, sinks);
+    if (key_tiles >= CHUNK_TILES) return fail(SKB_ERR_ARG, "%s: too many slots", what);  // 4 TB of workspace
+    c.key_tiles = (int)key_tiles;
+    c.roomy = key_tiles == chunk_row_tiles(max_chunk, max_pages, page_size, window, sinks) * rows;
     const ChunkWork at(tiles, c.key_tiles, n_kv_heads, rows, mass != nullptr);
     unsigned char* w = static_cast<unsigned char*>(work);
     c.qtiles = w + at.q;
@@ -1148,7 +1208,8 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     const int most = max_chunk < 1 ? 1 : (max_chunk < tokens ? max_chunk : tokens);
     const int tiles_x = (most + c.P - 1) / c.P;
     // key tiles of one row, at most
-    const long long row_tiles = chunk_key_tiles(1, most, max_pages, page_size, n_pages, window, sinks);
+    long long row_tiles = chunk_row_tiles(most, max_pages, page_size, window, sinks);
+    if (row_tiles > c.key_tiles) row_tiles = c.key_tiles;
     // CTAs that have work, at most; while they leave SMs idle, up to 8 share a
     // query tile's key tiles.  (Sharing where they fill the card already makes
     // clusters wait for SMs and adds the join: 8 prompts 199 us in pairs, 117 alone;

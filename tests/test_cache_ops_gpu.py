@@ -386,11 +386,12 @@ def seen_pages_only(c, lengths, window, sinks, spare=0):
     the table names none."""
     used = torch.zeros_like(c.table, dtype=torch.bool)
     for r, n in enumerate(lengths):
+        if n == 0:
+            continue
         filled = int(c.cached[r])
         first = max(0, filled - window + 1) if window else 0
         slots = torch.cat([torch.arange(min(sinks, first)), torch.arange(first, filled + n)]).cuda()
-        if n:
-            used[r, slots // c.page] = True
+        used[r, slots // c.page] = True
     pages = int(used.sum())
     order = torch.randperm(pages + spare, generator=c.gen, device="cuda")[:pages]
     pool = torch.full((pages + spare, *c.pool.shape[1:]), math.nan, device="cuda")
@@ -424,6 +425,45 @@ def test_chunk_attention_with_pages_of_seen_slots_alone(cached, lengths, page, w
     for r in range(c.rows):
         first = max(0, int(c.cached[r]) - window + 1)
         assert torch.equal(c.mass[r, :, min(sinks, first):first], mass[r, :, min(sinks, first):first])
+
+
+@pytest.mark.parametrize("rows,tokens", [(3, 6), (30, 90)])
+@pytest.mark.parametrize("broken", ["first", "every_second", "but_for_some_pages"])
+def test_rows_beside_rows_without_pages(rows, tokens, broken):
+    """Rows that claim more slots than the pool has, for which the table has no
+    pages, return NaN whole and cost no other row anything: with a grid of rows, and
+    with a list of them."""
+    from soraku_tts_b200 import kernels
+
+    window, sinks = 0, 0
+    sick = [0] if broken == "first" else list(range(0, rows, 2))
+    lengths = [tokens - r % 3 for r in range(rows)]
+    cached = [9000 // len(sick) + 2000 + r if r in sick else 100 + 7 * r for r in range(rows)]
+    c = Cache(cached, tokens, 4, 2, seed=63, max_pos=12000)
+    c.cached[sick] = -1
+    pool, table = seen_pages_only(c, [0 if r in sick else n for r, n in enumerate(lengths)], window, sinks, spare=5)
+    c.cached[sick] = torch.tensor(cached, dtype=torch.int32, device="cuda")[sick]
+    if broken == "but_for_some_pages":
+        free = torch.ones(pool.shape[0], dtype=torch.bool, device="cuda")
+        free[table[table >= 0].long()] = False
+        table[sick[-1], [0, 1, 2, 40, int(c.cached[sick[-1]]) // c.page]] = free.nonzero().flatten().to(torch.int32)
+    mass = c.mass.clone()
+    qkv = c.qkv(sum(lengths))
+    got = kernels.chunk_attention(qkv, chunk_start=starts(lengths), max_chunk=tokens, mass=c.mass,
+                                  **c.args(kv_pool=pool, page_table=table))
+    ill = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    ill[sick] = True
+    ill = ill.repeat_interleave(torch.tensor(lengths, device="cuda"))
+    assert torch.isnan(got[ill]).all()
+    c.cached[sick] = -1
+    want = c.want(qkv, lengths, window, sinks, True)
+    close(got[~ill], want[~ill])
+    fine = torch.tensor([r not in sick for r in range(rows)], device="cuda")
+    close(c.mass[fine], c.mass64[fine])
+    assert torch.equal(c.mass[~fine], mass[~fine])
+    free = torch.ones(pool.shape[0], dtype=torch.bool, device="cuda")
+    free[table[fine][table[fine] >= 0].long()] = False
+    assert torch.isnan(pool[free]).all()
 
 
 # ------------------------------------------------------------------- decode
