@@ -814,13 +814,14 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
         if (*abort) l = __int_as_float(0x7fffffff);  // a wait that ran out shows as NaN
         float* stage = reinterpret_cast<float*>(sm.stage) + row * CA_OUT_LD + part * CA_W;
         // rows that saw nothing, and dead ones, give zeros
-        const float f = l == 0.f || row >= sm.live ? 0.f : exp2_fast(E - 19.f) / l;
+        const bool none = l == 0.f || row >= sm.live;
+        const float f = exp2_fast(E - 19.f) / l;  // may be 0, and what it multiplies NaN
         if (splits == 1 && c.lse && part == 0 && row < sm.live) c.lse[sm.tile_at * 128 + row] = m + log2f(l);
 #pragma unroll
         for (int q = 0; q < CA_W / 4; ++q) {
             float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
             const float2 u = unpack2(acc[2 * q]), v = unpack2(acc[2 * q + 1]);
-            if (f != 0.f) w = make_float4(u.x * f, u.y * f, v.x * f, v.y * f);
+            if (!none) w = make_float4(u.x * f, u.y * f, v.x * f, v.y * f);
             *reinterpret_cast<float4*>(stage + 4 * q) = w;
         }
         if (part == 0) sm.m[row] = m;

@@ -299,6 +299,29 @@ def test_chunk_attention_value_scales(scale):
     close(got.double() / scale, want / scale)
 
 
+def set_slot(c, r, slot, key=None, value=1.0):
+    """Replaces a cached key, scales its value, in every head."""
+    page, at = int(c.table[r, slot // c.page]), slot % c.page
+    if key is not None:
+        c.pool[page, 0, :, at] = key
+    c.pool[page, 1, :, at] *= value
+    c.pool64[page, :, :, at] = c.pool[page, :, :, at].double()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_query_that_sees_nothing_finite_says_so(bad):
+    """The first tokens of a prompt, whose values are all not finite; so does one that
+    sees such a value behind zeros."""
+    c = Cache((0, 3), 4, 4, 2, seed=74)
+    qkv = c.qkv(5)
+    heads = qkv.view(5, 8, HD)
+    heads[:4, 6:] = bad
+    heads[4, 6:] = bad
+    for s in range(3):
+        set_slot(c, 1, s, None, 0.0)
+    close(*chunk(c, (4, 1), qkv=qkv))
+
+
 def test_chunk_attention_sharp_and_flat_scores():
     """Scores far apart (norm weights of 12: one slot takes all) and all alike."""
     for w in (12.0, 1e-3):
