@@ -326,8 +326,10 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const __grid_constan
                 const int row = row0 + part + 4 * q + i4, slot = first - row0 + row;
                 if (slot >= x.cached && slot <= last) continue;
                 d.put(q, c.kvtiles + at * (2 * UT_BYTES), row0 + part, row_scale(e), lane);
-                if ((lane & 7) == 0)
-                    c.meta[at * 128 + row] = value ? e : e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac : e;
+                if ((lane & 7) == 0)  // (a value that is not there counts among no exponents)
+                    c.meta[at * 128 + row] = value ? (unit[q] == UT_NONE ? __int_as_float(0x7fffffff) : e)
+                                             : e == e ? pow2_whole(fmaxf(e, -100.f) - 13.f) * qfac
+                                                      : e;
             }
         }
     }
@@ -388,16 +390,32 @@ constexpr int CA_STAGES = 3;
 constexpr uint32_t CA_TM_O = 256, CA_TM_Q = 384;
 constexpr int CA_OUT_LD = 132;  // floats of a staged output row
 constexpr int CA_MAX_SPLITS = 8;
+// Weights are held as p 2^(e - E + CA_UP) in fp16 pairs, e the exponent of the
+// value row, whose own numbers are below 2^14.  A pair resolves 2^-25 whatever it
+// holds, so what counts is where a query's largest contribution p 2^e lies.
+//   Values of like sizes: E is set by the first tile, CA_ABOVE above its largest e,
+//   and serves as long as every e in sight lies in [E - CA_SPREAD, E].  The factors
+//   2^(e - E + CA_UP) are then the same for all queries, and the key with the largest
+//   weight, 1/2 at least, gives 2^(CA_UP - CA_SPREAD - 1) = 4, or 2^27 times the resolution.
+//   Else (one large value that hardly anybody looks at, a zero one that all look
+//   at) E follows the query's largest contribution from that tile on, and each weight
+//   is formed by an exponential of its own beside the one that goes into the sum
+//   (8 prompts: 194 us a call instead of 166).
+// Which of them holds goes by the values that the query sees, and no other.
+constexpr float CA_UP = 12.f, CA_ABOVE = 2.f, CA_SPREAD = 9.f;
+constexpr float CA_SLACK = 3.f;  // how far a score, or a contribution, may pass its reference: 2^(12 + 3) fits fp16
 
 struct CaSmem {
     unsigned char stage[CA_STAGES][2 * UT_BYTES];
     float kc[2][128];                    // factor of a key's scores: its scale undone
     float ve[2][128];                    // exponent of a value row
-    float vg[2][128];                    // factor of its weights: 2^(exponent - E + 6)
-    float mx[2][CA_PARTS][128], ex[2][CA_PARTS][128];  // a row part's largest score and value exponent
+    float vg[2][128];                    // factor of its weights: 2^(exponent - E + CA_UP)
+    float mx[2][CA_PARTS][128];          // a row part's largest score,
+    float ex[2][CA_PARTS][128], lo[2][CA_PARTS][128];  // its largest and smallest value exponent,
+    float cx[CA_PARTS][128];             // its largest contribution
     float m[128], l[CA_PARTS][128];      // this split's statistics (sums of row parts)
-    float E[2];                          // running exponent of the values
-    float vtop[2][CA_PARTS];             // largest exponent of a part's values
+    float E[2];                          // E of the tiles that all queries see whole; inf: it follows the contributions
+    float top[2], low[2];                // largest and smallest exponent of a tile's values
     float own_vg[CA_SOFTMAX_WARPS][CA_W];  // a warp's factors in a tile that is not whole
     uint64_t q_landed, q_full, full[CA_STAGES], empty[CA_STAGES], s_full[2], p_full[2], pv_done[2], o_free, meta_full[2];
     uint64_t s_end, o_full;  // every product of warp M, of warp O
@@ -624,22 +642,24 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
             const int b = i & 1;
             const float* at = c.meta + place(sm.list.tile(sm.k0 + i)) * 256;
             const float4 k = reinterpret_cast<const float4*>(at)[lane], v = reinterpret_cast<const float4*>(at)[32 + lane];
-            // largest exponents (NaN aside): of each 32 values, of all
-            float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-            top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
-            top = fmaxf(top, __shfl_xor_sync(FULL, top, 4));
-            const float part_top = top;
-            top = warp_max(top);
+            // exponents, NaN aside
+            const float top = warp_max(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+            const float low = -warp_max(-fminf(fminf(v.x, v.y), fminf(v.z, v.w)));
             // the softmax of tile i - 2 is done with the buffers
             if (i >= 2 && !ut_wait(&sm.pv_done[b], ((i - 2) >> 1) & 1, abort)) break;
-            if (sm.k0 + i < sm.list.full && top > E) E = top + 3.f;  // 3 bits to spare: it rarely moves
+            if (sm.k0 + i < sm.list.full) {
+                if (i == 0) E = top + CA_ABOVE;
+                if (top > E || low < E - CA_SPREAD || low == UT_POISON_E) E = INFINITY;
+            }
             reinterpret_cast<float4*>(sm.kc[b])[lane] = k;
             reinterpret_cast<float4*>(sm.ve[b])[lane] = v;
-            reinterpret_cast<float4*>(sm.vg[b])[lane] = make_float4(exp2_fast(v.x - E + 6.f), exp2_fast(v.y - E + 6.f),
-                                                                    exp2_fast(v.z - E + 6.f), exp2_fast(v.w - E + 6.f));
-            if (lane == 0) sm.E[b] = E;
-            if ((lane & 7) == 0) sm.vtop[b][lane >> 3] = part_top;
+            reinterpret_cast<float4*>(sm.vg[b])[lane] = make_float4(exp2_fast(v.x - E + CA_UP), exp2_fast(v.y - E + CA_UP),
+                                                                    exp2_fast(v.z - E + CA_UP), exp2_fast(v.w - E + CA_UP));
+            if (lane == 0) {
+                sm.E[b] = E;
+                sm.top[b] = top;
+                sm.low[b] = low;
+            }
             __syncwarp();
             if (lane == 0) ut_arrive(&sm.meta_full[b]);
         }
@@ -647,9 +667,11 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
     } else if (warp < CA_SOFTMAX_WARPS) {
         const int part = warp >> 2, row = tid & 127;
         const uint32_t lane_tm = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        // m is a whole number, so that moving it and E multiplies by powers of two
         float m = CO_LOW, l = 0.f, E = UT_POISON_E;
+        bool own = false;  // E follows this query's contributions
         // A part of the output row, over the tiles before the newest, in
-        // units 2^(E - 13 - 6) of that tile's E and m; f_o takes it there.
+        // units 2^(E - 13 - CA_UP) of that tile's E and m; f_o takes it there.
         uint64_t acc[CA_W / 2];
 #pragma unroll
         for (int q = 0; q < CA_W / 2; ++q) acc[q] = 0;
@@ -686,10 +708,9 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
             ut_wait(&sm.meta_full[b], (i >> 1) & 1, abort);
             ut_wait(&sm.s_full[b], (i >> 1) & 1, abort);
             ut_fence_after();
-            // scores; the largest (and, where queries differ in what they
-            // see, the largest exponent among the values this query sees)
+            // scores and the largest
             float2 s[CA_W / 2];
-            float mx = CO_LOW, ex = UT_POISON_E;
+            float mx = CO_LOW;
             uint32_t seen = FULL;  // bit per key of the part
             if (!whole) {
                 const auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? FULL : (1u << n) - 1u; };
@@ -712,21 +733,18 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
             if (__all_sync(FULL, seen == FULL)) {
 #pragma unroll
                 for (int q = 0; q < 16; ++q) mx = fmaxf(fmaxf(mx, s[q].x), s[q].y);
-                ex = sm.vtop[b][part];
             } else {
 #pragma unroll
                 for (int q = 0; q < 16; ++q) {  // what is not seen weighs nothing from here on
                     if (!(seen >> (2 * q) & 1u)) s[q].x = -INFINITY;
                     if (!(seen >> (2 * q + 1) & 1u)) s[q].y = -INFINITY;
                     mx = fmaxf(fmaxf(mx, s[q].x), s[q].y);
-                    if (seen >> (2 * q) & 1u) ex = fmaxf(ex, ve[2 * q]);
-                    if (seen >> (2 * q + 1) & 1u) ex = fmaxf(ex, ve[2 * q + 1]);
                 }
             }
             float E_new = E;
             float2 sum;
             // Scores -> weights, scaled by their values' exponents, as hi | lo
-            // over the scores.  `vg`: the factors 2^(exponent - E + 6), if one
+            // over the scores.  `vg`: the factors 2^(exponent - E + CA_UP), if one
             // set holds for the warp; else (EACH) every thread forms its own.
             // MASKED: some keys are not seen, whatever their factors are.
             auto weigh = [&](const float2* vg, auto masked, auto each) {
@@ -741,7 +759,8 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
                         p = make_float2(exp2_fast(p.x), exp2_fast(p.y));
                         sum = add2(sum, p);
                         float2 f = vg[ch * 8 + q];
-                        if (decltype(each)::value) f = make_float2(exp2_fast(f.x - E_new + 6.f), exp2_fast(f.y - E_new + 6.f));
+                        if (decltype(each)::value)
+                            f = make_float2(exp2_fast(f.x - E + CA_UP), exp2_fast(f.y - E + CA_UP));
                         p = mul2(p, f);
                         if (decltype(masked)::value) {
                             if (!(seen >> (ch * 16 + 2 * q) & 1u)) p.x = 0.f;
@@ -753,38 +772,112 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
                     ut_st8(st + ch * 16 + 8, pl);
                 }
             };
-            // The running maximum follows only when it is passed by 2^8, the
-            // running exponent with 3 bits to spare: weights stay below 2^8,
-            // scaled ones below 2^14.  In a whole tile the exponent is every
-            // row's, and where no thread passed its maximum the row's parts
-            // need not tell one another theirs.
-            float f_l = 1.f;
-            if (whole) E_new = sm.E[b];
-            if (!whole || i == 0 || softmax_any(mx > m + 8.f && hi >= 0)) {
-                sm.mx[b][part][row] = mx;
-                if (!whole) sm.ex[b][part][row] = ex;
-                softmax_sync();
-                if (!whole) {
+            // The same where some of the warp's rows have an E that follows their
+            // contributions: factors are part of those rows' weights.  16 scores at a
+            // time, read again, so that the 32 held above are not held here as well.
+            auto weigh_mixed = [&]() {
+                sum = make_float2(0.f, 0.f);
+#pragma unroll 1
+                for (int k = 0; k < CA_W; k += 16) {
+                    uint32_t w[16], ph[8], pl[8];
+                    ut_ld16(st + k, w);
+                    ut_wait_ld();
+                    const float2* kf = reinterpret_cast<const float2*>(sm.kc[b] + part * CA_W + k);
+                    const float2* vf = reinterpret_cast<const float2*>(ve + k);
 #pragma unroll
-                    for (int q = 0; q < CA_PARTS; ++q) ex = fmaxf(ex, sm.ex[b][q][row]);
-                    if (ex > E) E_new = ex + 3.f;
+                    for (int q = 0; q < 8; ++q) {
+                        const bool sx = seen >> (k + 2 * q) & 1u, sy = seen >> (k + 2 * q + 1) & 1u;
+                        float2 x = mul2(make_float2(__uint_as_float(w[2 * q]), __uint_as_float(w[2 * q + 1])), kf[q]);
+                        x = make_float2(sx ? x.x - m : -INFINITY, sy ? x.y - m : -INFINITY);
+                        const float2 p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        sum = add2(sum, p);
+                        float2 f = make_float2(vf[q].x - E + CA_UP, vf[q].y - E + CA_UP);
+                        f = make_float2(exp2_fast(own ? x.x + f.x : f.x), exp2_fast(own ? x.y + f.y : f.y));
+                        f = make_float2(own ? f.x : p.x * f.x, own ? f.y : p.y * f.y);
+                        split2(make_float2(sx ? f.x : 0.f, sy ? f.y : 0.f), ph[q], pl[q]);
+                    }
+                    ut_st8(st + k, ph);
+                    ut_st8(st + k + 8, pl);
                 }
+            };
+            // The running maximum follows only when it is passed by 2^CA_SLACK.  In
+            // a whole tile the exponents are every row's, and where no thread passed
+            // its maximum the row's parts need not tell one another theirs.
+            // (Barriers are taken or not by what a barrier said, so that the warps agree
+            // also when a wait ran out and they read what is still being written.)
+            float d_m = 0.f;
+            bool mixed = false;
+            if (whole) E_new = sm.E[b];
+            if (!whole || i == 0 || softmax_any((mx > m + CA_SLACK && hi >= 0) || E_new == INFINITY)) {
+                // Exponents of the values that a row sees, where those of the tile
+                // do not tell all there is to know; the smallest only where it may be too small.
+                const float top = sm.top[b], low = sm.low[b];
+                const bool ask = !whole && hi >= 0 && !own, fresh = E == UT_POISON_E;
+                const bool look = __any_sync(FULL, ask && (fresh || top > E || low < E - CA_SPREAD));
+                const bool wide = __any_sync(FULL, ask && (low < (fresh ? top + CA_ABOVE : E) - CA_SPREAD || low == UT_POISON_E));
+                float ex = UT_POISON_E, lo = INFINITY;
+                if (look) {
+#pragma unroll 1  // once a query tile, and registers are scarce
+                    for (int q = 0; q < CA_W / 4; ++q) {
+                        const float4 f = reinterpret_cast<const float4*>(ve)[q];
+                        const uint32_t w = seen >> (4 * q);
+                        ex = fmaxf(fmaxf(ex, w & 1u ? f.x : ex), w & 2u ? f.y : ex);
+                        ex = fmaxf(fmaxf(ex, w & 4u ? f.z : ex), w & 8u ? f.w : ex);
+                    }
+                    sm.ex[b][part][row] = ex;
+                    if (wide) {
+#pragma unroll 4
+                        for (int q = 0; q < CA_W; ++q)
+                            if (seen >> q & 1u) lo = fminf(lo, ve[q]);
+                        sm.lo[b][part][row] = lo;
+                    }
+                }
+                sm.mx[b][part][row] = mx;
+                // some row's E follows its contributions, or may have to
+                mixed = softmax_any(whole ? E_new == INFINITY
+                                          : hi >= 0 && (own || (fresh ? wide : ex > E || lo < E - CA_SPREAD || lo == UT_POISON_E)));
 #pragma unroll
                 for (int q = 0; q < CA_PARTS; ++q) mx = fmaxf(mx, sm.mx[b][q][row]);
-                const float m_new = mx > m + 8.f && hi >= 0 ? mx : m;
-                f_l = exp2_fast(m - m_new);
+                const float m_new = mx > m + CA_SLACK && hi >= 0 ? ceilf(mx) : m;
+                d_m = m - m_new;
                 m = m_new;
+                l *= exp2_fast(d_m);
+                if (look) {
+#pragma unroll
+                    for (int q = 0; q < CA_PARTS; ++q) ex = fmaxf(ex, sm.ex[b][q][row]);
+                    if (wide) {
+#pragma unroll
+                        for (int q = 0; q < CA_PARTS; ++q) lo = fminf(lo, sm.lo[b][q][row]);
+                    }
+                    if (fresh && ex > UT_POISON_E) E_new = ex + CA_ABOVE;
+                    own = own || ex > E_new || lo < E_new - CA_SPREAD || lo == UT_POISON_E;
+                }
             }
-            if (whole) {
+            if (whole) own = E_new == INFINITY;
+            if (mixed) {
+                float cx = CO_LOW;
+#pragma unroll
+                for (int q = 0; q < 16; ++q) cx = fmaxf(fmaxf(cx, s[q].x - m + ve[2 * q]), s[q].y - m + ve[2 * q + 1]);
+                sm.cx[part][row] = cx;
+                softmax_sync();
+#pragma unroll
+                for (int q = 0; q < CA_PARTS; ++q) cx = fmaxf(cx, sm.cx[q][row]);
+                if (own) E_new = cx > E + d_m + CA_SLACK ? ceilf(cx) : E + d_m;  // else where it was
+            }
+            const float f_new = i == 0 ? 0.f : exp2_fast(d_m + (E - E_new));
+            E = E_new;
+            if (mixed) {
+                weigh_mixed();
+            } else if (whole) {
                 weigh(reinterpret_cast<const float2*>(sm.vg[b] + part * CA_W), std::false_type{}, std::false_type{});
-            } else if (__all_sync(FULL, E_new == __shfl_sync(FULL, E_new, 0))) {
-                sm.own_vg[warp][lane] = exp2_fast(ve[lane] - E_new + 6.f);
+            } else if (const float E_0 = __shfl_sync(FULL, E, 0); __all_sync(FULL, hi < 0 || E == E_0)) {
+                sm.own_vg[warp][lane] = exp2_fast(ve[lane] - E_0 + CA_UP);
                 __syncwarp();
                 weigh(reinterpret_cast<const float2*>(sm.own_vg[warp]), std::true_type{}, std::false_type{});
             } else {
                 weigh(reinterpret_cast<const float2*>(ve), std::true_type{}, std::true_type{});
             }
-            l = fmaf(l, f_l, sum.x + sum.y);
+            l += sum.x + sum.y;
             ut_wait_st();
             ut_fence_before();
             __syncwarp();
@@ -797,8 +890,7 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
                 __syncwarp();
                 if (lane == 0) ut_arrive(&sm.o_free);
             }
-            f_o = i == 0 ? 0.f : f_l * exp2_fast(E - E_new);
-            E = E_new;
+            f_o = f_new;
         }
         // ---- this split's output over its own sum, staged in shared memory
         if (nt > 0) {
@@ -813,15 +905,16 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
         for (int q = 0; q < CA_PARTS; ++q) l += sm.l[q][row];
         if (*abort) l = __int_as_float(0x7fffffff);  // a wait that ran out shows as NaN
         float* stage = reinterpret_cast<float*>(sm.stage) + row * CA_OUT_LD + part * CA_W;
-        // rows that saw nothing, and dead ones, give zeros
+        // rows that saw nothing, and dead ones, give zeros.  2^E in two steps: E
+        // itself may lie below what a normal number holds
         const bool none = l == 0.f || row >= sm.live;
-        const float f = exp2_fast(E - 19.f) / l;  // may be 0, and what it multiplies NaN
+        const float half = rintf(0.5f * E), f = exp2_fast(half - 13.f - CA_UP) / l, g = exp2_fast(E - half);
         if (splits == 1 && c.lse && part == 0 && row < sm.live) c.lse[sm.tile_at * 128 + row] = m + log2f(l);
 #pragma unroll
         for (int q = 0; q < CA_W / 4; ++q) {
             float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
             const float2 u = unpack2(acc[2 * q]), v = unpack2(acc[2 * q + 1]);
-            if (!none) w = make_float4(u.x * f, u.y * f, v.x * f, v.y * f);
+            if (!none) w = make_float4(u.x * f * g, u.y * f * g, v.x * f * g, v.y * f * g);
             *reinterpret_cast<float4*>(stage + 4 * q) = w;
         }
         if (part == 0) sm.m[row] = m;

@@ -299,6 +299,19 @@ def test_chunk_attention_value_scales(scale):
     close(got.double() / scale, want / scale)
 
 
+def aimed(c, tokens):
+    """Rotations off and queries near one direction: [tokens, ...] new heads, and a
+    key along that direction whose score is about sqrt(128) times its factor."""
+    c.cos.fill_(1.0)
+    c.sin.zero_()
+    c.qn.fill_(1.0)
+    u = torch.randn(HD, generator=c.gen, device="cuda")
+    qkv = c.qkv(tokens)
+    heads = qkv.view(tokens, c.H + 2 * c.G, HD)
+    heads[:, :c.H] = u + 0.1 * heads[:, :c.H]
+    return qkv, u / u.norm() * math.sqrt(HD)
+
+
 def set_slot(c, r, slot, key=None, value=1.0):
     """Replaces a cached key, scales its value, in every head."""
     page, at = int(c.table[r, slot // c.page]), slot % c.page
@@ -306,6 +319,71 @@ def set_slot(c, r, slot, key=None, value=1.0):
         c.pool[page, 0, :, at] = key
     c.pool[page, 1, :, at] *= value
     c.pool64[page, :, :, at] = c.pool[page, :, :, at].double()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 2)])
+@pytest.mark.parametrize("factor", [10.0, 1e3, 1e6, 2.0**30, 1e20])
+def test_large_values_of_next_to_no_weight(factor, window, sinks):
+    """Slots whose values are far larger than the others' and whose scores lie so far
+    below that they weigh 2^-40 / factor or less: the others decide the output,
+    and keep their digits.  In tiles that all queries see whole, at the window's
+    edge, among the sinks and the newest slots; the same through decode."""
+    for slots in ((1,), (390,), (505,), (1, 390, 505, 600)):
+        c = Cache((620, 514), 90, 4, 2, seed=71, max_pos=1000)
+        lengths = (90, 3)
+        qkv, along = aimed(c, sum(lengths))
+        down = -(40 + math.log2(factor)) * math.log(2) / math.sqrt(HD)
+        for r in range(2):
+            for s in slots:
+                if s < int(c.cached[r]):
+                    set_slot(c, r, s, along * down, factor)
+        saved = c.pool.clone(), c.pool64.clone()
+        got, want = chunk(c, lengths, window, sinks, mass=True, qkv=qkv)
+        close(got, want)
+        c.check_mass()
+        c.pool, c.pool64 = saved
+        from soraku_tts_b200 import kernels
+
+        one = qkv[[0, 90]].contiguous()
+        got = kernels.window_decode_attention(one, window=window, sinks=sinks, **c.args())
+        close(got, c.want(one, (1, 1), window, sinks))
+
+
+@pytest.mark.parametrize("value", [0.0, 1e-30, 1e-6])
+@pytest.mark.parametrize("slot", [0, 200, 600])
+def test_small_values_of_nearly_all_weight(value, slot):
+    """A slot that takes nearly all the weight (a sink) and whose value is next to
+    nothing: the output is what little the others give."""
+    c = Cache((620, 700), 70, 4, 2, seed=72, max_pos=1000)
+    qkv, along = aimed(c, 73)
+    for r in range(2):
+        set_slot(c, r, slot, along * (20 / math.sqrt(HD)), value)
+    got, want = chunk(c, (70, 3), 650, 1, mass=True, qkv=qkv)
+    # a score of 20 formed of parts of one sign, so that roundings do not average out:
+    # the query's norm and scale and the key's factor, four of 2^-24, and the product's
+    # sum, which tensor memory adds up in 8 steps of 16 that each cut it towards zero by
+    # up to 2^-23 (16 of 2^-24).  All of them times 20 is what the weights are off by.
+    d = got.double() - want
+    assert float(d.abs().max()) <= ATOL * float(want.abs().max())
+    assert float(d.norm()) <= (REL + 20 * (4 + 16) * 2**-24) * float(want.norm()), float(d.norm() / want.norm())
+    c.check_mass()
+
+
+@pytest.mark.parametrize("spread", [4, 12, 40])
+@pytest.mark.parametrize("cached,lengths", [((0, 0), (100, 130)), ((700, 1300), (65, 9)), ((5000,), (40,))])
+def test_value_rows_of_all_sizes(spread, cached, lengths):
+    """Every value row has a size of its own, 2^-spread to 2^spread."""
+    c = Cache(cached, max(lengths), 4, 2, seed=73 + spread, max_pos=6000)
+    c.pool[:, 1] *= torch.exp2((2 * torch.rand(c.pool.shape[0], 2, c.page, 1, generator=c.gen, device="cuda") - 1) * spread)
+    c.pool64 = c.pool.double()
+    qkv = c.qkv(sum(lengths))
+    heads = qkv.view(-1, 8, HD)
+    heads[:, 6:] *= torch.exp2((2 * torch.rand(heads.shape[0], 2, 1, generator=c.gen, device="cuda") - 1) * spread)
+    got, want = chunk(c, lengths, qkv=qkv)
+    # per query, as each has outputs of its own size: its weights are off by at most ATOL,
+    # which is the bound where few contribute; twice that where they partly cancel
+    err = (got.double() - want).view(-1, 4, HD).norm(dim=-1) / want.view(-1, 4, HD).norm(dim=-1)
+    assert float(err.max()) <= 2 * ATOL and float(err.square().mean().sqrt()) <= REL, (float(err.max()), float(err.square().mean().sqrt()))
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
@@ -320,6 +398,22 @@ def test_a_query_that_sees_nothing_finite_says_so(bad):
     for s in range(3):
         set_slot(c, 1, s, None, 0.0)
     close(*chunk(c, (4, 1), qkv=qkv))
+
+
+@pytest.mark.parametrize("later", [1e9, 1e30, math.nan])
+def test_unseen_values_change_no_bit(later):
+    """What a query does not see changes none of its bits, whatever its size: later
+    tokens of the chunk, slots that fell out of its window."""
+    runs = []
+    for size in (1.0, later):
+        c = Cache((300, 140), 90, 4, 2, seed=75)
+        qkv = c.qkv(180)
+        qkv.view(180, 8, HD)[[80, 90 + 30], 6:] *= size  # row 0's token 80, row 1's token 30
+        set_slot(c, 0, 100, None, size)  # behind a window of 250 from row 0's token 50 on
+        runs.append(chunk(c, (90, 90), 250, 3, qkv=qkv)[0])
+    a, b = runs
+    assert torch.equal(a[50:80], b[50:80]) and torch.equal(a[90:120], b[90:120])
+    assert torch.isfinite(a).all() and not torch.equal(a[80:90], b[80:90])
 
 
 def test_chunk_attention_sharp_and_flat_scores():
