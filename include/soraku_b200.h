@@ -226,6 +226,9 @@ int skb_window_decode_attention(const float *qkv, int rows, int n_heads, int n_k
  * filled slots, each kv head keeps the first `sinks`, the last `recent` and, of
  * those between, the heaviest (equal weights: the lower slot; NaN counts as
  * heaviest), in slot order; their keys and values move to the front in place.
+ * A kept slot whose page-table entry names no page has none to move: NaN goes to
+ * its new place, so that attention goes on to answer NaN where it is seen.  A
+ * new place without a page takes nothing.
  *   kept       device int32 [rows, n_kv_heads, budget]: where each kept slot
  *              was; -1 behind the last
  *   mass_out   device, like mass: the kept slots' weights, zeros behind them

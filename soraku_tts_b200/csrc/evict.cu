@@ -63,7 +63,7 @@ struct EvictSmem {
     int wcount[EV_WARPS][2];
     unsigned border;
     int left;
-    uint32_t src[EV_BLOCK], dst[EV_BLOCK];  // units in the pool; UT_NONE: nothing to move
+    uint32_t src[EV_BLOCK], dst[EV_BLOCK];  // units in the pool; src UT_NONE: nothing to move, UT_BAD: no page
 };
 
 // Unsigned keys in the order of the floats; NaN of either sign above all.
@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictArgs a)
                 u = a.kv.key_unit(r, __ldcg(kept + b0 + i), g);
                 d = a.kv.key_unit(r, b0 + i, g);
             }
-            const bool ok = u >= 0 && d >= 0;
-            sm.src[i] = ok ? (uint32_t)u : UT_NONE;
+            // a kept slot without a page: its new place must not go on holding another's row
+            sm.src[i] = d < 0 ? UT_NONE : u < 0 ? UT_BAD : (uint32_t)u;
             sm.dst[i] = (uint32_t)d;
         }
         __syncthreads();
@@ -310,7 +310,8 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictArgs a)
 #pragma unroll
             for (int j = 0; j < EV_UNROLL; ++j) {
                 const uint32_t u = sm.src[i0 + j * Shape::ROWS + tr];
-                if (u != UT_NONE) x[j] = __ldcg(pool4 + (long long)u * 32);
+                if (u < UT_BAD) x[j] = __ldcg(pool4 + (long long)u * 32);
+                else x[j].x = x[j].y = x[j].z = x[j].w = __int_as_float(0x7fffffff);
             }
         };
         auto store = [&](const float4 (&x)[EV_UNROLL], int i0) {

@@ -369,7 +369,8 @@ def evict_cache(mass: torch.Tensor, *, cached: torch.Tensor, kv_pool: torch.Tens
     slot order, in place; see skb_evict_cache in include/soraku_b200.h.  Returns
     (kept int32 [rows, n_kv_heads, budget], the slots that were kept, -1 behind
     the last; the weights moved alike, zeros behind them; the new ``cached``).
-    The pages behind ``ceil(cached / page_size)`` are then free."""
+    The pages behind ``ceil(cached / page_size)`` are then free.  A kept slot whose
+    page-table entry names no page becomes NaN where it moves to."""
     _whole(budget, "budget", 1)
     _whole(sinks, "sinks")
     _whole(recent, "recent")

@@ -739,6 +739,56 @@ def test_evict_long_and_many_rows():
     check_evict(Cache([int(x) for x in torch.randint(-1, 90, (70,), generator=g)], 1, 2, 1, seed=3), 33, 1, 5)
 
 
+@pytest.mark.parametrize("cached,budget", [((300, 260), 100), ((5000, 2600), 2100)])
+def test_evict_slots_without_a_page(cached, budget):
+    """Pages that are not in the pool under kept slots, evicted ones and new places:
+    NaN where a kept slot would have moved to, the other slots as ever, and nothing
+    written elsewhere."""
+    from soraku_tts_b200 import kernels
+
+    c = Cache(cached, 1, 2, 2, page=16, seed=7)
+    table = c.table.clone()
+    lost = [(0, 1, -1), (0, cached[0] // 2 // 16, 10**6), (1, cached[1] // 16 - 1, c.pool.shape[0]), (1, 2, -5)]
+    for r, page, bad in lost:
+        c.table[r, page] = bad
+    # every slot of the lost pages weighs most, but for row 1's page 2: all evicted
+    for r, page, _ in lost:
+        c.mass[r, :, page * 16:page * 16 + 16] = -1.0 if (r, page) == (1, 2) else 9.0
+    pool, before = c.pool.clone(), c.mass.clone()
+    whole = table.clone()
+    good = c.table
+    c.table = whole
+    want_kept, want_mass, _ = plain_evict(c, budget, 3, 20)
+    kept, mass, count = kernels.evict_cache(c.mass, cached=c.cached, kv_pool=c.pool, page_table=good, page_size=16,
+                                            budget=budget, sinks=3, recent=20)
+    assert torch.equal(kept.cpu(), want_kept) and torch.equal(mass, want_mass) and torch.equal(c.mass, before)
+    want = pool.clone()
+    moved = 0
+    gone = {(r, page) for r, page, _ in lost}
+    for r in range(2):
+        slot = want_kept[r].cuda().long()  # [G, budget]
+        at = torch.arange(budget, device="cuda").expand_as(slot)
+        g = torch.arange(2, device="cuda")[:, None].expand_as(slot)
+        rows = pool[whole[r][slot // 16].long(), :, g, slot % 16]  # [G, budget, 2, HD]
+        off = torch.zeros_like(slot, dtype=torch.bool)
+        skip = torch.zeros_like(off)
+        for rr, page in gone:
+            if rr == r:
+                off |= slot // 16 == page
+                skip |= at // 16 == page
+        off &= slot != at  # what stays in place stays as it is: without a page
+        rows[off] = math.nan
+        put = ~skip
+        want[whole[r][at[put] // 16].long(), :, g[put], at[put] % 16] = rows[put]
+        moved += int((off & put).sum())
+    assert moved > 20
+    assert torch.equal(torch.isnan(c.pool), torch.isnan(want)) and torch.equal(torch.nan_to_num(c.pool), torch.nan_to_num(want))
+    # and attention shows it
+    c.table, c.cached, c.pos = good, count, c.cached.clone()
+    out = kernels.window_decode_attention(c.qkv(2), **c.args(page_table=good))
+    assert torch.isnan(out).view(2, 2, HD).any(-1).all()
+
+
 def test_evict_counts_outside_the_cache():
     c = Cache((30, 30, 30), 2, 2, 2, seed=4)
     c.cached[0], c.cached[1] = c.slots + 1, -1
