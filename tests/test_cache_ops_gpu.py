@@ -739,6 +739,46 @@ def test_evict_long_and_many_rows():
     check_evict(Cache([int(x) for x in torch.randint(-1, 90, (70,), generator=g)], 1, 2, 1, seed=3), 33, 1, 5)
 
 
+def sorted_evict(c, budget, sinks, recent):
+    """plain_evict by a stable sort, for many long rows (no NaN among the weights)."""
+    kept, mass, pool = [], torch.zeros_like(c.mass), c.pool.clone()
+    for r in range(c.rows):
+        n = int(c.cached[r])
+        i = torch.arange(n, device="cuda").expand(c.G, -1)
+        w = c.mass[r, :, :n].clone()
+        w[(i < sinks) | (i >= n - recent)] = math.inf
+        k = torch.sort(torch.sort(w, dim=1, descending=True, stable=True).indices[:, :min(n, budget)], dim=1).values
+        kept.append(torch.nn.functional.pad(k, (0, budget - k.shape[1]), value=-1))
+        mass[r, :, :k.shape[1]] = torch.gather(c.mass[r], 1, k)
+        g = torch.arange(c.G, device="cuda")[:, None].expand_as(k)
+        at = torch.arange(k.shape[1], device="cuda").expand_as(k)
+        page = c.table[r].long()
+        pool[page[at // c.page], :, g, at % c.page] = c.pool[page[k // c.page], :, g, k % c.page]
+    return torch.stack(kept).to(torch.int32), mass, pool
+
+
+# Groups of two CTAs (38 of them or more) and of eight; rows whose keys a cluster
+# holds in registers (16384 slots for two CTAs, 65536 for eight) and rows that it
+# reads again; budgets of more rows than a CTA looks up at once (2048).
+@pytest.mark.parametrize("rows,kv_heads,shortest,longest,budget", [
+    (38, 1, 2049, 9000, 2100), (5, 8, 2049, 6000, 4097), (40, 1, 1500, 2600, 2050), (19, 2, 16300, 16900, 5000),
+    (38, 1, 17000, 20000, 2049), (1, 1, 66000, 66000, 30000), (1, 2, 65536, 65536, 2500)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_long_rows_of_many_groups(rows, kv_heads, shortest, longest, budget, ties):
+    from soraku_tts_b200 import kernels
+
+    cached = [longest - (longest - shortest) * r // max(1, rows - 1) for r in range(rows)]
+    c = Cache(cached, 1, kv_heads, kv_heads, page=64, seed=rows + budget, max_pos=64)
+    c.pool64 = c.mass64 = None
+    if ties:
+        c.mass = (c.mass * 5).floor()
+    want_kept, want_mass, want_pool = sorted_evict(c, budget, 5, 77)
+    kept, mass, count = kernels.evict_cache(c.mass, cached=c.cached, kv_pool=c.pool, page_table=c.table, page_size=64,
+                                            budget=budget, sinks=5, recent=77)
+    assert torch.equal(kept, want_kept) and torch.equal(mass, want_mass) and torch.equal(c.pool, want_pool)
+    assert torch.equal(count, torch.clamp(c.cached, max=budget))
+
+
 @pytest.mark.parametrize("cached,budget", [((300, 260), 100), ((5000, 2600), 2100)])
 def test_evict_slots_without_a_page(cached, budget):
     """Pages that are not in the pool under kept slots, evicted ones and new places:
