@@ -113,8 +113,13 @@ __device__ __forceinline__ bool row_mapped(const ChunkArgs& c, int r, const Chun
     return all;
 }
 // row_base where the rows see more than the pool can hold, so that some see
-// slots without a page: room for the others alone.
-__device__ __forceinline__ int row_base_mapped(const ChunkArgs& c, int r) {
+// slots without a page: room for the others alone.  Every warp goes through the
+// rows one by one, 1 us each, so only for up to CP_SORTED of them; of more, those
+// before the first that finds no room have theirs, in the plain order.
+constexpr int CP_SORTED = 512;   // more rows than that are taken as they come
+__device__ __forceinline__ int row_base_mapped(const ChunkArgs& c, int r, int before) {
+    if (c.a.rows > CP_SORTED)
+        return before + RowTiles(c, chunk_row(c, r)).n <= c.key_tiles ? before : -1;
     int base = 0;
     for (int p = 0; p <= r; ++p) {
         const ChunkRow x = chunk_row(c, p);
@@ -138,8 +143,9 @@ __device__ __forceinline__ int row_base(const ChunkArgs& c, int r) {
         all = min(all + RowTiles(c, chunk_row(c, p)).n, CHUNK_TILES);
         if (p < r) before = all;
     }
-    if (!c.roomy && __reduce_add_sync(FULL, all) > c.key_tiles) return row_base_mapped(c, r);
-    return __reduce_add_sync(FULL, before);
+    before = __reduce_add_sync(FULL, before);
+    if (!c.roomy && __reduce_add_sync(FULL, all) > c.key_tiles) return row_base_mapped(c, r, before);
+    return before;
 }
 
 // A whole number e with |q| < 2^e for every query in log2 units: a normed head
@@ -169,7 +175,6 @@ constexpr float CH_QSCALE = 0.08838834764831845f * CO_LOG2E;  // 1 / sqrt(128), 
 
 constexpr int CP_TILES = 64;     // blocks side by side over a row's key tiles
 constexpr int CP_NQ = 2;         // groups of four rows a warp holds at once
-constexpr int CP_SORTED = 512;   // more rows than that are taken as they come
 
 // The first `token_blocks` blocks: `per_block` new tokens each (1, 2 or 4), 8 /
 // per_block warps to a token, which take its head vectors in turn.  Few tokens
@@ -206,7 +211,7 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const __grid_constan
         if (i < 0 || i >= x.n) return;
         const RowTiles rt(c, x);
         int base = __reduce_add_sync(FULL, before);
-        if (!c.roomy && __reduce_add_sync(FULL, all) > c.key_tiles) base = row_base_mapped(c, r);
+        if (!c.roomy && __reduce_add_sync(FULL, all) > c.key_tiles) base = row_base_mapped(c, r, base);
         // (rows that begin before the one ahead ends are counted otherwise elsewhere)
         if (base < 0 || base + rt.n > c.key_tiles) x.bad = true;
         if (x.idle || x.bad) {
@@ -271,7 +276,7 @@ __global__ void __launch_bounds__(256, 4) chunk_prep_kernel(const __grid_constan
         __syncthreads();
         if (all > (unsigned long long)c.key_tiles) {  // rows without room are left out
             for (int p = warp; p < a.rows; p += 8)
-                if (row_base_mapped(c, p) < 0 && lane == 0) seen[p] = tiles[p] = 0;
+                if (row_base_mapped(c, p, 0) < 0 && lane == 0) seen[p] = tiles[p] = 0;
             __syncthreads();
         }
         for (int p = threadIdx.x; p < a.rows; p += 256) {

@@ -1073,6 +1073,32 @@ def test_row_counts_whose_sum_passes_32_bits():
     assert not pool[:, :, :, 8:].any()
 
 
+def test_many_rows_beside_rows_without_pages():
+    """More than 512 rows that claim more than the pool has: those before the first
+    row without pages are right, the others right or NaN with nothing written."""
+    from soraku_tts_b200 import kernels
+
+    rows, sick = 700, 300
+    c = Cache([40 + r % 9 for r in range(rows)], 2, 2, 1, seed=64, spare=2)
+    pool, mass = c.pool.clone(), c.mass.clone()
+    cached, table = c.cached.clone(), torch.full((rows, 2**16), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.max_pages] = c.table
+    table[sick] = -1
+    cached[sick] = 2**20 - 3
+    qkv = c.qkv(2 * rows)
+    got = kernels.chunk_attention(qkv, chunk_start=starts([2] * rows), max_chunk=2,
+                                  **c.args(page_table=table, cached=cached)).view(rows, 2, -1)
+    c.cached[sick] = -1
+    want = c.want(qkv, [2] * rows).view(rows, 2, -1)
+    fine = ~torch.isnan(got).view(rows, -1).any(-1)
+    assert fine[:sick].all() and not fine[sick]
+    close(got[fine].view(-1, 2 * HD), want[fine].view(-1, 2 * HD))
+    pages = c.table[~fine].long().flatten()
+    assert torch.equal(c.pool[pages], pool[pages])
+    pages = c.table[fine].long().flatten()
+    torch.testing.assert_close(c.pool[pages].double(), c.pool64[pages], rtol=0, atol=5e-6)
+
+
 def test_python_layer_refusals():
     from soraku_tts_b200 import kernels
 
