@@ -1099,6 +1099,38 @@ def test_many_rows_beside_rows_without_pages():
     torch.testing.assert_close(c.pool[pages].double(), c.pool64[pages], rtol=0, atol=5e-6)
 
 
+@pytest.mark.parametrize("heads", [(16, 8), (9, 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 3)])
+def test_value_rows_of_all_sizes_in_a_full_batch(heads, window, sinks):
+    """Values of very unlike sizes in some rows of a batch that goes by the list of
+    rows, zeros, and values that are not finite out of sight; the same bits twice."""
+    lengths = [(37 * r * r + 11 * r) % 330 for r in range(30)]
+    cached = [0 if r % 3 else (53 * r) % 400 for r in range(30)]
+    runs = []
+    for _ in range(2):
+        c = Cache(cached, 330, *heads, seed=77)
+        H, G = heads
+        size = torch.exp2((2 * torch.rand(sum(lengths), G, 1, generator=c.gen, device="cuda") - 1) * 30)
+        qkv = c.qkv(sum(lengths))
+        row = torch.repeat_interleave(torch.arange(30, device="cuda"), torch.tensor(lengths, device="cuda"))
+        v = qkv.view(-1, H + 2 * G, HD)[:, H + G:]
+        v *= torch.where((row % 4 == 1)[:, None, None], size, torch.ones_like(size))
+        v[row % 5 == 2] = 0.0
+        for r in range(0, 30, 3):
+            for s in range(0, cached[r], 7):
+                set_slot(c, r, s, None, 0.0 if s % 2 else 3e7)
+        got, want = chunk(c, lengths, window, sinks, mass=True, qkv=qkv)
+        runs.append((got, c.mass))
+    norm = want.view(-1, heads[0], HD).norm(dim=-1)
+    err = (got.double() - want).view(-1, heads[0], HD).norm(dim=-1)
+    some = norm > 0
+    assert torch.isfinite(got).all() and not err[~some].any()
+    rel = err[some] / norm[some]  # bounds as in test_value_rows_of_all_sizes
+    assert float(rel.max()) <= 2 * ATOL and float(rel.square().mean().sqrt()) <= REL, (float(rel.max()), float(rel.square().mean().sqrt()))
+    c.check_mass()
+    assert torch.equal(runs[0][0], runs[1][0]) and torch.equal(runs[0][1], runs[1][1])
+
+
 def test_python_layer_refusals():
     from soraku_tts_b200 import kernels
 
