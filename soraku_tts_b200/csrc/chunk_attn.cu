@@ -398,7 +398,8 @@ constexpr int CA_MAX_SPLITS = 8;
 // Weights are held as p 2^(e - E + CA_UP) in fp16 pairs, e the exponent of the
 // value row, whose own numbers are below 2^14.  A pair resolves 2^-25 whatever it
 // holds, so what counts is where a query's largest contribution p 2^e lies.
-//   Values of like sizes: E is set by the first tile, CA_ABOVE above its largest e,
+//   Values of like sizes: E is set by the first tile, CA_ABOVE above its largest e
+//   (or, where queries see different parts of it, above one e that they share),
 //   and serves as long as every e in sight lies in [E - CA_SPREAD, E].  The factors
 //   2^(e - E + CA_UP) are then the same for all queries, and the key with the largest
 //   weight, 1/2 at least, gives 2^(CA_UP - CA_SPREAD - 1) = 4, or 2^27 times the resolution.
@@ -407,7 +408,7 @@ constexpr int CA_MAX_SPLITS = 8;
 //   is formed by an exponential of its own beside the one that goes into the sum
 //   (8 prompts: 194 us a call instead of 166).
 // Which of them holds goes by the values that the query sees, and no other.
-constexpr float CA_UP = 12.f, CA_ABOVE = 2.f, CA_SPREAD = 9.f;
+constexpr float CA_UP = 12.f, CA_ABOVE = 3.f, CA_SPREAD = 9.f;
 constexpr float CA_SLACK = 3.f;  // how far a score, or a contribution, may pass its reference: 2^(12 + 3) fits fp16
 
 struct CaSmem {
@@ -814,33 +815,33 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
             bool mixed = false;
             if (whole) E_new = sm.E[b];
             if (!whole || i == 0 || softmax_any((mx > m + CA_SLACK && hi >= 0) || E_new == INFINITY)) {
-                // Exponents of the values that a row sees, where those of the tile
-                // do not tell all there is to know; the smallest only where it may be too small.
+                // A row without E takes it from one value that it sees, the same
+                // for as many rows as can be.  The exponents that a row sees are looked
+                // through only where those of the tile do not all fit.
                 const float top = sm.top[b], low = sm.low[b];
-                const bool ask = !whole && hi >= 0 && !own, fresh = E == UT_POISON_E;
-                const bool look = __any_sync(FULL, ask && (fresh || top > E || low < E - CA_SPREAD));
-                const bool wide = __any_sync(FULL, ask && (low < (fresh ? top + CA_ABOVE : E) - CA_SPREAD || low == UT_POISON_E));
-                float ex = UT_POISON_E, lo = INFINITY;
+                const bool ask = !whole && hi >= 0 && !own;
+                if (ask && E == UT_POISON_E) {
+                    const int first = base_slot - part * CA_W;
+                    const int one = first < a.sinks ? first : min(max(sm.own[0], first), first + 127);
+                    const float e = sm.ve[b][one - first];
+                    if (one <= hi && (one > lo || one < a.sinks) && e > UT_POISON_E) E_new = e + CA_ABOVE;
+                }
+                const bool look = __any_sync(FULL, ask && (E_new == UT_POISON_E || top > E_new || low < E_new - CA_SPREAD));
+                float ex = UT_POISON_E, bot = INFINITY;
                 if (look) {
-#pragma unroll 1  // once a query tile, and registers are scarce
-                    for (int q = 0; q < CA_W / 4; ++q) {
-                        const float4 f = reinterpret_cast<const float4*>(ve)[q];
-                        const uint32_t w = seen >> (4 * q);
-                        ex = fmaxf(fmaxf(ex, w & 1u ? f.x : ex), w & 2u ? f.y : ex);
-                        ex = fmaxf(fmaxf(ex, w & 4u ? f.z : ex), w & 8u ? f.w : ex);
+#pragma unroll 1
+                    for (int q = 0; q < CA_W; ++q) {
+                        if (!(seen >> q & 1u)) continue;
+                        ex = fmaxf(ex, ve[q]);
+                        bot = fminf(bot, ve[q]);
                     }
                     sm.ex[b][part][row] = ex;
-                    if (wide) {
-#pragma unroll 4
-                        for (int q = 0; q < CA_W; ++q)
-                            if (seen >> q & 1u) lo = fminf(lo, ve[q]);
-                        sm.lo[b][part][row] = lo;
-                    }
+                    sm.lo[b][part][row] = bot;
                 }
                 sm.mx[b][part][row] = mx;
                 // some row's E follows its contributions, or may have to
                 mixed = softmax_any(whole ? E_new == INFINITY
-                                          : hi >= 0 && (own || (fresh ? wide : ex > E || lo < E - CA_SPREAD || lo == UT_POISON_E)));
+                                          : hi >= 0 && (own || (E_new == UT_POISON_E ? bot < INFINITY : ex > E_new || bot < E_new - CA_SPREAD)));
 #pragma unroll
                 for (int q = 0; q < CA_PARTS; ++q) mx = fmaxf(mx, sm.mx[b][q][row]);
                 const float m_new = mx > m + CA_SLACK && hi >= 0 ? ceilf(mx) : m;
@@ -849,13 +850,12 @@ __global__ void __launch_bounds__(CA_THREADS, 1) chunk_attn_kernel(const __grid_
                 l *= exp2_fast(d_m);
                 if (look) {
 #pragma unroll
-                    for (int q = 0; q < CA_PARTS; ++q) ex = fmaxf(ex, sm.ex[b][q][row]);
-                    if (wide) {
-#pragma unroll
-                        for (int q = 0; q < CA_PARTS; ++q) lo = fminf(lo, sm.lo[b][q][row]);
+                    for (int q = 0; q < CA_PARTS; ++q) {
+                        ex = fmaxf(ex, sm.ex[b][q][row]);
+                        bot = fminf(bot, sm.lo[b][q][row]);
                     }
-                    if (fresh && ex > UT_POISON_E) E_new = ex + CA_ABOVE;
-                    own = own || ex > E_new || lo < E_new - CA_SPREAD || lo == UT_POISON_E;
+                    if (ask && E_new == UT_POISON_E && ex > UT_POISON_E) E_new = ex + CA_ABOVE;
+                    own = own || (ask && (ex > E_new || bot < E_new - CA_SPREAD || bot == UT_POISON_E));
                 }
             }
             if (whole) own = E_new == INFINITY;
