@@ -1310,9 +1310,12 @@ extern "C" int skb_chunk_attention(const float* qkv, int tokens, int rows, int n
     long long row_tiles = chunk_row_tiles(most, max_pages, page_size, window, sinks);
     if (row_tiles > c.key_tiles) row_tiles = c.key_tiles;
     // CTAs that have work, at most; while they leave SMs idle, up to 8 share a
-    // query tile's key tiles.  (Sharing where they fill the card already makes
-    // clusters wait for SMs and adds the join: 8 prompts 199 us in pairs, 117 alone;
-    // two rows of five tokens 13.7 us alone, 12.5 in eights.)
+    // query tile's key tiles, as long as no SM gets two.  (Sharing where they fill
+    // the card already makes clusters wait for SMs and adds the join: 8 prompts 199 us
+    // in pairs, 117 alone.  Calls alone, in pairs, in threes: 512 tokens behind 8192
+    // slots, 64 CTAs, 193, 112 with the two that this rule gives, 149; 640, 80 CTAs,
+    // 174 alone as it gives, 190, 151; 1152, 144 CTAs, 232, 251, 300.  Two rows of
+    // five tokens 18.5 alone, 17.3 in threes, one for each of their key tiles.)
     long long ctas = (long long)rows * tiles_x;
     if (ctas > tiles) ctas = tiles;
     ctas *= n_kv_heads;

@@ -20,10 +20,12 @@
 //           without any order between them.  Where rows come from and go to is looked up
 //           for EV_BLOCK rows at once, so that a round waits for its data alone,
 //           and two rounds are on their way at a time.
-// Bound by memory: each kept slot that moves is 1 KB in and 1 KB out (128 groups
-// of 5k to 8k slots to 2k: 119 us, 70 % of a plain copy's rate; two rounds are what
-// the registers hold, and a longer ring in shared memory, with fewer CTAs an SM,
-// took 122 us, and 142 instead of 120 at 32k slots).
+// Each kept slot that moves is 1 KB in and 1 KB out.  128 groups of 5k to 8k slots
+// to 2k take 121 us, 69 % of a plain copy's rate; with weights that keep the
+// first slots, so that only the 256 recent ones move, 34.  So about a quarter is
+// the search, which all groups do at the same time while memory is idle, and the move
+// runs near a copy's rate (a longer ring in shared memory, with fewer CTAs an
+// SM, took 122 us, and 142 instead of 120 at 32k slots).
 #include "cache_ops.cuh"
 
 namespace skb {
@@ -373,8 +375,12 @@ extern "C" int skb_evict_cache(const float* mass, const int32_t* cached, int row
     a.mass_out = mass_out;
     a.cached_out = cached_out;
     // 8 CTAs a group while all of them fit the card at once (two on each of
-    // 148 SMs); more groups take whole rows, which memory likes better: 128
-    // groups of 8k slots to 2k 120 us, against 126 in halves and 160 in quarters
+    // 148 SMs); more groups take whole rows.  Measured, us a call in eights, fours
+    // (no variant here) and twos, rows of up to 8k slots to 2k: 32 groups 41, 43, 57;
+    // 40 groups 71, 51, 61; 64 groups 86, 68, 72; 96 groups 124, 106, 100; 128 groups
+    // 161, 129, 121; rows of up to 842 slots to 512: 40 groups 27, 20, 18.  40 and 64
+    // groups of 20k slots to 5k: 133, 105, 154 and 157, 147, 174: there eights would
+    // be the better of the two that there are.
     const int ctas = (long long)rows * n_kv_heads * 8 <= 296 ? 8 : 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, n_kv_heads, rows);

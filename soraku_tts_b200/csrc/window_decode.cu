@@ -366,8 +366,14 @@ static cudaError_t window_decode_launch(const WdArgs& w, cudaStream_t stream) {
     static std::atomic<unsigned long long> done;
     cudaError_t e = smem_attrs_once(window_decode_kernel<NR>, smem, done);
     if (e != cudaSuccess) return e;
-    // Enough CTAs to fill 148 SMs twice over while the cluster stays within
-    // the portable 8.
+    // Up to 592 CTAs, two waves of two an SM (four of one for 3 and 4 heads a kv
+    // head), while the cluster stays within the portable 8.  Measured, us a call with
+    // at most 296, 592 and 1184 CTAs: two heads, 296 groups of 1000 to 2000 slots 77, 79,
+    // 82; 160 groups of 3000 to 6000 137, 132, 122; 128 of 4000 to 8000 131, 129,
+    // 129; 72 of 3000 to 6000 60, 63, 63.  Four heads, in the same order: 89, 98, 131;
+    // 173, 144, 144; 141, 149, 190; 74, 92, 92.  No limit is best for all.  128 short rows
+    // (120 to 842 slots, 8 kv heads, a CTA a group) with 1, 2, 3 and 4 heads a kv
+    // head: 83, 88, 109 and 120 us for 79 us of bytes at a copy's rate.
     const long long groups = (long long)w.a.rows * w.a.kv.KVH;
     int C = WD_MAXC;
     while (C > 1 && groups * C > 592) C >>= 1;
