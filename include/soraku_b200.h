@@ -174,12 +174,13 @@ int skb_decode_attention_noalloc(const float *qkv, int rows, int n_heads, int n_
  * Rows with cached < 0 are idle: zeros out, the cache untouched.  A row whose
  * counts or positions lie outside the inputs, the cache or the RoPE tables
  * returns NaN and leaves the cache untouched, and so does every query that
- * sees a slot whose page-table entry names no page (where the rows of a chunk
+ * sees a slot whose page-table entry names no page.  (Where the rows of a chunk
  * call see more slots than the pool has, a row that sees such a slot returns NaN
  * whole and leaves the cache untouched; no other row is touched by it, unless
- * the call has more than 512 rows: then the rows behind it may be).  Slots that a query does
- * not see cannot change its output, whatever they hold; a query head that sees
- * a key or value that is not finite returns 128 numbers that are not all finite.
+ * the call has more than 512 rows: then the rows behind it may be.)  Slots that
+ * a query does not see need no page and cannot change its output, whatever they
+ * hold; a query head that sees a key or value that is not finite returns 128
+ * numbers that are not all finite.  Outputs overlap no input.
  * `mass` (optional): device [rows, n_kv_heads, max_pages * page_size], the
  * softmax weights a slot received, added up over the queries and the heads of
  * the group; the slots of new tokens begin at zero.
