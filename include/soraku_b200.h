@@ -241,6 +241,64 @@ int skb_evict_cache(const float *mass, const int32_t *cached, int rows, int n_kv
                     const int32_t *page_table, int max_pages, int page_size, int n_pages, int budget, int sinks,
                     int recent, int32_t *kept, float *mass_out, int32_t *cached_out, cudaStream_t stream);
 
+/* ------------------------------------------------------------------------
+ * A decoding step in 8-bit integers, up to the drawn token.  Types of rows:
+ * values in FP32, BF16 or FP16, or 8-bit codes with a scale for each row.
+ * ---------------------------------------------------------------------- */
+#define SKB_F32 0
+#define SKB_BF16 1
+#define SKB_F16 2
+#define SKB_I8 3
+
+/* Rows [rows, K] (row stride ldx elements) to codes and scales: with y = x, or
+ * x * norm_weight in FP32, and s = max(max |y| / 127, 2^-126),
+ *   q[k] = round(y[k] / s) (the FP32 quotient, halves to even),
+ *   scale = s, or s / sqrt(mean(x^2) + eps) with a norm,
+ * so that q * scale is about the row, RMS-normed where norm_weight [K] is not
+ * NULL.  A row that holds something not finite becomes zeros with the scale NaN.
+ * Rows of q begin on 16 bytes (ldq a multiple of 16, at least K rounded up to
+ * one); what lies between K and that is set to 0.  K: 1 to 131071. */
+int skb_quantize_rows(const void *x, int x_type, int64_t ldx, int rows, int K, const float *norm_weight, float eps,
+                      int8_t *q, int64_t ldq, float *scale, cudaStream_t stream);
+
+/* out[t, n] = (sum_k xq[t, k] w[n, k]) x_scale[t] w_scale[n] + bias[n] + residual[t, n]
+ * for T rows x: values, which become codes as by skb_quantize_rows (x_scale
+ * NULL; norm_weight NULL: no norm), or codes with x_scale [T].  The sum is
+ * exact, the rest is FP32, rounded once to out_type.  w [N, K] codes with
+ * w_scale [N]; rows of codes begin on 16 bytes and are readable up to K rounded
+ * up to 16 (what lies there counts for nothing).  bias [N] FP32 and residual
+ * [T, N] (of out_type; may be out itself) may be NULL.  Row strides ldx, ldr,
+ * ldo are in elements.  out overlaps no other input.  Workspace of
+ * skb_int8_workspace(T, K, x_type) bytes, 16-byte aligned (NULL where that is 0). */
+int64_t skb_int8_workspace(int T, int K, int x_type);
+int skb_int8_linear(const void *x, int x_type, int64_t ldx, const float *x_scale, const float *norm_weight, float eps,
+                    int T, int K, const int8_t *w, int64_t ldw, const float *w_scale, int N, const float *bias,
+                    const void *residual, int64_t ldr, void *out, int out_type, int64_t ldo, void *workspace,
+                    int64_t workspace_bytes, cudaStream_t stream);
+
+/* out[t, i] = silu(g) u, with g and u the products of row t with gate and up
+ * [I, K], as skb_int8_linear forms them. */
+int skb_int8_swiglu(const void *x, int x_type, int64_t ldx, const float *x_scale, const float *norm_weight, float eps,
+                    int T, int K, const int8_t *gate, int64_t ldg, const float *gate_scale, const int8_t *up, int64_t ldu,
+                    const float *up_scale, int I, void *out, int out_type, int64_t ldo, void *workspace,
+                    int64_t workspace_bytes, cudaStream_t stream);
+
+/* One token of each row of logits [rows, V] (V at most 2^18, row stride ld; a
+ * masked logit is -infinity) by its uniform number in [0, 1).  In the order
+ * (logit descending, index ascending), with e_j = exp((l_j - max) / temperature):
+ * the first top_k stay (<= 0: all); of those the shortest prefix whose mass is
+ * at least top_p of theirs (>= 1: all; never less than one token); of those the ones
+ * with e_j >= min_p.  tokens[row] is the first whose running sum of e passes
+ * uniform times the kept ones' sum, logprob[row] the logarithm of its share of
+ * that sum.  A temperature that is not above 0 takes the largest logit, the first of
+ * equal ones.  The settings are numbers, or device arrays [rows] where those are
+ * not NULL.  A row that is masked whole, or holds NaN: token -1, logprob NaN;
+ * logits of +infinity share all the mass.  Weights below 2^-45 count for nothing. */
+int skb_sample_tokens(const void *logits, int type, int64_t ld, int rows, int V, const float *uniform,
+                      const float *temperatures, float temperature, const int32_t *top_ks, int top_k,
+                      const float *top_ps, float top_p, const float *min_ps, float min_p, int64_t *tokens,
+                      float *logprob, cudaStream_t stream);
+
 /* Test hooks: the device exp used by the sampler, and raw Philox4x32-10.
  * ctr_key: device uint32 [n, 6] = (c0, c1, c2, c3, k0, k1); out: [n, 4]. */
 int skb_test_exp(const float *x, float *y, int n, cudaStream_t stream);

@@ -50,6 +50,17 @@ SIGNATURES = {
                                             c_void_p]),
     "skb_evict_cache": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
                                 c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "skb_quantize_rows": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_float, c_void_p, c_int64, c_void_p,
+                                  c_void_p]),
+    "skb_int8_workspace": (c_int64, [c_int] * 3),
+    "skb_int8_linear": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_float, c_int, c_int, c_void_p, c_int64,
+                                c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64,
+                                c_void_p]),
+    "skb_int8_swiglu": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_float, c_int, c_int, c_void_p, c_int64,
+                                c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_int64, c_void_p, c_int64,
+                                c_void_p]),
+    "skb_sample_tokens": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_int,
+                                  c_void_p, c_float, c_void_p, c_float, c_void_p, c_void_p, c_void_p]),
     "skb_test_exp": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
     "skb_test_philox": (c_int, [c_void_p, c_void_p, c_int, c_void_p]),
     "skb_test_wait_timeout": (c_int, [c_void_p, c_int, c_void_p]),

@@ -1,0 +1,164 @@
+// Products of a few tokens' codes with 8-bit weights, bound by the weights'
+// bytes: the tokens' rows become codes in every CTA's shared memory (one launch
+// for norm, codes and product), each warp streams whole weight rows, four a
+// step, and adds up products of four bytes an instruction.
+#include "int8_ops.cuh"
+
+namespace skb {
+
+constexpr int GV_THREADS = 256, GV_WARPS = 8;
+constexpr int GV_ROWS = 4;      // weight rows a warp takes at a time (2 gate and 2 up rows)
+constexpr int GV_CHUNK = 512;   // bytes of a row that a warp reads at once
+constexpr int GV_MAX_T = 8;
+constexpr int GV_MAX_X = 128 * 1024;  // bytes of codes in shared memory: one token of any length
+constexpr int GV_FUSED = 32 * 1024;   // up to here each CTA makes the codes itself
+
+// TT: tokens a CTA holds (the last ones may be missing).
+template <class TX, int TT, bool GLU>
+__global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args a) {
+    extern __shared__ __align__(16) int8_t gv_x[];  // [TT][kp]
+    __shared__ float red[2 * GV_WARPS];
+    __shared__ float sx[TT];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int K = a.in.K, kp = ceil16(K);
+    const int t0 = blockIdx.y * TT, nt = min(TT, a.in.T - t0);
+    constexpr int PER = GLU ? GV_ROWS / 2 : GV_ROWS;  // output columns a step
+    const int groups = (a.N + PER - 1) / PER;
+    const int chunks = (kp + GV_CHUNK - 1) / GV_CHUNK;
+    pdl_wait();
+    pdl_trigger();
+
+    auto fetch = [&](uint4 (&w)[GV_ROWS], int group, int chunk) {
+        const int k = chunk * GV_CHUNK + lane * 16;
+#pragma unroll
+        for (int r = 0; r < GV_ROWS; ++r) {
+            const int m = GLU ? r / PER : 0, n = group * PER + (GLU ? r % PER : r);
+            w[r] = make_uint4(0, 0, 0, 0);
+            if (group < groups && n < a.N && k < kp)
+                w[r] = __ldcg(reinterpret_cast<const uint4*>(a.w[m] + n * a.ldw[m] + k));
+        }
+    };
+    const int stride = gridDim.x * GV_WARPS;
+    int group = blockIdx.x * GV_WARPS + warp;
+    uint4 next[GV_ROWS];
+    fetch(next, group, 0);
+
+    // the tokens' codes
+    if constexpr (sizeof(TX) == 1) {
+        for (int i = tid; i < TT * (kp / 16); i += GV_THREADS) {
+            const int t = i / (kp / 16), k = i % (kp / 16) * 16;
+            uint4 c = make_uint4(0, 0, 0, 0);
+            if (t < nt) c = __ldcg(reinterpret_cast<const uint4*>(static_cast<const int8_t*>(a.in.x) + (t0 + t) * a.in.ld + k));
+            // whatever lies behind K counts for nothing, here and in the weights
+            uint32_t b[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int left = K - k - 4 * j;
+                if (left < 4) b[j] = left <= 0 ? 0u : b[j] & (0xffffffffu >> (32 - 8 * left));
+            }
+            *reinterpret_cast<uint4*>(gv_x + t * kp + k) = make_uint4(b[0], b[1], b[2], b[3]);
+        }
+        if (tid < TT) sx[tid] = tid < nt ? __ldcg(a.in.scale + t0 + tid) : 0.f;
+    } else {
+        constexpr int G = GV_THREADS / TT;
+        const int t = tid / G;
+        // a missing token repeats the last one, so that all threads take the same way
+        const TX* x = static_cast<const TX*>(a.in.x) + (long long)(t0 + min(t, nt - 1)) * a.in.ld;
+        const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+        const float s = quantize_row<TX, G, 16 / Vec<TX>::N>(x, a.in.nw, a.in.eps, K, aligned, gv_x + t * kp, tid % G,
+                                                             red + 2 * (t * G / 32));
+        if (tid % G == 0) sx[t] = s;
+    }
+    __syncthreads();
+
+    for (; group < groups; group += stride) {
+        int acc[GV_ROWS][TT];
+#pragma unroll
+        for (int r = 0; r < GV_ROWS; ++r)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[r][t] = 0;
+        for (int c = 0; c < chunks; ++c) {
+            uint4 w[GV_ROWS];
+#pragma unroll
+            for (int r = 0; r < GV_ROWS; ++r) w[r] = next[r];
+            if (c + 1 < chunks) fetch(next, group, c + 1);
+            else fetch(next, group + stride, 0);
+            const int k = c * GV_CHUNK + lane * 16;
+            if (k < kp) {
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    const int4 x = *reinterpret_cast<const int4*>(gv_x + t * kp + k);
+#pragma unroll
+                    for (int r = 0; r < GV_ROWS; ++r) {
+                        acc[r][t] = __dp4a((int)w[r].x, x.x, acc[r][t]);
+                        acc[r][t] = __dp4a((int)w[r].y, x.y, acc[r][t]);
+                        acc[r][t] = __dp4a((int)w[r].z, x.z, acc[r][t]);
+                        acc[r][t] = __dp4a((int)w[r].w, x.w, acc[r][t]);
+                    }
+                }
+            }
+        }
+        // lane (t, column) takes its sum
+        int v = 0, u = 0;
+#pragma unroll
+        for (int r = 0; r < GV_ROWS; ++r)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                const int sum = __reduce_add_sync(FULL, acc[r][t]);
+                if (lane == t * PER + (GLU ? r % PER : r)) {
+                    if (GLU && r >= PER) u = sum;
+                    else v = sum;
+                }
+            }
+        const int t = lane / PER, n = group * PER + lane % PER;
+        if (t < nt && lane < TT * PER && n < a.N) {
+            float y = (float)v * sx[t] * __ldcg(a.ws[0] + n);
+            if (GLU) {
+                y = silu(y) * ((float)u * sx[t] * __ldcg(a.ws[1] + n));
+            } else {
+                if (a.bias) y += __ldcg(a.bias + n);
+                if (a.residual) y += load_as_float(a.residual, a.out_type, (t0 + t) * a.ldr + n);
+            }
+            store_as(a.out, a.out_type, (t0 + t) * a.ldo + n, y);
+        }
+    }
+}
+
+bool int8_gemv_fuses(int T, int K) { return T <= GV_MAX_T && T * ceil16(K) <= GV_FUSED; }
+
+template <auto Kernel>
+static cudaError_t gemv_go(const Int8Args& a, dim3 grid, size_t smem, cudaStream_t s) {
+    const cudaError_t e = prepare_kernel<Kernel>(GV_MAX_X);
+    return e != cudaSuccess ? e : launch(Kernel, grid, dim3(GV_THREADS), smem, s, true, a);
+}
+
+template <class TX, bool GLU>
+static cudaError_t gemv_typed(const Int8Args& a, cudaStream_t s) {
+    const int T = a.in.T;
+    int tt = T == 1 ? 1 : T == 2 ? 2 : T <= 4 ? 4 : 8;
+    while (tt * ceil16(a.in.K) > GV_MAX_X) tt >>= 1;
+    const int per = GLU ? GV_ROWS / 2 : GV_ROWS;
+    const int blocks = ((a.N + per - 1) / per + GV_WARPS - 1) / GV_WARPS;
+    const dim3 grid(blocks < 296 ? blocks : 296, (T + tt - 1) / tt);
+    const size_t smem = (size_t)tt * ceil16(a.in.K);
+    if (tt == 1) return gemv_go<int8_gemv_kernel<TX, 1, GLU>>(a, grid, smem, s);
+    if (tt == 2) return gemv_go<int8_gemv_kernel<TX, 2, GLU>>(a, grid, smem, s);
+    if (tt == 4) return gemv_go<int8_gemv_kernel<TX, 4, GLU>>(a, grid, smem, s);
+    return gemv_go<int8_gemv_kernel<TX, 8, GLU>>(a, grid, smem, s);
+}
+
+template <class TX>
+static cudaError_t gemv_either(const Int8Args& a, bool glu, cudaStream_t s) {
+    return glu ? gemv_typed<TX, true>(a, s) : gemv_typed<TX, false>(a, s);
+}
+
+cudaError_t int8_gemv_launch(const Int8Args& a, bool glu, cudaStream_t s) {
+    switch (a.in.type) {
+        case SKB_F32: return gemv_either<float>(a, glu, s);
+        case SKB_BF16: return gemv_either<__nv_bfloat16>(a, glu, s);
+        case SKB_F16: return gemv_either<__half>(a, glu, s);
+        default: return gemv_either<int8_t>(a, glu, s);
+    }
+}
+
+}  // namespace skb

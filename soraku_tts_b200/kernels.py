@@ -16,6 +16,7 @@ CUDA tensors (float32, codes int64), as the reference's packed ABI requires
 from __future__ import annotations
 
 import functools
+from typing import NamedTuple
 
 import torch
 
@@ -391,3 +392,197 @@ def evict_cache(mass: torch.Tensor, *, cached: torch.Tensor, kv_pool: torch.Tens
             page_table.data_ptr(), max_pages, page_size, n_pages, budget, sinks, recent, kept.data_ptr(),
             mass_out.data_ptr(), cached_out.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
     return kept, mass_out, cached_out
+
+
+# ------------------------------------- a decoding step in 8-bit integers
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_I8 = torch.int8
+
+
+class Int8Rows(NamedTuple):
+    """Rows held as 8-bit codes: ``q`` int8 [rows, K], its rows beginning on 16
+    bytes, and ``scale`` FP32 [rows]; the values are about ``q * scale[:, None]``."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+def _rows(t, name: str, device: int) -> None:
+    """A [rows, K] CUDA tensor whose rows are contiguous."""
+    _dims(t, name, 2, "of two dimensions")
+    if t.get_device() != device:
+        raise ValueError(f"{name}: must be on the device of the others (cuda:{device}), is on {t.device}")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise ValueError(f"{name}: its rows must be contiguous")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}: its rows overlap")
+
+
+def _stride(t) -> int:
+    """Row stride; one row's is of no account, so that any will do."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) & -16
+
+
+def _codes(rows, name: str, device: int, inner: int | None):
+    try:
+        q, scale = rows
+    except (TypeError, ValueError):
+        raise ValueError(f"{name}: expected 8-bit rows and their scales (Int8Rows)") from None
+    _rows(q, name, device)
+    if q.dtype is not _I8:
+        raise ValueError(f"{name}: expected {_I8}, got {q.dtype}")
+    n, k = q.shape
+    if inner is not None and k != inner:
+        raise ValueError(f"{name}: expected rows of {inner}, got {k}")
+    _all(device, ((f"{name} scale", scale, (n,), _F32),))
+    return q, scale
+
+
+def quantize_rows(x: torch.Tensor, *, norm_weight: torch.Tensor | None = None, eps: float = 1e-6) -> Int8Rows:
+    """Rows of ``x`` [rows, K] (float32, bfloat16 or float16) as 8-bit codes with
+    a scale each: weights once, one row a channel, or activations that several
+    products share.  With ``norm_weight`` [K] the rows are RMS-normed first; see
+    skb_quantize_rows in include/soraku_b200.h."""
+    rows, k = _dims(x, "x", 2, "[rows, K]")
+    device = x.get_device()
+    _rows(x, "x", device)
+    kind = _TYPES.get(x.dtype)
+    if kind is None:
+        raise ValueError(f"x: expected float32, bfloat16 or float16, got {x.dtype}")
+    if k < 1:
+        raise ValueError("x: rows must hold at least one value")
+    if norm_weight is not None:
+        _all(device, (("norm_weight", norm_weight, (k,), _F32),))
+    q = torch.empty((rows, (k + 15) & -16), dtype=_I8, device=x.device)
+    scale = torch.empty(rows, dtype=_F32, device=x.device)
+    if rows > 0:
+        _on(device, _lib.call, "skb_quantize_rows", x.data_ptr(), kind, _stride(x), rows, k,
+            None if norm_weight is None else norm_weight.data_ptr(), float(eps), q.data_ptr(), q.shape[1],
+            scale.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
+    return Int8Rows(q[:, :k], scale)
+
+
+def _int8_product(name, x, weights, norm_weight, eps, bias, residual, out_dtype, out):
+    if isinstance(x, torch.Tensor):
+        codes, scale = x, None
+        rows, k = _dims(x, "x", 2, "[tokens, K]")
+        device = x.get_device()
+        _rows(x, "x", device)
+        kind = _TYPES.get(x.dtype)
+        if kind is None:
+            raise ValueError(f"x: expected float32, bfloat16 or float16, got {x.dtype}")
+        dtype = x.dtype
+    else:
+        if not isinstance(x, tuple) or len(x) != 2:
+            raise ValueError("x: expected a tensor, or 8-bit rows and their scales (Int8Rows)")
+        rows, k = _dims(x[0], "x", 2, "[tokens, K]")
+        device = x[0].get_device()
+        codes, scale = _codes(x, "x", device, None)
+        kind, dtype = 3, _F32
+        if norm_weight is not None:
+            raise ValueError("norm_weight: rows that are codes already take no norm")
+    if norm_weight is not None:
+        _all(device, (("norm_weight", norm_weight, (k,), _F32),))
+    args, n = [], None
+    for w, what in weights:
+        q, ws = _codes(w, what, device, k)
+        if n is not None and q.shape[0] != n:
+            raise ValueError(f"{what}: expected {n} rows, got {q.shape[0]}")
+        n = q.shape[0]
+        args += (q.data_ptr(), _stride(q), ws.data_ptr())
+    if k < 1 or n < 1:
+        raise ValueError("x and the weights must hold at least one value a row, and one row of weights")
+    if out is not None:
+        _rows(out, "out", device)
+        if out_dtype is None:
+            out_dtype = out.dtype
+        if out.dtype is not out_dtype or tuple(out.shape) != (rows, n):
+            raise ValueError(f"out: expected {out_dtype} [{rows}, {n}], got {out.dtype} {list(out.shape)}")
+    elif out_dtype is None:
+        out_dtype = dtype
+    out_kind = _TYPES.get(out_dtype)
+    if out_kind is None:
+        raise ValueError(f"out_dtype: expected float32, bfloat16 or float16, got {out_dtype}")
+    if out is None:
+        out = torch.empty((rows, n), dtype=out_dtype, device=codes.device)
+    args.append(n)
+    if name == "skb_int8_linear":
+        if bias is not None:
+            _all(device, (("bias", bias, (n,), _F32),))
+        ldr = 0
+        if residual is not None:
+            _rows(residual, "residual", device)
+            if residual.dtype is not out_dtype or tuple(residual.shape) != (rows, n):
+                raise ValueError(f"residual: expected {out_dtype} [{rows}, {n}], got {residual.dtype} {list(residual.shape)}")
+            ldr = _stride(residual)
+        args += (None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), ldr)
+    if rows == 0:  # nothing to do, and empty tensors have no address
+        return out
+    need = _workspace("skb_int8_workspace", rows, k, kind)
+    work = torch.empty(need, dtype=torch.uint8, device=codes.device) if need > 0 else None
+    _on(device, _lib.call, name, codes.data_ptr(), kind, _stride(codes), None if scale is None else scale.data_ptr(),
+        None if norm_weight is None else norm_weight.data_ptr(), float(eps), rows, k, *args, out.data_ptr(), out_kind,
+        _stride(out), None if work is None else work.data_ptr(), need, torch._C._cuda_getCurrentRawStream(device))
+    return out
+
+
+def int8_linear(x, weight, *, norm_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ weight.T + bias + residual`` in 8-bit integers; see skb_int8_linear
+    in include/soraku_b200.h.
+
+    ``x`` [tokens, K] is float32, bfloat16 or float16 and becomes 8-bit codes
+    with a scale for each token on the way (RMS-normed before if ``norm_weight`` is
+    given), or codes already (Int8Rows).  ``weight``: Int8Rows [N, K] from
+    ``quantize_rows``.  ``bias`` FP32 [N], ``residual`` [tokens, N] of the output's
+    type.  Returns [tokens, N] in ``out_dtype`` (default: x's type, FP32 for
+    codes), ``out`` if given, which may be ``residual`` and no other input."""
+    return _int8_product("skb_int8_linear", x, ((weight, "weight"),), norm_weight, eps, bias, residual, out_dtype, out)
+
+
+def int8_swiglu(x, gate, up, *, norm_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``silu(x @ gate.T) * (x @ up.T)`` in 8-bit integers, with ``gate`` and
+    ``up`` Int8Rows [I, K]; the rest as in ``int8_linear``."""
+    return _int8_product("skb_int8_swiglu", x, ((gate, "gate"), (up, "up")), norm_weight, eps, None, None, out_dtype, out)
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """A token for each row of ``logits`` [rows, V] (float32, bfloat16 or float16,
+    V up to 2^18) by its number in ``uniform`` (FP32 [rows], from [0, 1)), after
+    temperature, top-k, top-p and min-p; see skb_sample_tokens in
+    include/soraku_b200.h.  Each setting is a number, or a tensor [rows] (FP32;
+    ``top_k`` int32) with every row's own.  ``cfg_sample`` draws in the same order.
+    Returns (tokens int64 [rows], -1 for a row with nothing to draw from; the
+    logarithm of each token's probability among the kept ones, FP32 [rows])."""
+    rows, vocab = _dims(logits, "logits", 2, "[rows, V]")
+    device = logits.get_device()
+    _rows(logits, "logits", device)
+    kind = _TYPES.get(logits.dtype)
+    if kind is None:
+        raise ValueError(f"logits: expected float32, bfloat16 or float16, got {logits.dtype}")
+    if vocab < 1:
+        raise ValueError("logits: rows must hold at least one")
+    tensors, settings = [("uniform", uniform, (rows,), _F32)], []
+    for name, x in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+        if isinstance(x, torch.Tensor):
+            tensors.append((name, x, (rows,), _I32 if name == "top_k" else _F32))
+            settings += (x.data_ptr(), 0)
+        elif name == "top_k":
+            if type(x) is not int or abs(x) > 2**31 - 1:
+                raise ValueError(f"top_k: must be an int or an int32 tensor, got {x!r}")
+            settings += (None, x)
+        else:
+            x = float(x)
+            if x != x:
+                raise ValueError(f"{name}: must be a number")
+            settings += (None, x)
+    _all(device, tensors)
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprob = torch.empty(rows, dtype=_F32, device=logits.device)
+    if rows > 0:
+        _on(device, _lib.call, "skb_sample_tokens", logits.data_ptr(), kind, _stride(logits), rows, vocab,
+            uniform.data_ptr(), *settings, tokens.data_ptr(), logprob.data_ptr(),
+            torch._C._cuda_getCurrentRawStream(device))
+    return tokens, logprob
