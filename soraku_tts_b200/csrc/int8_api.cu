@@ -5,8 +5,8 @@
 namespace skb {
 
 static int check_rows(const char* what, const RowsIn& in, bool codes_too) {
-    if (in.T < 0 || in.K < 1 || in.K > I8_MAX_K)
-        return fail(SKB_ERR_ARG, "%s: bad sizes (%d rows of %d; 1 to %d values a row)", what, in.T, in.K, I8_MAX_K);
+    if (in.T < 0 || in.T > 1 << 30 || in.K < 1 || in.K > I8_MAX_K)
+        return fail(SKB_ERR_ARG, "%s: bad sizes (%d rows of %d; at most 2^30, of 1 to %d values)", what, in.T, in.K, I8_MAX_K);
     if (in.type < SKB_F32 || in.type > (codes_too ? SKB_I8 : SKB_F16))
         return fail(SKB_ERR_ARG, "%s: unknown type %d of the rows", what, in.type);
     if (!in.x) return fail(SKB_ERR_ARG, "%s: null pointer", what);
@@ -28,7 +28,7 @@ static int check_rows(const char* what, const RowsIn& in, bool codes_too) {
 static int check_product(const char* what, const Int8Args& a, int parts) {
     const int st = check_rows(what, a.in, true);
     if (st) return st;
-    if (a.N < 1) return fail(SKB_ERR_ARG, "%s: bad output width %d", what, a.N);
+    if (a.N < 1 || a.N > 1 << 30) return fail(SKB_ERR_ARG, "%s: bad output width %d", what, a.N);
     for (int i = 0; i < parts; ++i) {
         if (!a.w[i] || !a.ws[i]) return fail(SKB_ERR_ARG, "%s: null pointer", what);
         if (!aligned16(a.w[i]) || a.ldw[i] % 16 != 0 || a.ldw[i] < ceil16(a.in.K))
@@ -62,7 +62,7 @@ static int product(const char* what, Int8Args& a, bool glu, void* work, int64_t 
         if (e != cudaSuccess) return fail(SKB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
         a.in = {q, SKB_I8, kp, scale, nullptr, 0.f, a.in.T, a.in.K};
     }
-    const cudaError_t e = int8_gemv_launch(a, glu, s);
+    const cudaError_t e = a.in.T <= I8_FEW ? int8_gemv_launch(a, glu, s) : int8_gemm_launch(a, glu, s);
     return e == cudaSuccess ? SKB_OK : fail(SKB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 

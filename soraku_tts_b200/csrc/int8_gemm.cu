@@ -1,0 +1,372 @@
+// Products of 8-bit codes on the 5th-generation tensor cores
+// (tcgen05.mma kind::i8, sums in 32-bit integers in tensor memory):
+//   D[n][t] = sum_k W[n][k] X[t][k]
+// Weights are the M operand, so that a product of few tokens costs few columns,
+// and a thread of the epilogue holds one output channel: its scale and bias
+// stay in registers, and a warp writes 32 neighbouring channels of a token.
+//
+// A CTA takes tiles of 128 channels x TN tokens (for SwiGLU the 128 gate rows
+// and the 128 up rows of the same channels, two accumulators).  Warps:
+//   0 (one thread)   TMA: K in blocks of 128 bytes, the width of the 128-byte
+//                    swizzle, into a ring of stages; rows and bytes past the
+//                    end arrive as zeros, which add nothing;
+//   1 (one thread)   four MMAs of 32 bytes a block and part;
+//   4-11             the epilogue of one tile while the next one is added up
+//                    (two accumulators take turns).
+// Where tiles are fewer than SMs, a cluster of CTAs splits a tile's K: whole
+// numbers, so that the order of their sum does not matter.  Every CTA leaves
+// its sums in its shared memory and finishes its share of the tile's tokens.
+#include <cudaTypedefs.h>
+
+#include "int8_ops.cuh"
+#include "umma.cuh"
+
+namespace skb {
+
+constexpr int GM_THREADS = 384, GM_EPI = 256;
+constexpr int GM_MAX_SPLIT = 8;
+constexpr int GM_RING = 196 * 1024;
+
+struct GemmMaps {
+    CUtensorMap x, w[2];
+};
+
+template <int TN, bool GLU>
+struct GemmShape {
+    static constexpr int PARTS = GLU ? 2 : 1;
+    static constexpr int A_BYTES = 128 * 128, B_BYTES = TN * 128;
+    static constexpr int STAGE = PARTS * A_BYTES + B_BYTES;
+    static constexpr int STAGES = GM_RING / STAGE < 8 ? GM_RING / STAGE : 8;
+    static constexpr int COLS = PARTS * TN;       // of one accumulator
+    static constexpr int TMEM = 2 * COLS < 32 ? 32 : 2 * COLS;
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE;
+    static constexpr bool SPLITS = COLS * 512 <= STAGES * STAGE;  // sums fit the ring
+};
+
+struct GemmShared {
+    uint64_t full[8], empty[8], acc_full[2], acc_free[2];
+    uint32_t tmem;
+    int abort;
+};
+
+__device__ __forceinline__ void gm_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+// D S32, A and B S8, both K-major, M = 128.
+__host__ __device__ constexpr uint32_t gm_idesc(int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void gm_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t gm_peer(uint32_t addr, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ int gm_peer_load(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void gm_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// One channel's finish.
+template <bool GLU>
+struct Channel {
+    float s0, s1, bias;
+    bool has_bias;
+    __device__ __forceinline__ void load(const Int8Args& a, int n) {
+        const bool in = n < a.N;
+        s0 = in ? __ldcg(a.ws[0] + n) : 0.f;
+        s1 = GLU && in ? __ldcg(a.ws[1] + n) : 0.f;
+        has_bias = !GLU && a.bias != nullptr;
+        bias = has_bias && in ? __ldcg(a.bias + n) : 0.f;
+    }
+    __device__ __forceinline__ float operator()(int v, int u, float sx) const {
+        float y = (float)v * sx * s0;
+        if (GLU) y = silu(y) * ((float)u * sx * s1);
+        else if (has_bias) y += bias;
+        return y;
+    }
+};
+
+template <int TN, bool GLU>
+__global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args a, const __grid_constant__ GemmMaps maps, int split) {
+    using S = GemmShape<TN, GLU>;
+    extern __shared__ unsigned char gm_raw[];
+    __shared__ GemmShared sm;
+    unsigned char* base = gm_raw + ((1024u - (smem_u32(gm_raw) & 1023u)) & 1023u);
+    const uint32_t ring = smem_u32(base);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; ++i) mbar_init(&sm.full[i], 1), mbar_init(&sm.empty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&sm.acc_full[i], 1), mbar_init(&sm.acc_free[i], GM_EPI / 32);
+        sm.abort = 0;
+        mbar_fence_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.x)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.w[0])) : "memory");
+        if (GLU) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.w[1])) : "memory");
+    }
+    if (warp == 2) ut_alloc<S::TMEM>(&sm.tmem);
+    ut_fence_before();
+    __syncthreads();
+    ut_fence_after();
+    const uint32_t tmem = sm.tmem;
+    volatile int* abort = &sm.abort;
+
+    const int tiles_n = (a.N + 127) / 128, tiles_t = (a.in.T + TN - 1) / TN;
+    const long long tiles = (long long)tiles_n * tiles_t;
+    const int blocks = (a.in.K + 127) / 128;
+    const int z = blockIdx.x % split;  // rank in the cluster
+    const int k0 = (int)((long long)z * blocks / split), k1 = (int)((long long)(z + 1) * blocks / split);
+    const long long first = blockIdx.x / split, step = gridDim.x / split;
+    pdl_wait();
+    pdl_trigger();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            long long it = 0;
+            bool go = true;
+            for (long long tile = first; tile < tiles && go; tile += step) {
+                const int n0 = (int)(tile % tiles_n) * 128, t0 = (int)(tile / tiles_n) * TN;
+                for (int kb = k0; kb < k1; ++kb, ++it) {
+                    const int s = (int)(it % S::STAGES);
+                    if (it >= S::STAGES && !ut_wait(&sm.empty[s], (uint32_t)(it / S::STAGES - 1) & 1u, abort)) {
+                        go = false;
+                        break;
+                    }
+                    const uint32_t at = ring + s * S::STAGE;
+                    mbar_expect_tx(&sm.full[s], S::STAGE);
+                    gm_load(at, &maps.w[0], kb * 128, n0, &sm.full[s]);
+                    if (GLU) gm_load(at + S::A_BYTES, &maps.w[1], kb * 128, n0, &sm.full[s]);
+                    gm_load(at + S::PARTS * S::A_BYTES, &maps.x, kb * 128, t0, &sm.full[s]);
+                }
+            }
+            // no copy may land after the CTA has gone: the MMAs wait for each of
+            // them; where those gave up, wait here
+            if (*abort)
+                for (long long i = it > S::STAGES ? it - S::STAGES : 0; i < it; ++i)
+                    mbar_wait(&sm.full[i % S::STAGES], (uint32_t)(i / S::STAGES) & 1u, nullptr);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            long long it = 0;
+            int i = 0;
+            bool go = true;
+            for (long long tile = first; tile < tiles && go; tile += step, ++i) {
+                const int b = i & 1;
+                if (i >= 2 && !ut_wait(&sm.acc_free[b], (uint32_t)((i >> 1) - 1) & 1u, abort)) break;
+                ut_fence_after();
+                const uint32_t d = tmem + b * S::COLS;
+                for (int kb = k0; kb < k1; ++kb, ++it) {
+                    const int s = (int)(it % S::STAGES);
+                    if (!ut_wait(&sm.full[s], (uint32_t)(it / S::STAGES) & 1u, abort)) {
+                        go = false;
+                        break;
+                    }
+                    ut_fence_after();
+                    const uint32_t at = ring + s * S::STAGE;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint64_t x = ut_desc(at + S::PARTS * S::A_BYTES, k * 32, false);
+#pragma unroll
+                        for (int p = 0; p < S::PARTS; ++p)
+                            gm_mma(d + p * TN, ut_desc(at + p * S::A_BYTES, k * 32, false), x, gm_idesc(TN), kb > k0 || k > 0);
+                    }
+                    ut_commit(&sm.empty[s]);
+                }
+                if (go) ut_commit(&sm.acc_full[b]);
+            }
+            // what was issued ends before tensor memory is given back
+            if (*abort) {
+                ut_commit(&sm.acc_full[0]);
+                for (int n = 0; n < 2; ++n) mbar_wait_limit(&sm.acc_full[0], n, nullptr, 1000000ull);
+            }
+        }
+    } else if (warp >= 4) {
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
+        constexpr int CH = TN / 2 < 32 ? TN / 2 : 32;  // columns at a time
+        int i = 0;
+        for (long long tile = first; tile < tiles; tile += step, ++i) {
+            const int n0 = (int)(tile % tiles_n) * 128, t0 = (int)(tile / tiles_n) * TN;
+            const int n = n0 + 32 * q + lane, b = i & 1;
+            Channel<GLU> ch;
+            if (split == 1) ch.load(a, n);
+            const bool ok = ut_wait(&sm.acc_full[b], (uint32_t)(i >> 1) & 1u, abort);
+            __syncwarp();
+            ut_fence_after();
+            for (int c = half * (TN / 2); c < (half + 1) * (TN / 2); c += CH) {
+                if (t0 + c >= a.in.T) break;
+                uint32_t v[CH], u[GLU ? CH : 1];
+                if constexpr (CH == 32) {
+                    ut_ld32(lanes + b * S::COLS + c, v);
+                    if constexpr (GLU) ut_ld32(lanes + b * S::COLS + TN + c, u);
+                } else {
+                    ut_ld16(lanes + b * S::COLS + c, v);
+                    if constexpr (GLU) ut_ld16(lanes + b * S::COLS + TN + c, u);
+                }
+                if (split > 1) {
+                    ut_wait_ld();
+                    int* sums = reinterpret_cast<int*>(base);
+#pragma unroll
+                    for (int j = 0; j < CH; ++j) {
+                        sums[(c + j) * 128 + 32 * q + lane] = (int)v[j];
+                        if constexpr (GLU) sums[(TN + c + j) * 128 + 32 * q + lane] = (int)u[j];
+                    }
+                    continue;
+                }
+                const int left = a.in.T - t0 - c;  // tokens there are
+                const float mine = lane < left && lane < CH ? __ldcg(a.in.scale + t0 + c + lane) : 0.f;
+                float r[CH];
+                const bool has_r = !GLU && a.residual != nullptr;
+                if (has_r) {
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        r[j] = j < left && n < a.N ? load_as_float(a.residual, a.out_type, (long long)(t0 + c + j) * a.ldr + n) : 0.f;
+                }
+                ut_wait_ld();
+#pragma unroll
+                for (int j = 0; j < CH; ++j) {
+                    const float sx = __shfl_sync(FULL, mine, j);
+                    float y = ch((int)v[j], GLU ? (int)u[GLU ? j : 0] : 0, sx);
+                    if (has_r) y += r[j];
+                    if (!ok) y = __int_as_float(0x7fffffff);  // a wait that ran out shows as NaN
+                    if (j < left && n < a.N) store_as(a.out, a.out_type, (long long)(t0 + c + j) * a.ldo + n, y);
+                }
+            }
+            ut_fence_before();
+            __syncwarp();
+            if (lane == 0) ut_arrive(&sm.acc_free[b]);
+        }
+    }
+    if (split > 1) {
+        __syncwarp();
+        gm_cluster_sync();
+        const int n0 = (int)(first % tiles_n) * 128, t0 = (int)(first / tiles_n) * TN;
+        if (warp >= 4) {
+            bool bad = false;
+            for (int p = 0; p < split; ++p) bad |= gm_peer_load(gm_peer(smem_u32(&sm.abort), p)) != 0;
+            const int nt = min(TN, a.in.T - t0), c = tid & 127, n = n0 + c;
+            Channel<GLU> ch;
+            ch.load(a, n);
+            for (int t = z * nt / split + ((tid - 128) >> 7); t < (z + 1) * nt / split; t += 2) {
+                int v[GM_MAX_SPLIT], u[GLU ? GM_MAX_SPLIT : 1];
+#pragma unroll
+                for (int p = 0; p < GM_MAX_SPLIT; ++p) {
+                    v[p] = p < split ? gm_peer_load(gm_peer(ring + (t * 128 + c) * 4, p)) : 0;
+                    if constexpr (GLU) u[p] = p < split ? gm_peer_load(gm_peer(ring + ((TN + t) * 128 + c) * 4, p)) : 0;
+                }
+                int vs = 0, us = 0;
+#pragma unroll
+                for (int p = 0; p < GM_MAX_SPLIT; ++p) {
+                    vs += v[p];
+                    if constexpr (GLU) us += u[p];
+                }
+                if (n >= a.N) continue;
+                float y = ch(vs, us, __ldcg(a.in.scale + t0 + t));
+                if (!GLU && a.residual) y += load_as_float(a.residual, a.out_type, (long long)(t0 + t) * a.ldr + n);
+                if (bad) y = __int_as_float(0x7fffffff);
+                store_as(a.out, a.out_type, (long long)(t0 + t) * a.ldo + n, y);
+            }
+        }
+        __syncwarp();
+        gm_cluster_sync();  // peers have read this CTA's sums
+    }
+    ut_fence_before();
+    __syncthreads();
+    if (warp == 2) ut_free<S::TMEM>(tmem);
+}
+
+static PFN_cuTensorMapEncodeTiled_v12000 gm_encoder() {
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> known{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 f = known.load(std::memory_order_acquire);
+    if (f) return f;
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    known.store(f, std::memory_order_release);
+    return f;
+}
+
+// Rows of K bytes, boxes of 128 bytes x `box` rows, 128-byte swizzle, zeros outside.
+static bool gm_map(CUtensorMap* m, const void* p, int K, int rows, long long ld, int box) {
+    const PFN_cuTensorMapEncodeTiled_v12000 encode = gm_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t size[2] = {128, (cuuint32_t)box}, es[2] = {1, 1};
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, size, es,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int TN, bool GLU>
+static cudaError_t gemm_launch(const Int8Args& a, cudaStream_t s) {
+    using S = GemmShape<TN, GLU>;
+    const cudaError_t e = prepare_kernel<int8_gemm_kernel<TN, GLU>>(S::SMEM);
+    if (e != cudaSuccess) return e;
+    GemmMaps maps;
+    if (!gm_map(&maps.x, a.in.x, a.in.K, a.in.T, a.in.ld, TN) || !gm_map(&maps.w[0], a.w[0], a.in.K, a.N, a.ldw[0], 128))
+        return cudaErrorNotSupported;
+    if (GLU) {
+        if (!gm_map(&maps.w[1], a.w[1], a.in.K, a.N, a.ldw[1], 128)) return cudaErrorNotSupported;
+    } else {
+        maps.w[1] = maps.w[0];
+    }
+    constexpr int SMS = 148;
+    const long long tiles = (long long)((a.N + 127) / 128) * ((a.in.T + TN - 1) / TN);
+    const int blocks = (a.in.K + 127) / 128;
+    int split = 1;
+    if (S::SPLITS && tiles * 2 <= SMS) {
+        split = (int)(SMS / tiles);
+        if (split > blocks) split = blocks;
+        if (split > GM_MAX_SPLIT) split = GM_MAX_SPLIT;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < SMS ? tiles : SMS));
+    cfg.blockDim = dim3(GM_THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = split;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, int8_gemm_kernel<TN, GLU>, a, maps, split);
+}
+
+// Rows as codes.  Tiles as narrow as the tokens are few.
+cudaError_t int8_gemm_launch(const Int8Args& a, bool glu, cudaStream_t s) {
+    const int T = a.in.T;
+    if (glu) {
+        if (T <= 32) return gemm_launch<32, true>(a, s);
+        if (T <= 64) return gemm_launch<64, true>(a, s);
+        return gemm_launch<128, true>(a, s);
+    }
+    if (T <= 32) return gemm_launch<32, false>(a, s);
+    if (T <= 64) return gemm_launch<64, false>(a, s);
+    const long long wide = (long long)((a.N + 127) / 128) * ((T + 255) / 256);
+    if (T <= 128 || wide < 148) return gemm_launch<128, false>(a, s);
+    return gemm_launch<256, false>(a, s);
+}
+
+}  // namespace skb

@@ -9,7 +9,6 @@ namespace skb {
 constexpr int GV_THREADS = 256, GV_WARPS = 8;
 constexpr int GV_ROWS = 4;      // weight rows a warp takes at a time (2 gate and 2 up rows)
 constexpr int GV_CHUNK = 512;   // bytes of a row that a warp reads at once
-constexpr int GV_MAX_T = 8;
 constexpr int GV_MAX_X = 128 * 1024;  // bytes of codes in shared memory: one token of any length
 constexpr int GV_FUSED = 32 * 1024;   // up to here each CTA makes the codes itself
 
@@ -124,7 +123,7 @@ __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args
     }
 }
 
-bool int8_gemv_fuses(int T, int K) { return T <= GV_MAX_T && T * ceil16(K) <= GV_FUSED; }
+bool int8_gemv_fuses(int T, int K) { return T <= I8_FEW && T * ceil16(K) <= GV_FUSED; }
 
 template <auto Kernel>
 static cudaError_t gemv_go(const Int8Args& a, dim3 grid, size_t smem, cudaStream_t s) {

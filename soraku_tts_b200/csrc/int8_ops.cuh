@@ -67,8 +67,10 @@ cudaError_t prepare_kernel(size_t dyn_bytes) {
 }
 
 cudaError_t quantize_launch(const RowsIn& in, int8_t* q, long long ldq, float* scale, cudaStream_t s);
+constexpr int I8_FEW = 8;  // tokens that int8_gemv.cu serves
 bool int8_gemv_fuses(int T, int K);
 cudaError_t int8_gemv_launch(const Int8Args& a, bool glu, cudaStream_t s);
+cudaError_t int8_gemm_launch(const Int8Args& a, bool glu, cudaStream_t s);
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
