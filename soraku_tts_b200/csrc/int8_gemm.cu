@@ -18,6 +18,8 @@
 // its sums in its shared memory and finishes its share of the tile's tokens.
 #include <cudaTypedefs.h>
 
+#include <cstddef>
+
 #include "int8_ops.cuh"
 #include "umma.cuh"
 
@@ -47,7 +49,9 @@ struct GemmShared {
     uint64_t full[8], empty[8], acc_full[2], acc_free[2];
     uint32_t tmem;
     int abort;
+    alignas(16) float sx[GM_EPI / 32][128];  // scales of a warp's tokens, read four at a time
 };
+static_assert(offsetof(GemmShared, sx) % 16 == 0 && alignof(GemmShared) % 16 == 0, "16-byte reads");
 
 __device__ __forceinline__ void gm_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
     asm volatile(
@@ -79,27 +83,7 @@ __device__ __forceinline__ void gm_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// One channel's finish.
-template <bool GLU>
-struct Channel {
-    float s0, s1, bias;
-    bool has_bias;
-    __device__ __forceinline__ void load(const Int8Args& a, int n) {
-        const bool in = n < a.N;
-        s0 = in ? __ldcg(a.ws[0] + n) : 0.f;
-        s1 = GLU && in ? __ldcg(a.ws[1] + n) : 0.f;
-        has_bias = !GLU && a.bias != nullptr;
-        bias = has_bias && in ? __ldcg(a.bias + n) : 0.f;
-    }
-    __device__ __forceinline__ float operator()(int v, int u, float sx) const {
-        float y = (float)v * sx * s0;
-        if (GLU) y = silu(y) * ((float)u * sx * s1);
-        else if (has_bias) y += bias;
-        return y;
-    }
-};
-
-template <int TN, bool GLU>
+template <int TN, bool GLU, class TO>
 __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args a, const __grid_constant__ GemmMaps maps, int split) {
     using S = GemmShape<TN, GLU>;
     extern __shared__ unsigned char gm_raw[];
@@ -196,53 +180,68 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
         const int q = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
         constexpr int CH = TN / 2 < 32 ? TN / 2 : 32;  // columns at a time
+        float* sx = sm.sx[warp - 4];
         int i = 0;
         for (long long tile = first; tile < tiles; tile += step, ++i) {
-            const int n0 = (int)(tile % tiles_n) * 128, t0 = (int)(tile / tiles_n) * TN;
-            const int n = n0 + 32 * q + lane, b = i & 1;
-            Channel<GLU> ch;
-            if (split == 1) ch.load(a, n);
-            const bool ok = ut_wait(&sm.acc_full[b], (uint32_t)(i >> 1) & 1u, abort);
+            const int n = (int)(tile % tiles_n) * 128 + 32 * q + lane, t0 = (int)(tile / tiles_n) * TN + half * (TN / 2);
+            const int b = i & 1;
+            const bool in = n < a.N;
+            const float s0 = in ? __ldcg(a.ws[0] + n) : 0.f, s1 = GLU && in ? __ldcg(a.ws[1] + n) : 0.f;
+            const float bias = !GLU && a.bias != nullptr && in ? __ldcg(a.bias + n) : 0.f;
+            const TO* res = GLU ? nullptr : static_cast<const TO*>(a.residual);
+            __syncwarp();
+            for (int j = lane; j < TN / 2; j += 32) sx[j] = t0 + j < a.in.T ? __ldcg(a.in.scale + t0 + j) : 0.f;
+            // a wait that ran out shows as NaN
+            const float poison = ut_wait(&sm.acc_full[b], (uint32_t)(i >> 1) & 1u, abort) ? 1.f : __int_as_float(0x7fffffff);
             __syncwarp();
             ut_fence_after();
-            for (int c = half * (TN / 2); c < (half + 1) * (TN / 2); c += CH) {
-                if (t0 + c >= a.in.T) break;
+#pragma unroll 1
+            for (int c = 0; c < TN / 2 && t0 + c < a.in.T; c += CH) {
                 uint32_t v[CH], u[GLU ? CH : 1];
+                const uint32_t col = lanes + b * S::COLS + half * (TN / 2) + c;
                 if constexpr (CH == 32) {
-                    ut_ld32(lanes + b * S::COLS + c, v);
-                    if constexpr (GLU) ut_ld32(lanes + b * S::COLS + TN + c, u);
+                    ut_ld32(col, v);
+                    if constexpr (GLU) ut_ld32(col + TN, u);
                 } else {
-                    ut_ld16(lanes + b * S::COLS + c, v);
-                    if constexpr (GLU) ut_ld16(lanes + b * S::COLS + TN + c, u);
+                    ut_ld16(col, v);
+                    if constexpr (GLU) ut_ld16(col + TN, u);
                 }
                 if (split > 1) {
                     ut_wait_ld();
-                    int* sums = reinterpret_cast<int*>(base);
+                    int* sums = reinterpret_cast<int*>(base) + (half * (TN / 2) + c) * 128 + 32 * q + lane;
 #pragma unroll
                     for (int j = 0; j < CH; ++j) {
-                        sums[(c + j) * 128 + 32 * q + lane] = (int)v[j];
-                        if constexpr (GLU) sums[(TN + c + j) * 128 + 32 * q + lane] = (int)u[j];
+                        sums[j * 128] = (int)v[j];
+                        if constexpr (GLU) sums[(TN + j) * 128] = (int)u[j];
                     }
                     continue;
                 }
-                const int left = a.in.T - t0 - c;  // tokens there are
-                const float mine = lane < left && lane < CH ? __ldcg(a.in.scale + t0 + c + lane) : 0.f;
-                float r[CH];
-                const bool has_r = !GLU && a.residual != nullptr;
-                if (has_r) {
+                const int left = in ? a.in.T - t0 - c : 0;  // tokens there are
+                float r[GLU ? 1 : CH];
+                if constexpr (!GLU) {
+                    const TO* p = res + (long long)(t0 + c) * a.ldr + n;
 #pragma unroll
-                    for (int j = 0; j < CH; ++j)
-                        r[j] = j < left && n < a.N ? load_as_float(a.residual, a.out_type, (long long)(t0 + c + j) * a.ldr + n) : 0.f;
+                    for (int j = 0; j < CH; ++j, p += a.ldr) r[j] = res != nullptr && j < left ? to_float(__ldcg(p)) : 0.f;
                 }
                 ut_wait_ld();
+                TO* p = static_cast<TO*>(a.out) + (long long)(t0 + c) * a.ldo + n;
+                auto put = [&](bool all) {
 #pragma unroll
-                for (int j = 0; j < CH; ++j) {
-                    const float sx = __shfl_sync(FULL, mine, j);
-                    float y = ch((int)v[j], GLU ? (int)u[GLU ? j : 0] : 0, sx);
-                    if (has_r) y += r[j];
-                    if (!ok) y = __int_as_float(0x7fffffff);  // a wait that ran out shows as NaN
-                    if (j < left && n < a.N) store_as(a.out, a.out_type, (long long)(t0 + c + j) * a.ldo + n, y);
-                }
+                    for (int j0 = 0; j0 < CH; j0 += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4*>(sx + c + j0);
+                        const float sj[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k, p += a.ldo) {
+                            const int j = j0 + k;
+                            float y;
+                            if constexpr (GLU) y = finish_glu((int)v[j], (int)u[j], sj[k], s0 * poison, s1);
+                            else y = finish((int)v[j], sj[k], s0 * poison, bias) + r[j];
+                            if (all || j < left) store_out(p, y);
+                        }
+                    }
+                };
+                if (left >= CH) put(true);
+                else put(false);
             }
             ut_fence_before();
             __syncwarp();
@@ -257,8 +256,10 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
             bool bad = false;
             for (int p = 0; p < split; ++p) bad |= gm_peer_load(gm_peer(smem_u32(&sm.abort), p)) != 0;
             const int nt = min(TN, a.in.T - t0), c = tid & 127, n = n0 + c;
-            Channel<GLU> ch;
-            ch.load(a, n);
+            const bool in = n < a.N;
+            const float s0 = in ? __ldcg(a.ws[0] + n) : 0.f, s1 = GLU && in ? __ldcg(a.ws[1] + n) : 0.f;
+            const float bias = !GLU && a.bias != nullptr && in ? __ldcg(a.bias + n) : 0.f;
+            const TO* res = GLU ? nullptr : static_cast<const TO*>(a.residual);
             for (int t = z * nt / split + ((tid - 128) >> 7); t < (z + 1) * nt / split; t += 2) {
                 int v[GM_MAX_SPLIT], u[GLU ? GM_MAX_SPLIT : 1];
 #pragma unroll
@@ -273,10 +274,12 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
                     if constexpr (GLU) us += u[p];
                 }
                 if (n >= a.N) continue;
-                float y = ch(vs, us, __ldcg(a.in.scale + t0 + t));
-                if (!GLU && a.residual) y += load_as_float(a.residual, a.out_type, (long long)(t0 + t) * a.ldr + n);
+                const float sx = __ldcg(a.in.scale + t0 + t);
+                float y;
+                if constexpr (GLU) y = finish_glu(vs, us, sx, s0, s1);
+                else y = finish(vs, sx, s0, bias) + (res ? to_float(__ldcg(res + (long long)(t0 + t) * a.ldr + n)) : 0.f);
                 if (bad) y = __int_as_float(0x7fffffff);
-                store_as(a.out, a.out_type, (long long)(t0 + t) * a.ldo + n, y);
+                store_out(static_cast<TO*>(a.out) + (long long)(t0 + t) * a.ldo + n, y);
             }
         }
         __syncwarp();
@@ -315,10 +318,10 @@ static bool gm_map(CUtensorMap* m, const void* p, int K, int rows, long long ld,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int TN, bool GLU>
+template <int TN, bool GLU, class TO>
 static cudaError_t gemm_launch(const Int8Args& a, cudaStream_t s) {
     using S = GemmShape<TN, GLU>;
-    const cudaError_t e = prepare_kernel<int8_gemm_kernel<TN, GLU>>(S::SMEM);
+    const cudaError_t e = prepare_kernel<int8_gemm_kernel<TN, GLU, TO>>(S::SMEM);
     if (e != cudaSuccess) return e;
     GemmMaps maps;
     if (!gm_map(&maps.x, a.in.x, a.in.K, a.in.T, a.in.ld, TN) || !gm_map(&maps.w[0], a.w[0], a.in.K, a.N, a.ldw[0], 128))
@@ -351,22 +354,27 @@ static cudaError_t gemm_launch(const Int8Args& a, cudaStream_t s) {
     at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, int8_gemm_kernel<TN, GLU>, a, maps, split);
+    return cudaLaunchKernelEx(&cfg, int8_gemm_kernel<TN, GLU, TO>, a, maps, split);
+}
+
+template <class TO>
+static cudaError_t gemm_typed(const Int8Args& a, bool glu, cudaStream_t s) {
+    const int T = a.in.T;
+    if (glu) {
+        if (T <= 32) return gemm_launch<32, true, TO>(a, s);
+        if (T <= 64) return gemm_launch<64, true, TO>(a, s);
+        return gemm_launch<128, true, TO>(a, s);
+    }
+    if (T <= 32) return gemm_launch<32, false, TO>(a, s);
+    if (T <= 64) return gemm_launch<64, false, TO>(a, s);
+    const long long wide = (long long)((a.N + 127) / 128) * ((T + 255) / 256);
+    if (T <= 128 || wide < 148) return gemm_launch<128, false, TO>(a, s);
+    return gemm_launch<256, false, TO>(a, s);
 }
 
 // Rows as codes.  Tiles as narrow as the tokens are few.
 cudaError_t int8_gemm_launch(const Int8Args& a, bool glu, cudaStream_t s) {
-    const int T = a.in.T;
-    if (glu) {
-        if (T <= 32) return gemm_launch<32, true>(a, s);
-        if (T <= 64) return gemm_launch<64, true>(a, s);
-        return gemm_launch<128, true>(a, s);
-    }
-    if (T <= 32) return gemm_launch<32, false>(a, s);
-    if (T <= 64) return gemm_launch<64, false>(a, s);
-    const long long wide = (long long)((a.N + 127) / 128) * ((T + 255) / 256);
-    if (T <= 128 || wide < 148) return gemm_launch<128, false>(a, s);
-    return gemm_launch<256, false>(a, s);
+    return with_type(a.out_type, [&](auto to) { return gemm_typed<decltype(to)>(a, glu, s); });
 }
 
 }  // namespace skb

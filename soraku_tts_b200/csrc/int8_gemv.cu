@@ -13,7 +13,7 @@ constexpr int GV_MAX_X = 128 * 1024;  // bytes of codes in shared memory: one to
 constexpr int GV_FUSED = 32 * 1024;   // up to here each CTA makes the codes itself
 
 // TT: tokens a CTA holds (the last ones may be missing).
-template <class TX, int TT, bool GLU>
+template <class TX, class TO, int TT, bool GLU>
 __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args a) {
     extern __shared__ __align__(16) int8_t gv_x[];  // [TT][kp]
     __shared__ float red[2 * GV_WARPS];
@@ -111,14 +111,14 @@ __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args
             }
         const int t = lane / PER, n = group * PER + lane % PER;
         if (t < nt && lane < TT * PER && n < a.N) {
-            float y = (float)v * sx[t] * __ldcg(a.ws[0] + n);
-            if (GLU) {
-                y = silu(y) * ((float)u * sx[t] * __ldcg(a.ws[1] + n));
+            float y;
+            if constexpr (GLU) {
+                y = finish_glu(v, u, sx[t], __ldcg(a.ws[0] + n), __ldcg(a.ws[1] + n));
             } else {
-                if (a.bias) y += __ldcg(a.bias + n);
-                if (a.residual) y += load_as_float(a.residual, a.out_type, (t0 + t) * a.ldr + n);
+                y = finish(v, sx[t], __ldcg(a.ws[0] + n), a.bias ? __ldcg(a.bias + n) : 0.f);
+                if (a.residual) y += to_float(__ldcg(static_cast<const TO*>(a.residual) + (t0 + t) * a.ldr + n));
             }
-            store_as(a.out, a.out_type, (t0 + t) * a.ldo + n, y);
+            store_out(static_cast<TO*>(a.out) + (t0 + t) * a.ldo + n, y);
         }
     }
 }
@@ -131,7 +131,7 @@ static cudaError_t gemv_go(const Int8Args& a, dim3 grid, size_t smem, cudaStream
     return e != cudaSuccess ? e : launch(Kernel, grid, dim3(GV_THREADS), smem, s, true, a);
 }
 
-template <class TX, bool GLU>
+template <class TX, class TO, bool GLU>
 static cudaError_t gemv_typed(const Int8Args& a, cudaStream_t s) {
     const int T = a.in.T;
     int tt = T == 1 ? 1 : T == 2 ? 2 : T <= 4 ? 4 : 8;
@@ -140,24 +140,19 @@ static cudaError_t gemv_typed(const Int8Args& a, cudaStream_t s) {
     const int blocks = ((a.N + per - 1) / per + GV_WARPS - 1) / GV_WARPS;
     const dim3 grid(blocks < 296 ? blocks : 296, (T + tt - 1) / tt);
     const size_t smem = (size_t)tt * ceil16(a.in.K);
-    if (tt == 1) return gemv_go<int8_gemv_kernel<TX, 1, GLU>>(a, grid, smem, s);
-    if (tt == 2) return gemv_go<int8_gemv_kernel<TX, 2, GLU>>(a, grid, smem, s);
-    if (tt == 4) return gemv_go<int8_gemv_kernel<TX, 4, GLU>>(a, grid, smem, s);
-    return gemv_go<int8_gemv_kernel<TX, 8, GLU>>(a, grid, smem, s);
-}
-
-template <class TX>
-static cudaError_t gemv_either(const Int8Args& a, bool glu, cudaStream_t s) {
-    return glu ? gemv_typed<TX, true>(a, s) : gemv_typed<TX, false>(a, s);
+    if (tt == 1) return gemv_go<int8_gemv_kernel<TX, TO, 1, GLU>>(a, grid, smem, s);
+    if (tt == 2) return gemv_go<int8_gemv_kernel<TX, TO, 2, GLU>>(a, grid, smem, s);
+    if (tt == 4) return gemv_go<int8_gemv_kernel<TX, TO, 4, GLU>>(a, grid, smem, s);
+    return gemv_go<int8_gemv_kernel<TX, TO, 8, GLU>>(a, grid, smem, s);
 }
 
 cudaError_t int8_gemv_launch(const Int8Args& a, bool glu, cudaStream_t s) {
-    switch (a.in.type) {
-        case SKB_F32: return gemv_either<float>(a, glu, s);
-        case SKB_BF16: return gemv_either<__nv_bfloat16>(a, glu, s);
-        case SKB_F16: return gemv_either<__half>(a, glu, s);
-        default: return gemv_either<int8_t>(a, glu, s);
-    }
+    return with_type(a.out_type, [&](auto to) {
+        auto go = [&](auto x) {
+            return glu ? gemv_typed<decltype(x), decltype(to), true>(a, s) : gemv_typed<decltype(x), decltype(to), false>(a, s);
+        };
+        return a.in.type == SKB_I8 ? go(int8_t()) : with_type(a.in.type, go);
+    });
 }
 
 }  // namespace skb

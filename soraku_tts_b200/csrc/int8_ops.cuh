@@ -76,42 +76,84 @@ __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
-// Largest of |a|, |b|; NaN if one of them is.
-__device__ __forceinline__ float max_abs(float a, float b) {
+// Largest of |a|, |b|, |c|; NaN if one of them is.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
     float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+// Of numbers that are not negative, a warp's largest, NaN above all: in the order
+// of their bits.
+__device__ __forceinline__ float warp_top(float a) {
+    return __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(a) & 0x7fffffffu));
 }
 // s = max / 127, and no smaller than the smallest normal number, where the
 // quotient by it stays finite.  NaN for a row that holds something not finite.
 __device__ __forceinline__ float step_of(float top) {
     return top <= 3.402823466e38f ? fmaxf(__fdiv_rn(top, 127.f), 1.17549435e-38f) : __int_as_float(0x7fffffff);
 }
-// round(y / s) with the FP32 quotient: y times 1 / s is within 3e-5 of it
-// (|q| <= 127, three roundings), so only near halves is it formed.
-__device__ __forceinline__ int code_of(float y, float s, float r) {
-    const float t = y * r;
-    float q = rintf(t);
-    if (fabsf(fabsf(t - q) - 0.5f) < 1e-4f) q = rintf(__fdiv_rn(y, s));
-    return (int)q;
-}
 
-// VEC consecutive values: 16 bytes of the type.
+// 16 bytes of a row's values.
 template <class TX>
 struct Vec {
     static constexpr int N = 16 / sizeof(TX);
-};
-template <class TX>
-__device__ __forceinline__ void load_vec(const TX* p, int left, bool aligned, float (&v)[Vec<TX>::N]) {
-    if (aligned && left >= Vec<TX>::N) {
-        const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p));
-        const TX* e = reinterpret_cast<const TX*>(&u);
+    union {
+        uint4 raw;
+        TX e[N];
+    };
+    __device__ __forceinline__ Vec() {}
+    // the `left` values at p, zeros behind them
+    __device__ __forceinline__ void load(const TX* p, int left, bool aligned) {
+        if (aligned && left >= N) {
+            raw = __ldcg(reinterpret_cast<const uint4*>(p));
+        } else {
+            raw = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < Vec<TX>::N; ++i) v[i] = to_float(e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < Vec<TX>::N; ++i) v[i] = i < left ? to_float(__ldcg(p + i)) : 0.f;
+            for (int i = 0; i < N; ++i)
+                if (i < left) e[i] = __ldcg(p + i);
+        }
     }
+    __device__ __forceinline__ void get(float (&v)[N]) const {
+        if constexpr (sizeof(TX) == 4) {
+            v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y);
+            v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = to_float(e[i]);
+        }
+    }
+};
+
+// Codes of N values, four bytes a word: round(y / s) with the FP32 quotient, halves
+// to even.  Adding 1.5 2^23 rounds y times 1 / s and leaves the code in the low
+// byte.  That product is within 3e-5 of the quotient (|q| <= 127, three
+// roundings), so only values next to a half need the division: one in five
+// thousand, looked for once in N.  s NaN: zeros.
+template <int N>
+__device__ __forceinline__ void encode(const float (&y)[N], float s, float r, uint32_t (&word)[N / 4]) {
+    constexpr float MAGIC = 12582912.f;
+    uint32_t q[N];
+    float off = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float t = __fmul_rn(y[i], r), m = __fadd_rn(t, MAGIC);
+        q[i] = __float_as_uint(m);
+        off = fmaxf(off, fabsf(__fsub_rn(t, __fsub_rn(m, MAGIC))));
+    }
+    if (off > 0.4999f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = __float_as_uint(__fadd_rn(__fdiv_rn(y[i], s), MAGIC));
+    }
+#pragma unroll
+    for (int h = 0; h < N / 4; ++h) {
+        word[h] = __byte_perm(__byte_perm(q[4 * h], q[4 * h + 1], 0x0040), __byte_perm(q[4 * h + 2], q[4 * h + 3], 0x0040), 0x5410);
+        if (!(s == s)) word[h] = 0;
+    }
+}
+template <int N>
+__device__ __forceinline__ void put_codes(int8_t* q, const uint32_t (&word)[N / 4]) {
+    if constexpr (N == 4) *reinterpret_cast<uint32_t*>(q) = word[0];
+    else *reinterpret_cast<uint2*>(q) = make_uint2(word[0], word[1]);
 }
 
 // One row by a group of G threads (G a multiple of 32; `t`: place in it):
@@ -128,11 +170,14 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
     float v[CH][V];
     float top = 0.f, ss = 0.f;
     auto load = [&](int base) {
+        Vec<TX> raw[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k = base + (c * G + t) * V;
-            load_vec<TX>(x + k, K - k, x_aligned, v[c]);
+            raw[c].load(x + k, K - k, x_aligned);
         }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) raw[c].get(v[c]);
     };
     auto weigh = [&](int base, bool first) {
 #pragma unroll
@@ -141,19 +186,21 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
             if (nw != nullptr) {
 #pragma unroll
                 for (int h = 0; h < V / 4; ++h) {
+                    Vec<float> raw;
+                    raw.load(nw + k + 4 * h, K - k - 4 * h, w_aligned);
                     float w[4];
-                    load_vec<float>(nw + k + 4 * h, K - k - 4 * h, w_aligned, w);
+                    raw.get(w);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float& y = v[c][4 * h + i];
                         if (first) ss = fmaf(y, y, ss);
-                        y = k + 4 * h + i < K ? __fmul_rn(y, w[i]) : 0.f;
+                        y = __fmul_rn(y, w[i]);
                     }
                 }
             }
             if (first) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) top = max_abs(top, v[c][i]);
+                for (int i = 0; i < V; i += 2) top = max_abs(top, v[c][i], v[c][i + 1]);
             }
         }
     };
@@ -163,40 +210,24 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
         weigh(base, true);
         if (base + PIECE >= K) break;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        top = max_abs(top, __shfl_xor_sync(FULL, top, o));
-        ss += __shfl_xor_sync(FULL, ss, o);
-    }
+    top = warp_top(top);
+    if (nw != nullptr) ss = warp_sum(ss);
     if (G > 32) {
         if ((t & 31) == 0) red[2 * (t >> 5)] = top, red[2 * (t >> 5) + 1] = ss;
         __syncthreads();
         top = 0.f, ss = 0.f;
 #pragma unroll
-        for (int w = 0; w < G / 32; ++w) top = max_abs(top, red[2 * w]), ss += red[2 * w + 1];
+        for (int w = 0; w < G / 32; ++w) top = max_abs(top, red[2 * w], 0.f), ss += red[2 * w + 1];
     }
-    const float s = step_of(top);
-    const bool bad = !(s == s);
-    const float r = __fdiv_rn(1.f, s);
+    const float s = step_of(top), r = __fdiv_rn(1.f, s);
     for (;;) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k = base + (c * G + t) * V;
             if (k >= ceil16(K)) continue;
             uint32_t word[V / 4];
-#pragma unroll
-            for (int h = 0; h < V / 4; ++h) {
-                word[h] = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int code = bad ? 0 : code_of(v[c][4 * h + i], s, r);
-                    word[h] |= (uint32_t)(code & 0xff) << (8 * i);
-                }
-            }
-            if (V == 4)
-                *reinterpret_cast<uint32_t*>(q + k) = word[0];
-            else
-                *reinterpret_cast<uint2*>(q + k) = make_uint2(word[0], word[V / 4 - 1]);
+            encode<V>(v[c], s, r, word);
+            put_codes<V>(q + k, word);
         }
         if (base == 0) break;
         base -= PIECE;
@@ -206,15 +237,30 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
     return nw != nullptr ? s * rsqrtf(ss / (float)K + eps) : s;
 }
 
-__device__ __forceinline__ float load_as_float(const void* p, int type, long long i) {
-    if (type == SKB_F32) return __ldcg(static_cast<const float*>(p) + i);
-    if (type == SKB_BF16) return __bfloat162float(__ldcg(static_cast<const __nv_bfloat16*>(p) + i));
-    return __half2float(__ldcg(static_cast<const __half*>(p) + i));
+// A sum's way to its result; the same operations in every kernel, so that a
+// token's result does not depend on how many stand beside it.  `bias`: 0 without.
+__device__ __forceinline__ float finish(int sum, float sx, float sw, float bias) {
+    return fmaf(__fmul_rn((float)sum, sx), sw, bias);
 }
-__device__ __forceinline__ void store_as(void* p, int type, long long i, float v) {
-    if (type == SKB_F32) static_cast<float*>(p)[i] = v;
-    else if (type == SKB_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+// silu by the hardware's exponential and reciprocal: each is within 2^-22 of
+// its value, where the product's own roundings are 2^-22 already, and the
+// argument's rounding counts |g| 2^-24, as that of g itself does.  (The exact
+// ones took 30 instructions more of each result.)
+__device__ __forceinline__ float finish_glu(int gate, int up, float sx, float sg, float su) {
+    const float g = finish(gate, sx, sg, 0.f);
+    return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, __expf(-g))), finish(up, sx, su, 0.f));
+}
+
+__device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
+
+// f(TO()) with the output's type.
+template <class F>
+inline cudaError_t with_type(int type, F f) {
+    if (type == SKB_F32) return f(float());
+    if (type == SKB_BF16) return f(__nv_bfloat16());
+    return f(__half());
 }
 
 }  // namespace skb

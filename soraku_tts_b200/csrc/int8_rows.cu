@@ -1,38 +1,138 @@
 // Rows of values to rows of 8-bit codes, each with its scale (int8_ops.cuh has
-// the definition).  Activations before a product, weights once.
+// the definition).  Activations before a product, weights once.  Bound by memory
+// where rows are many, by latency where they are few.
 #include "int8_ops.cuh"
 
 namespace skb {
 
-// Rows of up to 1024 values: a warp each, the values in its registers between
-// the largest's search and the codes.  Longer ones: a CTA each, up to 8192
-// values in registers, the rest read again from L2.
-template <class TX, int G>
+// G threads a row, which hold it in registers, CH vectors each, between the
+// search for the largest and the codes.  A CTA takes rows one after the other:
+// the norm's weights stay in registers, and the next row is on its way while this
+// one is finished.
+template <class TX, int G, int CH, bool NORM>
 __global__ void __launch_bounds__(256) quantize_kernel(const RowsIn in, int8_t* __restrict__ q, long long ldq,
                                                        float* __restrict__ scale) {
+    constexpr int V = Vec<TX>::N, ROWS = 256 / G, WARPS = G / 32;
+    __shared__ float red[2][ROWS][WARPS][2];
+    const int slot = threadIdx.x / G, t = threadIdx.x % G;
+    const int K = in.K, kp = ceil16(K);
+    pdl_wait();
+    pdl_trigger();
+    float w[NORM ? CH : 1][V];
+    if constexpr (NORM) {
+        const bool aligned = (reinterpret_cast<uintptr_t>(in.nw) & 15) == 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int h = 0; h < V / 4; ++h) {
+                const int k = (c * G + t) * V + 4 * h;
+                Vec<float> raw;
+                raw.load(in.nw + k, K - k, aligned);
+                float f[4];
+                raw.get(f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[c][4 * h + i] = f[i];
+            }
+    }
+    Vec<TX> next[CH];
+    auto load = [&](long long row) {
+        const TX* x = static_cast<const TX*>(in.x) + row * in.ld;
+        const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int k = (c * G + t) * V;
+            next[c].load(x + k, row < in.T ? K - k : 0, aligned);
+        }
+    };
+    const long long step = (long long)gridDim.x * ROWS;
+    long long row = (long long)blockIdx.x * ROWS + slot;
+    load(row);
+    for (int turn = 0; row - slot < in.T; row += step, turn ^= 1) {
+        float v[CH][V], top = 0.f, ss = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            next[c].get(v[c]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if constexpr (NORM) {
+                    ss = fmaf(v[c][i], v[c][i], ss);
+                    v[c][i] = __fmul_rn(v[c][i], w[c][i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; i += 2) top = max_abs(top, v[c][i], v[c][i + 1]);
+        }
+        if (row - slot + step < in.T) load(row + step);
+        top = warp_top(top);
+        if (NORM) ss = warp_sum(ss);
+        if constexpr (G > 32) {
+            // two places in turn, so that one barrier a row is enough
+            if ((t & 31) == 0) red[turn][slot][t >> 5][0] = top, red[turn][slot][t >> 5][1] = ss;
+            __syncthreads();
+            top = 0.f, ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < WARPS; ++i) top = max_abs(top, red[turn][slot][i][0], 0.f), ss += red[turn][slot][i][1];
+        }
+        if (row >= in.T) continue;
+        const float s = step_of(top), r = __fdiv_rn(1.f, s);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int k = (c * G + t) * V;
+            if (k < kp) {
+                uint32_t word[V / 4];
+                encode<V>(v[c], s, r, word);
+                put_codes<V>(q + row * ldq + k, word);
+            }
+        }
+        if (t == 0) scale[row] = NORM ? s * rsqrtf(ss / (float)K + in.eps) : s;
+    }
+}
+
+// Rows of more than 8192 values: a CTA each, all but the last piece read again.
+template <class TX>
+__global__ void __launch_bounds__(256) quantize_long_kernel(const RowsIn in, int8_t* __restrict__ q, long long ldq,
+                                                            float* __restrict__ scale) {
     __shared__ float red[16];
     pdl_wait();
     pdl_trigger();
-    const long long row = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
-    if (G < 256 && row >= in.T) return;  // whole warps
-    const int t = threadIdx.x % G;
+    const long long row = blockIdx.x;
     const TX* x = static_cast<const TX*>(in.x) + row * in.ld;
     const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    const float s = quantize_row<TX, G, 32 / Vec<TX>::N>(x, in.nw, in.eps, in.K, aligned, q + row * ldq, t, red);
-    if (t == 0) scale[row] = s;
+    const float s = quantize_row<TX, 256, 32 / Vec<TX>::N>(x, in.nw, in.eps, in.K, aligned, q + row * ldq, threadIdx.x, red);
+    if (threadIdx.x == 0) scale[row] = s;
+}
+
+template <class TX, int G, int CH>
+static cudaError_t rows_launch(const RowsIn& in, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
+    constexpr int ROWS = 256 / G;
+    const int need = (int)(((long long)in.T + ROWS - 1) / ROWS), most = 148 * 4;
+    const dim3 grid(need < most ? need : most);
+    return in.nw ? launch(quantize_kernel<TX, G, CH, true>, grid, dim3(256), 0, s, true, in, q, ldq, scale)
+                 : launch(quantize_kernel<TX, G, CH, false>, grid, dim3(256), 0, s, true, in, q, ldq, scale);
 }
 
 template <class TX>
 static cudaError_t quantize_typed(const RowsIn& in, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
-    if (in.K <= 1024)
-        return launch(quantize_kernel<TX, 32>, dim3((in.T + 7) / 8), dim3(256), 0, s, true, in, q, ldq, scale);
-    return launch(quantize_kernel<TX, 256>, dim3(in.T), dim3(256), 0, s, true, in, q, ldq, scale);
+    constexpr int V = Vec<TX>::N;
+    const int vectors = (in.K + V - 1) / V;
+    // rows that are few: as many threads as a row has vectors
+    if (in.T <= 296) {
+        if (vectors <= 32) return rows_launch<TX, 32, 1>(in, q, ldq, scale, s);
+        if (vectors <= 256) return rows_launch<TX, 256, 1>(in, q, ldq, scale, s);
+        if (vectors <= 512) return rows_launch<TX, 256, 2>(in, q, ldq, scale, s);
+    }
+    if (vectors <= 128) return rows_launch<TX, 32, 4>(in, q, ldq, scale, s);
+    if (vectors <= 256) return rows_launch<TX, 64, 4>(in, q, ldq, scale, s);
+    if (vectors <= 512) return rows_launch<TX, 128, 4>(in, q, ldq, scale, s);
+    if (vectors <= 1024) return rows_launch<TX, 256, 4>(in, q, ldq, scale, s);
+    if constexpr (V == 4) {
+        if (vectors <= 2048) return rows_launch<TX, 256, 8>(in, q, ldq, scale, s);
+    }
+    return launch(quantize_long_kernel<TX>, dim3(in.T), dim3(256), 0, s, true, in, q, ldq, scale);
 }
 
 cudaError_t quantize_launch(const RowsIn& in, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
-    if (in.type == SKB_F32) return quantize_typed<float>(in, q, ldq, scale, s);
-    if (in.type == SKB_BF16) return quantize_typed<__nv_bfloat16>(in, q, ldq, scale, s);
-    return quantize_typed<__half>(in, q, ldq, scale, s);
+    return with_type(in.type, [&](auto x) { return quantize_typed<decltype(x)>(in, q, ldq, scale, s); });
 }
 
 }  // namespace skb
