@@ -79,12 +79,18 @@ __device__ __forceinline__ int gm_peer_load(uint32_t addr) {
     asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ int4 gm_peer_load4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void gm_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <int TN, bool GLU, class TO>
-__global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args a, const __grid_constant__ GemmMaps maps, int split) {
+__global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args a, const __grid_constant__ GemmMaps maps, int split,
+                                                                  bool early) {
     using S = GemmShape<TN, GLU>;
     extern __shared__ unsigned char gm_raw[];
     __shared__ GemmShared sm;
@@ -113,6 +119,19 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
     const int z = blockIdx.x % split;  // rank in the cluster
     const int k0 = (int)((long long)z * blocks / split), k1 = (int)((long long)(z + 1) * blocks / split);
     const long long first = blockIdx.x / split, step = gridDim.x / split;
+    // blocks whose weights are asked for before the wait
+    int ahead = 0;
+    auto load_w = [&](long long tile, int kb, uint32_t at, uint64_t* bar) {
+        const int n0 = (int)(tile % tiles_n) * 128;
+        gm_load(at, &maps.w[0], kb * 128, n0, bar);
+        if (GLU) gm_load(at + S::A_BYTES, &maps.w[1], kb * 128, n0, bar);
+    };
+    if (early && tid == 0 && first < tiles) {
+        for (; ahead < S::STAGES && k0 + ahead < k1; ++ahead) {
+            mbar_expect_tx(&sm.full[ahead], S::STAGE);
+            load_w(first, k0 + ahead, ring + ahead * S::STAGE, &sm.full[ahead]);
+        }
+    }
     pdl_wait();
     pdl_trigger();
 
@@ -121,7 +140,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
             long long it = 0;
             bool go = true;
             for (long long tile = first; tile < tiles && go; tile += step) {
-                const int n0 = (int)(tile % tiles_n) * 128, t0 = (int)(tile / tiles_n) * TN;
+                const int t0 = (int)(tile / tiles_n) * TN;
                 for (int kb = k0; kb < k1; ++kb, ++it) {
                     const int s = (int)(it % S::STAGES);
                     if (it >= S::STAGES && !ut_wait(&sm.empty[s], (uint32_t)(it / S::STAGES - 1) & 1u, abort)) {
@@ -129,9 +148,10 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
                         break;
                     }
                     const uint32_t at = ring + s * S::STAGE;
-                    mbar_expect_tx(&sm.full[s], S::STAGE);
-                    gm_load(at, &maps.w[0], kb * 128, n0, &sm.full[s]);
-                    if (GLU) gm_load(at + S::A_BYTES, &maps.w[1], kb * 128, n0, &sm.full[s]);
+                    if (it >= ahead) {
+                        mbar_expect_tx(&sm.full[s], S::STAGE);
+                        load_w(tile, kb, at, &sm.full[s]);
+                    }
                     gm_load(at + S::PARTS * S::A_BYTES, &maps.x, kb * 128, t0, &sm.full[s]);
                 }
             }
@@ -218,14 +238,14 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
                 }
                 const int left = in ? a.in.T - t0 - c : 0;  // tokens there are
                 float r[GLU ? 1 : CH];
-                if constexpr (!GLU) {
+                if (!GLU && res != nullptr) {
                     const TO* p = res + (long long)(t0 + c) * a.ldr + n;
 #pragma unroll
-                    for (int j = 0; j < CH; ++j, p += a.ldr) r[j] = res != nullptr && j < left ? to_float(__ldcg(p)) : 0.f;
+                    for (int j = 0; j < CH; ++j, p += a.ldr) r[GLU ? 0 : j] = j < left ? to_float(__ldcg(p)) : 0.f;
                 }
                 ut_wait_ld();
                 TO* p = static_cast<TO*>(a.out) + (long long)(t0 + c) * a.ldo + n;
-                auto put = [&](bool all) {
+                auto put = [&](bool all, bool add) {
 #pragma unroll
                     for (int j0 = 0; j0 < CH; j0 += 4) {
                         const float4 s4 = *reinterpret_cast<const float4*>(sx + c + j0);
@@ -235,13 +255,15 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
                             const int j = j0 + k;
                             float y;
                             if constexpr (GLU) y = finish_glu((int)v[j], (int)u[j], sj[k], s0 * poison, s1);
-                            else y = finish((int)v[j], sj[k], s0 * poison, bias) + r[j];
+                            else y = finish((int)v[j], sj[k], s0 * poison, bias);
+                            if (add) y += r[GLU ? 0 : j];
                             if (all || j < left) store_out(p, y);
                         }
                     }
                 };
-                if (left >= CH) put(true);
-                else put(false);
+                if (!GLU && res != nullptr) put(false, true);
+                else if (left >= CH) put(true, false);
+                else put(false, false);
             }
             ut_fence_before();
             __syncwarp();
@@ -255,31 +277,51 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
         if (warp >= 4) {
             bool bad = false;
             for (int p = 0; p < split; ++p) bad |= gm_peer_load(gm_peer(smem_u32(&sm.abort), p)) != 0;
-            const int nt = min(TN, a.in.T - t0), c = tid & 127, n = n0 + c;
-            const bool in = n < a.N;
-            const float s0 = in ? __ldcg(a.ws[0] + n) : 0.f, s1 = GLU && in ? __ldcg(a.ws[1] + n) : 0.f;
-            const float bias = !GLU && a.bias != nullptr && in ? __ldcg(a.bias + n) : 0.f;
+            // a warp takes a token, a lane four channels; two tokens' sums are on their way
+            const int nt = min(TN, a.in.T - t0), c = 4 * lane, n = n0 + c;
             const TO* res = GLU ? nullptr : static_cast<const TO*>(a.residual);
-            for (int t = z * nt / split + ((tid - 128) >> 7); t < (z + 1) * nt / split; t += 2) {
-                int v[GM_MAX_SPLIT], u[GLU ? GM_MAX_SPLIT : 1];
+            float s0[4], s1[4], bias[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool in = n + k < a.N;
+                s0[k] = in ? __ldcg(a.ws[0] + n + k) : 0.f;
+                s1[k] = GLU && in ? __ldcg(a.ws[1] + n + k) : 0.f;
+                bias[k] = !GLU && a.bias != nullptr && in ? __ldcg(a.bias + n + k) : 0.f;
+                if (bad) s0[k] = __int_as_float(0x7fffffff);
+            }
+            constexpr int W = GM_EPI / 32;
+            const int t_end = (z + 1) * nt / split;
+            for (int t = z * nt / split + warp - 4; t < t_end; t += 2 * W) {
+                int v[2][4] = {}, u[2][4] = {};
 #pragma unroll
                 for (int p = 0; p < GM_MAX_SPLIT; ++p) {
-                    v[p] = p < split ? gm_peer_load(gm_peer(ring + (t * 128 + c) * 4, p)) : 0;
-                    if constexpr (GLU) u[p] = p < split ? gm_peer_load(gm_peer(ring + ((TN + t) * 128 + c) * 4, p)) : 0;
-                }
-                int vs = 0, us = 0;
+                    if (p >= split) break;
 #pragma unroll
-                for (int p = 0; p < GM_MAX_SPLIT; ++p) {
-                    vs += v[p];
-                    if constexpr (GLU) us += u[p];
+                    for (int h = 0; h < 2; ++h) {
+                        if (t + h * W >= t_end) continue;
+                        const int4 x = gm_peer_load4(gm_peer(ring + ((t + h * W) * 128 + c) * 4, p));
+                        v[h][0] += x.x, v[h][1] += x.y, v[h][2] += x.z, v[h][3] += x.w;
+                        if constexpr (GLU) {
+                            const int4 y = gm_peer_load4(gm_peer(ring + ((TN + t + h * W) * 128 + c) * 4, p));
+                            u[h][0] += y.x, u[h][1] += y.y, u[h][2] += y.z, u[h][3] += y.w;
+                        }
+                    }
                 }
-                if (n >= a.N) continue;
-                const float sx = __ldcg(a.in.scale + t0 + t);
-                float y;
-                if constexpr (GLU) y = finish_glu(vs, us, sx, s0, s1);
-                else y = finish(vs, sx, s0, bias) + (res ? to_float(__ldcg(res + (long long)(t0 + t) * a.ldr + n)) : 0.f);
-                if (bad) y = __int_as_float(0x7fffffff);
-                store_out(static_cast<TO*>(a.out) + (long long)(t0 + t) * a.ldo + n, y);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int tt = t + h * W;
+                    if (tt >= t_end) break;
+                    const float sx = __ldcg(a.in.scale + t0 + tt);
+                    TO* o = static_cast<TO*>(a.out) + (long long)(t0 + tt) * a.ldo + n;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (n + k >= a.N) break;
+                        float y;
+                        if constexpr (GLU) y = finish_glu(v[h][k], u[h][k], sx, s0[k], s1[k]);
+                        else y = finish(v[h][k], sx, s0[k], bias[k]) + (res ? to_float(__ldcg(res + (long long)(t0 + tt) * a.ldr + n + k)) : 0.f);
+                        store_out(o + k, y);
+                    }
+                }
             }
         }
         __syncwarp();
@@ -319,7 +361,7 @@ static bool gm_map(CUtensorMap* m, const void* p, int K, int rows, long long ld,
 }
 
 template <int TN, bool GLU, class TO>
-static cudaError_t gemm_launch(const Int8Args& a, cudaStream_t s) {
+static cudaError_t gemm_launch(const Int8Args& a, bool early, cudaStream_t s) {
     using S = GemmShape<TN, GLU>;
     const cudaError_t e = prepare_kernel<int8_gemm_kernel<TN, GLU, TO>>(S::SMEM);
     if (e != cudaSuccess) return e;
@@ -354,27 +396,29 @@ static cudaError_t gemm_launch(const Int8Args& a, cudaStream_t s) {
     at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, int8_gemm_kernel<TN, GLU, TO>, a, maps, split);
+    return cudaLaunchKernelEx(&cfg, int8_gemm_kernel<TN, GLU, TO>, a, maps, split, early);
 }
 
+// Tiles as narrow as lets all of them run at once: the weights are read again
+// for each from L2, which costs less than SMs that stand idle.
 template <class TO>
-static cudaError_t gemm_typed(const Int8Args& a, bool glu, cudaStream_t s) {
-    const int T = a.in.T;
+static cudaError_t gemm_typed(const Int8Args& a, bool glu, bool early, cudaStream_t s) {
+    const long long cols = (a.N + 127) / 128;
+    auto fits = [&](int tn) { return cols * ((a.in.T + tn - 1) / tn) <= 148; };
     if (glu) {
-        if (T <= 32) return gemm_launch<32, true, TO>(a, s);
-        if (T <= 64) return gemm_launch<64, true, TO>(a, s);
-        return gemm_launch<128, true, TO>(a, s);
+        if (fits(32)) return gemm_launch<32, true, TO>(a, early, s);
+        if (fits(64)) return gemm_launch<64, true, TO>(a, early, s);
+        return gemm_launch<128, true, TO>(a, early, s);
     }
-    if (T <= 32) return gemm_launch<32, false, TO>(a, s);
-    if (T <= 64) return gemm_launch<64, false, TO>(a, s);
-    const long long wide = (long long)((a.N + 127) / 128) * ((T + 255) / 256);
-    if (T <= 128 || wide < 148) return gemm_launch<128, false, TO>(a, s);
-    return gemm_launch<256, false, TO>(a, s);
+    if (fits(32)) return gemm_launch<32, false, TO>(a, early, s);
+    if (fits(64)) return gemm_launch<64, false, TO>(a, early, s);
+    if (fits(128)) return gemm_launch<128, false, TO>(a, early, s);
+    return gemm_launch<256, false, TO>(a, early, s);
 }
 
-// Rows as codes.  Tiles as narrow as the tokens are few.
-cudaError_t int8_gemm_launch(const Int8Args& a, bool glu, cudaStream_t s) {
-    return with_type(a.out_type, [&](auto to) { return gemm_typed<decltype(to)>(a, glu, s); });
+// Rows as codes; early: see int8_gemv_launch.
+cudaError_t int8_gemm_launch(const Int8Args& a, bool glu, bool early, cudaStream_t s) {
+    return with_type(a.out_type, [&](auto to) { return gemm_typed<decltype(to)>(a, glu, early, s); });
 }
 
 }  // namespace skb

@@ -7,40 +7,47 @@
 namespace skb {
 
 constexpr int GV_THREADS = 256, GV_WARPS = 8;
-constexpr int GV_ROWS = 4;      // weight rows a warp takes at a time (2 gate and 2 up rows)
 constexpr int GV_CHUNK = 512;   // bytes of a row that a warp reads at once
 constexpr int GV_MAX_X = 128 * 1024;  // bytes of codes in shared memory: one token of any length
-constexpr int GV_FUSED = 32 * 1024;   // up to here each CTA makes the codes itself
+constexpr int GV_FUSED_T = 2, GV_FUSED = 32 * 1024;  // tokens, and values, up to which each CTA makes the codes itself
 
-// TT: tokens a CTA holds (the last ones may be missing).
-template <class TX, class TO, int TT, bool GLU>
-__global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args a) {
+// TT: tokens a CTA holds (the last ones may be missing); R: weight rows a warp
+// takes at a time (with SwiGLU R / 2 gate rows and their up rows).  8 / R chunks of
+// each are on their way: 4 KB a warp.
+template <class TX, int TT, int R, bool GLU>
+__global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args a, bool early) {
     extern __shared__ __align__(16) int8_t gv_x[];  // [TT][kp]
     __shared__ float red[2 * GV_WARPS];
     __shared__ float sx[TT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int K = a.in.K, kp = ceil16(K);
     const int t0 = blockIdx.y * TT, nt = min(TT, a.in.T - t0);
-    constexpr int PER = GLU ? GV_ROWS / 2 : GV_ROWS;  // output columns a step
+    constexpr int D = 8 / R;
+    constexpr int PER = GLU ? R / 2 : R;  // output columns a step
     const int groups = (a.N + PER - 1) / PER;
     const int chunks = (kp + GV_CHUNK - 1) / GV_CHUNK;
-    pdl_wait();
-    pdl_trigger();
-
-    auto fetch = [&](uint4 (&w)[GV_ROWS], int group, int chunk) {
-        const int k = chunk * GV_CHUNK + lane * 16;
-#pragma unroll
-        for (int r = 0; r < GV_ROWS; ++r) {
-            const int m = GLU ? r / PER : 0, n = group * PER + (GLU ? r % PER : r);
-            w[r] = make_uint4(0, 0, 0, 0);
-            if (group < groups && n < a.N && k < kp)
-                w[r] = __ldcg(reinterpret_cast<const uint4*>(a.w[m] + n * a.ldw[m] + k));
-        }
-    };
     const int stride = gridDim.x * GV_WARPS;
     int group = blockIdx.x * GV_WARPS + warp;
-    uint4 next[GV_ROWS];
-    fetch(next, group, 0);
+
+    // the next chunk to fetch, of this group or the next
+    int f_group = group, f_chunk = 0;
+    auto fetch = [&](uint4 (&w)[R]) {
+        const int k = f_chunk * GV_CHUNK + lane * 16;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int m = GLU ? r / PER : 0, n = f_group * PER + (GLU ? r % PER : r);
+            w[r] = make_uint4(0, 0, 0, 0);
+            if (f_group < groups && n < a.N && k < kp)
+                w[r] = __ldcg(reinterpret_cast<const uint4*>(a.w[m] + n * a.ldw[m] + k));
+        }
+        if (++f_chunk == chunks) f_chunk = 0, f_group += stride;
+    };
+    uint4 w[D][R];
+    if (!early) pdl_wait();
+#pragma unroll
+    for (int d = 0; d < D; ++d) fetch(w[d]);
+    if (early) pdl_wait();
+    pdl_trigger();
 
     // the tokens' codes
     if constexpr (sizeof(TX) == 1) {
@@ -70,40 +77,15 @@ __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args
     }
     __syncthreads();
 
-    for (; group < groups; group += stride) {
-        int acc[GV_ROWS][TT];
-#pragma unroll
-        for (int r = 0; r < GV_ROWS; ++r)
-#pragma unroll
-            for (int t = 0; t < TT; ++t) acc[r][t] = 0;
-        for (int c = 0; c < chunks; ++c) {
-            uint4 w[GV_ROWS];
-#pragma unroll
-            for (int r = 0; r < GV_ROWS; ++r) w[r] = next[r];
-            if (c + 1 < chunks) fetch(next, group, c + 1);
-            else fetch(next, group + stride, 0);
-            const int k = c * GV_CHUNK + lane * 16;
-            if (k < kp) {
-#pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const int4 x = *reinterpret_cast<const int4*>(gv_x + t * kp + k);
-#pragma unroll
-                    for (int r = 0; r < GV_ROWS; ++r) {
-                        acc[r][t] = __dp4a((int)w[r].x, x.x, acc[r][t]);
-                        acc[r][t] = __dp4a((int)w[r].y, x.y, acc[r][t]);
-                        acc[r][t] = __dp4a((int)w[r].z, x.z, acc[r][t]);
-                        acc[r][t] = __dp4a((int)w[r].w, x.w, acc[r][t]);
-                    }
-                }
-            }
-        }
+    auto finish_group = [&](int group, int (&acc)[R][TT]) {
         // lane (t, column) takes its sum
         int v = 0, u = 0;
 #pragma unroll
-        for (int r = 0; r < GV_ROWS; ++r)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
                 const int sum = __reduce_add_sync(FULL, acc[r][t]);
+                acc[r][t] = 0;
                 if (lane == t * PER + (GLU ? r % PER : r)) {
                     if (GLU && r >= PER) u = sum;
                     else v = sum;
@@ -116,43 +98,87 @@ __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args
                 y = finish_glu(v, u, sx[t], __ldcg(a.ws[0] + n), __ldcg(a.ws[1] + n));
             } else {
                 y = finish(v, sx[t], __ldcg(a.ws[0] + n), a.bias ? __ldcg(a.bias + n) : 0.f);
-                if (a.residual) y += to_float(__ldcg(static_cast<const TO*>(a.residual) + (t0 + t) * a.ldr + n));
+                if (a.residual) y += load_as(a.residual, a.out_type, (t0 + t) * a.ldr + n);
             }
-            store_out(static_cast<TO*>(a.out) + (t0 + t) * a.ldo + n, y);
+            store_as(a.out, a.out_type, (t0 + t) * a.ldo + n, y);
+        }
+    };
+    int acc[R][TT];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[r][t] = 0;
+    int c = 0;
+    while (group < groups) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (group < groups) {
+                const int k = c * GV_CHUNK + lane * 16;
+                if (k < kp) {
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) {
+                        const int4 x = *reinterpret_cast<const int4*>(gv_x + t * kp + k);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            acc[r][t] = __dp4a((int)w[d][r].x, x.x, acc[r][t]);
+                            acc[r][t] = __dp4a((int)w[d][r].y, x.y, acc[r][t]);
+                            acc[r][t] = __dp4a((int)w[d][r].z, x.z, acc[r][t]);
+                            acc[r][t] = __dp4a((int)w[d][r].w, x.w, acc[r][t]);
+                        }
+                    }
+                }
+                fetch(w[d]);
+                if (++c == chunks) {
+                    c = 0;
+                    finish_group(group, acc);
+                    group += stride;
+                }
+            }
         }
     }
 }
 
-bool int8_gemv_fuses(int T, int K) { return T <= I8_FEW && T * ceil16(K) <= GV_FUSED; }
+bool int8_gemv_fuses(int T, int K) { return T <= GV_FUSED_T && T * ceil16(K) <= GV_FUSED; }
 
 template <auto Kernel>
-static cudaError_t gemv_go(const Int8Args& a, dim3 grid, size_t smem, cudaStream_t s) {
+static cudaError_t gemv_go(const Int8Args& a, int R, int tt, bool glu, bool early, cudaStream_t s) {
     const cudaError_t e = prepare_kernel<Kernel>(GV_MAX_X);
-    return e != cudaSuccess ? e : launch(Kernel, grid, dim3(GV_THREADS), smem, s, true, a);
+    if (e != cudaSuccess) return e;
+    const int per = glu ? R / 2 : R, blocks = ((a.N + per - 1) / per + GV_WARPS - 1) / GV_WARPS;
+    const dim3 grid(blocks < 296 ? blocks : 296, (a.in.T + tt - 1) / tt);
+    return launch(Kernel, grid, dim3(GV_THREADS), (size_t)tt * ceil16(a.in.K), s, true, a, early);
 }
 
-template <class TX, class TO, bool GLU>
-static cudaError_t gemv_typed(const Int8Args& a, cudaStream_t s) {
+template <class TX, int TT, bool GLU>
+static cudaError_t gemv_rows(const Int8Args& a, bool early, cudaStream_t s) {
+    const long long rows = (long long)a.N * (GLU ? 2 : 1);
+    if (rows > 2 * GV_WARPS * 296) return gemv_go<int8_gemv_kernel<TX, TT, 4, GLU>>(a, 4, TT, GLU, early, s);
+    if constexpr (!GLU) {
+        if (rows <= GV_WARPS * 296) return gemv_go<int8_gemv_kernel<TX, TT, 1, GLU>>(a, 1, TT, GLU, early, s);
+    }
+    return gemv_go<int8_gemv_kernel<TX, TT, 2, GLU>>(a, 2, TT, GLU, early, s);
+}
+
+template <class TX, bool GLU>
+static cudaError_t gemv_typed(const Int8Args& a, bool early, cudaStream_t s) {
     const int T = a.in.T;
     int tt = T == 1 ? 1 : T == 2 ? 2 : T <= 4 ? 4 : 8;
     while (tt * ceil16(a.in.K) > GV_MAX_X) tt >>= 1;
-    const int per = GLU ? GV_ROWS / 2 : GV_ROWS;
-    const int blocks = ((a.N + per - 1) / per + GV_WARPS - 1) / GV_WARPS;
-    const dim3 grid(blocks < 296 ? blocks : 296, (T + tt - 1) / tt);
-    const size_t smem = (size_t)tt * ceil16(a.in.K);
-    if (tt == 1) return gemv_go<int8_gemv_kernel<TX, TO, 1, GLU>>(a, grid, smem, s);
-    if (tt == 2) return gemv_go<int8_gemv_kernel<TX, TO, 2, GLU>>(a, grid, smem, s);
-    if (tt == 4) return gemv_go<int8_gemv_kernel<TX, TO, 4, GLU>>(a, grid, smem, s);
-    return gemv_go<int8_gemv_kernel<TX, TO, 8, GLU>>(a, grid, smem, s);
+    if (tt == 1) return gemv_rows<TX, 1, GLU>(a, early, s);
+    if (tt == 2) return gemv_rows<TX, 2, GLU>(a, early, s);
+    if constexpr (sizeof(TX) == 1) {
+        if (tt == 4) return gemv_rows<TX, 4, GLU>(a, early, s);
+        return gemv_rows<TX, 8, GLU>(a, early, s);
+    }
+    return cudaErrorInvalidValue;
 }
 
-cudaError_t int8_gemv_launch(const Int8Args& a, bool glu, cudaStream_t s) {
-    return with_type(a.out_type, [&](auto to) {
-        auto go = [&](auto x) {
-            return glu ? gemv_typed<decltype(x), decltype(to), true>(a, s) : gemv_typed<decltype(x), decltype(to), false>(a, s);
-        };
-        return a.in.type == SKB_I8 ? go(int8_t()) : with_type(a.in.type, go);
-    });
+// early: the kernel before this one in the stream is quantize_launch's of the same
+// call, which has waited for all before it when it lets this one begin; so the
+// weights are there, and only the codes are waited for.
+cudaError_t int8_gemv_launch(const Int8Args& a, bool glu, bool early, cudaStream_t s) {
+    auto go = [&](auto x) { return glu ? gemv_typed<decltype(x), true>(a, early, s) : gemv_typed<decltype(x), false>(a, early, s); };
+    return a.in.type == SKB_I8 ? go(int8_t()) : with_type(a.in.type, go);
 }
 
 }  // namespace skb

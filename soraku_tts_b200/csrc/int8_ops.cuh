@@ -69,8 +69,8 @@ cudaError_t prepare_kernel(size_t dyn_bytes) {
 cudaError_t quantize_launch(const RowsIn& in, int8_t* q, long long ldq, float* scale, cudaStream_t s);
 constexpr int I8_FEW = 8;  // tokens that int8_gemv.cu serves
 bool int8_gemv_fuses(int T, int K);
-cudaError_t int8_gemv_launch(const Int8Args& a, bool glu, cudaStream_t s);
-cudaError_t int8_gemm_launch(const Int8Args& a, bool glu, cudaStream_t s);
+cudaError_t int8_gemv_launch(const Int8Args& a, bool glu, bool early, cudaStream_t s);
+cudaError_t int8_gemm_launch(const Int8Args& a, bool glu, bool early, cudaStream_t s);
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -254,6 +254,17 @@ __device__ __forceinline__ float finish_glu(int gate, int up, float sx, float sg
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
+
+__device__ __forceinline__ float load_as(const void* p, int type, long long i) {
+    if (type == SKB_F32) return __ldcg(static_cast<const float*>(p) + i);
+    if (type == SKB_BF16) return __bfloat162float(__ldcg(static_cast<const __nv_bfloat16*>(p) + i));
+    return __half2float(__ldcg(static_cast<const __half*>(p) + i));
+}
+__device__ __forceinline__ void store_as(void* p, int type, long long i, float v) {
+    if (type == SKB_F32) store_out(static_cast<float*>(p) + i, v);
+    else if (type == SKB_BF16) store_out(static_cast<__nv_bfloat16*>(p) + i, v);
+    else store_out(static_cast<__half*>(p) + i, v);
+}
 
 // f(TO()) with the output's type.
 template <class F>
