@@ -75,6 +75,14 @@ cudaError_t int8_gemm_launch(const Int8Args& a, bool glu, bool early, cudaStream
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
 // Largest of |a|, |b|, |c|; NaN if one of them is.
 __device__ __forceinline__ float max_abs(float a, float b, float c) {
@@ -251,9 +259,8 @@ __device__ __forceinline__ float finish_glu(int gate, int up, float sx, float sg
     return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, __expf(-g))), finish(up, sx, su, 0.f));
 }
 
-__device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void store_out(__half* p, float v) { *p = __float2half_rn(v); }
+template <class T>
+__device__ __forceinline__ void store_out(T* p, float v) { *p = from_float<T>(v); }
 
 __device__ __forceinline__ float load_as(const void* p, int type, long long i) {
     if (type == SKB_F32) return __ldcg(static_cast<const float*>(p) + i);

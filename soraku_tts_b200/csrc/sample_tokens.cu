@@ -15,7 +15,7 @@
 // is less than the last step 2^-24 of a uniform number.  A cluster of CTAs holds
 // the row in shared memory, read once from the device's.
 //
-// With a top-k of up to 1536: the k-th largest of the threads' own largest logits
+// With a top-k of up to 1280: the k-th largest of the threads' own largest logits (four each)
 // bounds the k-th logit from below, and hardly more than k logits are above it
 // (k = 1000 of 151,936: about 1150).  Those alone are gathered in one CTA, put in
 // order and weighed.
@@ -31,17 +31,19 @@
 // index), as often as it takes (st_general).
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "int8_ops.cuh"
 
 namespace skb {
 namespace cg = cooperative_groups;
 
-constexpr int ST_THREADS = 512, ST_WARPS = ST_THREADS / 32;
+constexpr int ST_WARPS = 32;        // most of a CTA
 constexpr int ST_BINS = 2048;
 constexpr int ST_LIST = 512;        // logits of one gathered bin
 constexpr int ST_SORT = 2048;       // logits that are gathered to be put in order
-constexpr int ST_QUICK_K = 1536;
-constexpr int ST_FOUR = ST_SORT / ST_THREADS;  // listed logits a thread holds, and bins
+constexpr int ST_QUICK_K = 1280;
+constexpr int ST_OWN = 4;           // parts of a thread's logits that have a largest of their own
 static_assert(ST_BINS == ST_SORT, "as many bins as listed logits");
 constexpr int ST_MAX_V = 1 << 18;
 constexpr double ST_ONE = 17592186044416.0;  // 2^44: the largest logit's weight
@@ -73,32 +75,35 @@ struct Bin {
     int bin;
 };
 
-// Bins [b0, b1] about an answer.
+// Bins [b0, b1] about an answer; none: {-1, -1}.
 struct Window {
     int b0, b1;
 };
 
 struct SampleShared {
+    float top, low;            // this CTA's
     Window window[3];          // apart and in order; written by the first CTA, to all
-    int windows;               // -1: no list can hold them
+    int go_on;                 // 1: the list has the answer, 0: st_general has to
     u64 part[5];               // this CTA's masses: before each window, all, passing min-p
     unsigned before[3];        // logits before each window
-    float approx[4];
+    unsigned listed;           // logits that this CTA has listed
+    int few[3];                // logits of one fine bin, for each question
     int answer[3];
-    u64 delta[3];
-    int starts[3];
-    float top, low;            // this CTA's
+    int hit[3];                // the fine bin that a sum reaches its target in
+    u64 hit_mass[3];
+    unsigned hit_count[3];
+    Found reached[3];
+    float approx[2];
     u64 mass, mass_min_p;      // this CTA's totals
     unsigned count;
     u64 lo, hi;                // smallest and largest key of a bin, this CTA's
     Bin bin;                   // written by the CTA that found it, to all
     Found found;
-    unsigned listed;           // logits that this CTA has listed
     u64 warp_mass[ST_WARPS];
     unsigned warp_count[ST_WARPS];
-    float red[2 * ST_WARPS];
-    u64 prefix[3];
-    double power[32];          // 2^(i / 32)
+    unsigned red[2][ST_WARPS];
+    u64 warp_part[5][ST_WARPS];
+    double power[128];         // 2^(i / 128)
 };
 
 // (logit descending, index ascending) as ascending whole numbers.
@@ -122,65 +127,109 @@ __device__ __forceinline__ u64 drawn_at(float u, u64 mass) {
     return t >= (double)mass ? mass : !(t >= 1.0) ? 1ull : (u64)t + 1;  // + 1 in whole numbers: past 2^53 a double has none
 }
 
-template <class TX>
+// This CTA's part of a row: 16-byte vectors, in shared memory (HELD) or the
+// device's; what lies before the first logit or behind the last reads as -infinity.
+template <class TX, int NT, bool HELD>
 struct Row {
-    const TX* data;  // this CTA's slice in shared memory
+    static constexpr int VN = Vec<TX>::N;
+    const TX* data;  // on 16 bytes
     const double* power;
-    int n, first;    // logits, and the first one's index
+    int off, n, first;  // the first logit's place, how many there are, and its index in the row
     float top, cut, inv_width;
-    double inv_t, scale;  // 1 / T, and 32 log2(e) / T
+    double inv_t, scale;  // 1 / T, and 128 log2(e) / T
     // how far below the largest; beyond `cut`: without weight
     __device__ __forceinline__ float gap(float l) const { return l == top ? 0.f : top - l; }
-    __device__ __forceinline__ bool counts(float l) const { return gap(l) <= cut && l > -INFINITY; }
-    __device__ __forceinline__ int bin(float l) const { return min((int)fminf(gap(l) * inv_width, 3e4f), ST_BINS - 1); }
+    __device__ __forceinline__ bool counts(float l) const { return gap(l) <= cut; }
+    // along the bins, [0, ST_BINS - 1], of what counts; and the nearest one, by an
+    // addition that leaves it in the low bits
+    __device__ __forceinline__ float place(float g) const { return g * inv_width; }
+    __device__ __forceinline__ int bin_at(float g) const { return __float_as_int(fmaf(g, inv_width, 8388608.f)) & 4095; }
+    __device__ __forceinline__ int bin(float l) const { return bin_at(gap(l)); }
     __device__ __forceinline__ double score(float l) const { return l == top ? 0.0 : ((double)l - (double)top) * inv_t; }
-    // exp((l - top) / T) 2^44 for a logit that counts: 2^(n / 32) from a table and the
-    // power series of what is left, |x| <= log(2) / 64, to its fifth power (the sixth is
-    // 2^-48).  The exponent is at least 44 - 48: no underflow.
+    // exp((l - top) / T) 2^44 for a logit that counts: 2^(n / 128) from a table and the
+    // power series of what is left, |x| <= log(2) / 256, to its third power (the fourth
+    // is 2^-38).  The exponent is at least 44 - 48: no underflow.  top is finite.
     __device__ __forceinline__ double weight(float l) const {
-        if (l == top) return ST_ONE;
-        constexpr double MAGIC = 6755399441055744.0, LN2_32 = 0.021660849392498290;
+        constexpr double MAGIC = 6755399441055744.0, LN = 0.69314718055994531 / 128;
         const double y = ((double)l - (double)top) * scale;
         const double m = y + MAGIC;
         const int n = __double2loint(m);
-        const double x = (y - (m - MAGIC)) * LN2_32;
-        double p = fma(x, 1.0 / 120, 1.0 / 24);
-        p = fma(p, x, 1.0 / 6);
-        p = fma(p, x, 0.5);
-        p = fma(p, x, 1.0);
-        p = fma(p, x, 1.0) * power[n & 31];
-        return __hiloint2double(__double2hiint(p) + (((n >> 5) + 44) << 20), __double2loint(p));
+        const double x = y - (m - MAGIC);
+        const double p = fma(fma(fma(LN * LN * LN / 6, x, LN * LN / 2), x, LN), x, 1.0) * power[n & 127];
+        return __hiloint2double(__double2hiint(p) + (((n >> 7) + 44) << 20), __double2loint(p));
     }
-    __device__ __forceinline__ static u64 mass(double weight) {
-        // up to 2^44, rounded by adding 2^52
-        return (u64)__double_as_longlong(weight + 4503599627370496.0) & 0xfffffffffffffull;
+    // rounded by adding 2^52: weights are up to 2^44
+    __device__ __forceinline__ static double whole(double weight) { return __dadd_rn(__dadd_rn(weight, 4503599627370496.0), -4503599627370496.0); }
+    __device__ __forceinline__ u64 mass(float l) const {
+        return l == top ? (u64)ST_ONE : (u64)__double_as_longlong(weight(l) + 4503599627370496.0) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ double safe_weight(float l) const { return l == top ? ST_ONE : weight(l); }
+    // f(logits, index of the first) for every vector, B of them read at a time.
+    template <int B, class F>
+    __device__ __forceinline__ void each(F f) const {
+        const int end = off + n;
+        for (int i = threadIdx.x * VN; i < end; i += B * NT * VN) {
+            Vec<TX> v[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int at = i + b * NT * VN;
+                if (HELD ? at < end : at >= off && at + VN <= end) {
+                    if (HELD) v[b].raw = *reinterpret_cast<const uint4*>(data + at);
+                    else v[b].raw = __ldcg(reinterpret_cast<const uint4*>(data + at));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VN; ++j)
+                        v[b].e[j] = !HELD && at + j >= off && at + j < end ? __ldcg(data + at + j) : from_float<TX>(-INFINITY);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                float l[VN];
+                v[b].get(l);
+                f(l, first + i + b * NT * VN - off);
+            }
+        }
     }
 };
 
-template <class TX, int C>
+template <class TX, int C, int NT, bool HELD>
 struct Sampler {
+    static constexpr int VN = Vec<TX>::N, WARPS = NT / 32;
+    static constexpr int PER = ST_BINS / NT;   // bins of a thread, and listed logits
+    static constexpr int SHARE = ST_BINS / C;  // bins that a CTA adds up for the cluster
+    static_assert(ST_BINS == ST_SORT, "as many bins as listed logits");
+    using R = Row<TX, NT, HELD>;
+
     SampleShared& sm;
-    u64 *key, *weight;             // the list
-    unsigned *count, *low, *high;  // bins of this CTA's logits: number, and mass in two words
+    unsigned* count;               // bins of this CTA's logits
+    unsigned *low, *high;          // their masses, in two words
+    u64* key;                      // this CTA's list, in the place of the masses
     unsigned* pre_count;           // of this CTA's share of the bins, cluster-wide: what stands before each
     u64* pre_mass;
-    const Row<TX>& row;
-    cg::cluster_group cl;
+    const R& row;
     int tid, rank;
     u64 all_mass, mass_min_p;
     unsigned all_count;
     bool fresh;  // the bins hold the whole row
 
-    template <class T>
-    __device__ __forceinline__ T* at(T* p, int r) { return C == 1 ? p : cl.map_shared_rank(p, r); }
-    __device__ __forceinline__ void sync() {
-        if (C == 1) __syncthreads();
-        else cl.sync();
+    __device__ __forceinline__ Sampler(SampleShared& sm, unsigned char* raw, const R& row, int rank)
+        : sm(sm), row(row), tid(threadIdx.x), rank(rank), all_mass(0), mass_min_p(0), all_count(0), fresh(false) {
+        count = reinterpret_cast<unsigned*>(raw);
+        low = count + ST_BINS, high = low + ST_BINS;
+        key = reinterpret_cast<u64*>(low);
+        pre_mass = reinterpret_cast<u64*>(high + ST_BINS);
+        pre_count = reinterpret_cast<unsigned*>(pre_mass + SHARE + 2);
     }
+    static constexpr int BYTES = 3 * ST_BINS * 4 + (SHARE + 2) * 8 + (SHARE + 4) * 4;  // a multiple of 16
 
+    template <class T>
+    __device__ __forceinline__ T* at(T* p, int r) const { return C == 1 ? p : cg::this_cluster().map_shared_rank(p, r); }
+    __device__ __forceinline__ void sync() const {
+        if (C == 1) __syncthreads();
+        else cg::this_cluster().sync();
+    }
     __device__ __forceinline__ void clear() {
-        for (int i = tid; i < ST_BINS; i += ST_THREADS) count[i] = low[i] = high[i] = 0;
-        __syncthreads();
+        for (int i = tid; i < 3 * ST_BINS / 4; i += NT) reinterpret_cast<uint4*>(count)[i] = make_uint4(0, 0, 0, 0);
     }
     __device__ __forceinline__ void add(int b, u64 m) {
         atomicAdd(&count[b], 1u);
@@ -189,18 +238,355 @@ struct Sampler {
         const unsigned hi = (unsigned)(m >> 32) + (old + lo < old ? 1u : 0u);
         if (hi) atomicAdd(&high[b], hi);
     }
+    __device__ __forceinline__ u64 bin_mass(int b) const { return ((u64)high[b] << 32) + low[b]; }
+    // What stands before this thread in the CTA, and all of it.
+    template <class A, class B>
+    __device__ __forceinline__ void scan(A& n, B& m, A& all_n, B& all_m, A* warp_n, B* warp_m) const {
+        const int lane = tid & 31, warp = tid >> 5;
+        auto in_warp = [&](A& x, B& y) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const A p = __shfl_up_sync(FULL, x, o);
+                const B q = __shfl_up_sync(FULL, y, o);
+                if (lane >= o) x += p, y += q;
+            }
+        };
+        const A own_n = n;
+        const B own_m = m;
+        in_warp(n, m);
+        if (lane == 31) warp_n[warp] = n, warp_m[warp] = m;
+        __syncthreads();
+        A wn = lane < WARPS ? warp_n[lane] : A(0);
+        B wm = lane < WARPS ? warp_m[lane] : B(0);
+        in_warp(wn, wm);
+        all_n = __shfl_sync(FULL, wn, 31), all_m = __shfl_sync(FULL, wm, 31);
+        const A pn = __shfl_sync(FULL, wn, (warp + 31) & 31);
+        const B pm = __shfl_sync(FULL, wm, (warp + 31) & 31);
+        n = n - own_n + (warp > 0 ? pn : A(0)), m = m - own_m + (warp > 0 ? pm : B(0));
+        __syncthreads();  // the arrays may be used again
+    }
 
+    // ---- the list ------------------------------------------------------
+    __device__ __forceinline__ void list(float l, int index) {
+        const unsigned p = atomicAdd(&sm.listed, 1u);
+        if (p < ST_SORT) key[p] = st_key(l, index);
+    }
+
+    // The first CTA: the answers from everybody's lists.  The listed logits are
+    // those of `windows` windows of bins; part: the masses before them, of all, and of
+    // what min-p lets stay (known, but for a list that has the first k).
+    // False if the list does not have them.
+    __device__ __forceinline__ bool answer(int windows, bool first_k, int top_k, float top_p, double min_weight, float u, u64 (&part)[5],
+                                           int64_t* token, float* logprob) {
+        unsigned from[C], n = 0;
+#pragma unroll
+        for (int r = 0; r < C; ++r) from[r] = *at(&sm.listed, r);
+#pragma unroll
+        for (int r = 0; r < C; ++r) {
+            const unsigned x = from[r];
+            from[r] = n, n += x;
+        }
+        if (n > ST_SORT) return false;
+        const Window w0 = sm.window[0], w1 = sm.window[1], w2 = sm.window[2];
+        const int each = windows == 1 ? ST_BINS : windows == 2 ? ST_BINS / 2 : ST_BINS / 3;
+        const float per0 = (float)each / (float)(w0.b1 - w0.b0 + 1), per1 = (float)each / (float)(w1.b1 - w1.b0 + 1),
+                    per2 = (float)each / (float)(w2.b1 - w2.b0 + 1);
+        u64 k[PER], m[PER], passing = 0;
+        int fine[PER], in[PER];
+        if (tid < 3) sm.few[tid] = 0, sm.hit[tid] = -1, sm.reached[tid].index = -1;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const unsigned i = j * NT + tid;
+            k[j] = ~0ull, m[j] = 0, fine[j] = -1, in[j] = 0;
+            if (i < n) {
+                u64* list = at(key, 0);
+                unsigned base = 0;
+#pragma unroll
+                for (int r = 1; r < C; ++r)
+                    if (i >= from[r]) list = at(key, r), base = from[r];
+                k[j] = list[i - base];
+                const float l = st_logit(k[j]), g = top_gap(l), x = row.place(g);
+                const double w = row.safe_weight(l);
+                m[j] = (u64)R::whole(w);
+                if (!(w < min_weight)) passing += m[j];
+                const int b = row.bin_at(g);
+                in[j] = (windows > 1 && b >= w1.b0 ? 1 : 0) + (windows > 2 && b >= w2.b0 ? 1 : 0);
+                const float f = (x + 0.5f - (float)(in[j] == 0 ? w0.b0 : in[j] == 1 ? w1.b0 : w2.b0)) * (in[j] == 0 ? per0 : in[j] == 1 ? per1 : per2);
+                fine[j] = in[j] * each + max(0, min((int)f, each - 1));
+            }
+        }
+        const bool small = n <= NT / 4;
+        u64 all = 0;
+        unsigned all_n = n;
+        // small: of this thread's logit, else of its fine bins: what stands before, and how much it is
+        u64 before[PER], size[PER];
+        unsigned count_before[PER], number[PER];
+        __syncthreads();
+        if (small) {
+            // four threads a logit add up what stands before it in its window
+            if (tid < (int)n) key[tid] = k[0], key[NT / 4 + tid] = m[0], count[tid] = in[0];
+            __syncthreads();
+            const int i = tid >> 2;
+            u64 mass = 0, mine = 0;
+            unsigned cnt = 0;
+            int q = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) k[j] = ~0ull, m[j] = 0, fine[j] = -1, before[j] = 0, size[j] = 0, count_before[j] = 0, number[j] = 0;
+            if (i < (int)n) {
+                mine = key[i], q = count[i];
+                for (int j = tid & 3; j < (int)n; j += 4) {
+                    const u64 w = key[NT / 4 + j];
+                    all += w;
+                    if (key[j] < mine && (int)count[j] == q) mass += w, cnt += 1;
+                }
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                mass += __shfl_xor_sync(FULL, mass, o), cnt += __shfl_xor_sync(FULL, cnt, o);
+                all += __shfl_xor_sync(FULL, all, o);
+            }
+            if (i < (int)n && (tid & 3) == 0) {
+                k[0] = mine, m[0] = key[NT / 4 + i], fine[0] = i;
+                before[0] = mass, size[0] = m[0], count_before[0] = cnt, number[0] = 1;
+                if (!first_k) before[0] += q == 0 ? part[0] : q == 1 ? part[1] : part[2], count_before[0] += sm.before[q];
+            }
+            // the sum of all is known where there is a logit: in the first warp
+            if (tid == 0) sm.warp_mass[0] = all;
+            __syncthreads();
+            all = sm.warp_mass[0];
+            __syncthreads();
+        } else {
+            clear();
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (fine[j] >= 0) add(fine[j], m[j]);
+            __syncthreads();
+            // sums along the fine bins; each window begins with what stands before it
+            unsigned cnt = 0;
+            u64 mass = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                number[j] = count[tid * PER + j], size[j] = bin_mass(tid * PER + j);
+                cnt += number[j], mass += size[j];
+            }
+            scan(cnt, mass, all_n, all, sm.warp_count, sm.warp_mass);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                before[j] = mass, count_before[j] = cnt;
+                mass += size[j], cnt += number[j];
+            }
+            if (!first_k) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const int b = tid * PER + j;
+                    if (b % each == 0 && b / each < 3) sm.part[b / each] = before[j], sm.answer[b / each] = (int)count_before[j];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const int q = min((tid * PER + j) / each, windows - 1);
+                    before[j] += (q == 0 ? part[0] : q == 1 ? part[1] : part[2]) - sm.part[q];
+                    count_before[j] += sm.before[q] - (unsigned)sm.answer[q];
+                }
+            }
+        }
+        if (first_k && min_weight > 0) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) passing += __shfl_xor_sync(FULL, passing, o);
+            if ((tid & 31) == 0) sm.warp_part[0][tid >> 5] = passing;
+            __syncthreads();
+            passing = (tid & 31) < WARPS ? sm.warp_part[0][tid & 31] : 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) passing += __shfl_xor_sync(FULL, passing, o);
+        }
+        u64 kept = first_k ? all : part[3];
+        const u64 allowed = first_k ? passing : part[4];
+        // where top-k ends, where top-p does, and what is drawn
+#pragma unroll 1
+        for (int question = 0; question < 3; ++question) {
+            u64 target;
+            if (question == 0) {
+                if (top_k <= 0 || (unsigned)top_k >= (first_k ? all_n : all_count)) continue;
+                target = (u64)top_k;
+            } else if (question == 1) {
+                if (!(top_p < 1.f)) continue;
+                target = share_of(top_p, kept);
+            } else {
+                if (min_weight > 0) kept = min(kept, allowed);
+                target = drawn_at(u, kept);
+            }
+            const bool by_count = question == 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const u64 start = by_count ? (u64)count_before[j] : before[j], extent = by_count ? (u64)number[j] : size[j];
+                if (start < target && target <= start + extent) {
+                    if (small) sm.reached[question] = {before[j] + size[j], st_logit(k[j]), (int)(k[j] & (ST_MAX_V - 1))};
+                    else sm.hit[question] = tid * PER + j, sm.hit_mass[question] = before[j], sm.hit_count[question] = count_before[j];
+                }
+            }
+            __syncthreads();
+            if (!small) {
+                const int b = sm.hit[question];
+                if (b < 0) return false;  // the windows missed
+#pragma unroll
+                for (int j = 0; j < PER; ++j)
+                    if (fine[j] == b) {
+                        const int i = atomicAdd(&sm.few[question], 1);
+                        if (i < ST_SORT / 2) key[i] = k[j], key[ST_SORT / 2 + i] = m[j];
+                    }
+                __syncthreads();
+                const int few = sm.few[question];
+                if (few > ST_SORT / 2) return false;
+                for (int i = tid; i < few; i += NT) {
+                    const u64 mine = key[i], w = key[ST_SORT / 2 + i];
+                    u64 mass = sm.hit_mass[question], cnt = sm.hit_count[question];
+                    for (int j = 0; j < few; ++j)
+                        if (key[j] < mine) cnt += 1, mass += key[ST_SORT / 2 + j];
+                    if (by_count ? cnt + 1 == target : mass < target && target <= mass + w)
+                        sm.reached[question] = {mass + w, st_logit(mine), (int)(mine & (ST_MAX_V - 1))};
+                }
+                __syncthreads();
+            }
+            if (sm.reached[question].index < 0) return false;
+            if (question < 2) kept = sm.reached[question].mass;
+        }
+        if (tid == 0) {
+            *token = sm.reached[2].index;
+            *logprob = (float)(row.score(sm.reached[2].logit) - log((double)kept / ST_ONE));
+        }
+        return true;
+    }
+    __device__ __forceinline__ float top_gap(float l) const { return row.gap(l); }
+
+    // The first CTA: windows about where the answers will be, to all.  total: its bins'
+    // counts; step: a bin's width by T.  How many windows, 0: no list can hold them.
+    __device__ __forceinline__ int choose_windows(const unsigned* total, float step, int top_k, float top_p, float min_p, float u) {
+        // mass by the weight at the middle of each bin
+        unsigned c[PER], cnt = 0, everyone;
+        float m[PER], mass = 0.f, all;
+        float* warp_mass = reinterpret_cast<float*>(sm.red[0]);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int b = tid * PER + j;
+            c[j] = total[b];
+            m[j] = b == 0 ? (float)c[j] : (float)c[j] * __expf(-(float)b * step);
+            cnt += c[j], mass += m[j];
+        }
+        if (tid < 3) sm.answer[tid] = -1;
+        if (tid == 3) sm.approx[0] = sm.approx[1] = -1.f;
+        scan(cnt, mass, everyone, all, sm.warp_count, warp_mass);
+        all_count = everyone;
+        unsigned cb[PER + 1];
+        float mb[PER + 1];
+        cb[0] = cnt, mb[0] = mass;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) cb[j + 1] = cb[j] + c[j], mb[j + 1] = mb[j] + m[j];
+        const bool with_k = top_k > 0 && (unsigned)top_k < everyone;
+        // the last bin that min-p lets stay
+        const float edge = min_p > 0.f ? fminf(-__logf(fminf(min_p, 1.f)) / step + 0.5f, 3e4f) : 3e4f;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int b = tid * PER + j;
+            if (with_k && cb[j] < (unsigned)top_k && (unsigned)top_k <= cb[j + 1]) sm.answer[2] = b, sm.approx[0] = 0.5f * (mb[j] + mb[j + 1]);
+            if ((int)edge == b) sm.approx[1] = mb[j + 1];
+        }
+        __syncthreads();
+        float kept = with_k ? sm.approx[0] : all;
+        auto locate = [&](int which, float target) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (c[j] > 0 && mb[j] <= target && target < mb[j + 1]) sm.answer[which] = tid * PER + j;
+        };
+        const bool with_p = top_p < 1.f;
+        if (with_p) {
+            kept *= fmaxf(top_p, 0.f);
+            locate(1, kept);
+        }
+        if (sm.approx[1] >= 0.f) kept = fminf(kept, sm.approx[1]);
+        locate(0, kept * fminf(fmaxf(u, 0.f), 1.f));
+        __syncthreads();
+        // in order: what is drawn, top-p's end, top-k's
+        const int at_k = sm.answer[2];
+        int at_p = sm.answer[1], at_d = sm.answer[0];
+        if (with_p && at_p < 0) at_p = at_k >= 0 ? at_k : ST_BINS - 1;  // rounding of the sums
+        if (at_d < 0) at_d = at_p >= 0 ? at_p : at_k >= 0 ? at_k : ST_BINS - 1;
+        // 384 logits to each side, or as many as the list has room for
+#pragma unroll 1
+        for (unsigned room = 384;; room = room > 100 ? room / 4 : 0) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int b = tid * PER + j;
+                if (b == at_d) sm.window[0] = {b, b}, sm.before[0] = cb[j], sm.part[0] = cb[j + 1];
+                if (b == at_p) sm.window[1] = {b, b}, sm.before[1] = cb[j], sm.part[1] = cb[j + 1];
+            }
+            if (tid == 0) sm.listed = 0;
+            __syncthreads();
+            const unsigned d0 = sm.before[0], d1 = (unsigned)sm.part[0], p0 = sm.before[1], p1 = (unsigned)sm.part[1];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int b = tid * PER + j;
+                if (b < at_d && d0 - cb[j] <= room) atomicMin(&sm.window[0].b0, b);
+                if (b > at_d && cb[j + 1] - d1 <= room) atomicMax(&sm.window[0].b1, b);
+                if (with_p && b < at_p && p0 - cb[j] <= room) atomicMin(&sm.window[1].b0, b);
+                if (with_p && b > at_p && cb[j + 1] - p1 <= room) atomicMax(&sm.window[1].b1, b);
+            }
+            __syncthreads();
+            // those that touch become one
+            const Window none = {-1, -1};
+            Window w0 = sm.window[0], w1 = none, w2 = none;
+            if (with_p) {
+                const Window p = sm.window[1];
+                if (p.b0 <= w0.b1 + 1) w0.b0 = min(w0.b0, p.b0), w0.b1 = max(w0.b1, p.b1);
+                else w1 = p;
+            }
+            if (at_k >= 0) {
+                const Window k = {at_k, at_k};
+                Window& last = w1.b0 >= 0 ? w1 : w0;
+                if (k.b0 <= last.b1 + 1) last.b0 = min(last.b0, k.b0), last.b1 = max(last.b1, k.b1);
+                else if (w1.b0 >= 0) w2 = k;
+                else w1 = k;
+            }
+            __syncthreads();
+            // logits in them, and before them
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int b = tid * PER + j;
+                if (b == w0.b0) sm.before[0] = cb[j], atomicSub(&sm.listed, cb[j]);
+                if (b == w1.b0) sm.before[1] = cb[j], atomicSub(&sm.listed, cb[j]);
+                if (b == w2.b0) sm.before[2] = cb[j], atomicSub(&sm.listed, cb[j]);
+                if (b == w0.b1) atomicAdd(&sm.listed, cb[j + 1]);
+                if (b == w1.b1) atomicAdd(&sm.listed, cb[j + 1]);
+                if (b == w2.b1) atomicAdd(&sm.listed, cb[j + 1]);
+            }
+            __syncthreads();
+            const unsigned listed = sm.listed;
+            if (listed > ST_SORT && room > 0) continue;
+            const int windows = listed > ST_SORT ? 0 : 1 + (w1.b0 >= 0) + (w2.b0 >= 0);
+            if (tid < C) {
+                SampleShared* peer = at(&sm, tid);
+                peer->window[0] = w0, peer->window[1] = w1, peer->window[2] = w2;
+                peer->go_on = windows > 0;
+            }
+            __syncthreads();
+            if (tid == 0) sm.listed = 0;
+            return windows;
+        }
+    }
+
+    // ---- bins with masses, again and again -----------------------------
     // Every CTA's bins into running sums over the cluster's, each CTA a share of the bins.
     // passing: this thread's mass of what min-p lets stay.
     __device__ __forceinline__ void total(u64 passing) {
         sync();
-        constexpr int SHARE = ST_BINS / C, PER = SHARE > ST_THREADS ? SHARE / ST_THREADS : 1;
-        const int b0 = tid * PER;
-        unsigned n = 0, cn[PER];
-        u64 m = 0, cm[PER];
+        constexpr int EACH = SHARE > NT ? SHARE / NT : 1;
+        const int b0 = tid * EACH;
+        unsigned n = 0, cn[EACH];
+        u64 m = 0, cm[EACH];
         if (b0 < SHARE) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
+            for (int j = 0; j < EACH; ++j) {
                 cn[j] = n, cm[j] = m;
                 const int b = rank * SHARE + b0 + j;
 #pragma unroll
@@ -211,23 +597,13 @@ struct Sampler {
                 }
             }
         }
-        unsigned in = n;
-        u64 im = m;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned a = __shfl_up_sync(FULL, in, o);
-            const u64 b = __shfl_up_sync(FULL, im, o);
-            if ((tid & 31) >= o) in += a, im += b;
-            passing += __shfl_xor_sync(FULL, passing, o);
-        }
-        if ((tid & 31) == 31) sm.warp_count[tid >> 5] = in, sm.warp_mass[tid >> 5] = im;
+        for (int o = 16; o > 0; o >>= 1) passing += __shfl_xor_sync(FULL, passing, o);
         if ((tid & 31) == 0 && passing) atomicAdd(&sm.mass_min_p, passing);
-        __syncthreads();
-        unsigned wn = 0;
-        u64 wm = 0;
-        for (int w = 0; w < (tid >> 5); ++w) wn += sm.warp_count[w], wm += sm.warp_mass[w];
-        in += wn, im += wm;
-        if (tid == ST_THREADS - 1) sm.count = in, sm.mass = im;
+        unsigned all_n;
+        u64 all_m;
+        scan(n, m, all_n, all_m, sm.warp_count, sm.warp_mass);
+        if (tid == 0) sm.count = all_n, sm.mass = all_m;
         sync();
         unsigned before = 0;
         u64 before_mass = 0;
@@ -242,30 +618,29 @@ struct Sampler {
         }
         if (b0 < SHARE) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                pre_count[b0 + j] = before + in - n + cn[j];
-                pre_mass[b0 + j] = before_mass + im - m + cm[j];
-            }
-            if (b0 + PER == SHARE) {
-                pre_count[SHARE] = before + in;
-                pre_mass[SHARE] = before_mass + im;
+            for (int j = 0; j < EACH; ++j) {
+                pre_count[b0 + j] = before + n + cn[j];
+                pre_mass[b0 + j] = before_mass + m + cm[j];
             }
         }
+        if (tid == 0) pre_count[SHARE] = before + all_n, pre_mass[SHARE] = before_mass + all_m;
         __syncthreads();
     }
     // The whole row's bins.
     __device__ __forceinline__ void fill(double min_weight) {
+        __syncthreads();
         clear();
+        __syncthreads();
         u64 passing = 0;
-        for (int i = tid; i < row.n; i += ST_THREADS) {
-            const float l = to_float(row.data[i]);
-            if (row.counts(l)) {
-                const double w = row.weight(l);
-                const u64 m = row.mass(w);
-                add(row.bin(l), m);
-                if (!(w < min_weight)) passing += m;
-            }
-        }
+        row.template each<1>([&](const float (&l)[VN], int) {
+#pragma unroll
+            for (int j = 0; j < VN; ++j)
+                if (row.counts(l[j])) {
+                    const u64 m = row.mass(l[j]);
+                    add(row.bin(l[j]), m);
+                    if (!(row.safe_weight(l[j]) < min_weight)) passing += m;
+                }
+        });
         total(passing);
         fresh = true;
     }
@@ -273,9 +648,8 @@ struct Sampler {
     // The bin in which the count or the mass reaches `target` (1 to the whole).
     // Nothing is listed any more.
     __device__ __forceinline__ Bin find(bool by_count, u64 target, u64 mass_before, unsigned count_before) {
-        constexpr int SHARE = ST_BINS / C;
         if (tid == 0) sm.listed = 0;
-        for (int i = tid; i < SHARE; i += ST_THREADS) {
+        for (int i = tid; i < SHARE; i += NT) {
             const u64 m0 = mass_before + pre_mass[i], m1 = mass_before + pre_mass[i + 1];
             const unsigned n0 = count_before + pre_count[i], n1 = count_before + pre_count[i + 1];
             if (by_count ? n0 < target && target <= n1 : m0 < target && target <= m1) {
@@ -288,131 +662,6 @@ struct Sampler {
         __syncthreads();
         return b;
     }
-
-    // What `wanted` says, into this CTA's list.
-    template <class F>
-    __device__ __forceinline__ void list(F wanted) {
-        for (int i = tid; i < row.n; i += ST_THREADS) {
-            const float l = to_float(row.data[i]);
-            if (wanted(l)) {
-                const unsigned p = atomicAdd(&sm.listed, 1u);
-                if (p < ST_SORT) key[p] = st_key(l, row.first + i);
-            }
-        }
-    }
-    // The first CTA: everybody's lists, in order, to its own.  `fine`: bins [0, ST_BINS)
-    // along the order, the finer the better.  The number of logits; more than
-    // ST_SORT: nothing was done.
-    template <class F>
-    __device__ __forceinline__ int collect(F fine) {
-        unsigned from[C + 1];
-        from[0] = 0;
-#pragma unroll
-        for (int r = 0; r < C; ++r) from[r + 1] = from[r] + *at(&sm.listed, r);
-        const int n = (int)min(from[C], (unsigned)ST_SORT + 1);
-        if (n > ST_SORT) return n;
-        u64 k[ST_FOUR];
-        unsigned slot[ST_FOUR];
-        int bin[ST_FOUR];
-#pragma unroll
-        for (int j = 0; j < ST_FOUR; ++j) {
-            const int i = j * ST_THREADS + tid;
-            k[j] = ~0ull;
-            if (i < n) {
-                int r = 0;
-                while (from[r + 1] <= (unsigned)i) ++r;
-                k[j] = at(key, r)[i - from[r]];
-            }
-        }
-        for (int i = tid; i < ST_BINS; i += ST_THREADS) count[i] = 0;
-        if (tid == 0) sm.answer[0] = 0;
-        __syncthreads();
-        if (n <= 128) {
-            // few: each counts those before it
-            if (tid < n) key[tid] = k[0];
-            __syncthreads();
-            const int i = tid >> 2;  // four threads each
-            unsigned before = 0;
-            u64 mine = 0;
-            if (i < n) {
-                mine = key[i];
-                for (int j = tid & 3; j < n; j += 4) before += key[j] < mine;
-            }
-            before += __shfl_xor_sync(FULL, before, 1);
-            before += __shfl_xor_sync(FULL, before, 2);
-            __syncthreads();
-            if (i < n && (tid & 3) == 0) key[before] = mine;
-            __syncthreads();
-            return n;
-        }
-        int crowd = 0;
-#pragma unroll
-        for (int j = 0; j < ST_FOUR; ++j)
-            if (j * ST_THREADS + tid < n) {
-                bin[j] = fine(st_logit(k[j]));
-                slot[j] = atomicAdd(&count[bin[j]], 1u);
-                crowd = max(crowd, (int)slot[j]);
-            }
-        crowd = __reduce_max_sync(FULL, crowd);
-        if ((tid & 31) == 0 && crowd > 32) sm.answer[0] = 1;
-        __syncthreads();
-        if (sm.answer[0]) {  // many equal ones
-#pragma unroll
-            for (int j = 0; j < ST_FOUR; ++j)
-                if (j * ST_THREADS + tid < n) key[j * ST_THREADS + tid] = k[j];
-            __syncthreads();
-            sort(n);
-            return n;
-        }
-        // bins' counts to where they begin; then each place within a bin
-        const uint4 c = reinterpret_cast<const uint4*>(count)[tid];
-        unsigned sum = c.x + c.y + c.z + c.w, upto = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned x = __shfl_up_sync(FULL, upto, o);
-            if ((tid & 31) >= o) upto += x;
-        }
-        if ((tid & 31) == 31) sm.warp_count[tid >> 5] = upto;
-        __syncthreads();
-        unsigned at0 = upto - sum;
-        for (int w = 0; w < (tid >> 5); ++w) at0 += sm.warp_count[w];
-        reinterpret_cast<uint4*>(count)[tid] = make_uint4(at0, at0 + c.x, at0 + c.x + c.y, at0 + c.x + c.y + c.z);
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < ST_FOUR; ++j)
-            if (j * ST_THREADS + tid < n) key[count[bin[j]] + slot[j]] = k[j];
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < ST_FOUR; ++j)
-            if (j * ST_THREADS + tid < n) {
-                const unsigned b0 = count[bin[j]], b1 = bin[j] + 1 < ST_BINS ? count[bin[j] + 1] : (unsigned)n;
-                slot[j] = b0;
-                for (unsigned i = b0; i < b1; ++i) slot[j] += key[i] < k[j];
-            }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < ST_FOUR; ++j)
-            if (j * ST_THREADS + tid < n) key[slot[j]] = k[j];
-        __syncthreads();
-        return n;
-    }
-
-    // What `wanted` says, into the first CTA's list; how many there are, listed or not.
-    template <class F>
-    __device__ __forceinline__ unsigned gather(int room, F wanted) {
-        unsigned* listed = at(&sm.listed, 0);
-        u64* keys = at(key, 0);
-        for (int i = tid; i < row.n; i += ST_THREADS) {
-            const float l = to_float(row.data[i]);
-            if (wanted(l, row.first + i)) {
-                const unsigned p = atomicAdd(listed, 1u);
-                if (p < room) keys[p] = st_key(l, row.first + i);
-            }
-        }
-        sync();
-        return *listed;
-    }
-    __device__ __forceinline__ u64 weigh(u64 k) { return row.mass(row.weight(st_logit(k))); }
 
     // The logit at which the count or the mass reaches `target`.
     __device__ __forceinline__ Found select(bool by_count, u64 target) {
@@ -428,15 +677,14 @@ struct Sampler {
         while (b.count > ST_LIST) {
             // the smallest and largest key there is between lo and hi
             u64 a = ~0ull, z = 0;
-            for (int i = tid; i < row.n; i += ST_THREADS) {
-                const float l = to_float(row.data[i]);
-                if (inside(l, row.first + i)) {
-                    const u64 k = st_key(l, row.first + i);
-                    a = min(a, k), z = max(z, k);
-                }
-            }
+            row.template each<1>([&](const float (&l)[VN], int i) {
+#pragma unroll
+                for (int j = 0; j < VN; ++j)
+                    if (inside(l[j], i + j)) a = min(a, st_key(l[j], i + j)), z = max(z, st_key(l[j], i + j));
+            });
             if (tid == 0) sm.lo = ~0ull, sm.hi = 0;
             clear();
+            __syncthreads();
             if (a <= z) {
                 atomicMin(&sm.lo, a);
                 atomicMax(&sm.hi, z);
@@ -446,39 +694,42 @@ struct Sampler {
 #pragma unroll
             for (int r = 0; r < C; ++r) a = min(a, *at(&sm.lo, r)), z = max(z, *at(&sm.hi, r));
             const int width = 64 - __clzll((long long)(z - a)), shift = max(0, width - 11);
-            for (int i = tid; i < row.n; i += ST_THREADS) {
-                const float l = to_float(row.data[i]);
-                if (inside(l, row.first + i)) add((int)((st_key(l, row.first + i) - a) >> shift), row.mass(row.weight(l)));
-            }
+            row.template each<1>([&](const float (&l)[VN], int i) {
+#pragma unroll
+                for (int j = 0; j < VN; ++j)
+                    if (inside(l[j], i + j)) add((int)((st_key(l[j], i + j) - a) >> shift), row.mass(l[j]));
+            });
             total(0);
             fresh = false;
             b = find(by_count, target, b.mass_before, b.count_before);
             lo = a + ((u64)b.bin << shift);
             hi = lo + ((1ull << shift) - 1);
         }
-        const int n = min(gather(ST_LIST, inside), (unsigned)ST_LIST);
-        if (rank == 0) {
-            for (int i = tid; i < n; i += ST_THREADS) weight[i] = weigh(key[i]);
-            __syncthreads();
-            // two threads each add up what stands before one
-            for (int i0 = 0; i0 < n; i0 += ST_THREADS / 2) {
-                const int i = i0 + (tid >> 1);
-                unsigned cnt = 0;
-                u64 mass = 0;
-                if (i < n) {
-                    const u64 mine = key[i];
-                    for (int j = tid & 1; j < n; j += 2)
-                        if (key[j] < mine) cnt += 1, mass += weight[j];
+        // into the first CTA's list
+        unsigned* listed = at(&sm.listed, 0);
+        u64* keys = at(key, 0);
+        row.template each<1>([&](const float (&l)[VN], int i) {
+#pragma unroll
+            for (int j = 0; j < VN; ++j)
+                if (inside(l[j], i + j)) {
+                    const unsigned p = atomicAdd(listed, 1u);
+                    if (p < ST_LIST) keys[p] = st_key(l[j], i + j);
                 }
-                cnt += __shfl_xor_sync(FULL, cnt, 1);
-                mass += __shfl_xor_sync(FULL, mass, 1);
-                if (i < n && (tid & 1) == 0) {
-                    cnt += b.count_before, mass += b.mass_before;
-                    const u64 w = weight[i];
-                    if (by_count ? cnt + 1 == target : mass < target && target <= mass + w) {
-                        const Found f = {mass + w, st_logit(key[i]), (int)(key[i] & (ST_MAX_V - 1))};
-                        for (int r = 0; r < C; ++r) *at(&sm.found, r) = f;
-                    }
+        });
+        sync();
+        if (rank == 0) {
+            const int n = min((int)sm.listed, ST_LIST);
+            u64* weight = key + ST_LIST;
+            for (int i = tid; i < n; i += NT) weight[i] = row.mass(st_logit(key[i]));
+            __syncthreads();
+            for (int i = tid; i < n; i += NT) {
+                const u64 mine = key[i], w = weight[i];
+                u64 mass = b.mass_before, cnt = b.count_before;
+                for (int j = 0; j < n; ++j)
+                    if (key[j] < mine) cnt += 1, mass += weight[j];
+                if (by_count ? cnt + 1 == target : mass < target && target <= mass + w) {
+                    const Found f = {mass + w, st_logit(mine), (int)(mine & (ST_MAX_V - 1))};
+                    for (int r = 0; r < C; ++r) *at(&sm.found, r) = f;
                 }
             }
         }
@@ -487,182 +738,18 @@ struct Sampler {
         __syncthreads();
         return f;
     }
-
-    // The first CTA: windows about where the answers will be, to all.  total: its bins'
-    // counts; span: the logits they cover.
-    __device__ __forceinline__ void choose_windows(const unsigned* total, float span, double t, int top_k, float top_p, float min_p,
-                                                   float u) {
-        const int lane = tid & 31, warp = tid >> 5;
-        const uint4 c4 = reinterpret_cast<const uint4*>(total)[tid];
-        const unsigned c[ST_FOUR] = {c4.x, c4.y, c4.z, c4.w};
-        // mass by the weight at the middle of each bin (nothing of the first is above its beginning)
-        const float step = (float)(span / ST_BINS / t);
-        float m[ST_FOUR], mass = 0.f;
-        unsigned cnt = 0;
-#pragma unroll
-        for (int j = 0; j < ST_FOUR; ++j) {
-            const int b = tid * ST_FOUR + j;
-            m[j] = c[j] == 0 ? 0.f : b == 0 ? 1.f + (float)(c[j] - 1) * __expf(-0.5f * step) : (float)c[j] * __expf(-((float)b + 0.5f) * step);
-            mass += m[j], cnt += c[j];
-        }
-        float mass_at = mass;
-        unsigned cnt_at = cnt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const float x = __shfl_up_sync(FULL, mass_at, o);
-            const unsigned y = __shfl_up_sync(FULL, cnt_at, o);
-            if (lane >= o) mass_at += x, cnt_at += y;
-        }
-        float* warp_mass = sm.red;
-        if (lane == 31) warp_mass[warp] = mass_at, sm.warp_count[warp] = cnt_at;
-        if (tid < 3) sm.answer[tid] = -1, sm.approx[tid] = -1.f;
-        __syncthreads();
-        mass_at -= mass, cnt_at -= cnt;
-        float all = 0.f;
-        unsigned everyone = 0;
-        for (int w = 0; w < ST_WARPS; ++w) {
-            if (w < warp) mass_at += warp_mass[w], cnt_at += sm.warp_count[w];
-            all += warp_mass[w], everyone += sm.warp_count[w];
-        }
-        // what stands up to each of this thread's bins
-        float mb[ST_FOUR + 1];
-        unsigned cb[ST_FOUR + 1];
-        mb[0] = mass_at, cb[0] = cnt_at;
-#pragma unroll
-        for (int j = 0; j < ST_FOUR; ++j) mb[j + 1] = mb[j] + m[j], cb[j + 1] = cb[j] + c[j];
-        const bool with_k = top_k > 0 && (unsigned)top_k < everyone;
-        // the last bin that min-p lets stay
-        const float edge = min_p > 0.f ? fminf(-__logf(fminf(min_p, 1.f)) / step, 3e4f) : 3e4f;
-#pragma unroll
-        for (int j = 0; j < ST_FOUR; ++j) {
-            const int b = tid * ST_FOUR + j;
-            if (with_k && cb[j] < (unsigned)top_k && (unsigned)top_k <= cb[j + 1]) sm.answer[0] = b, sm.approx[0] = 0.5f * (mb[j] + mb[j + 1]);
-            if ((int)edge == b) sm.approx[1] = mb[j + 1];
-        }
-        __syncthreads();
-        float kept = with_k ? sm.approx[0] : all;
-        auto locate = [&](int which, float target) {
-#pragma unroll
-            for (int j = 0; j < ST_FOUR; ++j)
-                if (c[j] > 0 && mb[j] <= target && target < mb[j + 1]) sm.answer[which] = tid * ST_FOUR + j;
-        };
-        if (top_p < 1.f) {
-            kept *= fmaxf(top_p, 0.f);
-            locate(1, kept);
-        }
-        if (sm.approx[1] >= 0.f) kept = fminf(kept, sm.approx[1]);
-        locate(2, kept * fminf(fmaxf(u, 0.f), 1.f));
-        __syncthreads();
-        // as many logits to each side as the list has room for
-        int at[3] = {sm.answer[0], sm.answer[1], sm.answer[2]};
-        if (at[1] < 0 && top_p < 1.f) at[1] = ST_BINS - 1;  // rounding of the sums
-        if (at[2] < 0) at[2] = at[1] >= 0 ? at[1] : ST_BINS - 1;
-        int n = 0;
-        for (unsigned room = 384;; room = room > 100 ? room / 4 : 0) {
-            __syncthreads();
-            if (tid < 3) sm.window[tid] = {at[tid], at[tid]};
-#pragma unroll
-            for (int q = 0; q < 3; ++q)
-                if (at[q] >= 0 && at[q] / ST_FOUR == tid) {
-#pragma unroll
-                    for (int j = 0; j < ST_FOUR; ++j)
-                        if (at[q] % ST_FOUR == j) sm.before[q] = cb[j], sm.starts[q] = (int)cb[j + 1];
-                }
-            __syncthreads();
-#pragma unroll
-            for (int q = 1; q < 3; ++q)
-                if (at[q] >= 0) {
-#pragma unroll
-                    for (int j = 0; j < ST_FOUR; ++j) {
-                        const int b = tid * ST_FOUR + j;
-                        if (b < at[q] && sm.before[q] - cb[j] <= room) atomicMin(&sm.window[q].b0, b);
-                        if (b > at[q] && cb[j + 1] - (unsigned)sm.starts[q] <= room) atomicMax(&sm.window[q].b1, b);
-                    }
-                }
-            __syncthreads();
-            // in order, and those that touch as one
-            Window w[3];
-            n = 0;
-            int order[3] = {2, 1, 0};  // what is drawn comes first, top-k's end last
-#pragma unroll
-            for (int q = 0; q < 3; ++q) {
-                if (at[order[q]] < 0) continue;
-                const Window x = sm.window[order[q]];
-                int i = n;
-                while (i > 0 && w[i - 1].b0 > x.b0) w[i] = w[i - 1], --i;
-                w[i] = x;
-                ++n;
-            }
-            int k = 0;
-            for (int q = 1; q < n; ++q) {
-                if (w[q].b0 <= w[k].b1 + 1) w[k].b1 = max(w[k].b1, w[q].b1);
-                else w[++k] = w[q];
-            }
-            n = k + 1;
-            // how many logits there are in them, and before them
-            __syncthreads();
-            if (tid == 0) sm.listed = 0;
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < ST_FOUR; ++j) {
-                const int b = tid * ST_FOUR + j;
-                for (int q = 0; q < n; ++q) {
-                    if (w[q].b0 == b) sm.before[q] = cb[j], atomicSub(&sm.listed, cb[j]);
-                    if (w[q].b1 == b) atomicAdd(&sm.listed, cb[j + 1]);
-                }
-            }
-            __syncthreads();
-            const unsigned listed = sm.listed;
-            if (listed <= ST_SORT || room == 0) {
-                if (listed > ST_SORT) n = -1;
-                if (tid < C) {
-                    SampleShared* peer = at_rank(tid);
-                    peer->windows = n;
-                    for (int q = 0; q < 3; ++q) peer->window[q] = q < n ? w[q] : Window{-1, -1};
-                    for (int q = 0; q < 5; ++q) peer->part[q] = 0;
-                }
-                __syncthreads();
-                if (tid == 0) sm.listed = 0;
-                return;
-            }
-        }
-    }
-    __device__ __forceinline__ SampleShared* at_rank(int r) { return at(&sm, r); }
-
-    // The n listed keys in ascending order, the first CTA's threads all.
-    __device__ __forceinline__ void sort(int n) {
-        int size = 32;
-        while (size < n) size <<= 1;
-        for (int i = n + tid; i < size; i += ST_THREADS) key[i] = ~0ull;
-        __syncthreads();
-        for (int k = 2; k <= size; k <<= 1)
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                for (int p = tid; p < size / 2; p += ST_THREADS) {
-                    const int i = 2 * p - (p & (j - 1)), o = i + j;
-                    const u64 x = key[i], y = key[o];
-                    if ((x > y) == ((i & k) == 0)) key[i] = y, key[o] = x;
-                }
-                __syncthreads();
-            }
-        __syncthreads();
-    }
 };
 
 // The row by bins with their masses, binned again as often as it takes.
-template <class TX, int C>
-__device__ __noinline__ void st_general(const SampleArgs& a, Row<TX> row, SampleShared& sm, unsigned* count, int r, int rank,
-                                        int top_k, float top_p, double min_weight, float u) {
-    u64* pre_mass = reinterpret_cast<u64*>(count) - (ST_BINS / C + 2) - (ST_BINS / C + 4) / 2;
-    unsigned* pre_count = reinterpret_cast<unsigned*>(pre_mass + ST_BINS / C + 2);
-    u64* key = reinterpret_cast<u64*>(count + ST_BINS);
-    Sampler<TX, C> s = {sm, key, key + ST_LIST, count, count + ST_BINS, count + 2 * ST_BINS, pre_count, pre_mass, row,
-                        cg::this_cluster(), (int)threadIdx.x, rank, 0, 0, 0, false};
+template <class TX, int C, int NT, bool HELD>
+__device__ __noinline__ void st_general(Row<TX, NT, HELD> row, SampleShared& sm, unsigned char* raw, int rank, int top_k, float top_p,
+                                        double min_weight, float u, int64_t* token, float* logprob) {
+    Sampler<TX, C, NT, HELD> s(sm, raw, row, rank);
     s.sync();  // whatever was being read in this CTA's shared memory has been
     s.fill(min_weight);
     u64 kept = s.all_mass;
     const u64 passing = min_weight > 0 ? s.mass_min_p : kept;
     Found f;
-    // where top-k ends, where top-p does, and what is drawn
 #pragma unroll 1
     for (int question = 0; question < 3; ++question) {
         u64 target;
@@ -680,30 +767,26 @@ __device__ __noinline__ void st_general(const SampleArgs& a, Row<TX> row, Sample
         if (question < 2) kept = f.mass;
     }
     if (rank == 0 && threadIdx.x == 0) {
-        a.tokens[r] = f.index;
-        a.logprob[r] = (float)(row.score(f.logit) - log((double)kept / ST_ONE));
+        *token = f.index;
+        *logprob = (float)(row.score(f.logit) - log((double)kept / ST_ONE));
     }
     s.sync();
 }
 
-template <class TX, int C>
-__global__ void __launch_bounds__(ST_THREADS, 2) sample_kernel(const SampleArgs a) {
+template <class TX, int C, int NT, bool HELD>
+__global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs a) {
+    using S = Sampler<TX, C, NT, HELD>;
+    constexpr int VN = Vec<TX>::N, WARPS = NT / 32;
     extern __shared__ __align__(16) unsigned char st_raw[];
     __shared__ SampleShared sm;
-    u64* pre_mass = reinterpret_cast<u64*>(st_raw);
-    unsigned* pre_count = reinterpret_cast<unsigned*>(pre_mass + ST_BINS / C + 2);
-    unsigned* count = pre_count + ST_BINS / C + 4;
-    // the list lies over the bins' masses: those are summed up before anything is listed
-    u64* key = reinterpret_cast<u64*>(count + ST_BINS);
-    static_assert(ST_SORT * 8 <= 2 * ST_BINS * 4, "the list fits");
-    TX* data = reinterpret_cast<TX*>(count + 3 * ST_BINS);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / C;
-    cg::cluster_group cl = cg::this_cluster();
-    const int rank = C == 1 ? 0 : (int)cl.block_rank();
-    if (tid < 32) sm.power[tid] = exp2(tid / 32.0);
-    for (int i = tid; i < ST_BINS; i += ST_THREADS) count[i] = 0;
-    if (tid == 0) sm.listed = 0;
+    const int rank = C == 1 ? 0 : (int)cg::this_cluster().block_rank();
+    Row<TX, NT, HELD> row;
+    S s(sm, st_raw, row, rank);
+    if (tid < 128) sm.power[tid] = exp2(tid / 128.0);
+    if (tid == 128) sm.listed = 0, sm.mass_min_p = 0, sm.go_on = 1;
+    s.clear();
 
     pdl_wait();
     pdl_trigger();
@@ -713,70 +796,72 @@ __global__ void __launch_bounds__(ST_THREADS, 2) sample_kernel(const SampleArgs 
     int top_k = a.top_k ? __ldcg(a.top_k + r) : a.top_k0;
     const float u = __ldcg(a.uniform + r);
 
-    // the slice, in the places mod 16 bytes that it has in memory
-    Row<TX> row;
     row.power = sm.power;
     row.first = rank * a.slice;
     row.n = max(0, min(a.slice, a.V - row.first));
-    float mine = -INFINITY;  // this thread's largest
-    {
-        constexpr int VN = Vec<TX>::N;
-        const TX* src = static_cast<const TX*>(a.logits) + (long long)r * a.ld + row.first;
-        const int off = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(TX));
-        row.data = data + off;
-        float lo = INFINITY;
-        auto see = [&](float l) {
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(mine) : "f"(l));
-            if (l > -INFINITY) lo = fminf(lo, l);
-        };
-#pragma unroll 4
-        for (int i = tid * VN; i < row.n + off; i += ST_THREADS * VN) {
-            Vec<TX> v;
-            if (i >= off && i + VN <= row.n + off) {
-                v.raw = __ldcs(reinterpret_cast<const uint4*>(src + (i - off)));
-                *reinterpret_cast<uint4*>(data + i) = v.raw;
-                float f[VN];
-                v.get(f);
+    float mine[ST_OWN], low = INFINITY;  // largest of this thread's parts, and its smallest that is finite
 #pragma unroll
-                for (int j = 0; j < VN; ++j) see(f[j]);
-            } else {
-                for (int j = max(i, off); j < min(i + VN, row.n + off); ++j) {
-                    const TX e = __ldcs(src + (j - off));
-                    data[j] = e;
-                    see(to_float(e));
+    for (int q = 0; q < ST_OWN; ++q) mine[q] = -INFINITY;
+    {
+        const TX* src = static_cast<const TX*>(a.logits) + (long long)r * a.ld + row.first;
+        row.off = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(TX));
+        src -= row.off;
+        TX* held = reinterpret_cast<TX*>(st_raw + S::BYTES);
+        row.data = HELD ? held : src;
+        constexpr int B = 32 / VN / 2;
+        const int end = row.off + row.n;
+        for (int i = tid * VN; i < end; i += B * NT * VN) {
+            Vec<TX> v[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int at = i + b * NT * VN;
+                if (at >= row.off && at + VN <= end) {
+                    v[b].raw = HELD ? __ldcs(reinterpret_cast<const uint4*>(src + at)) : __ldcg(reinterpret_cast<const uint4*>(src + at));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VN; ++j)
+                        v[b].e[j] = at + j >= row.off && at + j < end ? __ldcg(src + at + j) : from_float<TX>(-INFINITY);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int at = i + b * NT * VN;
+                if (HELD && at < end) *reinterpret_cast<uint4*>(held + at) = v[b].raw;
+                float l[VN];
+                v[b].get(l);
+#pragma unroll
+                for (int j = 0; j < VN; ++j) {
+                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(mine[(b * VN + j) * ST_OWN / (B * VN)]) : "f"(l[j]));
+                    low = fminf(low, l[j] > -INFINITY ? l[j] : INFINITY);
                 }
             }
         }
-        float hi = mine;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float h = __shfl_xor_sync(FULL, hi, o);
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(h));
-            lo = fminf(lo, __shfl_xor_sync(FULL, lo, o));
-        }
-        if (lane == 0) sm.red[warp] = hi, sm.red[ST_WARPS + warp] = lo;
-        __syncthreads();
-        if (warp == 0) {
-            hi = lane < ST_WARPS ? sm.red[lane] : -INFINITY;
-            lo = lane < ST_WARPS ? sm.red[ST_WARPS + lane] : INFINITY;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const float h = __shfl_xor_sync(FULL, hi, o);
-                asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(h));
-                lo = fminf(lo, __shfl_xor_sync(FULL, lo, o));
-            }
-            if (lane == 0) sm.top = hi, sm.low = lo, sm.mass_min_p = 0, sm.windows = 0;
-        }
     }
-    Sampler<TX, C> s = {sm, key, key + ST_LIST, count, count + ST_BINS, count + 2 * ST_BINS, pre_count, pre_mass, row, cl,
-                        tid, rank, 0, 0, 0, false};
-    s.sync();
-    float top = -INFINITY, low = INFINITY;
+    // the order of numbers as that of whole ones, NaN (max.NaN gives the positive one) on top
+    auto up = [](float x) {
+        const unsigned b = __float_as_uint(x);
+        return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+    };
+    auto down = [](unsigned b) { return __uint_as_float(b ^ ((b >> 31) ? 0x80000000u : 0xffffffffu)); };
+    {
+        float most = mine[0];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const float h = s.at(&sm, c)->top;
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(h));
-        low = fminf(low, s.at(&sm, c)->low);
+        for (int q = 1; q < ST_OWN; ++q) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(mine[q]));
+        const unsigned h = __reduce_max_sync(FULL, up(most)), l = __reduce_min_sync(FULL, up(low));
+        if (lane == 0) sm.red[0][warp] = h, sm.red[1][warp] = l;
+    }
+    __syncthreads();
+    float top = down(__reduce_max_sync(FULL, lane < WARPS ? sm.red[0][lane] : 0u));
+    low = down(__reduce_min_sync(FULL, lane < WARPS ? sm.red[1][lane] : 0xffffffffu));
+    if (C > 1) {
+        if (tid == 0) sm.top = top, sm.low = low;
+        s.sync();
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const float h = s.at(&sm, c)->top;
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(h));
+            low = fminf(low, s.at(&sm, c)->low);
+        }
     }
     if (!(top > -INFINITY)) {  // nothing to draw from, or not a number
         if (rank == 0 && tid == 0) {
@@ -790,222 +875,155 @@ __global__ void __launch_bounds__(ST_THREADS, 2) sample_kernel(const SampleArgs 
     if (!(temperature > 0.f)) t = 1.0, top_k = 1, top_p = 1.f, min_p = 0.f;  // the largest logit, the first of equal ones
     row.top = top;
     row.inv_t = 1.0 / t;
-    row.scale = 46.166241308446828 / t;
+    row.scale = 184.66496523378731 / t;
     row.cut = (float)fmin(32.0 * t, 3e38);
     const float span = fmaxf(fminf(row.cut, top == low ? 1.f : top - low), 1e-30f);
-    row.inv_width = (float)ST_BINS / span;
+    row.inv_width = (float)(ST_BINS - 1) / span;
     const double min_weight = min_p > 0.f ? (double)fminf(min_p, 1.f) * ST_ONE : 0.0;
     const bool quick = top_k > 0 && top_k <= ST_QUICK_K;
 
+    if (top == INFINITY) {  // which cannot be subtracted
+        st_general<TX, C, NT, HELD>(row, sm, st_raw, rank, top_k, top_p, min_weight, u, a.tokens + r, a.logprob + r);
+        return;
+    }
     u64 part[5] = {};  // masses before each window, of all, and of what min-p lets stay
+    int windows = 1;
     if (quick) {
         // the bin of the k-th of the threads' largest: all that is in later bins
-        // comes behind the first k.  (Not in a bin: weighs nothing.)
-        if (row.counts(mine)) atomicAdd(s.at(&count[row.bin(mine)], 0), 1u);
+        // comes behind the first k
+#pragma unroll
+        for (int q = 0; q < ST_OWN; ++q)
+            if (top - mine[q] <= row.cut) atomicAdd(s.at(&s.count[row.bin_at(top - mine[q])], 0), 1u);
         s.sync();
         if (rank == 0) {
-            const uint4 c4 = reinterpret_cast<const uint4*>(count)[tid];
-            const unsigned c[ST_FOUR] = {c4.x, c4.y, c4.z, c4.w}, sum = c4.x + c4.y + c4.z + c4.w;
-            unsigned at = sum;
+            unsigned c[S::PER], at = 0, zero = 0, all, none;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned x = __shfl_up_sync(FULL, at, o);
-                if (lane >= o) at += x;
-            }
-            if (lane == 31) sm.warp_count[warp] = at;
+            for (int j = 0; j < S::PER; ++j) c[j] = s.count[tid * S::PER + j], at += c[j];
             if (tid == 0) sm.answer[0] = ST_BINS - 1;
-            __syncthreads();
-            at -= sum;
-            for (int w = 0; w < warp; ++w) at += sm.warp_count[w];
+            s.scan(at, zero, all, none, sm.warp_count, sm.red[0]);
 #pragma unroll
-            for (int j = 0; j < ST_FOUR; ++j) {
-                if (at < (unsigned)top_k && (unsigned)top_k <= at + c[j]) sm.answer[0] = tid * ST_FOUR + j;
+            for (int j = 0; j < S::PER; ++j) {
+                if (at < (unsigned)top_k && (unsigned)top_k <= at + c[j]) sm.answer[0] = tid * S::PER + j;
                 at += c[j];
             }
             __syncthreads();
-            if (tid < C) *s.at(&sm.window[0], tid) = {0, sm.answer[0]};
+            if (tid < C) s.at(&sm, tid)->window[0] = {0, sm.answer[0]};
         }
         s.sync();
         const int last = sm.window[0].b1;
-        s.list([&](float l) { return row.counts(l) && row.bin(l) <= last; });
+        // bins up to `last` reach half a bin behind it; with room for rounding, that is as
+        // far as a vector's largest has to be looked at
+        const float reach = last == ST_BINS - 1 ? -INFINITY : top - ((float)last + 1.f) * (span / (ST_BINS - 1)) - fabsf(top) * 1e-6f;
+        row.template each<4>([&](const float (&l)[VN], int i) {
+            float most = l[0];
+#pragma unroll
+            for (int j = 1; j < VN; ++j) most = fmaxf(most, l[j]);
+            if (most < reach) return;
+#pragma unroll
+            for (int j = 0; j < VN; ++j)
+                if (top - l[j] <= row.cut && row.bin_at(top - l[j]) <= last) s.list(l[j], i + j);
+        });
         s.sync();
     } else {
-        for (int i = tid; i < row.n; i += ST_THREADS) {
-            const float l = to_float(row.data[i]);
-            if (row.counts(l)) atomicAdd(&count[row.bin(l)], 1u);
-        }
+        row.template each<1>([&](const float (&l)[VN], int) {
+#pragma unroll
+            for (int j = 0; j < VN; ++j)
+                if (top - l[j] <= row.cut) atomicAdd(&s.count[row.bin_at(top - l[j])], 1u);
+        });
         s.sync();
         // each CTA adds up a share of the bins, into the first one's list
-        constexpr int SHARE = ST_BINS / C;
-        unsigned* total = reinterpret_cast<unsigned*>(key);
-        for (int i = tid; i < SHARE; i += ST_THREADS) {
+        unsigned* total = reinterpret_cast<unsigned*>(s.key);
+        for (int i = tid; i < S::SHARE; i += NT) {
             unsigned n = 0;
 #pragma unroll
-            for (int c = 0; c < C; ++c) n += *s.at(&count[rank * SHARE + i], c);
-            s.at(total, 0)[rank * SHARE + i] = n;
+            for (int c = 0; c < C; ++c) n += *s.at(&s.count[rank * S::SHARE + i], c);
+            s.at(total, 0)[rank * S::SHARE + i] = n;
         }
         s.sync();
-        if (rank == 0) s.choose_windows(total, span, t, top_k, top_p, min_p, u);
+        if (rank == 0) {
+            windows = s.choose_windows(total, (float)((double)(span / (ST_BINS - 1)) * row.inv_t), top_k, top_p, min_p, u);
+        }
         s.sync();
-        const int windows = sm.windows;
-        if (windows < 0) {
-            st_general<TX, C>(a, row, sm, count, r, rank, top_k, top_p, min_weight, u);
+        if (!sm.go_on) {
+            st_general<TX, C, NT, HELD>(row, sm, st_raw, rank, top_k, top_p, min_weight, u, a.tokens + r, a.logprob + r);
             return;
         }
         const Window w0 = sm.window[0], w1 = sm.window[1], w2 = sm.window[2];
-        for (int i = tid; i < row.n; i += ST_THREADS) {
-            const float l = to_float(row.data[i]);
-            if (!row.counts(l)) continue;
-            const double w = row.weight(l);
-            const u64 m = row.mass(w);
-            const int b = row.bin(l);
-            part[3] += m;
-            if (!(w < min_weight)) part[4] += m;
-            if (b < w0.b0) part[0] += m;
-            if (b < w1.b0) part[1] += m;
-            if (b < w2.b0) part[2] += m;
-            if ((w0.b0 <= b && b <= w0.b1) || (w1.b0 <= b && b <= w1.b1) || (w2.b0 <= b && b <= w2.b1)) {
-                const unsigned p = atomicAdd(&sm.listed, 1u);
-                if (p < ST_SORT) key[p] = st_key(l, row.first + i);
-            }
-        }
+        // a thread's masses add up to 2^52 at most, whole numbers, as doubles
+        double sum[5] = {};
+        auto weigh = [&](auto three) {
+            row.template each<1>([&](const float (&l)[VN], int i) {
+                double m[VN], w[VN];
+                int b[VN];
+#pragma unroll
+                for (int j = 0; j < VN; ++j) {
+                    const float g = top - l[j];
+                    const bool in = g <= row.cut;
+                    w[j] = row.weight(in ? l[j] : top);
+                    m[j] = in ? row.whole(w[j]) : 0.0;
+                    b[j] = in ? row.bin_at(g) : ST_BINS;
+                }
+#pragma unroll
+                for (int j = 0; j < VN; ++j) {
+                    sum[3] += m[j];
+                    if (!(w[j] < min_weight)) sum[4] += m[j];
+                    if (b[j] < w0.b0) sum[0] += m[j];
+                    if (b[j] < w1.b0) sum[1] += m[j];
+                    bool listed = (w0.b0 <= b[j] && b[j] <= w0.b1) || (w1.b0 <= b[j] && b[j] <= w1.b1);
+                    if (decltype(three)::value) {
+                        if (b[j] < w2.b0) sum[2] += m[j];
+                        listed |= w2.b0 <= b[j] && b[j] <= w2.b1;
+                    }
+                    if (listed) s.list(l[j], i + j);
+                }
+            });
+        };
+        if (w2.b0 < 0) weigh(std::false_type());
+        else weigh(std::true_type());
 #pragma unroll
         for (int j = 0; j < 5; ++j) {
+            // in two halves of 26 bits, which a warp's sum keeps within 32
+            const u64 x = (u64)sum[j];
+            const unsigned lo = __reduce_add_sync(FULL, (unsigned)x & 0x3ffffffu), hi = __reduce_add_sync(FULL, (unsigned)(x >> 26));
+            if (lane == 0) sm.warp_part[j][warp] = ((u64)hi << 26) + lo;
+        }
+        __syncthreads();
+        if (warp < 5) {
+            u64 x = lane < WARPS ? sm.warp_part[warp][lane] : 0;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) part[j] += __shfl_xor_sync(FULL, part[j], o);
-            if (lane == 0) atomicAdd(&sm.part[j], part[j]);
+            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(FULL, x, o);
+            if (lane == 0) sm.part[warp] = x;
         }
         s.sync();
+        if (rank == 0) {
+#pragma unroll
+            for (int j = 0; j < 5; ++j) {
+                part[j] = 0;
+#pragma unroll
+                for (int c = 0; c < C; ++c) part[j] += s.at(&sm, c)->part[j];
+            }
+            __syncthreads();
+        }
     }
     // the first CTA reads the answers off the list
     if (rank == 0) {
-        float lo[3], per[3];  // where each window begins, and its fine bins' width
-        const int windows = quick ? 1 : sm.windows, each = ST_BINS / windows;
-#pragma unroll
-        for (int j = 0; j < 3; ++j) {
-            lo[j] = (float)sm.window[j].b0;
-            per[j] = (float)each / (float)(sm.window[j].b1 - sm.window[j].b0 + 1);
-        }
-        auto window_of = [&](int b) {
-            return (windows > 1 && b >= sm.window[1].b0 ? 1 : 0) + (windows > 2 && b >= sm.window[2].b0 ? 1 : 0);
-        };
-        const int n = s.collect([&](float l) {
-            const int w = window_of(row.bin(l));
-            const float at = (fminf(row.gap(l) * row.inv_width, (float)ST_BINS) - (w == 0 ? lo[0] : w == 1 ? lo[1] : lo[2])) *
-                             (w == 0 ? per[0] : w == 1 ? per[1] : per[2]);
-            return w * each + max(0, min((int)at, each - 1));
-        });
-        bool found = n <= ST_SORT;
-        if (found) {
-            if (tid < 3) sm.prefix[tid] = ~0ull, sm.starts[tid] = 0;
-            if (!quick && tid < 5) {
-                u64 m = 0;
-                for (int c = 0; c < C; ++c) m += s.at(&sm, c)->part[tid];
-                sm.delta[tid < 3 ? tid : 0] = 0;
-                sm.warp_mass[tid] = m;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < 5; ++j) part[j] = quick ? 0 : sm.warp_mass[j];
-            __syncthreads();
-            // `run` in a row to a thread
-            const int run = (n + ST_THREADS - 1) / ST_THREADS;
-            u64 w[ST_FOUR], sum = 0;
-            int passing = 0, in[ST_FOUR];
-#pragma unroll
-            for (int j = 0; j < ST_FOUR; ++j) {
-                const int i = tid * run + j;
-                w[j] = 0, in[j] = 0;
-                if (j < run && i < n) {
-                    const float l = st_logit(key[i]);
-                    const double x = row.weight(l);
-                    w[j] = row.mass(x);
-                    if (!(x < min_weight) && (!quick || i < top_k)) passing = i + 1;
-                    in[j] = window_of(row.bin(l));
-                }
-                sum += w[j];
-            }
-            u64 upto = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 x = __shfl_up_sync(FULL, upto, o);
-                if (lane >= o) upto += x;
-            }
-            passing = __reduce_max_sync(FULL, passing);
-            if (lane == 31) sm.warp_mass[warp] = upto;
-            if (lane == 0) sm.warp_count[warp] = passing;
-            __syncthreads();
-            u64 all = 0, at = upto - sum;
-            for (int q = 0; q < ST_WARPS; ++q) {
-                if (q < warp) at += sm.warp_mass[q];
-                all += sm.warp_mass[q];
-                passing = max(passing, (int)sm.warp_count[q]);
-            }
-            // sums in the list to sums in the row: windows begin with what stands before them
-            u64 ends[ST_FOUR];
-            u64 before = at;
-#pragma unroll
-            for (int j = 0; j < ST_FOUR; ++j) {
-                const int i = tid * run + j;
-                if (j < run && i < n && (i == 0 || in[j] != window_of(row.bin(st_logit(key[i - 1])))))
-                    sm.delta[in[j]] = (quick ? 0 : part[in[j] == 0 ? 0 : in[j] == 1 ? 1 : 2]) - before, sm.starts[in[j]] = i;
-                before += w[j];
-            }
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < ST_FOUR; ++j) {
-                const int i = tid * run + j;
-                at += w[j];
-                ends[j] = at + sm.delta[in[j]];
-                if (j >= run || i >= n) ends[j] = 0, w[j] = 0;
-                else {
-                    const unsigned nth = (quick ? 0u : sm.before[in[j]]) + (unsigned)(i - sm.starts[in[j]]) + 1;
-                    if (top_k > 0 && nth == (unsigned)top_k) sm.prefix[0] = ends[j];
-                    if (quick && i + 1 == passing) sm.prefix[2] = ends[j];
-                }
-            }
-            __syncthreads();
-            u64 kept = sm.prefix[0];  // of the first k, if there are as many
-            if (kept == ~0ull) kept = quick ? all : part[3];
-            const u64 target = share_of(top_p, kept);
-#pragma unroll
-            for (int j = 0; j < ST_FOUR; ++j)
-                if (top_p < 1.f && ends[j] - w[j] < target && target <= ends[j]) sm.prefix[1] = ends[j];
-            __syncthreads();
-            if (top_p < 1.f) {
-                if (sm.prefix[1] == ~0ull) found = false;  // the window missed
-                kept = min(kept, sm.prefix[1]);
-            }
-            kept = min(kept, quick ? sm.prefix[2] : min_weight > 0 ? part[4] : ~0ull);
-            const u64 drawn = drawn_at(u, kept);
-            int here = 0;
-#pragma unroll
-            for (int j = 0; j < ST_FOUR; ++j) {
-                if (found && ends[j] - w[j] < drawn && drawn <= ends[j]) {
-                    const u64 k = key[tid * run + j];
-                    a.tokens[r] = (int64_t)(k & (ST_MAX_V - 1));
-                    a.logprob[r] = (float)(row.score(st_logit(k)) - log((double)kept / ST_ONE));
-                    here = 1;
-                }
-            }
-            if (!quick) found = __syncthreads_or(here) != 0;
-        }
+        const bool found = s.answer(windows, quick, top_k, top_p, min_weight, u, part, a.tokens + r, a.logprob + r);
         __syncthreads();
-        if (tid < C) s.at(&sm, tid)->windows = found ? 0 : -1;
+        if (tid < C) s.at(&sm, tid)->go_on = found;
     }
-    s.sync();  // no CTA leaves while another may read its shared memory
-    if (sm.windows < 0) st_general<TX, C>(a, row, sm, count, r, rank, top_k, top_p, min_weight, u);
+    s.sync();  // and no CTA leaves while another may read its shared memory
+    if (!sm.go_on) st_general<TX, C, NT, HELD>(row, sm, st_raw, rank, top_k, top_p, min_weight, u, a.tokens + r, a.logprob + r);
 }
 
-template <class TX, int C>
+template <class TX, int C, int NT, bool HELD>
 static cudaError_t sample_launch(SampleArgs a, cudaStream_t s) {
     a.slice = ((a.V + C - 1) / C + 7) & ~7;
-    const size_t smem = (ST_BINS / C + 2) * 8 + (ST_BINS / C + 4) * 4 + 3 * ST_BINS * 4 + (size_t)a.slice * sizeof(TX) + 16;
-    cudaError_t e = prepare_kernel<sample_kernel<TX, C>>(200 * 1024);
+    const size_t smem = Sampler<TX, C, NT, HELD>::BYTES + (HELD ? (size_t)a.slice * sizeof(TX) + 32 : 0);
+    cudaError_t e = prepare_kernel<sample_kernel<TX, C, NT, HELD>>(200 * 1024);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.rows * C);
-    cfg.blockDim = dim3(ST_THREADS);
+    cfg.blockDim = dim3(NT);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[2];
@@ -1017,13 +1035,14 @@ static cudaError_t sample_launch(SampleArgs a, cudaStream_t s) {
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, sample_kernel<TX, C>, a);
+    return cudaLaunchKernelEx(&cfg, sample_kernel<TX, C, NT, HELD>, a);
 }
 
 template <class TX>
 static cudaError_t sample_typed(const SampleArgs& a, cudaStream_t s) {
-    if (a.V <= 8192) return sample_launch<TX, 1>(a, s);
-    return sample_launch<TX, 8>(a, s);
+    if (a.V <= 8192) return sample_launch<TX, 1, 512, true>(a, s);
+    if (a.rows <= 32) return sample_launch<TX, 8, 1024, true>(a, s);
+    return sample_launch<TX, 1, 1024, false>(a, s);
 }
 
 }  // namespace skb
