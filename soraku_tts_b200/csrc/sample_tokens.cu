@@ -279,8 +279,9 @@ struct Sampler {
     __device__ __forceinline__ bool answer(int windows, bool first_k, int top_k, float top_p, double min_weight, float u, u64 (&part)[5],
                                            int64_t* token, float* logprob) {
         unsigned from[C], n = 0;
+        const unsigned theirs = (tid & 31) < C ? *at(&sm.listed, tid & 31) : 0;
 #pragma unroll
-        for (int r = 0; r < C; ++r) from[r] = *at(&sm.listed, r);
+        for (int r = 0; r < C; ++r) from[r] = __shfl_sync(FULL, theirs, r);
 #pragma unroll
         for (int r = 0; r < C; ++r) {
             const unsigned x = from[r];
@@ -856,12 +857,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     if (C > 1) {
         if (tid == 0) sm.top = top, sm.low = low;
         s.sync();
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const float h = s.at(&sm, c)->top;
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(h));
-            low = fminf(low, s.at(&sm, c)->low);
-        }
+        // a lane for each CTA: a peer's memory is asked once a warp
+        top = down(__reduce_max_sync(FULL, lane < C ? up(s.at(&sm, lane)->top) : 0u));
+        low = down(__reduce_min_sync(FULL, lane < C ? up(s.at(&sm, lane)->low) : 0xffffffffu));
     }
     if (!(top > -INFINITY)) {  // nothing to draw from, or not a number
         if (rank == 0 && tid == 0) {
@@ -996,12 +994,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         }
         s.sync();
         if (rank == 0) {
+            if (warp < 5) {
+                u64 x = lane < C ? s.at(&sm, lane)->part[warp] : 0;
 #pragma unroll
-            for (int j = 0; j < 5; ++j) {
-                part[j] = 0;
-#pragma unroll
-                for (int c = 0; c < C; ++c) part[j] += s.at(&sm, c)->part[j];
+                for (int o = 1; o < C; o <<= 1) x += __shfl_xor_sync(FULL, x, o);
+                if (lane == 0) sm.warp_part[0][warp] = x;
             }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 5; ++j) part[j] = sm.warp_part[0][j];
             __syncthreads();
         }
     }
