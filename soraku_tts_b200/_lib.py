@@ -139,6 +139,28 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_bind = None
+
+
+def bind():
+    """The short way (csrc/bind.cpp) to the functions that a decoding step calls
+    most: loaded once, and given their addresses.  Raises if it has not been built."""
+    global _bind
+    if _bind is None:
+        import torch  # noqa: F401 - its libraries come first
+
+        try:
+            from . import _bind as module
+        except ImportError as e:
+            raise RuntimeError(
+                f"{os.path.join(HERE, '_bind.so')} is missing or does not fit this torch: build it with "
+                "`python -c 'import __graft_entry__ as g; g.build()'`") from e
+        names = ("skb_quantize_rows", "skb_int8_workspace", "skb_int8_linear", "skb_int8_swiglu", "skb_sample_tokens")
+        module.connect(*(ctypes.cast(getattr(lib(), n), c_void_p).value for n in names))
+        _bind = module
+    return _bind
+
+
 def last_error() -> str:
     msg = lib().skb_last_error()
     return msg.decode() if msg else ""

@@ -1,8 +1,9 @@
-"""Build libsoraku_b200.so (sm_100a) in-tree with nvcc.
+"""Build libsoraku_b200.so (sm_100a) in-tree with nvcc, and _bind.so with g++.
 
 Each .cu under csrc/ compiles to an object in _build/ (in parallel), then
 nvcc links the shared library next to this file.  Objects are rebuilt when
-their source or any header changed.
+their source or any header changed.  _bind.so (csrc/bind.cpp) is the short way
+from Python to some of the library's functions; it uses torch's own libraries.
 """
 
 from __future__ import annotations
@@ -17,9 +18,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libsoraku_b200.so")
+BIND = os.path.join(HERE, "_bind.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+CXX = os.environ.get("CXX", "g++")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I", INCLUDE]
 
@@ -44,6 +47,27 @@ def _compile(src: str, hdr_mtime: float, verbose: bool) -> str:
     return obj
 
 
+def _build_bind(force: bool) -> None:
+    import sysconfig
+
+    import torch
+
+    src = os.path.join(CSRC, "bind.cpp")
+    needs = [src, os.path.join(INCLUDE, "soraku_b200.h"), torch.__file__]
+    if not force and os.path.exists(BIND) and os.path.getmtime(BIND) >= max(os.path.getmtime(p) for p in needs):
+        return
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(NVCC)))
+    system = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+              os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", INCLUDE, *(f"-isystem{p}" for p in system), src, "-o", BIND, "-L", os.path.join(root, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for {src}:\n{res.stdout}\n{res.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
@@ -51,8 +75,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if force:
         for o in glob.glob(os.path.join(BUILD, "*.o")):
             os.remove(o)
-    with ThreadPoolExecutor(max_workers=max(1, min(len(srcs), os.cpu_count() or 4))) as ex:
+    with ThreadPoolExecutor(max_workers=max(1, min(len(srcs) + 1, os.cpu_count() or 4))) as ex:
+        bind = ex.submit(_build_bind, force)
         objs = list(ex.map(lambda s: _compile(s, hdr, verbose), srcs))
+    bind.result()
     newest = max(os.path.getmtime(o) for o in objs)
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < newest:
         cmd = [NVCC, *ARCH, "-shared", "-o", LIB, *objs]

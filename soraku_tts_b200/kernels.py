@@ -443,6 +443,10 @@ def quantize_rows(x: torch.Tensor, *, norm_weight: torch.Tensor | None = None, e
     a scale each: weights once, one row a channel, or activations that several
     products share.  With ``norm_weight`` [K] the rows are RMS-normed first; see
     skb_quantize_rows in include/soraku_b200.h."""
+    done = _lib.bind().quantize(x, norm_weight, eps)
+    if done is not None:
+        return Int8Rows(*done)
+    # rows that are out of the ordinary, or refused
     rows, k = _dims(x, "x", 2, "[rows, K]")
     device = x.get_device()
     _rows(x, "x", device)
@@ -463,6 +467,8 @@ def quantize_rows(x: torch.Tensor, *, norm_weight: torch.Tensor | None = None, e
 
 
 def _int8_product(name, x, weights, norm_weight, eps, bias, residual, out_dtype, out):
+    """A product that is out of the ordinary (one row of weights, another device
+    than the current one, nothing to do), or refused: what is wrong with it."""
     if isinstance(x, torch.Tensor):
         codes, scale = x, None
         rows, k = _dims(x, "x", 2, "[tokens, K]")
@@ -538,6 +544,9 @@ def int8_linear(x, weight, *, norm_weight: torch.Tensor | None = None, eps: floa
     ``quantize_rows``.  ``bias`` FP32 [N], ``residual`` [tokens, N] of the output's
     type.  Returns [tokens, N] in ``out_dtype`` (default: x's type, FP32 for
     codes), ``out`` if given, which may be ``residual`` and no other input."""
+    done = _lib.bind().product(x, weight, None, norm_weight, eps, bias, residual, out_dtype, out)
+    if done is not None:
+        return done
     return _int8_product("skb_int8_linear", x, ((weight, "weight"),), norm_weight, eps, bias, residual, out_dtype, out)
 
 
@@ -545,6 +554,9 @@ def int8_swiglu(x, gate, up, *, norm_weight: torch.Tensor | None = None, eps: fl
                 out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``silu(x @ gate.T) * (x @ up.T)`` in 8-bit integers, with ``gate`` and
     ``up`` Int8Rows [I, K]; the rest as in ``int8_linear``."""
+    done = _lib.bind().product(x, gate, up, norm_weight, eps, None, None, out_dtype, out) if up is not None else None
+    if done is not None:
+        return done
     return _int8_product("skb_int8_swiglu", x, ((gate, "gate"), (up, "up")), norm_weight, eps, None, None, out_dtype, out)
 
 
@@ -556,6 +568,10 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     ``top_k`` int32) with every row's own.  ``cfg_sample`` draws in the same order.
     Returns (tokens int64 [rows], -1 for a row with nothing to draw from; the
     logarithm of each token's probability among the kept ones, FP32 [rows])."""
+    done = _lib.bind().sample(logits, uniform, temperature, top_k, top_p, min_p)
+    if done is not None:
+        return done
+    # rows that are out of the ordinary, or refused
     rows, vocab = _dims(logits, "logits", 2, "[rows, V]")
     device = logits.get_device()
     _rows(logits, "logits", device)
