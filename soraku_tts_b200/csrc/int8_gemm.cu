@@ -42,7 +42,7 @@ struct GemmShape {
     static constexpr int COLS = PARTS * TN;       // of one accumulator
     static constexpr int TMEM = 2 * COLS < 32 ? 32 : 2 * COLS;
     static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE;
-    static constexpr bool SPLITS = COLS * 512 <= STAGES * STAGE;  // sums fit the ring
+    static_assert(COLS * 512 <= STAGES * STAGE, "a split's sums fit the ring");
 };
 
 struct GemmShared {
@@ -348,8 +348,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 gm_encoder() {
     return f;
 }
 
-// Rows of K bytes, boxes of 128 bytes x `box` rows, 128-byte swizzle, zeros outside.
-static bool gm_map(CUtensorMap* m, const void* p, int K, int rows, long long ld, int box) {
+bool int8_map(CUtensorMap* m, const void* p, int K, int rows, long long ld, int box) {
     const PFN_cuTensorMapEncodeTiled_v12000 encode = gm_encoder();
     if (!encode) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
@@ -360,28 +359,34 @@ static bool gm_map(CUtensorMap* m, const void* p, int K, int rows, long long ld,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool out_map(CUtensorMap* m, void* p, int type, int N, int T, long long ld, int tokens) {
+    const PFN_cuTensorMapEncodeTiled_v12000 encode = gm_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)T};
+    const cuuint64_t strides[1] = {(cuuint64_t)(ld * type_size(type))};
+    const cuuint32_t size[2] = {32, (cuuint32_t)tokens}, es[2] = {1, 1};
+    return encode(m, type == SKB_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                     : type == SKB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  2, p, dims, strides, size, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int TN, bool GLU, class TO>
-static cudaError_t gemm_launch(const Int8Args& a, bool early, cudaStream_t s) {
+static cudaError_t gemm_launch(const Int8Args& a, int split, bool early, cudaStream_t s) {
     using S = GemmShape<TN, GLU>;
     const cudaError_t e = prepare_kernel<int8_gemm_kernel<TN, GLU, TO>>(S::SMEM);
     if (e != cudaSuccess) return e;
     GemmMaps maps;
-    if (!gm_map(&maps.x, a.in.x, a.in.K, a.in.T, a.in.ld, TN) || !gm_map(&maps.w[0], a.w[0], a.in.K, a.N, a.ldw[0], 128))
+    if (!int8_map(&maps.x, a.in.x, a.in.K, a.in.T, a.in.ld, TN) || !int8_map(&maps.w[0], a.w[0], a.in.K, a.N, a.ldw[0], 128))
         return cudaErrorNotSupported;
     if (GLU) {
-        if (!gm_map(&maps.w[1], a.w[1], a.in.K, a.N, a.ldw[1], 128)) return cudaErrorNotSupported;
+        if (!int8_map(&maps.w[1], a.w[1], a.in.K, a.N, a.ldw[1], 128)) return cudaErrorNotSupported;
     } else {
         maps.w[1] = maps.w[0];
     }
     constexpr int SMS = 148;
     const long long tiles = (long long)((a.N + 127) / 128) * ((a.in.T + TN - 1) / TN);
-    const int blocks = (a.in.K + 127) / 128;
-    int split = 1;
-    if (S::SPLITS && tiles * 2 <= SMS) {
-        split = (int)(SMS / tiles);
-        if (split > blocks) split = blocks;
-        if (split > GM_MAX_SPLIT) split = GM_MAX_SPLIT;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < SMS ? tiles : SMS));
     cfg.blockDim = dim3(GM_THREADS);
@@ -399,21 +404,78 @@ static cudaError_t gemm_launch(const Int8Args& a, bool early, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, int8_gemm_kernel<TN, GLU, TO>, a, maps, split, early);
 }
 
-// Tiles as narrow as lets all of them run at once: the weights are read again
-// for each from L2, which costs less than SMs that stand idle.
+// How many clusters of `split` CTAs run at once on the current device.
+template <int TN, bool GLU, class TO>
+static int clusters_at_once(int split) {
+    static std::atomic<int> known[64][GM_MAX_SPLIT + 1];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    const int k = known[dev][split].load(std::memory_order_relaxed);
+    if (k > 0) return k - 1;
+    using S = GemmShape<TN, GLU>;
+    if (prepare_kernel<int8_gemm_kernel<TN, GLU, TO>>(S::SMEM) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split);
+    cfg.blockDim = dim3(GM_THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = split;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, int8_gemm_kernel<TN, GLU, TO>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    known[dev][split].store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+
+// Tile width and split of K, of those that run at once: the least time by what was
+// measured at 9 to 512 tokens, 1024 to 4096 channels and K of 1024 to 8192 (us):
+// 0.22 + TN / 1000 a block of K, half as much again with two weights; a split costs
+// 0.5 and 0.025 a token to hand sums over, which is a tenth of that without.  False if
+// nothing fits: then tiles are as wide as they get, and CTAs take them in turn.
+template <class TO, bool GLU>
+static bool gemm_choose(const Int8Args& a, int& width, int& split) {
+    const long long cols = (a.N + 127) / 128;
+    const int blocks = (a.in.K + 127) / 128, T = a.in.T;
+    float best = 3e38f;
+    auto look = [&](int tn, int at_once, int s) {
+        const long long tiles = cols * ((T + tn - 1) / tn);
+        if (s > blocks || tiles > at_once) return;
+        const float t = (float)((blocks + s - 1) / s) * (0.22f + 0.001f * tn) * (GLU ? 1.5f : 1.f) +
+                        (s > 1 ? 0.5f + 0.025f * (float)(T < tn ? T : tn) * (GLU ? 2 : 1) : 0.004f * (float)(T < tn ? T : tn));
+        if (t < best) best = t, width = tn, split = s;
+    };
+    look(32, 148, 1), look(64, 148, 1), look(128, 148, 1);
+    for (int s = 2; s <= GM_MAX_SPLIT; s *= 2) {
+        if (cols * s > 148) break;
+        look(32, clusters_at_once<32, GLU, TO>(s), s);
+        look(64, clusters_at_once<64, GLU, TO>(s), s);
+        look(128, clusters_at_once<128, GLU, TO>(s), s);
+    }
+    return best < 3e38f;
+}
+
 template <class TO>
 static cudaError_t gemm_typed(const Int8Args& a, bool glu, bool early, cudaStream_t s) {
-    const long long cols = (a.N + 127) / 128;
-    auto fits = [&](int tn) { return cols * ((a.in.T + tn - 1) / tn) <= 148; };
-    if (glu) {
-        if (fits(32)) return gemm_launch<32, true, TO>(a, early, s);
-        if (fits(64)) return gemm_launch<64, true, TO>(a, early, s);
-        return gemm_launch<128, true, TO>(a, early, s);
+    int width = 0, split = 1;
+    if (glu ? gemm_choose<TO, true>(a, width, split) : gemm_choose<TO, false>(a, width, split)) {
+        if (glu) {
+            if (width == 32) return gemm_launch<32, true, TO>(a, split, early, s);
+            if (width == 64) return gemm_launch<64, true, TO>(a, split, early, s);
+            return gemm_launch<128, true, TO>(a, split, early, s);
+        }
+        if (width == 32) return gemm_launch<32, false, TO>(a, split, early, s);
+        if (width == 64) return gemm_launch<64, false, TO>(a, split, early, s);
+        return gemm_launch<128, false, TO>(a, split, early, s);
     }
-    if (fits(32)) return gemm_launch<32, false, TO>(a, early, s);
-    if (fits(64)) return gemm_launch<64, false, TO>(a, early, s);
-    if (fits(128)) return gemm_launch<128, false, TO>(a, early, s);
-    return gemm_launch<256, false, TO>(a, early, s);
+    if (int8_wide_serves(a)) return int8_wide_launch(a, glu, early, s);
+    return glu ? gemm_launch<128, true, TO>(a, 1, early, s) : gemm_launch<256, false, TO>(a, 1, early, s);
 }
 
 // Rows as codes; early: see int8_gemv_launch.

@@ -13,6 +13,7 @@
 // is FP32 from there, rounded once to the output's type.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -67,6 +68,12 @@ cudaError_t prepare_kernel(size_t dyn_bytes) {
 }
 
 cudaError_t quantize_launch(const RowsIn& in, int8_t* q, long long ldq, float* scale, cudaStream_t s);
+// Tensor maps: rows of K bytes in boxes of 128 bytes x `box` rows, 128-byte swizzle,
+// zeros outside; an output in boxes of 32 columns x `tokens` rows.
+bool int8_map(CUtensorMap* m, const void* p, int K, int rows, long long ld, int box);
+bool out_map(CUtensorMap* m, void* p, int type, int N, int T, long long ld, int tokens);
+bool int8_wide_serves(const Int8Args& a);
+cudaError_t int8_wide_launch(const Int8Args& a, bool glu, bool early, cudaStream_t s);
 constexpr int I8_FEW = 8;  // tokens that int8_gemv.cu serves
 bool int8_gemv_fuses(int T, int K);
 cudaError_t int8_gemv_launch(const Int8Args& a, bool glu, bool early, cudaStream_t s);

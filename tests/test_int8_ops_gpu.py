@@ -188,6 +188,27 @@ def test_linear_at_size(K, t, n, k):
     check_linear(K, t, n, k, "bf16", residual=True, out_dtype="f32")
 
 
+# more tiles than SMs: pairs of CTAs, with edges in every direction, and outputs off and on 16 bytes
+@pytest.mark.parametrize("t,n,k", [(1500, 2048, 1024), (2111, 2052, 1000), (1281, 2304, 130), (1300, 2049, 256), (6541, 1024, 64),
+                                   (300, 20008, 96)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_linear_of_many_tiles(K, t, n, k, dtype):
+    check_linear(K, t, n, k, dtype, norm=True, bias=True)
+    check_linear(K, t, n, k, dtype, codes=True)
+    check_linear(K, t, n, k, dtype, residual=True, in_place=n % 8 == 0)
+
+
+@pytest.mark.parametrize("t,n,k", [(1500, 1536, 1024), (2111, 1028, 1000), (1281, 2001, 130), (5003, 520, 64)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_swiglu_of_many_tiles(K, t, n, k, dtype):
+    check_swiglu(K, t, n, k, dtype, norm=True)
+    check_swiglu(K, t, n, k, dtype, codes=True)
+    wide = torch.full((t + 1, n + 24), 7.0, device="cuda").to(DT[dtype])
+    check_swiglu(K, t, n, k, dtype, out=wide[:t, 8:8 + n])
+    wide[:t, 8:8 + n] = 7.0
+    assert (wide == 7.0).all()
+
+
 def test_the_largest_sums_are_exact(K):
     """All codes at their ends: sums near 2^31, which FP32 or a 16-bit step on the way would not hold."""
     for t in (1, 5, 33, 140):
@@ -285,6 +306,8 @@ def test_a_row_goes_by_itself(K):
     """A token's result is the same in any batch, to the bit, when it comes as codes."""
     x, w = K.quantize_rows(rows_in((300, 512), 3, torch.float32)), weights(200, 512, 4)
     whole, glu = K.int8_linear(x, w), K.int8_swiglu(x, w, w)
+    more = K.Int8Rows(x.q.repeat(40, 1), x.scale.repeat(40))
+    assert torch.equal(K.int8_linear(more, w), whole.repeat(40, 1)) and torch.equal(K.int8_swiglu(more, w, w), glu.repeat(40, 1))
     for a, b in ((0, 1), (5, 7), (10, 26), (0, 100), (17, 217)):
         part = K.Int8Rows(x.q[a:b], x.scale[a:b])
         assert torch.equal(K.int8_linear(part, w), whole[a:b])
