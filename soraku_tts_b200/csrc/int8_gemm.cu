@@ -114,66 +114,71 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
     volatile int* abort = &sm.abort;
 
     const int tiles_n = (a.N + 127) / 128, tiles_t = (a.in.T + TN - 1) / TN;
-    const long long tiles = (long long)tiles_n * tiles_t;
+    const int tiles = tiles_n * tiles_t;  // the launch has seen that they are fewer than 2^30
     const int blocks = (a.in.K + 127) / 128;
     const int z = blockIdx.x % split;  // rank in the cluster
     const int k0 = (int)((long long)z * blocks / split), k1 = (int)((long long)(z + 1) * blocks / split);
-    const long long first = blockIdx.x / split, step = gridDim.x / split;
+    const int first = blockIdx.x / split, step = gridDim.x / split;
     // blocks whose weights are asked for before the wait
     int ahead = 0;
-    auto load_w = [&](long long tile, int kb, uint32_t at, uint64_t* bar) {
-        const int n0 = (int)(tile % tiles_n) * 128;
+    auto load_w = [&](int n0, int kb, uint32_t at, uint64_t* bar) {
         gm_load(at, &maps.w[0], kb * 128, n0, bar);
         if (GLU) gm_load(at + S::A_BYTES, &maps.w[1], kb * 128, n0, bar);
     };
     if (early && tid == 0 && first < tiles) {
         for (; ahead < S::STAGES && k0 + ahead < k1; ++ahead) {
             mbar_expect_tx(&sm.full[ahead], S::STAGE);
-            load_w(first, k0 + ahead, ring + ahead * S::STAGE, &sm.full[ahead]);
+            load_w(first % tiles_n * 128, k0 + ahead, ring + ahead * S::STAGE, &sm.full[ahead]);
         }
     }
     pdl_wait();
     pdl_trigger();
 
+    // One thread issues a copy or a product, against whatever the other warps run: no
+    // division on its way, stages and phases are counted along.
     if (warp == 0) {
         if (lane == 0) {
-            long long it = 0;
+            int s = 0, asked = 0;  // stage; blocks asked for, of the first round alone
+            uint32_t phase = 1;    // of the ring's barriers: the first round waits for nothing
             bool go = true;
-            for (long long tile = first; tile < tiles && go; tile += step) {
-                const int t0 = (int)(tile / tiles_n) * TN;
-                for (int kb = k0; kb < k1; ++kb, ++it) {
-                    const int s = (int)(it % S::STAGES);
-                    if (it >= S::STAGES && !ut_wait(&sm.empty[s], (uint32_t)(it / S::STAGES - 1) & 1u, abort)) {
+            for (int tile = first; tile < tiles && go; tile += step) {
+                const int n0 = tile % tiles_n * 128, t0 = tile / tiles_n * TN;
+                for (int kb = k0; kb < k1; ++kb) {
+                    if (asked >= S::STAGES && !ut_wait(&sm.empty[s], phase, abort)) {
                         go = false;
                         break;
                     }
                     const uint32_t at = ring + s * S::STAGE;
-                    if (it >= ahead) {
+                    if (asked >= ahead) {
                         mbar_expect_tx(&sm.full[s], S::STAGE);
-                        load_w(tile, kb, at, &sm.full[s]);
+                        load_w(n0, kb, at, &sm.full[s]);
                     }
                     gm_load(at + S::PARTS * S::A_BYTES, &maps.x, kb * 128, t0, &sm.full[s]);
+                    asked = min(asked + 1, S::STAGES);
+                    if (++s == S::STAGES) s = 0, phase ^= 1;
                 }
             }
             // no copy may land after the CTA has gone: the MMAs wait for each of
-            // them; where those gave up, wait here
+            // them; where those gave up, wait here, from the oldest on
             if (*abort)
-                for (long long i = it > S::STAGES ? it - S::STAGES : 0; i < it; ++i)
-                    mbar_wait(&sm.full[i % S::STAGES], (uint32_t)(i / S::STAGES) & 1u, nullptr);
+                for (int i = 0; i < asked; ++i) {
+                    const bool wrapped = asked == S::STAGES && s + i >= S::STAGES;
+                    const int at = asked < S::STAGES ? i : (wrapped ? s + i - S::STAGES : s + i);
+                    mbar_wait(&sm.full[at], asked < S::STAGES ? 0u : (wrapped ? phase ^ 1 : phase), nullptr);
+                }
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            long long it = 0;
-            int i = 0;
+            int s = 0, i = 0;
+            uint32_t phase = 0;
             bool go = true;
-            for (long long tile = first; tile < tiles && go; tile += step, ++i) {
+            for (int tile = first; tile < tiles && go; tile += step, ++i) {
                 const int b = i & 1;
                 if (i >= 2 && !ut_wait(&sm.acc_free[b], (uint32_t)((i >> 1) - 1) & 1u, abort)) break;
                 ut_fence_after();
                 const uint32_t d = tmem + b * S::COLS;
-                for (int kb = k0; kb < k1; ++kb, ++it) {
-                    const int s = (int)(it % S::STAGES);
-                    if (!ut_wait(&sm.full[s], (uint32_t)(it / S::STAGES) & 1u, abort)) {
+                for (int kb = k0; kb < k1; ++kb) {
+                    if (!ut_wait(&sm.full[s], phase, abort)) {
                         go = false;
                         break;
                     }
@@ -187,6 +192,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
                             gm_mma(d + p * TN, ut_desc(at + p * S::A_BYTES, k * 32, false), x, gm_idesc(TN), kb > k0 || k > 0);
                     }
                     ut_commit(&sm.empty[s]);
+                    if (++s == S::STAGES) s = 0, phase ^= 1;
                 }
                 if (go) ut_commit(&sm.acc_full[b]);
             }
@@ -202,8 +208,8 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
         constexpr int CH = TN / 2 < 32 ? TN / 2 : 32;  // columns at a time
         float* sx = sm.sx[warp - 4];
         int i = 0;
-        for (long long tile = first; tile < tiles; tile += step, ++i) {
-            const int n = (int)(tile % tiles_n) * 128 + 32 * q + lane, t0 = (int)(tile / tiles_n) * TN + half * (TN / 2);
+        for (int tile = first; tile < tiles; tile += step, ++i) {
+            const int n = tile % tiles_n * 128 + 32 * q + lane, t0 = tile / tiles_n * TN + half * (TN / 2);
             const int b = i & 1;
             const bool in = n < a.N;
             const float s0 = in ? __ldcg(a.ws[0] + n) : 0.f, s1 = GLU && in ? __ldcg(a.ws[1] + n) : 0.f;
@@ -273,7 +279,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
     if (split > 1) {
         __syncwarp();
         gm_cluster_sync();
-        const int n0 = (int)(first % tiles_n) * 128, t0 = (int)(first / tiles_n) * TN;
+        const int n0 = first % tiles_n * 128, t0 = first / tiles_n * TN;
         if (warp >= 4) {
             bool bad = false;
             for (int p = 0; p < split; ++p) bad |= gm_peer_load(gm_peer(smem_u32(&sm.abort), p)) != 0;
@@ -387,6 +393,7 @@ static cudaError_t gemm_launch(const Int8Args& a, int split, bool early, cudaStr
     }
     constexpr int SMS = 148;
     const long long tiles = (long long)((a.N + 127) / 128) * ((a.in.T + TN - 1) / TN);
+    if (tiles >= 1 << 30) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < SMS ? tiles : SMS));
     cfg.blockDim = dim3(GM_THREADS);

@@ -257,13 +257,20 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
 __device__ __forceinline__ float finish(int sum, float sx, float sw, float bias) {
     return fmaf(__fmul_rn((float)sum, sx), sw, bias);
 }
+// (float)v without the conversion unit, which a SwiGLU's exponentials and
+// reciprocals share: two exact halves, rounded as they are joined.
+__device__ __forceinline__ float whole_to_float(int v) {
+    const float hi = __fsub_rn(__int_as_float(0x4b400000 + (v >> 16)), 12582912.f);
+    const float lo = __fsub_rn(__int_as_float(0x4b000000 | (v & 0xffff)), 8388608.f);
+    return fmaf(hi, 65536.f, lo);
+}
 // silu by the hardware's exponential and reciprocal: each is within 2^-22 of
 // its value, where the product's own roundings are 2^-22 already, and the
 // argument's rounding counts |g| 2^-24, as that of g itself does.  (The exact
 // ones took 30 instructions more of each result.)
 __device__ __forceinline__ float finish_glu(int gate, int up, float sx, float sg, float su) {
     const float g = finish(gate, sx, sg, 0.f);
-    return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, __expf(-g))), finish(up, sx, su, 0.f));
+    return __fmul_rn(__fdividef(g, __fadd_rn(1.0f, __expf(-g))), fmaf(__fmul_rn(whole_to_float(up), sx), su, 0.f));
 }
 
 template <class T>

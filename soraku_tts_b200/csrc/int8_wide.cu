@@ -7,9 +7,9 @@
 // CTA holds its own 128 weight rows and half of the tokens, 32 KB a stage.
 //
 // Warps of each CTA: 0 copies (into its own memory, on the first CTA's barriers), 1 of
-// the first CTA issues the products for both, 4-11 finish one tile while the next
+// the first CTA issues the products for both, 4-19 finish one tile while the next
 // is added up.  A thread of these holds a channel; its results go to shared memory,
-// 32 channels x 32 tokens a warp, and out by TMA, which knows the output's edges.
+// 32 channels x 16 tokens a warp, and out by TMA, which knows the output's edges.
 // For SwiGLU a CTA's rows are 64 of the gate and the same 64 of up: the warps of a
 // gate row and of its up row hand each other half of their tokens.
 #include <cudaTypedefs.h>
@@ -21,7 +21,8 @@
 
 namespace skb {
 
-constexpr int WD_THREADS = 384, WD_EPI_WARPS = 8;
+constexpr int WD_THREADS = 640, WD_EPI_WARPS = 16;
+constexpr int WD_CH = 16;  // tokens a warp takes at a time
 constexpr int WD_STAGE = 32 * 1024, WD_A = 16 * 1024;
 constexpr int WD_MAX_STAGES = 6;
 
@@ -31,20 +32,20 @@ struct WideMaps {
 
 template <bool GLU, class TO>
 struct WideShape {
-    static constexpr int TOKENS = GLU ? 16 : 32;                     // of one store
+    static constexpr int TOKENS = GLU ? WD_CH / 2 : WD_CH;           // of one store
     static constexpr int OUT = 32 * TOKENS * (int)sizeof(TO);        // bytes of one store
-    static constexpr int SWAP = GLU ? 16 * 32 * 4 : 0;               // sums for the other warp
+    static constexpr int SWAP = GLU ? WD_CH / 2 * 32 * 4 : 0;        // sums for the other warp
     static constexpr int WARP = 2 * OUT + 2 * SWAP;
     static constexpr int STAGES = (224 * 1024 - WD_EPI_WARPS * WARP) / WD_STAGE;
     static constexpr size_t SMEM = 1024 + (size_t)STAGES * WD_STAGE + WD_EPI_WARPS * WARP;
-    static_assert(STAGES <= WD_MAX_STAGES && STAGES >= 4 && WARP % 1024 == 0, "ring");
+    static_assert(STAGES <= WD_MAX_STAGES && STAGES >= 4 && WARP % 512 == 0, "ring");
 };
 
 struct WideShared {
     uint64_t full[WD_MAX_STAGES], empty[WD_MAX_STAGES], acc_full[2], acc_free[2];
     uint32_t tmem;
     int abort;
-    alignas(16) float sx[WD_EPI_WARPS][32];  // scales of a warp's tokens, read four at a time
+    alignas(16) float sx[WD_EPI_WARPS][WD_CH];  // scales of a warp's tokens, read four at a time
 };
 static_assert(offsetof(WideShared, sx) % 16 == 0, "16-byte reads");
 
@@ -82,8 +83,10 @@ __device__ __forceinline__ uint32_t wd_peer(uint32_t addr, int rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// What it hands over is tensor memory, behind tcgen05's own fence: a release to the
+// cluster would wait for all stores on their way (1900 cycles a tile).
 __device__ __forceinline__ void wd_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void wd_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -122,12 +125,11 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
 
     constexpr int COLS = GLU ? 128 : 256;  // output columns of a tile
     const int tiles_n = (a.N + COLS - 1) / COLS, tiles_t = (a.in.T + 255) / 256;
-    const long long tiles = (long long)tiles_n * tiles_t;
+    const int tiles = tiles_n * tiles_t;  // the launch has seen that they are fewer than 2^30
     const int blocks = (a.in.K + 127) / 128;
-    const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
     const uint32_t full0 = wd_peer(smem_u32(&sm.full[0]), 0);  // the first CTA's
-    auto load_w = [&](long long tile, int kb, int s) {
-        const int n0 = (int)(tile % tiles_n) * COLS + rank * (COLS / 2);
+    auto load_w = [&](int n0, int kb, int s) {
         const uint32_t at = ring + s * WD_STAGE;
         if (GLU) {
             wd_load(at, &maps.w[0], kb * 128, n0, full0 + s * 8);
@@ -141,48 +143,54 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
     if (early && tid == 0 && first < tiles)
         for (; ahead < S::STAGES && ahead < blocks; ++ahead) {
             if (rank == 0) mbar_expect_tx(&sm.full[ahead], 2 * WD_STAGE);
-            load_w(first, ahead, ahead);
+            load_w(first % tiles_n * COLS + rank * (COLS / 2), ahead, ahead);
         }
     pdl_wait();
     pdl_trigger();
 
+    // One thread issues a copy or a product, against whatever the other warps run: no
+    // division on its way, stages and phases are counted along.
     if (warp == 0) {
         if (lane == 0) {
-            long long it = 0;
+            int s = 0, asked = 0;  // stage; blocks asked for, of the first round alone
+            uint32_t phase = 1;    // of the ring's barriers: the first round waits for nothing
             bool go = true;
-            for (long long tile = first; tile < tiles && go; tile += step) {
-                const int t0 = (int)(tile / tiles_n) * 256 + rank * 128;
-                for (int kb = 0; kb < blocks; ++kb, ++it) {
-                    const int s = (int)(it % S::STAGES);
-                    if (it >= S::STAGES && !ut_wait(&sm.empty[s], (uint32_t)(it / S::STAGES - 1) & 1u, abort)) {
+            for (int tile = first; tile < tiles && go; tile += step) {
+                const int n0 = tile % tiles_n * COLS + rank * (COLS / 2), t0 = tile / tiles_n * 256 + rank * 128;
+                for (int kb = 0; kb < blocks; ++kb) {
+                    if (asked >= S::STAGES && !ut_wait(&sm.empty[s], phase, abort)) {
                         go = false;
                         break;
                     }
-                    if (it >= ahead) {
+                    if (asked >= ahead) {
                         if (rank == 0) mbar_expect_tx(&sm.full[s], 2 * WD_STAGE);
-                        load_w(tile, kb, s);
+                        load_w(n0, kb, s);
                     }
                     wd_load(ring + s * WD_STAGE + WD_A, &maps.x, kb * 128, t0, full0 + s * 8);
+                    asked = min(asked + 1, S::STAGES);
+                    if (++s == S::STAGES) s = 0, phase ^= 1;
                 }
             }
             // no copy may land after the CTAs have gone: the products wait for each of
-            // them; where those gave up, wait here
+            // them; where those gave up, wait here, from the oldest on
             if (*abort && rank == 0)
-                for (long long i = it > S::STAGES ? it - S::STAGES : 0; i < it; ++i)
-                    mbar_wait(&sm.full[i % S::STAGES], (uint32_t)(i / S::STAGES) & 1u, nullptr);
+                for (int i = 0; i < asked; ++i) {
+                    const bool wrapped = asked == S::STAGES && s + i >= S::STAGES;
+                    const int at = asked < S::STAGES ? i : (wrapped ? s + i - S::STAGES : s + i);
+                    mbar_wait(&sm.full[at], asked < S::STAGES ? 0u : (wrapped ? phase ^ 1 : phase), nullptr);
+                }
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
-            long long it = 0;
-            int i = 0;
+            int s = 0, i = 0;
+            uint32_t phase = 0;
             bool go = true;
-            for (long long tile = first; tile < tiles && go; tile += step, ++i) {
+            for (int tile = first; tile < tiles && go; tile += step, ++i) {
                 const int b = i & 1;
                 if (i >= 2 && !ut_wait(&sm.acc_free[b], (uint32_t)((i >> 1) - 1) & 1u, abort)) break;
                 ut_fence_after();
-                for (int kb = 0; kb < blocks; ++kb, ++it) {
-                    const int s = (int)(it % S::STAGES);
-                    if (!ut_wait(&sm.full[s], (uint32_t)(it / S::STAGES) & 1u, abort)) {
+                for (int kb = 0; kb < blocks; ++kb) {
+                    if (!ut_wait(&sm.full[s], phase, abort)) {
                         go = false;
                         break;
                     }
@@ -192,6 +200,7 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
                     for (int k = 0; k < 4; ++k)
                         wd_mma(tmem + b * 256, ut_desc(at, k * 32, false), ut_desc(at + WD_A, k * 32, false), kb > 0 || k > 0);
                     wd_commit(&sm.empty[s]);
+                    if (++s == S::STAGES) s = 0, phase ^= 1;
                 }
                 if (go) wd_commit(&sm.acc_full[b]);
             }
@@ -202,8 +211,8 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
             }
         }
     } else if (warp >= 4) {
-        const int e = warp - 4, q = e & 3, half = e >> 2;
-        const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + half * 128;
+        const int e = warp - 4, q = e & 3, part = e >> 2;  // lanes 32 q, tokens 64 part of the tile
+        const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16) + part * 64;
         unsigned char* mine = base + S::STAGES * WD_STAGE + e * S::WARP;
         TO* stage = reinterpret_cast<TO*>(mine);
         int* give = reinterpret_cast<int*>(mine + 2 * S::OUT);
@@ -213,59 +222,61 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
         float* sx = sm.sx[e];
         const uint32_t free0 = wd_peer(smem_u32(&sm.acc_free[0]), 0);
         int i = 0, turn = 0;
-        for (long long tile = first; tile < tiles; tile += step, ++i) {
-            const int n0 = (int)(tile % tiles_n) * COLS + rank * (COLS / 2) + 32 * (GLU ? q & 1 : q), n = n0 + lane;
-            const int t0 = (int)(tile / tiles_n) * 256 + half * 128;
+        for (int tile = first; tile < tiles; tile += step, ++i) {
+            const int n0 = tile % tiles_n * COLS + rank * (COLS / 2) + 32 * (GLU ? q & 1 : q), n = n0 + lane;
+            const int t0 = tile / tiles_n * 256 + part * 64;
             const int b = i & 1;
             const bool in = n < a.N;
             float s0 = in ? __ldcg(a.ws[0] + n) : 0.f, s1 = GLU && in ? __ldcg(a.ws[1] + n) : 0.f;
             const float bias = !GLU && a.bias != nullptr && in ? __ldcg(a.bias + n) : 0.f;
             const TO* res = GLU ? nullptr : static_cast<const TO*>(a.residual);
-            float next = t0 + lane < a.in.T ? __ldcg(a.in.scale + t0 + lane) : 0.f;
+            auto scale_of = [&](int t) { return lane < WD_CH && t + lane < a.in.T ? __ldcg(a.in.scale + t + lane) : 0.f; };
+            float next = scale_of(t0);
             // a wait that ran out shows as NaN
             if (!ut_wait(&sm.acc_full[b], (uint32_t)(i >> 1) & 1u, abort)) s0 = __int_as_float(0x7fffffff);
             __syncwarp();
             ut_fence_after();
-            const int chunks = min(4, (a.in.T - t0 + 31) / 32);
+            const int chunks = min(64 / WD_CH, (a.in.T - t0 + WD_CH - 1) / WD_CH);
 #pragma unroll 1
             for (int c = 0; c < chunks; ++c, ++turn) {
-                const int t = t0 + 32 * c;
-                uint32_t v[32];
-                ut_ld32(lanes + b * 256 + 32 * c, v);
-                sx[lane] = next;
-                next = t + 32 + lane < a.in.T ? __ldcg(a.in.scale + t + 32 + lane) : 0.f;
+                const int t = t0 + WD_CH * c;
+                uint32_t v[WD_CH];
+                ut_ld16(lanes + b * 256 + WD_CH * c, v);
+                if (lane < WD_CH) sx[lane] = next;
+                next = scale_of(t + WD_CH);
                 TO* out = stage + (turn & 1) * (S::OUT / (int)sizeof(TO));
                 // the store that read this buffer two turns ago has read it
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                 if constexpr (GLU) {
+                    constexpr int H = WD_CH / 2;
                     int* to = give + (turn & 1) * (S::SWAP / 4);
                     const int* from = take + (turn & 1) * (S::SWAP / 4);
                     ut_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) to[j * 32 + lane] = (int)v[is_up ? j : 16 + j];
-                    asm volatile("bar.sync %0, 64;" ::"r"(1 + half * 2 + (q & 1)) : "memory");
+                    for (int j = 0; j < H; ++j) to[j * 32 + lane] = (int)v[is_up ? j : H + j];
+                    asm volatile("bar.sync %0, 64;" ::"r"(1 + part * 2 + (q & 1)) : "memory");
 #pragma unroll
-                    for (int j0 = 0; j0 < 16; j0 += 4) {
-                        const float4 s4 = *reinterpret_cast<const float4*>(sx + (is_up ? 16 : 0) + j0);
+                    for (int j0 = 0; j0 < H; j0 += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4*>(sx + (is_up ? H : 0) + j0);
                         const float sj[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const int j = j0 + k, own = (int)v[is_up ? 16 + j : j], other = from[j * 32 + lane];
+                            const int j = j0 + k, own = (int)v[is_up ? H + j : j], other = from[j * 32 + lane];
                             store_out(out + j * 32 + lane, finish_glu(is_up ? other : own, is_up ? own : other, sj[k], s0, s1));
                         }
                     }
                 } else {
-                    float r[32];
+                    float r[WD_CH];
                     if (res != nullptr) {
                         const TO* p = res + (long long)t * a.ldr + n;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j, p += a.ldr) r[j] = in && t + j < a.in.T ? to_float(__ldcg(p)) : 0.f;
+                        for (int j = 0; j < WD_CH; ++j, p += a.ldr) r[j] = in && t + j < a.in.T ? to_float(__ldcg(p)) : 0.f;
                     }
                     ut_wait_ld();
                     __syncwarp();
                     auto put = [&](bool add) {
 #pragma unroll
-                        for (int j0 = 0; j0 < 32; j0 += 4) {
+                        for (int j0 = 0; j0 < WD_CH; j0 += 4) {
                             const float4 s4 = *reinterpret_cast<const float4*>(sx + j0);
                             const float sj[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
@@ -287,7 +298,7 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    const int y = t + (is_up ? 16 : 0);
+                    const int y = t + (is_up ? S::TOKENS : 0);
                     if (n0 < a.N && y < a.in.T) wd_store(&maps.out, n0, y, smem_u32(out));
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
@@ -324,6 +335,7 @@ static cudaError_t wide_typed(const Int8Args& a, bool early, cudaStream_t s) {
         !out_map(&maps.out, a.out, a.out_type, a.N, a.in.T, a.ldo, S::TOKENS))
         return cudaErrorNotSupported;
     const long long tiles = (long long)((a.N + (GLU ? 127 : 255)) / (GLU ? 128 : 256)) * ((a.in.T + 255) / 256);
+    if (tiles >= 1 << 30) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)(tiles < 74 ? tiles : 74));
     cfg.blockDim = dim3(WD_THREADS);
