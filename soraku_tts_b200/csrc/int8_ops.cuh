@@ -18,8 +18,10 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "ops.cuh"
+#include "umma.cuh"
 
 namespace skb {
 
@@ -132,6 +134,10 @@ struct Vec {
         if constexpr (sizeof(TX) == 4) {
             v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y);
             v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
+        } else if constexpr (std::is_same<TX, __nv_bfloat16>::value) {
+            const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = to_float(e[i]);
@@ -147,13 +153,14 @@ struct Vec {
 template <int N>
 __device__ __forceinline__ void encode(const float (&y)[N], float s, float r, uint32_t (&word)[N / 4]) {
     constexpr float MAGIC = 12582912.f;
+    const float2 r2 = make_float2(r, r), up = make_float2(MAGIC, MAGIC), down = make_float2(-MAGIC, -MAGIC), minus = make_float2(-1.f, -1.f);
     uint32_t q[N];
     float off = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float t = __fmul_rn(y[i], r), m = __fadd_rn(t, MAGIC);
-        q[i] = __float_as_uint(m);
-        off = fmaxf(off, fabsf(__fsub_rn(t, __fsub_rn(m, MAGIC))));
+    for (int i = 0; i < N; i += 2) {
+        const float2 t = mul2(make_float2(y[i], y[i + 1]), r2), m = add2(t, up), d = fma2(add2(m, down), minus, t);
+        q[i] = __float_as_uint(m.x), q[i + 1] = __float_as_uint(m.y);
+        off = max_abs(off, d.x, d.y);
     }
     if (off > 0.4999f) {
 #pragma unroll

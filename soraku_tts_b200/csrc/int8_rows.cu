@@ -10,7 +10,7 @@ namespace skb {
 // the norm's weights stay in registers, and the next row is on its way while this
 // one is finished.
 template <class TX, int G, int CH, bool NORM>
-__global__ void __launch_bounds__(256) quantize_kernel(const RowsIn in, int8_t* __restrict__ q, long long ldq,
+__global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::N > 16 ? 2 : NORM ? 3 : 4) quantize_kernel(const RowsIn in, int8_t* __restrict__ q, long long ldq,
                                                        float* __restrict__ scale) {
     constexpr int V = Vec<TX>::N, ROWS = 256 / G, WARPS = G / 32;
     __shared__ float red[2][ROWS][WARPS][2];
@@ -49,19 +49,21 @@ __global__ void __launch_bounds__(256) quantize_kernel(const RowsIn in, int8_t* 
     load(row);
     for (int turn = 0; row - slot < in.T; row += step, turn ^= 1) {
         float v[CH][V], top = 0.f, ss = 0.f;
+        float2 squares = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             next[c].get(v[c]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
+            for (int i = 0; i < V; i += 2) {
                 if constexpr (NORM) {
-                    ss = fmaf(v[c][i], v[c][i], ss);
-                    v[c][i] = __fmul_rn(v[c][i], w[c][i]);
+                    const float2 x = make_float2(v[c][i], v[c][i + 1]), y = mul2(x, make_float2(w[c][i], w[c][i + 1]));
+                    squares = fma2(x, x, squares);
+                    v[c][i] = y.x, v[c][i + 1] = y.y;
                 }
+                top = max_abs(top, v[c][i], v[c][i + 1]);
             }
-#pragma unroll
-            for (int i = 0; i < V; i += 2) top = max_abs(top, v[c][i], v[c][i + 1]);
         }
+        ss = squares.x + squares.y;
         if (row - slot + step < in.T) load(row + step);
         top = warp_top(top);
         if (NORM) ss = warp_sum(ss);
@@ -102,13 +104,33 @@ __global__ void __launch_bounds__(256) quantize_long_kernel(const RowsIn in, int
     if (threadIdx.x == 0) scale[row] = s;
 }
 
+// CTAs that are resident at once: rows are dealt out to just as many.
+template <auto Kernel>
+static int resident() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, 256, 0) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            n = 1;
+        }
+        n *= 148;
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+template <class TX, int G, int CH, bool NORM>
+static cudaError_t rows_go(const RowsIn& in, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
+    constexpr int ROWS = 256 / G;
+    const int need = (in.T + ROWS - 1) / ROWS, most = resident<quantize_kernel<TX, G, CH, NORM>>();
+    return launch(quantize_kernel<TX, G, CH, NORM>, dim3(need < most ? need : most), dim3(256), 0, s, true, in, q, ldq, scale);
+}
 template <class TX, int G, int CH>
 static cudaError_t rows_launch(const RowsIn& in, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
-    constexpr int ROWS = 256 / G;
-    const int need = (int)(((long long)in.T + ROWS - 1) / ROWS), most = 148 * 4;
-    const dim3 grid(need < most ? need : most);
-    return in.nw ? launch(quantize_kernel<TX, G, CH, true>, grid, dim3(256), 0, s, true, in, q, ldq, scale)
-                 : launch(quantize_kernel<TX, G, CH, false>, grid, dim3(256), 0, s, true, in, q, ldq, scale);
+    return in.nw ? rows_go<TX, G, CH, true>(in, q, ldq, scale, s) : rows_go<TX, G, CH, false>(in, q, ldq, scale, s);
 }
 
 template <class TX>
@@ -121,9 +143,12 @@ static cudaError_t quantize_typed(const RowsIn& in, int8_t* q, long long ldq, fl
         if (vectors <= 256) return rows_launch<TX, 256, 1>(in, q, ldq, scale, s);
         if (vectors <= 512) return rows_launch<TX, 256, 2>(in, q, ldq, scale, s);
     }
-    if (vectors <= 128) return rows_launch<TX, 32, 4>(in, q, ldq, scale, s);
-    if (vectors <= 256) return rows_launch<TX, 64, 4>(in, q, ldq, scale, s);
-    if (vectors <= 512) return rows_launch<TX, 128, 4>(in, q, ldq, scale, s);
+    // many: two vectors a thread, which leaves room for four CTAs an SM (6541 rows of
+    // 1024 with a norm 8.3 us; four vectors 9.7, one 14)
+    if (vectors <= 64) return rows_launch<TX, 32, 2>(in, q, ldq, scale, s);
+    if (vectors <= 128) return rows_launch<TX, 64, 2>(in, q, ldq, scale, s);
+    if (vectors <= 256) return rows_launch<TX, 128, 2>(in, q, ldq, scale, s);
+    if (vectors <= 512) return rows_launch<TX, 256, 2>(in, q, ldq, scale, s);
     if (vectors <= 1024) return rows_launch<TX, 256, 4>(in, q, ldq, scale, s);
     if constexpr (V == 4) {
         if (vectors <= 2048) return rows_launch<TX, 256, 8>(in, q, ldq, scale, s);
