@@ -62,7 +62,7 @@ static int product(const char* what, Int8Args& a, bool glu, void* work, int64_t 
         if (e != cudaSuccess) return fail(SKB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
         a.in = {q, SKB_I8, kp, scale, nullptr, 0.f, a.in.T, a.in.K};
     }
-    const cudaError_t e = a.in.T <= I8_FEW ? int8_gemv_launch(a, glu, need > 0, s) : int8_gemm_launch(a, glu, need > 0, s);
+    const cudaError_t e = int8_gemv_serves(a, glu) ? int8_gemv_launch(a, glu, need > 0, s) : int8_gemm_launch(a, glu, need > 0, s);
     return e == cudaSuccess ? SKB_OK : fail(SKB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 

@@ -9,7 +9,8 @@ namespace skb {
 constexpr int GV_THREADS = 256, GV_WARPS = 8;
 constexpr int GV_CHUNK = 512;   // bytes of a row that a warp reads at once
 constexpr int GV_MAX_X = 128 * 1024;  // bytes of codes in shared memory: one token of any length
-constexpr int GV_FUSED_T = 2, GV_FUSED = 32 * 1024;  // tokens, and values, up to which each CTA makes the codes itself
+constexpr int GV_FUSED_T = 2, GV_FUSED = 4096;  // tokens, and values in all, up to which each CTA makes the codes itself
+constexpr long long GV_READS = 6 << 20;         // bytes of weights, read once for every 8 tokens
 
 // TT: tokens a CTA holds (the last ones may be missing); R: weight rows a warp
 // takes at a time (with SwiGLU R / 2 gate rows and their up rows).  8 / R chunks of
@@ -138,7 +139,20 @@ __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args
     }
 }
 
+// Codes made by every CTA save a launch, 1.4 us, and cost what their values take:
+// 2 tokens of 1024 to 4096 channels 3.6 us, in two launches 4.0; of 4096 to 4096 8.4
+// and 6.9.
 bool int8_gemv_fuses(int T, int K) { return T <= GV_FUSED_T && T * ceil16(K) <= GV_FUSED; }
+
+// Here, or on the tensor cores.  Up to 4 tokens weights come in as fast either way and
+// there is less around them (4 tokens of 1024 to 32816 channels 10.9 us, 9 tokens
+// there 12.1).  With more, four-byte products take longer than the bytes, once for
+// every 8 tokens: 16 of 2048 to 1024 5.6 us here and 7.3 there, 8 of 1024 to 4096 4.8
+// and 6.5, 16 of these 7.5 and 6.7, 8 of 4096 to 4096 9.6 and 8.7.
+bool int8_gemv_serves(const Int8Args& a, bool glu) {
+    const int T = a.in.T;
+    return T <= 4 || (T <= 16 && (T + 7) / 8 * (long long)a.N * max(a.in.K, GV_CHUNK) * (glu ? 2 : 1) <= GV_READS);
+}
 
 template <auto Kernel>
 static cudaError_t gemv_go(const Int8Args& a, int R, int tt, bool glu, bool early, cudaStream_t s) {

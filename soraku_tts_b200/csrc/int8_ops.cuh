@@ -76,7 +76,7 @@ bool int8_map(CUtensorMap* m, const void* p, int K, int rows, long long ld, int 
 bool out_map(CUtensorMap* m, void* p, int type, int N, int T, long long ld, int tokens);
 bool int8_wide_serves(const Int8Args& a);
 cudaError_t int8_wide_launch(const Int8Args& a, bool glu, bool early, cudaStream_t s);
-constexpr int I8_FEW = 8;  // tokens that int8_gemv.cu serves
+bool int8_gemv_serves(const Int8Args& a, bool glu);
 bool int8_gemv_fuses(int T, int K);
 cudaError_t int8_gemv_launch(const Int8Args& a, bool glu, bool early, cudaStream_t s);
 cudaError_t int8_gemm_launch(const Int8Args& a, bool glu, bool early, cudaStream_t s);
