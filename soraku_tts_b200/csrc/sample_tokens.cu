@@ -43,6 +43,7 @@ constexpr int ST_BINS = 2048;
 constexpr int ST_LIST = 512;        // logits of one gathered bin
 constexpr int ST_SORT = 2048;       // logits that are gathered to be put in order
 constexpr int ST_QUICK_K = 1280;
+constexpr int ST_TURN = 16;         // logits that a thread reads at a time
 constexpr int ST_OWN = 4;           // parts of a thread's logits that have a largest of their own
 static_assert(ST_BINS == ST_SORT, "as many bins as listed logits");
 constexpr int ST_MAX_V = 1 << 18;
@@ -164,31 +165,34 @@ struct Row {
         return l == top ? (u64)ST_ONE : (u64)__double_as_longlong(weight(l) + 4503599627370496.0) & 0xfffffffffffffull;
     }
     __device__ __forceinline__ double safe_weight(float l) const { return l == top ? ST_ONE : weight(l); }
-    // f(logits, index of the first) for every vector, B of them read at a time.
+    // f(logits, index of the first) for B vectors from this thread's one at i on.
     template <int B, class F>
-    __device__ __forceinline__ void each(F f) const {
+    __device__ __forceinline__ void turn(int i, F f) const {
         const int end = off + n;
-        for (int i = threadIdx.x * VN; i < end; i += B * NT * VN) {
-            Vec<TX> v[B];
+        Vec<TX> v[B];
 #pragma unroll
-            for (int b = 0; b < B; ++b) {
-                const int at = i + b * NT * VN;
-                if (HELD ? at < end : at >= off && at + VN <= end) {
-                    if (HELD) v[b].raw = *reinterpret_cast<const uint4*>(data + at);
-                    else v[b].raw = __ldcg(reinterpret_cast<const uint4*>(data + at));
-                } else {
+        for (int b = 0; b < B; ++b) {
+            const int at = i + b * NT * VN;
+            if (HELD ? at < end : at >= off && at + VN <= end) {
+                if (HELD) v[b].raw = *reinterpret_cast<const uint4*>(data + at);
+                else v[b].raw = __ldcg(reinterpret_cast<const uint4*>(data + at));
+            } else {
 #pragma unroll
-                    for (int j = 0; j < VN; ++j)
-                        v[b].e[j] = !HELD && at + j >= off && at + j < end ? __ldcg(data + at + j) : from_float<TX>(-INFINITY);
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < B; ++b) {
-                float l[VN];
-                v[b].get(l);
-                f(l, first + i + b * NT * VN - off);
+                for (int j = 0; j < VN; ++j)
+                    v[b].e[j] = !HELD && at + j >= off && at + j < end ? __ldcg(data + at + j) : from_float<TX>(-INFINITY);
             }
         }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            float l[VN];
+            v[b].get(l);
+            f(l, first + i + b * NT * VN - off);
+        }
+    }
+    // f for every vector, B of them read at a time.
+    template <int B, class F>
+    __device__ __forceinline__ void each(F f) const {
+        for (int i = threadIdx.x * VN; i < off + n; i += B * NT * VN) turn<B>(i, f);
     }
 };
 
@@ -808,10 +812,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         row.off = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(TX));
         src -= row.off;
         TX* held = reinterpret_cast<TX*>(st_raw + S::BYTES);
+        float* largest = reinterpret_cast<float*>(st_raw + S::BYTES);  // of each thread's turns, where the row is not held
         row.data = HELD ? held : src;
-        constexpr int B = 32 / VN / 2;
+        constexpr int B = ST_TURN / VN;
         const int end = row.off + row.n;
-        for (int i = tid * VN; i < end; i += B * NT * VN) {
+        for (int i = tid * VN, turn = 0; i < end; i += B * NT * VN, ++turn) {
+            float most = -INFINITY;
             Vec<TX> v[B];
 #pragma unroll
             for (int b = 0; b < B; ++b) {
@@ -834,8 +840,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
                 for (int j = 0; j < VN; ++j) {
                     asm("max.NaN.f32 %0, %0, %1;" : "+f"(mine[(b * VN + j) * ST_OWN / (B * VN)]) : "f"(l[j]));
                     low = fminf(low, l[j] > -INFINITY ? l[j] : INFINITY);
+                    most = fmaxf(most, l[j]);
                 }
             }
+            if (!HELD) largest[turn * NT + tid] = most;
         }
     }
     // the order of numbers as that of whole ones, NaN (max.NaN gives the positive one) on top
@@ -873,7 +881,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
     if (!(temperature > 0.f)) t = 1.0, top_k = 1, top_p = 1.f, min_p = 0.f;  // the largest logit, the first of equal ones
     row.top = top;
     row.inv_t = 1.0 / t;
-    row.scale = 184.66496523378731 / t;
+    row.scale = 184.66496523378731 * row.inv_t;
     row.cut = (float)fmin(32.0 * t, 3e38);
     const float span = fmaxf(fminf(row.cut, top == low ? 1.f : top - low), 1e-30f);
     row.inv_width = (float)(ST_BINS - 1) / span;
@@ -912,7 +920,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
         // bins up to `last` reach half a bin behind it; with room for rounding, that is as
         // far as a vector's largest has to be looked at
         const float reach = last == ST_BINS - 1 ? -INFINITY : top - ((float)last + 1.f) * (span / (ST_BINS - 1)) - fabsf(top) * 1e-6f;
-        row.template each<4>([&](const float (&l)[VN], int i) {
+        auto see = [&](const float (&l)[VN], int i) {
             float most = l[0];
 #pragma unroll
             for (int j = 1; j < VN; ++j) most = fmaxf(most, l[j]);
@@ -920,10 +928,24 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
 #pragma unroll
             for (int j = 0; j < VN; ++j)
                 if (top - l[j] <= row.cut && row.bin_at(top - l[j]) <= last) s.list(l[j], i + j);
-        });
+        };
+        if constexpr (HELD) {
+            row.template each<4>(see);
+        } else {
+            // a thread reads again only the turns that reach so far: one in eight for the
+            // first 1000 of 151,936
+            const float* largest = reinterpret_cast<const float*>(st_raw + S::BYTES);
+            constexpr int STEP = ST_TURN * NT;
+            static_assert((ST_MAX_V + 8) / STEP + 1 <= 32, "a thread's turns as bits");
+            unsigned far = 0;
+            for (int i = tid * VN, turn = 0; i < row.off + row.n; i += STEP, ++turn)
+                if (!(largest[turn * NT + tid] < reach)) far |= 1u << turn;
+            // each lane its next one: a warp goes round as often as its busiest lane has any
+            for (; far != 0; far &= far - 1) row.template turn<ST_TURN / VN>(tid * VN + (__ffs(far) - 1) * STEP, see);
+        }
         s.sync();
     } else {
-        row.template each<1>([&](const float (&l)[VN], int) {
+        row.template each<4>([&](const float (&l)[VN], int) {
 #pragma unroll
             for (int j = 0; j < VN; ++j)
                 if (top - l[j] <= row.cut) atomicAdd(&s.count[row.bin_at(top - l[j])], 1u);
@@ -1019,7 +1041,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
 template <class TX, int C, int NT, bool HELD>
 static cudaError_t sample_launch(SampleArgs a, cudaStream_t s) {
     a.slice = ((a.V + C - 1) / C + 7) & ~7;
-    const size_t smem = Sampler<TX, C, NT, HELD>::BYTES + (HELD ? (size_t)a.slice * sizeof(TX) + 32 : 0);
+    const size_t smem = Sampler<TX, C, NT, HELD>::BYTES + (HELD ? (size_t)a.slice * sizeof(TX) + 32 : (size_t)((a.slice + 8 + NT * ST_TURN - 1) / (NT * ST_TURN)) * NT * 4);
     cudaError_t e = prepare_kernel<sample_kernel<TX, C, NT, HELD>>(200 * 1024);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
