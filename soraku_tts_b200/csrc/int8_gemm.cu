@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
     } else if (warp >= 4) {
         const int q = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(32 * q) << 16);
-        constexpr int CH = TN / 2 < 32 ? TN / 2 : 32;  // columns at a time
+        constexpr int CH = 16;  // columns at a time
         float* sx = sm.sx[warp - 4];
         int i = 0;
         for (int tile = first; tile < tiles; tile += step, ++i) {
@@ -217,6 +217,13 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
             const TO* res = GLU ? nullptr : static_cast<const TO*>(a.residual);
             __syncwarp();
             for (int j = lane; j < TN / 2; j += 32) sx[j] = t0 + j < a.in.T ? __ldcg(a.in.scale + t0 + j) : 0.f;
+            TO r_next[GLU ? 1 : CH];  // as it came: a conversion would wait for it
+            auto residual_of = [&](int c) {
+                const TO* p = res + (long long)(t0 + c) * a.ldr + n;
+#pragma unroll
+                for (int j = 0; j < CH; ++j, p += a.ldr) r_next[GLU ? 0 : j] = in && t0 + c + j < a.in.T ? __ldcg(p) : from_float<TO>(0.f);
+            };
+            if (!GLU && split == 1 && res != nullptr) residual_of(0);
             // a wait that ran out shows as NaN
             const float poison = ut_wait(&sm.acc_full[b], (uint32_t)(i >> 1) & 1u, abort) ? 1.f : __int_as_float(0x7fffffff);
             __syncwarp();
@@ -225,13 +232,8 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
             for (int c = 0; c < TN / 2 && t0 + c < a.in.T; c += CH) {
                 uint32_t v[CH], u[GLU ? CH : 1];
                 const uint32_t col = lanes + b * S::COLS + half * (TN / 2) + c;
-                if constexpr (CH == 32) {
-                    ut_ld32(col, v);
-                    if constexpr (GLU) ut_ld32(col + TN, u);
-                } else {
-                    ut_ld16(col, v);
-                    if constexpr (GLU) ut_ld16(col + TN, u);
-                }
+                ut_ld16(col, v);
+                if constexpr (GLU) ut_ld16(col + TN, u);
                 if (split > 1) {
                     ut_wait_ld();
                     int* sums = reinterpret_cast<int*>(base) + (half * (TN / 2) + c) * 128 + 32 * q + lane;
@@ -245,9 +247,9 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
                 const int left = in ? a.in.T - t0 - c : 0;  // tokens there are
                 float r[GLU ? 1 : CH];
                 if (!GLU && res != nullptr) {
-                    const TO* p = res + (long long)(t0 + c) * a.ldr + n;
 #pragma unroll
-                    for (int j = 0; j < CH; ++j, p += a.ldr) r[GLU ? 0 : j] = j < left ? to_float(__ldcg(p)) : 0.f;
+                    for (int j = 0; j < CH; ++j) r[GLU ? 0 : j] = to_float(r_next[GLU ? 0 : j]);
+                    if (c + CH < TN / 2) residual_of(c + CH);  // on their way while these are used
                 }
                 ut_wait_ld();
                 TO* p = static_cast<TO*>(a.out) + (long long)(t0 + c) * a.ldo + n;
@@ -441,48 +443,59 @@ static int clusters_at_once(int split) {
     return n;
 }
 
-// Tile width and split of K, of those that run at once: the least time by what was
-// measured at 9 to 512 tokens, 1024 to 4096 channels and K of 1024 to 8192 (us):
-// 0.22 + TN / 1000 a block of K, half as much again with two weights; a split costs
-// 0.5 and 0.025 a token to hand sums over, which is a tenth of that without.  False if
-// nothing fits: then tiles are as wide as they get, and CTAs take them in turn.
+// Which tiles: their width in tokens, how many CTAs split K, or pairs (width 0,
+// int8_wide.cu).  Of those that run at once the least time by what was measured at 9 to
+// 512 tokens, 1024 to 4096 channels and K of 1024 to 8192, in us: 0.22 + width / 1000 a
+// block of K, half as much again with two weights; a split 0.5 and 0.025 a token to hand
+// sums over, a token's finish 0.004 without.  Where nothing fits, tiles are as wide as
+// they get and CTAs take them in turn: a turn of a pair 1 to begin with, then 0.39 a
+// block or its finish, 4 (SwiGLU 5.8, with a residual 8), whichever is longer; of a
+// single CTA 0.48 a block (0.52) or 4.3 (3.9, 10).
 template <class TO, bool GLU>
-static bool gemm_choose(const Int8Args& a, int& width, int& split) {
+static void gemm_choose(const Int8Args& a, int& width, int& split) {
     const long long cols = (a.N + 127) / 128;
     const int blocks = (a.in.K + 127) / 128, T = a.in.T;
     float best = 3e38f;
     auto look = [&](int tn, int at_once, int s) {
-        const long long tiles = cols * ((T + tn - 1) / tn);
-        if (s > blocks || tiles > at_once) return;
+        if (s > blocks || cols * ((T + tn - 1) / tn) > at_once) return;
+        const float tokens = (float)(T < tn ? T : tn);
         const float t = (float)((blocks + s - 1) / s) * (0.22f + 0.001f * tn) * (GLU ? 1.5f : 1.f) +
-                        (s > 1 ? 0.5f + 0.025f * (float)(T < tn ? T : tn) * (GLU ? 2 : 1) : 0.004f * (float)(T < tn ? T : tn));
+                        (s > 1 ? 0.5f + 0.025f * tokens * (GLU ? 2 : 1) : 0.004f * tokens);
         if (t < best) best = t, width = tn, split = s;
     };
     look(32, 148, 1), look(64, 148, 1), look(128, 148, 1);
-    for (int s = 2; s <= GM_MAX_SPLIT; s *= 2) {
-        if (cols * s > 148) break;
+    for (int s = 2; s <= GM_MAX_SPLIT && cols * s <= 148; s *= 2) {
         look(32, clusters_at_once<32, GLU, TO>(s), s);
         look(64, clusters_at_once<64, GLU, TO>(s), s);
         look(128, clusters_at_once<128, GLU, TO>(s), s);
     }
-    return best < 3e38f;
+    if (best < 3e38f) return;
+    split = 1, width = GLU ? 128 : 256;
+    if (!int8_wide_serves(a)) return;
+    auto turn = [&](float block, float finish) { return (float)blocks * block > finish ? (float)blocks * block : finish; };
+    const long long singles = (cols * ((T + width - 1) / width) + 147) / 148;
+    const long long pairs = ((a.N + (GLU ? 127 : 255)) / (GLU ? 128 : 256) * (long long)((T + 255) / 256) + 73) / 74;
+    if (1.f + (float)pairs * turn(0.39f, GLU ? 5.8f : a.residual ? 8.f : 4.f) <
+        (float)singles * turn(GLU ? 0.52f : 0.48f, GLU ? 3.9f : a.residual ? 10.f : 4.3f))
+        width = 0;
 }
 
 template <class TO>
 static cudaError_t gemm_typed(const Int8Args& a, bool glu, bool early, cudaStream_t s) {
     int width = 0, split = 1;
-    if (glu ? gemm_choose<TO, true>(a, width, split) : gemm_choose<TO, false>(a, width, split)) {
-        if (glu) {
-            if (width == 32) return gemm_launch<32, true, TO>(a, split, early, s);
-            if (width == 64) return gemm_launch<64, true, TO>(a, split, early, s);
-            return gemm_launch<128, true, TO>(a, split, early, s);
-        }
-        if (width == 32) return gemm_launch<32, false, TO>(a, split, early, s);
-        if (width == 64) return gemm_launch<64, false, TO>(a, split, early, s);
-        return gemm_launch<128, false, TO>(a, split, early, s);
+    if (glu) {
+        gemm_choose<TO, true>(a, width, split);
+        if (width == 0) return int8_wide_launch(a, true, early, s);
+        if (width == 32) return gemm_launch<32, true, TO>(a, split, early, s);
+        if (width == 64) return gemm_launch<64, true, TO>(a, split, early, s);
+        return gemm_launch<128, true, TO>(a, split, early, s);
     }
-    if (int8_wide_serves(a)) return int8_wide_launch(a, glu, early, s);
-    return glu ? gemm_launch<128, true, TO>(a, 1, early, s) : gemm_launch<256, false, TO>(a, 1, early, s);
+    gemm_choose<TO, false>(a, width, split);
+    if (width == 0) return int8_wide_launch(a, false, early, s);
+    if (width == 32) return gemm_launch<32, false, TO>(a, split, early, s);
+    if (width == 64) return gemm_launch<64, false, TO>(a, split, early, s);
+    if (width == 128) return gemm_launch<128, false, TO>(a, split, early, s);
+    return gemm_launch<256, false, TO>(a, 1, early, s);
 }
 
 // Rows as codes; early: see int8_gemv_launch.
