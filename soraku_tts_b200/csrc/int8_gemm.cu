@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
         __syncwarp();
         gm_cluster_sync();  // peers have read this CTA's sums
     }
+    __syncwarp();
     ut_fence_before();
     __syncthreads();
     if (warp == 2) ut_free<S::TMEM>(tmem);

@@ -10,8 +10,8 @@ namespace skb {
 // the norm's weights stay in registers, and the next row is on its way while this
 // one is finished.
 template <class TX, int G, int CH, bool NORM>
-__global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::N > 16 ? 2 : NORM ? 3 : 4) quantize_kernel(const RowsIn in, int8_t* __restrict__ q, long long ldq,
-                                                       float* __restrict__ scale) {
+__global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::N > 16 ? 2 : NORM ? 3 : 4)
+    quantize_kernel(const RowsIn in, int8_t* __restrict__ q, long long ldq, float* __restrict__ scale) {
     constexpr int V = Vec<TX>::N, ROWS = 256 / G, WARPS = G / 32;
     __shared__ float red[2][ROWS][WARPS][2];
     const int slot = threadIdx.x / G, t = threadIdx.x % G;
