@@ -109,6 +109,10 @@ __device__ __forceinline__ float warp_top(float a) {
 __device__ __forceinline__ float step_of(float top) {
     return top <= 3.402823466e38f ? fmaxf(__fdiv_rn(top, 127.f), 1.17549435e-38f) : __int_as_float(0x7fffffff);
 }
+// About 1 / s, which is enough to find codes by (encode).
+__device__ __forceinline__ float codes_per(float top) {
+    return top > 1e-30f && top < 1e30f ? __fdividef(127.f, top) : __fdiv_rn(1.f, step_of(top));
+}
 
 // 16 bytes of a row's values.
 template <class TX>
@@ -147,11 +151,11 @@ struct Vec {
 
 // Codes of N values, four bytes a word: round(y / s) with the FP32 quotient, halves
 // to even.  Adding 1.5 2^23 rounds y times 1 / s and leaves the code in the low
-// byte.  That product is within 3e-5 of the quotient (|q| <= 127, three
-// roundings), so only values next to a half need the division: one in five
-// thousand, looked for once in N.  s NaN: zeros.
+// byte.  That product is within 6e-5 of the quotient (|q| <= 127; 2^-22 for r and
+// three roundings of 2^-24), so only values next to a half need s and the division:
+// one in five thousand, looked for once in N.  Not finite: zeros.
 template <int N>
-__device__ __forceinline__ void encode(const float (&y)[N], float s, float r, uint32_t (&word)[N / 4]) {
+__device__ __forceinline__ void encode(const float (&y)[N], float top, float r, uint32_t (&word)[N / 4]) {
     constexpr float MAGIC = 12582912.f;
     const float2 r2 = make_float2(r, r), up = make_float2(MAGIC, MAGIC), down = make_float2(-MAGIC, -MAGIC), minus = make_float2(-1.f, -1.f);
     uint32_t q[N];
@@ -163,13 +167,14 @@ __device__ __forceinline__ void encode(const float (&y)[N], float s, float r, ui
         off = max_abs(off, d.x, d.y);
     }
     if (off > 0.4999f) {
+        const float s = step_of(top);
 #pragma unroll
         for (int i = 0; i < N; ++i) q[i] = __float_as_uint(__fadd_rn(__fdiv_rn(y[i], s), MAGIC));
     }
 #pragma unroll
     for (int h = 0; h < N / 4; ++h) {
         word[h] = __byte_perm(__byte_perm(q[4 * h], q[4 * h + 1], 0x0040), __byte_perm(q[4 * h + 2], q[4 * h + 3], 0x0040), 0x5410);
-        if (!(s == s)) word[h] = 0;
+        if (!(top <= 3.402823466e38f)) word[h] = 0;
     }
 }
 template <int N>
@@ -241,14 +246,14 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
 #pragma unroll
         for (int w = 0; w < G / 32; ++w) top = max_abs(top, red[2 * w], 0.f), ss += red[2 * w + 1];
     }
-    const float s = step_of(top), r = __fdiv_rn(1.f, s);
+    const float r = codes_per(top);
     for (;;) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k = base + (c * G + t) * V;
             if (k >= ceil16(K)) continue;
             uint32_t word[V / 4];
-            encode<V>(v[c], s, r, word);
+            encode<V>(v[c], top, r, word);
             put_codes<V>(q + k, word);
         }
         if (base == 0) break;
@@ -256,6 +261,7 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
         load(base);
         weigh(base, false);
     }
+    const float s = step_of(top);
     return nw != nullptr ? s * rsqrtf(ss / (float)K + eps) : s;
 }
 

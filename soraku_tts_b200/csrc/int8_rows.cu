@@ -13,7 +13,7 @@ template <class TX, int G, int CH, bool NORM>
 __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::N > 16 ? 2 : NORM ? 3 : 4)
     quantize_kernel(const RowsIn in, int8_t* __restrict__ q, long long ldq, float* __restrict__ scale) {
     constexpr int V = Vec<TX>::N, ROWS = 256 / G, WARPS = G / 32;
-    __shared__ float red[2][ROWS][WARPS][2];
+    __shared__ float red[2][2][ROWS][WARPS];
     const int slot = threadIdx.x / G, t = threadIdx.x % G;
     const int K = in.K, kp = ceil16(K);
     pdl_wait();
@@ -35,9 +35,10 @@ __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::
             }
     }
     Vec<TX> next[CH];
+    const bool all_aligned = ((reinterpret_cast<uintptr_t>(in.x) | (uintptr_t)(in.ld * (long long)sizeof(TX))) & 15) == 0;
     auto load = [&](long long row) {
         const TX* x = static_cast<const TX*>(in.x) + row * in.ld;
-        const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+        const bool aligned = all_aligned || (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k = (c * G + t) * V;
@@ -69,24 +70,30 @@ __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::
         if (NORM) ss = warp_sum(ss);
         if constexpr (G > 32) {
             // two places in turn, so that one barrier a row is enough
-            if ((t & 31) == 0) red[turn][slot][t >> 5][0] = top, red[turn][slot][t >> 5][1] = ss;
+            if ((t & 31) == 0) red[0][turn][slot][t >> 5] = top, red[1][turn][slot][t >> 5] = ss;
             __syncthreads();
-            top = 0.f, ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < WARPS; ++i) top = max_abs(top, red[turn][slot][i][0], 0.f), ss += red[turn][slot][i][1];
+            top = warp_top(red[0][turn][slot][t % WARPS]);
         }
         if (row >= in.T) continue;
-        const float s = step_of(top), r = __fdiv_rn(1.f, s);
+        const float r = codes_per(top);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k = (c * G + t) * V;
             if (k < kp) {
                 uint32_t word[V / 4];
-                encode<V>(v[c], s, r, word);
+                encode<V>(v[c], top, r, word);
                 put_codes<V>(q + row * ldq + k, word);
             }
         }
-        if (t == 0) scale[row] = NORM ? s * rsqrtf(ss / (float)K + in.eps) : s;
+        if (t == 0) {
+            if constexpr (NORM && G > 32) {
+                ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < WARPS; ++i) ss += red[1][turn][slot][i];
+            }
+            const float s = step_of(top);
+            scale[row] = NORM ? s * rsqrtf(ss / (float)K + in.eps) : s;
+        }
     }
 }
 
