@@ -151,18 +151,18 @@ struct Vec {
 
 // Codes of N values, four bytes a word: round(y / s) with the FP32 quotient, halves
 // to even.  Adding 1.5 2^23 rounds y times 1 / s and leaves the code in the low
-// byte.  That product is within 6e-5 of the quotient (|q| <= 127; 2^-22 for r and
-// three roundings of 2^-24), so only values next to a half need s and the division:
+// byte.  That product is within 5e-5 of the quotient (|q| <= 127; 2^-22 for r and
+// two roundings of 2^-24), so only values next to a half need s and the division:
 // one in five thousand, looked for once in N.  Not finite: zeros.
 template <int N>
 __device__ __forceinline__ void encode(const float (&y)[N], float top, float r, uint32_t (&word)[N / 4]) {
     constexpr float MAGIC = 12582912.f;
-    const float2 r2 = make_float2(r, r), up = make_float2(MAGIC, MAGIC), down = make_float2(-MAGIC, -MAGIC), minus = make_float2(-1.f, -1.f);
+    const float2 r2 = make_float2(r, r), up = make_float2(MAGIC, MAGIC), minus = make_float2(-1.f, -1.f);
     uint32_t q[N];
     float off = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        const float2 t = mul2(make_float2(y[i], y[i + 1]), r2), m = add2(t, up), d = fma2(add2(m, down), minus, t);
+        const float2 t = make_float2(y[i], y[i + 1]), m = fma2(t, r2, up), d = fma2(t, r2, fma2(m, minus, up));
         q[i] = __float_as_uint(m.x), q[i + 1] = __float_as_uint(m.y);
         off = max_abs(off, d.x, d.y);
     }
