@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::
             for (int h = 0; h < V / 4; ++h) {
                 const int k = (c * G + t) * V + 4 * h;
                 Vec<float> raw;
-                raw.load(in.nw + k, K - k, aligned);
+                raw.template load<true>(in.nw + k, K - k, aligned);
                 float f[4];
                 raw.get(f);
 #pragma unroll
