@@ -133,9 +133,11 @@ struct Vec {
             raw = NEAR ? __ldca(v) : __ldcg(v);
         } else {
             raw = make_uint4(0, 0, 0, 0);
+            if (left > 0) {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i < left) e[i] = NEAR ? __ldca(p + i) : __ldcg(p + i);
+                for (int i = 0; i < N; ++i)
+                    if (i < left) e[i] = NEAR ? __ldca(p + i) : __ldcg(p + i);
+            }
         }
     }
     __device__ __forceinline__ void get(float (&v)[N]) const {

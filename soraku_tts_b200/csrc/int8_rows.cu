@@ -144,9 +144,10 @@ template <class TX>
 static cudaError_t quantize_typed(const RowsIn& in, int8_t* q, long long ldq, float* scale, cudaStream_t s) {
     constexpr int V = Vec<TX>::N;
     const int vectors = (in.K + V - 1) / V;
+    // a warp's one vector a lane (33000 rows of 256 BF16 values 8.5 us, by two a lane 10.8)
+    if (vectors <= 32) return rows_launch<TX, 32, 1>(in, q, ldq, scale, s);
     // rows that are few: as many threads as a row has vectors
     if (in.T <= 296) {
-        if (vectors <= 32) return rows_launch<TX, 32, 1>(in, q, ldq, scale, s);
         if (vectors <= 256) return rows_launch<TX, 256, 1>(in, q, ldq, scale, s);
         if (vectors <= 512) return rows_launch<TX, 256, 2>(in, q, ldq, scale, s);
     }
