@@ -2,6 +2,11 @@
 // bytes: the tokens' rows become codes in every CTA's shared memory (one launch
 // for norm, codes and product), each warp streams whole weight rows, four a
 // step, and adds up products of four bytes an instruction.
+//
+// 2 tokens of 1024 to 4096 channels 3.4 us, to 32816 10.7 (33.6 MB from device memory;
+// 6.7 from codes and L2): about 1.5 us to the first codes, the stream, and sums across a
+// warp for every row.  Rows announced to L2 four groups ahead (bulk prefetch) made it
+// 12.5, two rows a step in place of four 11.1.
 #include "int8_ops.cuh"
 
 namespace skb {

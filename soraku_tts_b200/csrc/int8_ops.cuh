@@ -93,6 +93,22 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
+// A value by way of L2, or of L1 (NEAR).  CUDA's own __ldcg and __ldca of 16-bit types
+// are not volatile: the compiler may take them out of the condition that guards them (a
+// residual that is not there was read, an illegal address) or past a wait.  Those of
+// whole numbers are.
+template <bool NEAR = false, class T>
+__device__ __forceinline__ T read(const T* p) {
+    if constexpr (sizeof(T) == 2) {
+        const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
+        const unsigned short bits = NEAR ? __ldca(u) : __ldcg(u);
+        if constexpr (std::is_same<T, __half>::value) return __ushort_as_half(bits);
+        else return __ushort_as_bfloat16(bits);
+    } else {
+        return NEAR ? __ldca(p) : __ldcg(p);
+    }
+}
+
 // Largest of |a|, |b|, |c|; NaN if one of them is.
 __device__ __forceinline__ float max_abs(float a, float b, float c) {
     float d;
@@ -136,7 +152,7 @@ struct Vec {
             if (left > 0) {
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (i < left) e[i] = NEAR ? __ldca(p + i) : __ldcg(p + i);
+                    if (i < left) e[i] = read<NEAR>(p + i);
             }
         }
     }
@@ -296,9 +312,9 @@ template <class T>
 __device__ __forceinline__ void store_out(T* p, float v) { *p = from_float<T>(v); }
 
 __device__ __forceinline__ float load_as(const void* p, int type, long long i) {
-    if (type == SKB_F32) return __ldcg(static_cast<const float*>(p) + i);
-    if (type == SKB_BF16) return __bfloat162float(__ldcg(static_cast<const __nv_bfloat16*>(p) + i));
-    return __half2float(__ldcg(static_cast<const __half*>(p) + i));
+    if (type == SKB_F32) return read(static_cast<const float*>(p) + i);
+    if (type == SKB_BF16) return to_float(read(static_cast<const __nv_bfloat16*>(p) + i));
+    return to_float(read(static_cast<const __half*>(p) + i));
 }
 __device__ __forceinline__ void store_as(void* p, int type, long long i, float v) {
     if (type == SKB_F32) store_out(static_cast<float*>(p) + i, v);

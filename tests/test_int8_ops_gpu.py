@@ -198,6 +198,14 @@ def test_linear_of_many_tiles(K, t, n, k, dtype):
     check_linear(K, t, n, k, dtype, residual=True, in_place=n % 8 == 0)
 
 
+@pytest.mark.parametrize("t,n,k", [(5281, 64, 384), (531, 1727, 104), (40, 700, 130), (9000, 64, 96), (181, 4736, 64), (300, 2048, 520)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_linear_with_and_without_residual(K, t, n, k, dtype):
+    """Tiles of every width; a residual that is not there is not read."""
+    check_linear(K, t, n, k, dtype, norm=True, bias=False)
+    check_linear(K, t, n, k, dtype, residual=True)
+
+
 @pytest.mark.parametrize("t,n,k", [(1500, 1536, 1024), (2111, 1028, 1000), (1281, 2001, 130), (5003, 520, 64)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_swiglu_of_many_tiles(K, t, n, k, dtype):
@@ -480,6 +488,24 @@ def test_sample_rows_anywhere(K):
 def test_sample_many_rows(K):
     check_sample(K, some_logits(1000, 300, 4), uniforms(1000, 4), 0.8, 20, 0.9, 0.0)
     check_sample(K, some_logits(300, 12000, 4), uniforms(300, 4), 0.8, 0, 0.9, 0.0)
+
+
+@pytest.mark.parametrize("rows", [5, 40])
+@pytest.mark.parametrize("v", [8193, 16385, 50001, 151936])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sample_by_clusters_and_streams(K, dtype, v, rows):
+    """Few and many rows of long lines, with one top-k and with each row's own."""
+    k = torch.tensor([50, 1000, 1, 0, 1280], dtype=torch.int32, device="cuda").repeat(rows // 5)
+    x = some_logits(rows, v, rows + v, DT[dtype])
+    x[1] = (x[1] * 2).round()  # many equal ones
+    x[2, ::3] = float("-inf")
+    x[3, 77], x[3, v - 1] = float("inf"), float("inf")
+    u = uniforms(rows, v)
+    for top_k in (k, 20, 0):
+        check_sample(K, x, u, 0.8, top_k, 0.9, 0.001)
+    x[0] = 1.5
+    check_sample(K, x, u, 1.0, k, 1.0, 0.0)
+    check_sample(K, x, u, 1.0, 1000, 1.0, 0.0)
 
 
 def test_sample_draws_as_the_frame_sampler_does(K):
