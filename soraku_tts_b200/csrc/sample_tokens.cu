@@ -29,6 +29,12 @@
 // Where the windows miss, or more equal logits share a bin than a list holds, the
 // bins are weighed too and the bin of each answer is binned again by (logit,
 // index), as often as it takes (st_general).
+//
+// Times: 64 rows of 2051 by top-k 50, top-p and min-p 7.4 us; one row of 151,936 by top-p
+// and min-p 26; 128 rows of those by top-k 1000, top-p and min-p 36 (78 MB, 11.9 us at a
+// copy's rate).  A small batch is bound by latency: code that runs once, barriers over
+// the cluster, and the first CTA putting its list in order, where phases by half of
+// its threads were no faster.  A large one by instructions a logit beside the stream.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -179,7 +185,7 @@ struct Row {
             } else {
 #pragma unroll
                 for (int j = 0; j < VN; ++j)
-                    v[b].e[j] = !HELD && at + j >= off && at + j < end ? __ldcg(data + at + j) : from_float<TX>(-INFINITY);
+                    v[b].e[j] = !HELD && at + j >= off && at + j < end ? read(data + at + j) : from_float<TX>(-INFINITY);
             }
         }
 #pragma unroll
@@ -827,7 +833,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
                 } else {
 #pragma unroll
                     for (int j = 0; j < VN; ++j)
-                        v[b].e[j] = at + j >= row.off && at + j < end ? __ldcg(src + at + j) : from_float<TX>(-INFINITY);
+                        v[b].e[j] = at + j >= row.off && at + j < end ? read(src + at + j) : from_float<TX>(-INFINITY);
                 }
             }
 #pragma unroll
@@ -1039,15 +1045,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_kernel(const SampleArgs 
 }
 
 template <class TX, int C, int NT, bool HELD>
+static size_t sample_smem(int slice) {
+    constexpr int TURN = NT * ST_TURN;
+    return Sampler<TX, C, NT, HELD>::BYTES + (HELD ? (size_t)slice * sizeof(TX) + 32 : (size_t)((slice + 8 + TURN - 1) / TURN) * NT * 4);
+}
+
+template <class TX, int C, int NT, bool HELD>
 static cudaError_t sample_launch(SampleArgs a, cudaStream_t s) {
     a.slice = ((a.V + C - 1) / C + 7) & ~7;
-    const size_t smem = Sampler<TX, C, NT, HELD>::BYTES + (HELD ? (size_t)a.slice * sizeof(TX) + 32 : (size_t)((a.slice + 8 + NT * ST_TURN - 1) / (NT * ST_TURN)) * NT * 4);
     cudaError_t e = prepare_kernel<sample_kernel<TX, C, NT, HELD>>(200 * 1024);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.rows * C);
     cfg.blockDim = dim3(NT);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = sample_smem<TX, C, NT, HELD>(a.slice);
     cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1061,10 +1072,48 @@ static cudaError_t sample_launch(SampleArgs a, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, sample_kernel<TX, C, NT, HELD>, a);
 }
 
+// Clusters of 8 that run at once on the current device: a CTA of theirs takes an SM, so
+// that the length of a row is of no account.
+template <class TX>
+static int sample_clusters() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    if (prepare_kernel<sample_kernel<TX, 8, 1024, true>>(200 * 1024) != cudaSuccess) return 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(8);
+    cfg.blockDim = dim3(1024);
+    cfg.dynamicSmemBytes = sample_smem<TX, 8, 1024, true>(ST_MAX_V / 8);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 8;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, sample_kernel<TX, 8, 1024, true>, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        return 1;
+    }
+    known[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+// Up to 8192 logits by half as many threads, held in one CTA's shared memory (8192 by
+// top-k 50 7.6 us, streamed 8.5).  More by a top-k that all rows share: a row
+// streams through one CTA, which has little to do but read it (one row of 16,000 8.5 us and
+// of 151,936 15.1; by a cluster 13.2 and 31.2).  By windows each logit costs more, and
+// a cluster shares that: 1 row of 32,000 20 us, of 151,936 26, streamed 27 and 75.  But
+// few clusters run at once: 16 rows 41 and 52 us, streamed 27 and 76, 32 rows of 151,936 79
+// and 75.
 template <class TX>
 static cudaError_t sample_typed(const SampleArgs& a, cudaStream_t s) {
     if (a.V <= 8192) return sample_launch<TX, 1, 512, true>(a, s);
-    if (a.rows <= 32) return sample_launch<TX, 8, 1024, true>(a, s);
+    if (a.top_k == nullptr && a.top_k0 > 0 && a.top_k0 <= ST_QUICK_K) return sample_launch<TX, 1, 1024, false>(a, s);
+    const int turns = (a.rows - 1) / sample_clusters<TX>() + 1;
+    if ((float)turns * (18.f + (float)a.V / 18000.f) < 14.f + (float)a.V / 2500.f) return sample_launch<TX, 8, 1024, true>(a, s);
     return sample_launch<TX, 1, 1024, false>(a, s);
 }
 
