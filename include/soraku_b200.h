@@ -251,7 +251,7 @@ int skb_evict_cache(const float *mass, const int32_t *cached, int rows, int n_kv
 #define SKB_I8 3
 
 /* Rows [rows, K] (row stride ldx elements) to codes and scales: with y = x, or
- * x * norm_weight in FP32, and s = max(max |y| / 127, 2^-126),
+ * x * norm_weight in FP32, and s = max(max |y| (1 / 127), 2^-126) in FP32,
  *   q[k] = round(y[k] / s) (the FP32 quotient, halves to even),
  *   scale = s, or s / sqrt(mean(x^2) + eps) with a norm,
  * so that q * scale is about the row, RMS-normed where norm_weight [K] is not

@@ -1,7 +1,7 @@
 // Shared pieces of the products in 8-bit integers (int8_rows.cu, int8_gemv.cu,
 // int8_gemm.cu).
 //
-// A row y of K values becomes codes q_k = round(y_k / s), s = max |y| / 127,
+// A row y of K values becomes codes q_k = round(y_k / s), s = max |y| (1 / 127),
 // so that y is about q s.  The quotient is the FP32 one, rounded to even: a
 // code is a definite number, the same from every kernel.  With a norm,
 // y_k = x_k w_k and the row's scale is s / sqrt(mean x^2 + eps): the root mean
@@ -120,10 +120,12 @@ __device__ __forceinline__ float max_abs(float a, float b, float c) {
 __device__ __forceinline__ float warp_top(float a) {
     return __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(a) & 0x7fffffffu));
 }
-// s = max / 127, and no smaller than the smallest normal number, where the
+// s = max times FP32's 1 / 127, as elementary operations on the device form max / 127 (a
+// true division gave another s in some rows, and there another code where y / s was
+// next to a half: one of 6.7 million); no smaller than the smallest normal number, where the
 // quotient by it stays finite.  NaN for a row that holds something not finite.
 __device__ __forceinline__ float step_of(float top) {
-    return top <= 3.402823466e38f ? fmaxf(__fdiv_rn(top, 127.f), 1.17549435e-38f) : __int_as_float(0x7fffffff);
+    return top <= 3.402823466e38f ? fmaxf(__fmul_rn(top, 1.f / 127.f), 1.17549435e-38f) : __int_as_float(0x7fffffff);
 }
 // About 1 / s, which is enough to find codes by (encode).
 __device__ __forceinline__ float codes_per(float top) {
@@ -173,8 +175,8 @@ struct Vec {
 
 // Codes of N values, four bytes a word: round(y / s) with the FP32 quotient, halves
 // to even.  Adding 1.5 2^23 rounds y times 1 / s and leaves the code in the low
-// byte.  That product is within 5e-5 of the quotient (|q| <= 127; 2^-22 for r and
-// two roundings of 2^-24), so only values next to a half need s and the division:
+// byte.  That product is within 6e-5 of the quotient (|q| <= 127; 2^-22 for r and
+// three roundings of 2^-24), so only values next to a half need s and the division:
 // one in five thousand, looked for once in N.  Not finite: zeros.
 template <int N>
 __device__ __forceinline__ void encode(const float (&y)[N], float top, float r, uint32_t (&word)[N / 4]) {
