@@ -23,7 +23,7 @@ constexpr long long GV_READS = 6 << 20;         // bytes of weights, read once f
 template <class TX, int TT, int R, bool GLU>
 __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args a, bool early) {
     extern __shared__ __align__(16) int8_t gv_x[];  // [TT][kp]
-    __shared__ float red[2 * GV_WARPS];
+    __shared__ alignas(16) float red[TT * ROW_RED];
     __shared__ float sx[TT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int K = a.in.K, kp = ceil16(K);
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args
         const TX* x = static_cast<const TX*>(a.in.x) + (long long)(t0 + min(t, nt - 1)) * a.in.ld;
         const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
         const float s = quantize_row<TX, G, 16 / Vec<TX>::N>(x, a.in.nw, a.in.eps, K, aligned, gv_x + t * kp, tid % G,
-                                                             red + 2 * (t * G / 32));
+                                                             red + t * ROW_RED);
         if (tid % G == 0) sx[t] = s;
     }
     __syncthreads();

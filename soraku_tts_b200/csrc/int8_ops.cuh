@@ -5,8 +5,9 @@
 // so that y is about q s.  The quotient is the FP32 one, rounded to even: a
 // code is a definite number, the same from every kernel.  With a norm,
 // y_k = x_k w_k and the row's scale is s / sqrt(mean x^2 + eps): the root mean
-// square divides a whole row, so it moves the scale and no code, and codes do
-// not depend on the order in which squares are added up.
+// square divides a whole row, so it moves the scale and no code.  Squares are added
+// up in one order (Squares below), so that neither codes nor scale depend on the
+// rows beside it or on the kernel.
 //
 // A product's sum over K is exact in 32 bits (K <= 131071), in any order;
 //   out = (sum_k q_x q_w) s_x s_w + bias + residual
@@ -207,19 +208,77 @@ __device__ __forceinline__ void put_codes(int8_t* q, const uint32_t (&word)[N / 
     else *reinterpret_cast<uint2*>(q) = make_uint2(word[0], word[1]);
 }
 
+// A row's sum of squares, added in one order that depends on nothing but the row, so that
+// its scale is the same in any batch and from every kernel.  A group of G threads holds a
+// row's 16-byte vectors 32 j + lane, j = c W + warp for a thread's c-th one (W = G / 32).
+// Vectors of a lane with equal j mod 8 are one chain, j ascending, even and odd values
+// apart; a chain's lanes are added in a butterfly, then the eight chains in order.  W
+// divides eight: a thread of a small group holds N chains, and none of them crosses a warp.
+// What is not there adds an exact zero.
+template <int G, int CH>
+struct Squares {
+    static constexpr int W = G / 32, N = CH < 8 / W ? CH : 8 / W, CHAINS = W * N;
+    static_assert(W <= 8 && 8 % W == 0 && N <= 2 && CH % N == 0, "chains of a thread");
+    float2 s[N];
+    __device__ __forceinline__ Squares() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = make_float2(0.f, 0.f);
+    }
+    __device__ __forceinline__ void add(int c, float2 x) { s[c % N] = fma2(x, x, s[c % N]); }
+    // This thread's chains, even and odd values together.
+    __device__ __forceinline__ float2 ends() const { return make_float2(s[0].x + s[0].y, N == 2 ? s[N - 1].x + s[N - 1].y : 0.f); }
+    // Over the warp: chain `warp` in lane 0, and, of two, chain W + warp in lane 16.
+    __device__ __forceinline__ static float over_lanes(float2 ends, int lane) {
+        float a = ends.x;
+        if constexpr (N == 2) {
+            const bool second = lane & 16;
+            const float other = __shfl_xor_sync(FULL, second ? ends.x : ends.y, 16);
+            a = (second ? ends.y : ends.x) + other;
+        } else {
+            a += __shfl_xor_sync(FULL, a, 16);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(FULL, a, o);
+        return a;
+    }
+    // Where a row's chains have the one that thread t holds then: lane 0, and, of two, lane 16.
+    __device__ __forceinline__ static int place(int t) { return N == 2 ? (t >> 5) + W * ((t >> 4) & 1) : t >> 5; }
+    __device__ __forceinline__ static bool holds(int t) { return (t & (N == 2 ? 15 : 31)) == 0; }
+    __device__ __forceinline__ static float total(const float* chains) {  // on 16 bytes
+        float sum = 0.f;
+        if constexpr (CHAINS % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < CHAINS; i += 4) {
+                const float4 c = *reinterpret_cast<const float4*>(chains + i);
+                sum = (((sum + c.x) + c.y) + c.z) + c.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CHAINS; ++i) sum += chains[i];
+        }
+        return sum;
+    }
+};
+
+// Floats that a row's threads leave for each other: largest of their warps, chains.
+constexpr int ROW_RED = 16;
+
 // One row by a group of G threads (G a multiple of 32; `t`: place in it):
 // codes to `q` (16-byte aligned, zeros up to ceil16(K)), the scale returned to
 // every thread.  A thread keeps CH vectors; longer rows are read twice, but for
-// the last piece.  `red`: 2 floats a warp of the group, if G > 32; then all
-// threads of the CTA have to call this together.
+// the last piece.  `red`: ROW_RED floats on 16 bytes; all threads of the CTA have to call this
+// together.
 template <class TX, int G, int CH>
 __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const float* __restrict__ nw, float eps, int K,
                                               bool x_aligned, int8_t* q, int t, float* red) {
     constexpr int V = Vec<TX>::N;
     constexpr int PIECE = G * CH * V;
+    using SQ = Squares<G, CH>;
+    static_assert(G > 32 && CH * (G / 32) % 8 == 0, "a piece goes on with the chains of the one before");
     const bool w_aligned = (reinterpret_cast<uintptr_t>(nw) & 15) == 0;
     float v[CH][V];
     float top = 0.f, ss = 0.f;
+    SQ squares;
     auto load = [&](int base) {
         Vec<TX> raw[CH];
 #pragma unroll
@@ -242,10 +301,10 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
                     float w[4];
                     raw.get(w);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float& y = v[c][4 * h + i];
-                        if (first) ss = fmaf(y, y, ss);
-                        y = __fmul_rn(y, w[i]);
+                    for (int i = 0; i < 4; i += 2) {
+                        float &y0 = v[c][4 * h + i], &y1 = v[c][4 * h + i + 1];
+                        if (first) squares.add(c, make_float2(y0, y1));
+                        y0 = __fmul_rn(y0, w[i]), y1 = __fmul_rn(y1, w[i + 1]);
                     }
                 }
             }
@@ -262,14 +321,16 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
         if (base + PIECE >= K) break;
     }
     top = warp_top(top);
-    if (nw != nullptr) ss = warp_sum(ss);
-    if (G > 32) {
-        if ((t & 31) == 0) red[2 * (t >> 5)] = top, red[2 * (t >> 5) + 1] = ss;
-        __syncthreads();
-        top = 0.f, ss = 0.f;
-#pragma unroll
-        for (int w = 0; w < G / 32; ++w) top = max_abs(top, red[2 * w], 0.f), ss += red[2 * w + 1];
+    if ((t & 31) == 0) red[t >> 5] = top;
+    if (nw != nullptr) {
+        ss = SQ::over_lanes(squares.ends(), t & 31);
+        if (SQ::holds(t)) red[8 + SQ::place(t)] = ss;
     }
+    __syncthreads();
+    top = 0.f;
+#pragma unroll
+    for (int w = 0; w < G / 32; ++w) top = max_abs(top, red[w], 0.f);
+    if (nw != nullptr) ss = SQ::total(red + 8);
     const float r = codes_per(top);
     for (;;) {
 #pragma unroll
@@ -289,8 +350,8 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
     return nw != nullptr ? s * rsqrtf(ss / (float)K + eps) : s;
 }
 
-// A sum's way to its result; the same operations in every kernel, so that a
-// token's result does not depend on how many stand beside it.  `bias`: 0 without.
+// A sum's way to its result; the same operations in every kernel, so that from its
+// codes and scale on a token's result does not depend on how many stand beside it.  `bias`: 0 without.
 __device__ __forceinline__ float finish(int sum, float sx, float sw, float bias) {
     return fmaf(__fmul_rn((float)sum, sx), sw, bias);
 }

@@ -19,8 +19,9 @@ namespace skb {
 template <class TX, int G, int CH, bool NORM>
 __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::N > 16 ? 2 : NORM ? 3 : 4)
     quantize_kernel(const RowsIn in, int8_t* __restrict__ q, long long ldq, float* __restrict__ scale) {
+    using SQ = Squares<G, CH>;
     constexpr int V = Vec<TX>::N, ROWS = 256 / G, WARPS = G / 32;
-    __shared__ float red[2][2][ROWS][WARPS];
+    __shared__ alignas(16) float red[2][2][ROWS][SQ::CHAINS];  // warps' largest; chains
     const int slot = threadIdx.x / G, t = threadIdx.x % G;
     const int K = in.K, kp = ceil16(K);
     pdl_wait();
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::
     load(row);
     for (int turn = 0; row - slot < in.T; row += step, turn ^= 1) {
         float v[CH][V], top = 0.f, ss = 0.f;
-        float2 squares = make_float2(0.f, 0.f);
+        SQ squares;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             next[c].get(v[c]);
@@ -65,21 +66,29 @@ __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::
             for (int i = 0; i < V; i += 2) {
                 if constexpr (NORM) {
                     const float2 x = make_float2(v[c][i], v[c][i + 1]), y = mul2(x, make_float2(w[c][i], w[c][i + 1]));
-                    squares = fma2(x, x, squares);
+                    squares.add(c, x);
                     v[c][i] = y.x, v[c][i + 1] = y.y;
                 }
                 top = max_abs(top, v[c][i], v[c][i + 1]);
             }
         }
-        ss = squares.x + squares.y;
+        float2 ends;
+        if constexpr (NORM) ends = squares.ends();
         if (row - slot + step < in.T) load(row + step);
         top = warp_top(top);
-        if (NORM) ss = warp_sum(ss);
+        if (NORM) ss = SQ::over_lanes(ends, t & 31);
         if constexpr (G > 32) {
             // two places in turn, so that one barrier a row is enough
-            if ((t & 31) == 0) red[0][turn][slot][t >> 5] = top, red[1][turn][slot][t >> 5] = ss;
+            if constexpr (NORM && SQ::N == 2) {
+                if ((t & 15) == 0) red[1][turn][slot][SQ::place(t)] = ss;
+                if ((t & 31) == 0) red[0][turn][slot][t >> 5] = top;
+            } else {
+                if ((t & 31) == 0) red[0][turn][slot][t >> 5] = top, red[1][turn][slot][t >> 5] = ss;
+            }
             __syncthreads();
             top = warp_top(red[0][turn][slot][t % WARPS]);
+        } else if constexpr (NORM && SQ::N == 2) {
+            ss += __shfl_sync(FULL, ss, 16);  // of use to lane 0: its chain, then the other
         }
         if (row >= in.T) continue;
         const float r = codes_per(top);
@@ -93,11 +102,7 @@ __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::
             }
         }
         if (t == 0) {
-            if constexpr (NORM && G > 32) {
-                ss = 0.f;
-#pragma unroll
-                for (int i = 0; i < WARPS; ++i) ss += red[1][turn][slot][i];
-            }
+            if constexpr (NORM && G > 32) ss = SQ::total(red[1][turn][slot]);
             const float s = step_of(top);
             scale[row] = NORM ? s * rsqrtf(ss / (float)K + in.eps) : s;
         }
@@ -108,7 +113,7 @@ __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::
 template <class TX>
 __global__ void __launch_bounds__(256) quantize_long_kernel(const RowsIn in, int8_t* __restrict__ q, long long ldq,
                                                             float* __restrict__ scale) {
-    __shared__ float red[16];
+    __shared__ alignas(16) float red[ROW_RED];
     pdl_wait();
     pdl_trigger();
     const long long row = blockIdx.x;

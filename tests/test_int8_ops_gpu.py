@@ -636,3 +636,20 @@ def test_the_same_call_twice_gives_the_same(K):
     lg, u = some_logits(30, 50000, 3), uniforms(30, 3)
     a, b = K.sample_tokens(lg, u, top_p=0.9), K.sample_tokens(lg, u, top_p=0.9)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("k", [1, 37, 256, 300, 520, 1024, 2048, 4100, 8192, 20000])
+def test_a_normed_row_goes_by_itself(K, dtype, k):
+    """A row's scale holds its sum of squares, added in the same order whatever stands beside it: by a product's own
+    CTAs for one or two tokens, by 32 to 256 threads a row in a batch.  To the bit."""
+    t = 700
+    x, nw = rows_in((t, k), k, DT[dtype], 3), 1 + 0.3 * torch.randn(k, device="cuda", generator=gen(1))
+    w, w2 = weights(70, k, 2), weights(70, k, 3)
+    kw = dict(norm_weight=nw, eps=EPS)
+    rows, lin, glu = K.quantize_rows(x, **kw), K.int8_linear(x, w, **kw), K.int8_swiglu(x, w, w2, **kw)
+    for a, b in ((0, 1), (699, 700), (5, 7), (0, 3), (10, 26), (300, 333), (17, 313), (17, 314)):
+        part = K.quantize_rows(x[a:b], **kw)
+        assert torch.equal(part.scale, rows.scale[a:b]) and torch.equal(part.q, rows.q[a:b])
+        assert torch.equal(K.int8_linear(x[a:b], w, **kw), lin[a:b])
+        assert torch.equal(K.int8_swiglu(x[a:b], w, w2, **kw), glu[a:b])
