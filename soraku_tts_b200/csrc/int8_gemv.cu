@@ -13,7 +13,8 @@ namespace skb {
 
 constexpr int GV_THREADS = 256, GV_WARPS = 8;
 constexpr int GV_CHUNK = 512;   // bytes of a row that a warp reads at once
-constexpr int GV_MAX_X = 128 * 1024;  // bytes of codes in shared memory: one token of any length
+constexpr int GV_MAX_K = 8192;        // values of a row; of two tokens' twice, of one's three times as many
+constexpr int GV_MAX_X = 8 * GV_MAX_K;  // bytes of codes in shared memory
 constexpr int GV_FUSED_T = 2, GV_FUSED = 4096;  // tokens, and values in all, up to which each CTA makes the codes itself
 constexpr long long GV_READS = 6 << 20;         // bytes of weights, read once for every 8 tokens
 
@@ -149,14 +150,20 @@ __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args
 // and 6.9.
 bool int8_gemv_fuses(int T, int K) { return T <= GV_FUSED_T && T * ceil16(K) <= GV_FUSED; }
 
-// Here, or on the tensor cores.  Up to 4 tokens weights come in as fast either way and
-// there is less around them (4 tokens of 1024 to 32816 channels 10.9 us, 9 tokens
-// there 12.1).  With more, four-byte products take longer than the bytes, once for
-// every 8 tokens: 16 of 2048 to 1024 5.6 us here and 7.3 there, 8 of 1024 to 4096 4.8
-// and 6.5, 16 of these 7.5 and 6.7, 8 of 4096 to 4096 9.6 and 8.7.
+// Here, or on the tensor cores; from codes, us.  Up to 4 tokens weights come in about as
+// fast either way and there is less around them (4 tokens of 1024 to 4096 channels 3.5 and
+// 6.5, to 32816 11.6 and 17; of 8192 to 4096 13.3 and 11.8).  With more, four-byte products
+// take longer than the bytes, once for every 8 tokens: 16 of 2048 to 1024 4.9 here and
+// 6.6 there, 5 of 1024 to 4096 4.6 and 6.5, 16 of these 7.5 and 6.5, 8 of 4096 to 4096
+// 9.6 and 8.7.  A warp takes a whole row by itself, so that long ones are slow:
+// 4 tokens of 16384 to 4096 22.5 and 16.7, one of 131071 to 1024 91 and 40.  To few channels
+// one or two tokens are faster a little further (2 of 16384 to 64 9.0 and 9.4, of 24000
+// 12.4 and 11.4; 1 of 20000 9.4 and 10.6, of 33000 14.2 and 13.8).
 bool int8_gemv_serves(const Int8Args& a, bool glu) {
     const int T = a.in.T;
-    return T <= 4 || (T <= 16 && (T + 7) / 8 * (long long)a.N * max(a.in.K, GV_CHUNK) * (glu ? 2 : 1) <= GV_READS);
+    const long long bytes = (long long)a.N * max(a.in.K, GV_CHUNK) * (glu ? 2 : 1);
+    if (a.in.K > GV_MAX_K) return T <= 2 && a.in.K <= (4 - T) * GV_MAX_K && bytes <= GV_READS;
+    return T <= 4 || (T <= 16 && (T + 7) / 8 * bytes <= GV_READS);
 }
 
 template <auto Kernel>
@@ -181,8 +188,7 @@ static cudaError_t gemv_rows(const Int8Args& a, bool early, cudaStream_t s) {
 template <class TX, bool GLU>
 static cudaError_t gemv_typed(const Int8Args& a, bool early, cudaStream_t s) {
     const int T = a.in.T;
-    int tt = T == 1 ? 1 : T == 2 ? 2 : T <= 4 ? 4 : 8;
-    while (tt * ceil16(a.in.K) > GV_MAX_X) tt >>= 1;
+    const int tt = T == 1 ? 1 : T == 2 ? 2 : T <= 4 ? 4 : 8;
     if (tt == 1) return gemv_rows<TX, 1, GLU>(a, early, s);
     if (tt == 2) return gemv_rows<TX, 2, GLU>(a, early, s);
     if constexpr (sizeof(TX) == 1) {

@@ -653,3 +653,34 @@ def test_a_normed_row_goes_by_itself(K, dtype, k):
         assert torch.equal(part.scale, rows.scale[a:b]) and torch.equal(part.q, rows.q[a:b])
         assert torch.equal(K.int8_linear(x[a:b], w, **kw), lin[a:b])
         assert torch.equal(K.int8_swiglu(x[a:b], w, w2, **kw), glu[a:b])
+
+
+@pytest.mark.parametrize("n,k", [(1024, 131071), (4096, 40000)])
+def test_fewer_tokens_take_no_longer(K, n, k):
+    """Rows so long that the tensor cores have them: one to four tokens in hardly more time than eight (they took up to
+    eight times as long, where every few tokens read all weights again)."""
+    weight = weights(n, k, 1)
+    rows = {t: K.quantize_rows(rows_in((t, k), t, torch.float32)) for t in (1, 2, 3, 4, 8)}
+    times = {t: [] for t in rows}
+    for turn in range(9):
+        for t, x in rows.items():
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            K.int8_linear(x, weight)
+            a.record()
+            for _ in range(4):
+                K.int8_linear(x, weight)
+            b.record()
+            torch.cuda.synchronize()
+            times[t].append(a.elapsed_time(b))
+    best = {t: min(v) for t, v in times.items()}
+    assert max(best[t] for t in (1, 2, 3, 4)) < 1.5 * best[8], best
+
+
+@pytest.mark.parametrize("t", [1, 2, 3, 4, 5, 16, 17])
+@pytest.mark.parametrize("k", [8192, 8193, 16384, 16385, 24576, 24577, 33000, 66000])
+def test_few_tokens_of_long_rows(K, t, k):
+    """About the borders at which long rows go to the tensor cores, with few channels and with many."""
+    check_linear(K, t, 37, k, bias=True)
+    check_linear(K, t, 700, k, "bf16", residual=True, codes=True)
+    check_swiglu(K, t, 21, k)
+    check_swiglu(K, t, 300, k, "f16")
