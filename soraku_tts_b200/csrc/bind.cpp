@@ -63,6 +63,13 @@ bool optional_vector(PyObject* o, int device, int64_t n, at::ScalarType type, vo
     *p = nullptr;
     return o == Py_None || vector(o, device, n, type, p);
 }
+// Other Python threads run while outputs are taken and kernels launched: a launch waits
+// where a stream has as many before it as its queue holds, as long as they take.  No
+// Python object is touched meanwhile.
+struct Released {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Released() { PyEval_RestoreThread(state); }
+};
 // 8-bit rows and their scales.
 struct Codes {
     Rows q;
@@ -122,21 +129,27 @@ PyObject* product(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         Py_RETURN_NONE;
     if (w.q.n < 2) Py_RETURN_NONE;
     const at::TensorOptions on = at::TensorOptions().device(at::kCUDA, device);
-    const at::Tensor out = out_given ? *out_given : at::empty({x.n, w.q.n}, on.dtype(type));
-    if (!o.read(&out, device) || o.n != x.n || o.k != w.q.n) Py_RETURN_NONE;
-    const int64_t need = int8_workspace((int)x.n, (int)x.k, x.type);
-    at::Tensor work;
-    if (need > 0) work = at::empty({need}, on.dtype(at::kByte));
-    void* space = need > 0 ? work.data_ptr() : nullptr;
-    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
-    const float *xs = static_cast<const float*>(xc.scale), *nw = static_cast<const float*>(norm);
-    const int status =
-        glu ? int8_swiglu(x.data, x.type, x.ld, xs, nw, eps, (int)x.n, (int)x.k, static_cast<const int8_t*>(w.q.data), w.q.ld,
-                          static_cast<const float*>(w.scale), static_cast<const int8_t*>(up.q.data), up.q.ld,
-                          static_cast<const float*>(up.scale), (int)w.q.n, o.data, out_type, o.ld, space, need, stream)
-            : int8_linear(x.data, x.type, x.ld, xs, nw, eps, (int)x.n, (int)x.k, static_cast<const int8_t*>(w.q.data), w.q.ld,
-                          static_cast<const float*>(w.scale), (int)w.q.n, static_cast<const float*>(bias), residual.data,
-                          residual.ld, o.data, out_type, o.ld, space, need, stream);
+    at::Tensor out;
+    if (out_given) out = *out_given;
+    int status = SKB_ERR_ARG;
+    {
+        const Released released;
+        if (!out_given) out = at::empty({x.n, w.q.n}, on.dtype(type));
+        if (o.read(&out, device) && o.n == x.n && o.k == w.q.n) {
+            const int64_t need = int8_workspace((int)x.n, (int)x.k, x.type);
+            at::Tensor work;
+            if (need > 0) work = at::empty({need}, on.dtype(at::kByte));
+            void* space = need > 0 ? work.data_ptr() : nullptr;
+            const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device).stream();
+            const float *xs = static_cast<const float*>(xc.scale), *nw = static_cast<const float*>(norm);
+            status = glu ? int8_swiglu(x.data, x.type, x.ld, xs, nw, eps, (int)x.n, (int)x.k, static_cast<const int8_t*>(w.q.data),
+                                       w.q.ld, static_cast<const float*>(w.scale), static_cast<const int8_t*>(up.q.data), up.q.ld,
+                                       static_cast<const float*>(up.scale), (int)w.q.n, o.data, out_type, o.ld, space, need, stream)
+                         : int8_linear(x.data, x.type, x.ld, xs, nw, eps, (int)x.n, (int)x.k, static_cast<const int8_t*>(w.q.data),
+                                       w.q.ld, static_cast<const float*>(w.scale), (int)w.q.n, static_cast<const float*>(bias),
+                                       residual.data, residual.ld, o.data, out_type, o.ld, space, need, stream);
+        }
+    }
     if (status != SKB_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
@@ -153,10 +166,15 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         !optional_vector(a[1], device, x.k, at::kFloat, &norm) || !number(a[2], &eps))
         Py_RETURN_NONE;
     const at::TensorOptions on = at::TensorOptions().device(at::kCUDA, device);
-    const at::Tensor q = at::empty({x.n, x.k}, on.dtype(at::kChar)), scale = at::empty({x.n}, on.dtype(at::kFloat));
-    if (quantize_rows(x.data, x.type, x.ld, (int)x.n, (int)x.k, static_cast<const float*>(norm), eps, q.data_ptr<int8_t>(), x.k,
-                      scale.data_ptr<float>(), c10::cuda::getCurrentCUDAStream(device).stream()) != SKB_OK)
-        Py_RETURN_NONE;
+    at::Tensor q, scale;
+    int status;
+    {
+        const Released released;
+        q = at::empty({x.n, x.k}, on.dtype(at::kChar)), scale = at::empty({x.n}, on.dtype(at::kFloat));
+        status = quantize_rows(x.data, x.type, x.ld, (int)x.n, (int)x.k, static_cast<const float*>(norm), eps, q.data_ptr<int8_t>(),
+                               x.k, scale.data_ptr<float>(), c10::cuda::getCurrentCUDAStream(device).stream());
+    }
+    if (status != SKB_OK) Py_RETURN_NONE;
     return PyTuple_Pack(2, THPObjectPtr(THPVariable_Wrap(q)).get(), THPObjectPtr(THPVariable_Wrap(scale)).get());
     END_HANDLE_TH_ERRORS
 }
@@ -187,12 +205,17 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         }
     }
     const at::TensorOptions on = at::TensorOptions().device(at::kCUDA, device);
-    const at::Tensor tokens = at::empty({x.n}, on.dtype(at::kLong)), logprob = at::empty({x.n}, on.dtype(at::kFloat));
-    if (sample_tokens(x.data, x.type, x.ld, (int)x.n, (int)x.k, static_cast<const float*>(u), static_cast<const float*>(each[0]),
-                      value[0], static_cast<const int32_t*>(each[1]), top_k, static_cast<const float*>(each[2]), value[2],
-                      static_cast<const float*>(each[3]), value[3], tokens.data_ptr<int64_t>(), logprob.data_ptr<float>(),
-                      c10::cuda::getCurrentCUDAStream(device).stream()) != SKB_OK)
-        Py_RETURN_NONE;
+    at::Tensor tokens, logprob;
+    int status;
+    {
+        const Released released;
+        tokens = at::empty({x.n}, on.dtype(at::kLong)), logprob = at::empty({x.n}, on.dtype(at::kFloat));
+        status = sample_tokens(x.data, x.type, x.ld, (int)x.n, (int)x.k, static_cast<const float*>(u), static_cast<const float*>(each[0]),
+                               value[0], static_cast<const int32_t*>(each[1]), top_k, static_cast<const float*>(each[2]), value[2],
+                               static_cast<const float*>(each[3]), value[3], tokens.data_ptr<int64_t>(), logprob.data_ptr<float>(),
+                               c10::cuda::getCurrentCUDAStream(device).stream());
+    }
+    if (status != SKB_OK) Py_RETURN_NONE;
     return PyTuple_Pack(2, THPObjectPtr(THPVariable_Wrap(tokens)).get(), THPObjectPtr(THPVariable_Wrap(logprob)).get());
     END_HANDLE_TH_ERRORS
 }

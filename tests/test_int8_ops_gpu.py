@@ -13,6 +13,8 @@ beyond), a square root's reciprocal (2 steps) and three more roundings:
 from __future__ import annotations
 
 import math
+import threading
+import time
 
 import numpy as np
 import pytest
@@ -684,3 +686,35 @@ def test_few_tokens_of_long_rows(K, t, k):
     check_linear(K, t, 700, k, "bf16", residual=True, codes=True)
     check_swiglu(K, t, 21, k)
     check_swiglu(K, t, 300, k, "f16")
+
+
+@pytest.mark.parametrize("call", ["sample_tokens", "int8_linear", "quantize_rows"])
+def test_other_threads_run_while_a_launch_waits(K, call):
+    """More calls than a stream's queue holds, behind half a second of other work: the launch that waits for room keeps
+    no other Python thread from running."""
+    x, u = torch.randn(4, 512, device="cuda", generator=gen(1)), torch.rand(4, device="cuda", generator=gen(2))
+    w = weights(64, 512, 3)
+    once = {"sample_tokens": lambda: K.sample_tokens(x, u), "int8_linear": lambda: K.int8_linear(x, w),
+            "quantize_rows": lambda: K.quantize_rows(x)}[call]
+    once()
+    torch.cuda.synchronize()
+    stop, longest = threading.Event(), [0.0]
+
+    def tick():
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            longest[0], last = max(longest[0], now - last), now
+
+    other = threading.Thread(target=tick)
+    other.start()
+    try:
+        torch.cuda._sleep(1_000_000_000)
+        for _ in range(3000):
+            once()
+        torch.cuda.synchronize()
+    finally:
+        stop.set()
+        other.join()
+    assert longest[0] < 0.2, longest[0]
