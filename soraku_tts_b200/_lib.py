@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsoraku_b200.so")
@@ -139,25 +140,40 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+class _NoBind:
+    """Stands where the short way is missing: takes no call, so that each goes through Python and ctypes."""
+
+    @staticmethod
+    def product(*args):
+        return None
+
+    quantize = sample = product
+
+
 _bind = None
 
 
 def bind():
     """The short way (csrc/bind.cpp) to the functions that a decoding step calls
-    most: loaded once, and given their addresses.  Raises if it has not been built."""
+    most: loaded once, and given their addresses.  Where it was not built, or does
+    not load, a stand-in that takes no call, and a warning."""
     global _bind
     if _bind is None:
         import torch  # noqa: F401 - its libraries come first
 
+        handle, short, why = lib(), None, ""
         try:
-            from . import _bind as module
+            from . import _bind as short
         except ImportError as e:
-            raise RuntimeError(
-                f"{os.path.join(HERE, '_bind.so')} is missing or does not fit this torch: build it with "
-                "`python -c 'import __graft_entry__ as g; g.build()'`") from e
-        names = ("skb_quantize_rows", "skb_int8_workspace", "skb_int8_linear", "skb_int8_swiglu", "skb_sample_tokens")
-        module.connect(*(ctypes.cast(getattr(lib(), n), c_void_p).value for n in names))
-        _bind = module
+            why = str(e)
+        if short is None:
+            warnings.warn(f"the extension module _bind does not serve ({why}): calls of the 8-bit operators take some microseconds more; "
+                          "build it with `python -c 'import __graft_entry__ as g; g.build()'`", RuntimeWarning, stacklevel=3)
+            short = _NoBind
+        else:
+            names = ("skb_quantize_rows", "skb_int8_workspace", "skb_int8_linear", "skb_int8_swiglu", "skb_sample_tokens")
+            short.connect(*(ctypes.cast(getattr(handle, n), c_void_p).value for n in names))
+        _bind = short
     return _bind
 
 

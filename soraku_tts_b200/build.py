@@ -3,7 +3,8 @@
 Each .cu under csrc/ compiles to an object in _build/ (in parallel), then
 nvcc links the shared library next to this file.  Objects are rebuilt when
 their source or any header changed.  _bind.so (csrc/bind.cpp) is the short way
-from Python to some of the library's functions; it uses torch's own libraries.
+from Python to some of the library's functions; it uses torch's own libraries.  The
+library does without it (_lib.bind), so that it is no error where it cannot be built.
 """
 
 from __future__ import annotations
@@ -12,6 +13,7 @@ import glob
 import os
 import subprocess
 import sys
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -78,13 +80,17 @@ def build(force: bool = False, verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=max(1, min(len(srcs) + 1, os.cpu_count() or 4))) as ex:
         bind = ex.submit(_build_bind, force)
         objs = list(ex.map(lambda s: _compile(s, hdr, verbose), srcs))
-    bind.result()
     newest = max(os.path.getmtime(o) for o in objs)
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < newest:
         cmd = [NVCC, *ARCH, "-shared", "-o", LIB, *objs]
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"nvcc link failed:\n{res.stdout}\n{res.stderr}")
+    try:
+        bind.result()
+    except Exception as e:  # no torch, no headers, no g++: the library stands
+        warnings.warn(f"{os.path.basename(BIND)} was not built, calls go the longer way through ctypes: {e}", RuntimeWarning,
+                      stacklevel=2)
     return LIB
 
 

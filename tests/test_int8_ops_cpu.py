@@ -4,6 +4,8 @@ so they are checked without one."""
 
 from __future__ import annotations
 
+import sys
+
 import pytest
 import torch
 
@@ -95,3 +97,36 @@ def test_python_layer_refuses_cpu_tensors():
                  lambda: K.sample_tokens(x, torch.zeros(2)), lambda: K.int8_linear(w, w), lambda: K.int8_linear(None, w)):
         with pytest.raises(ValueError):
             call()
+
+
+# ------------------------------------------------- the short way from Python
+def cut_off(monkeypatch):
+    """As if the extension module had not been built."""
+    import soraku_tts_b200
+    from soraku_tts_b200 import _lib
+
+    monkeypatch.setattr(_lib, "_bind", None)
+    monkeypatch.delattr(soraku_tts_b200, "_bind", raising=False)
+    monkeypatch.setitem(sys.modules, "soraku_tts_b200._bind", None)
+
+
+def test_without_the_short_way_calls_go_through_ctypes(lib, monkeypatch):
+    from soraku_tts_b200 import kernels as K
+
+    cut_off(monkeypatch)
+    with pytest.warns(RuntimeWarning, match="_bind"):
+        short = lib.bind()
+    assert short.product(*range(9)) is None and short.quantize(1, 2, 3) is None and short.sample(*range(6)) is None
+    with pytest.raises(ValueError, match="CUDA"):
+        K.quantize_rows(torch.zeros(2, 32))
+
+
+def test_the_library_is_built_without_the_short_way(lib, monkeypatch):
+    from soraku_tts_b200 import build
+
+    def fails(force):
+        raise RuntimeError("no headers")
+
+    monkeypatch.setattr(build, "_build_bind", fails)
+    with pytest.warns(RuntimeWarning, match="longer way"):
+        assert build.build() == build.LIB

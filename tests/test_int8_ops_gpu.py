@@ -718,3 +718,20 @@ def test_other_threads_run_while_a_launch_waits(K, call):
         stop.set()
         other.join()
     assert longest[0] < 0.2, longest[0]
+
+
+def test_the_longer_way_gives_the_same(K, monkeypatch):
+    """Through ctypes, where the short way was not built."""
+    from soraku_tts_b200 import _lib
+
+    x, nw, u = rows_in((40, 512), 1, torch.bfloat16), torch.rand(512, device="cuda", generator=gen(1)), torch.rand(40, device="cuda")
+    w, b = weights(96, 512, 2), torch.randn(96, device="cuda", generator=gen(3))
+
+    def step():
+        y = K.int8_linear(x, w, norm_weight=nw, bias=b, residual=x[:, :96])
+        q = K.quantize_rows(x, norm_weight=nw)
+        return y, *q, K.int8_swiglu(q, w, w), *K.sample_tokens(y, u, temperature=0.8, top_k=20, top_p=0.9, min_p=0.01)
+
+    short = step()
+    monkeypatch.setattr(_lib, "_bind", _lib._NoBind)
+    assert all(torch.equal(a, c) for a, c in zip(short, step()))
