@@ -155,15 +155,20 @@ _bind = None
 
 def bind():
     """The short way (csrc/bind.cpp) to the functions that a decoding step calls
-    most: loaded once, and given their addresses.  Where it was not built, or does
-    not load, a stand-in that takes no call, and a warning."""
+    most: loaded once, and given their addresses.  Where it was not built, or for
+    another torch than this one, a stand-in that takes no call, and a warning."""
     global _bind
     if _bind is None:
         import torch  # noqa: F401 - its libraries come first
 
+        from .build import bind_key
+
         handle, short, why = lib(), None, ""
         try:
             from . import _bind as short
+
+            if short.built_for != bind_key():
+                why, short = f"it was built for {short.built_for}, this is {bind_key()}", None
         except ImportError as e:
             why = str(e)
         if short is None:

@@ -1,10 +1,13 @@
-"""Build libsoraku_b200.so (sm_100a) in-tree with nvcc, and _bind.so with g++.
+"""Build libsoraku_b200.so (sm_100a) in-tree with nvcc, and the extension module _bind with g++.
 
 Each .cu under csrc/ compiles to an object in _build/ (in parallel), then
 nvcc links the shared library next to this file.  Objects are rebuilt when
-their source or any header changed.  _bind.so (csrc/bind.cpp) is the short way
-from Python to some of the library's functions; it uses torch's own libraries.  The
-library does without it (_lib.bind), so that it is no error where it cannot be built.
+their source or any header changed.  _bind (csrc/bind.cpp) is the short way from
+Python to some of the library's functions.  It is compiled against torch's headers and
+this interpreter's: its file name carries the interpreter's ABI, it says which torch it
+was compiled against (bind_key), and it is rebuilt when its command or either
+changes.  The library does without it (_lib.bind), so that it is no error where it
+cannot be built.
 """
 
 from __future__ import annotations
@@ -13,6 +16,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 import warnings
 from concurrent.futures import ThreadPoolExecutor
 
@@ -20,7 +24,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libsoraku_b200.so")
-BIND = os.path.join(HERE, "_bind.so")
+BIND = os.path.join(HERE, "_bind" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+BIND_STAMP = os.path.join(BUILD, "bind.txt")  # how BIND was built
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -49,25 +54,38 @@ def _compile(src: str, hdr_mtime: float, verbose: bool) -> str:
     return obj
 
 
-def _build_bind(force: bool) -> None:
-    import sysconfig
+def bind_key() -> str:
+    """What _bind has to have been compiled against: its headers' inline accessors know how this torch lays out a tensor."""
+    import torch
 
+    return f"torch {torch.__version__} {torch.version.git_version} c++11 abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+
+
+def _build_bind(force: bool) -> None:
     import torch
 
     src = os.path.join(CSRC, "bind.cpp")
-    needs = [src, os.path.join(INCLUDE, "soraku_b200.h"), torch.__file__]
-    if not force and os.path.exists(BIND) and os.path.getmtime(BIND) >= max(os.path.getmtime(p) for p in needs):
-        return
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(NVCC)))
     system = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-I", INCLUDE, *(f"-isystem{p}" for p in system), src, "-o", BIND, "-L", os.path.join(root, "lib"),
-           "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+           f'-DSKB_BIND_KEY="{bind_key()}"', "-I", INCLUDE, *(f"-isystem{p}" for p in system), src, "-o", BIND, "-L",
+           os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    stamp = "\n".join(cmd)
+    newest = max(os.path.getmtime(p) for p in (src, os.path.join(INCLUDE, "soraku_b200.h")))
+    if not force and os.path.exists(BIND) and os.path.getmtime(BIND) >= newest and os.path.exists(BIND_STAMP):
+        with open(BIND_STAMP) as f:
+            if f.read() == stamp:
+                return
+    for old in (BIND, BIND_STAMP, os.path.join(HERE, "_bind.so")):  # the last: a name without an ABI, which any interpreter loads
+        if os.path.exists(old):
+            os.remove(old)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{CXX} failed for {src}:\n{res.stdout}\n{res.stderr}")
+    with open(BIND_STAMP, "w") as f:
+        f.write(stamp)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

@@ -251,4 +251,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__bind() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__bind() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", SKB_BIND_KEY) < 0) Py_CLEAR(m);
+    return m;
+}

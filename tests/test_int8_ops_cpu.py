@@ -4,6 +4,7 @@ so they are checked without one."""
 
 from __future__ import annotations
 
+import subprocess
 import sys
 
 import pytest
@@ -119,6 +120,54 @@ def test_without_the_short_way_calls_go_through_ctypes(lib, monkeypatch):
     assert short.product(*range(9)) is None and short.quantize(1, 2, 3) is None and short.sample(*range(6)) is None
     with pytest.raises(ValueError, match="CUDA"):
         K.quantize_rows(torch.zeros(2, 32))
+
+
+def test_the_short_way_is_not_taken_with_another_torch(lib, monkeypatch):
+    from soraku_tts_b200 import build
+
+    assert lib.bind().built_for == build.bind_key()
+    monkeypatch.setattr(lib, "_bind", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    with pytest.warns(RuntimeWarning, match="torch 1.0.0"):
+        assert lib.bind().product(*range(9)) is None
+
+
+@pytest.mark.parametrize("change", [dict(CXX="other-g++"), dict(torch="9.9.9"), dict(file="elsewhere"), dict(stamp=None), dict(fail=1)])
+def test_the_short_way_is_built_again_when_what_it_was_built_for_changes(lib, monkeypatch, tmp_path, change):
+    from soraku_tts_b200 import build
+
+    runs = []
+
+    def run(cmd, **kw):
+        runs.append(cmd)
+        if "fail" not in change:
+            open(cmd[cmd.index("-o") + 1], "w").close()
+        return subprocess.CompletedProcess(cmd, 1 if "fail" in change else 0, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build, "HERE", str(tmp_path))
+    monkeypatch.setattr(build, "BIND", str(tmp_path / "_bind.x.so"))
+    monkeypatch.setattr(build, "BIND_STAMP", str(tmp_path / "bind.txt"))
+    (tmp_path / "_bind.so").touch()  # of a build that gave it no ABI
+    if "fail" in change:  # what was there before is not loaded
+        with pytest.raises(RuntimeError):
+            build._build_bind(False)
+        assert not list(tmp_path.iterdir())
+        return
+    build._build_bind(False)
+    build._build_bind(False)
+    assert len(runs) == 1 and not (tmp_path / "_bind.so").exists()
+    if "CXX" in change:
+        monkeypatch.setattr(build, "CXX", change["CXX"])
+    elif "torch" in change:
+        monkeypatch.setattr(torch, "__version__", change["torch"])
+    elif "file" in change:
+        monkeypatch.setattr(torch, "__file__", str(tmp_path / change["file"] / "__init__.py"))
+    else:
+        (tmp_path / "bind.txt").unlink()
+    build._build_bind(False)
+    build._build_bind(False)
+    assert len(runs) == 2
 
 
 def test_the_library_is_built_without_the_short_way(lib, monkeypatch):
