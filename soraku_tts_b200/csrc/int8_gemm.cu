@@ -74,11 +74,6 @@ __device__ __forceinline__ void gm_mma(uint32_t d, uint64_t a, uint64_t b, uint3
         "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
-__device__ __forceinline__ uint32_t gm_peer(uint32_t addr, int rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
 __device__ __forceinline__ int gm_peer_load(uint32_t addr) {
     int v;
     asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -88,9 +83,6 @@ __device__ __forceinline__ int4 gm_peer_load4(uint32_t addr) {
     int4 v;
     asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
-}
-__device__ __forceinline__ void gm_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <int TN, bool GLU, class TO>
@@ -285,11 +277,11 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
     }
     if (split > 1) {
         __syncwarp();
-        gm_cluster_sync();
+        cluster_sync();
         const int n0 = first % tiles_n * 128, t0 = first / tiles_n * TN;
         if (warp >= 4) {
             bool bad = false;
-            for (int p = 0; p < split; ++p) bad |= gm_peer_load(gm_peer(smem_u32(&sm.abort), p)) != 0;
+            for (int p = 0; p < split; ++p) bad |= gm_peer_load(cluster_addr(smem_u32(&sm.abort), p)) != 0;
             // a warp takes a token, a lane four channels; two tokens' sums are on their way
             const int nt = min(TN, a.in.T - t0), c = 4 * lane, n = n0 + c;
             const TO* res = GLU ? nullptr : static_cast<const TO*>(a.residual);
@@ -312,10 +304,10 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (t + h * W >= t_end) continue;
-                        const int4 x = gm_peer_load4(gm_peer(ring + ((t + h * W) * 128 + c) * 4, p));
+                        const int4 x = gm_peer_load4(cluster_addr(ring + ((t + h * W) * 128 + c) * 4, p));
                         v[h][0] += x.x, v[h][1] += x.y, v[h][2] += x.z, v[h][3] += x.w;
                         if constexpr (GLU) {
-                            const int4 y = gm_peer_load4(gm_peer(ring + ((TN + t + h * W) * 128 + c) * 4, p));
+                            const int4 y = gm_peer_load4(cluster_addr(ring + ((TN + t + h * W) * 128 + c) * 4, p));
                             u[h][0] += y.x, u[h][1] += y.y, u[h][2] += y.z, u[h][3] += y.w;
                         }
                     }
@@ -338,7 +330,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1) int8_gemm_kernel(const Int8Args
             }
         }
         __syncwarp();
-        gm_cluster_sync();  // peers have read this CTA's sums
+        cluster_sync();  // peers have read this CTA's sums
     }
     __syncwarp();
     ut_fence_before();

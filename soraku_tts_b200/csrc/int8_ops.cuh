@@ -110,12 +110,16 @@ __device__ __forceinline__ T read(const T* p) {
     }
 }
 
-// Largest of |a|, |b|, |c|; NaN if one of them is.
-__device__ __forceinline__ float max_abs(float a, float b, float c) {
-    float d;
-    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
+// The place of this CTA's shared memory in that of a CTA of its cluster; all of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
 }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Of numbers that are not negative, a warp's largest, NaN above all: in the order
 // of their bits.
 __device__ __forceinline__ float warp_top(float a) {
@@ -189,7 +193,7 @@ __device__ __forceinline__ void encode(const float (&y)[N], float top, float r, 
     for (int i = 0; i < N; i += 2) {
         const float2 t = make_float2(y[i], y[i + 1]), m = fma2(t, r2, up), d = fma2(t, r2, fma2(m, minus, up));
         q[i] = __float_as_uint(m.x), q[i + 1] = __float_as_uint(m.y);
-        off = max_abs(off, d.x, d.y);
+        off = max3_abs(off, d.x, d.y);
     }
     if (off > 0.4999f) {
         const float s = step_of(top);
@@ -310,7 +314,7 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
             }
             if (first) {
 #pragma unroll
-                for (int i = 0; i < V; i += 2) top = max_abs(top, v[c][i], v[c][i + 1]);
+                for (int i = 0; i < V; i += 2) top = max3_abs(top, v[c][i], v[c][i + 1]);
             }
         }
     };
@@ -329,7 +333,7 @@ __device__ __forceinline__ float quantize_row(const TX* __restrict__ x, const fl
     __syncthreads();
     top = 0.f;
 #pragma unroll
-    for (int w = 0; w < G / 32; ++w) top = max_abs(top, red[w], 0.f);
+    for (int w = 0; w < G / 32; ++w) top = max3_abs(top, red[w], 0.f);
     if (nw != nullptr) ss = SQ::total(red + 8);
     const float r = codes_per(top);
     for (;;) {

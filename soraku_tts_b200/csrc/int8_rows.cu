@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256, CH * Vec<TX>::N <= 8 ? 4 : CH * Vec<TX>::
                     squares.add(c, x);
                     v[c][i] = y.x, v[c][i + 1] = y.y;
                 }
-                top = max_abs(top, v[c][i], v[c][i + 1]);
+                top = max3_abs(top, v[c][i], v[c][i + 1]);
             }
         }
         float2 ends;

@@ -86,18 +86,10 @@ __device__ __forceinline__ void wd_commit(uint64_t* bar) {
         "h"((uint16_t)3)
         : "memory");
 }
-__device__ __forceinline__ uint32_t wd_peer(uint32_t addr, int rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
 // What it hands over is tensor memory, behind tcgen05's own fence: a release to the
 // cluster would wait for all stores on their way (1900 cycles a tile).
 __device__ __forceinline__ void wd_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void wd_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <bool GLU, class TO>
@@ -126,7 +118,7 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
     }
     ut_fence_before();
     __syncthreads();
-    wd_cluster_sync();  // the peer's barriers and tensor memory are there
+    cluster_sync();  // the peer's barriers and tensor memory are there
     ut_fence_after();
     const uint32_t tmem = sm.tmem;
     volatile int* abort = &sm.abort;
@@ -136,7 +128,7 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
     const int tiles = tiles_n * tiles_t;  // the launch has seen that they are fewer than 2^30
     const int blocks = (a.in.K + 127) / 128;
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
-    const uint32_t full0 = wd_peer(smem_u32(&sm.full[0]), 0);  // the first CTA's
+    const uint32_t full0 = cluster_addr(smem_u32(&sm.full[0]), 0);  // the first CTA's
     auto load_w = [&](int n0, int kb, int s) {
         const uint32_t at = ring + s * WD_STAGE;
         if (GLU) {
@@ -228,7 +220,7 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
         const int* take = reinterpret_cast<const int*>(base + S::STAGES * WD_STAGE + (e ^ 2) * S::WARP + 2 * S::OUT);
         const bool is_up = GLU && q >= 2;
         float* sx = sm.sx[e];
-        const uint32_t free0 = wd_peer(smem_u32(&sm.acc_free[0]), 0);
+        const uint32_t free0 = cluster_addr(smem_u32(&sm.acc_free[0]), 0);
         int i = 0, turn = 0;
         for (int tile = first; tile < tiles; tile += step, ++i) {
             const int n0 = tile % tiles_n * COLS + rank * (COLS / 2) + 32 * (GLU ? q & 1 : q), n = n0 + lane;
@@ -328,7 +320,7 @@ __global__ void __launch_bounds__(WD_THREADS, 1) int8_wide_kernel(const Int8Args
     }
     __syncwarp();
     ut_fence_before();
-    wd_cluster_sync();  // neither CTA goes while the other's copies, products or arrivals reach it
+    cluster_sync();  // neither CTA goes while the other's copies, products or arrivals reach it
     if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
 }
 

@@ -207,7 +207,6 @@ struct Sampler {
     static constexpr int VN = Vec<TX>::N, WARPS = NT / 32;
     static constexpr int PER = ST_BINS / NT;   // bins of a thread, and listed logits
     static constexpr int SHARE = ST_BINS / C;  // bins that a CTA adds up for the cluster
-    static_assert(ST_BINS == ST_SORT, "as many bins as listed logits");
     using R = Row<TX, NT, HELD>;
 
     SampleShared& sm;
