@@ -167,8 +167,9 @@ def bind():
         try:
             from . import _bind as short
 
-            if short.built_for != bind_key():
-                why, short = f"it was built for {short.built_for}, this is {bind_key()}", None
+            built_for = getattr(short, "built_for", "something unknown")
+            if built_for != bind_key():
+                why, short = f"it was built for {built_for}, this is {bind_key()}", None
         except ImportError as e:
             why = str(e)
         if short is None:

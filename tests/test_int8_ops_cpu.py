@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import subprocess
 import sys
+import types
 
 import pytest
 import torch
@@ -129,6 +130,15 @@ def test_the_short_way_is_not_taken_with_another_torch(lib, monkeypatch):
     monkeypatch.setattr(lib, "_bind", None)
     monkeypatch.setattr(torch, "__version__", "1.0.0")
     with pytest.warns(RuntimeWarning, match="torch 1.0.0"):
+        assert lib.bind().product(*range(9)) is None
+
+
+def test_the_short_way_is_not_taken_when_it_does_not_say_what_it_was_built_for(lib, monkeypatch):
+    import soraku_tts_b200
+
+    monkeypatch.setattr(lib, "_bind", None)
+    monkeypatch.setattr(soraku_tts_b200, "_bind", types.ModuleType("_bind"), raising=False)
+    with pytest.warns(RuntimeWarning, match="unknown"):
         assert lib.bind().product(*range(9)) is None
 
 
