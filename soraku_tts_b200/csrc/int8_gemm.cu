@@ -17,10 +17,10 @@
 // numbers, so that the order of their sum does not matter.  Every CTA leaves
 // its sums in its shared memory and finishes its share of the tile's tokens.
 //
-// What bounds it, 128 tokens of 1024 to 4096 channels (128 CTAs of 128 x 32, 4.8 us): the
+// What bounds it, 128 tokens of 1024 to 4096 channels (128 CTAs of 128 x 32, 5.1 us): the
 // products take 0.3 us and the bytes 1.0; the rest is a chain of latencies, launch and
 // barriers, the first copy, eight blocks, the sums out.  77 tokens to 2 x 2048 channels
-// 5.5 us.
+// 5.7 to 6.0 us.
 #include <cudaTypedefs.h>
 
 #include <cstddef>
@@ -445,10 +445,12 @@ static int clusters_at_once(int split) {
 // int8_wide.cu).  Of those that run at once the least time by what was measured at 9 to
 // 512 tokens, 1024 to 4096 channels and K of 1024 to 8192, in us: 0.22 + width / 1000 a
 // block of K, half as much again with two weights; a split 0.5 and 0.025 a token to hand
-// sums over, a token's finish 0.004 without.  Where nothing fits, tiles are as wide as
-// they get and CTAs take them in turn: a turn of a pair 1 to begin with, then 0.39 a
-// block or its finish, 4 (SwiGLU 5.8, with a residual 8), whichever is longer; of a
-// single CTA 0.48 a block (0.52) or 4.3 (3.9, 10).
+// sums over, a token's finish 0.004 without.  Narrow tiles go in one turn alone; in several
+// they are not measured.  Where nothing fits, tiles are as wide as they get and CTAs take
+// them in turn, which is dear for few tokens: 5 to 100 of 1024 to 32816 channels 16 us with
+// most columns empty, 128 13.1, where four go by four-byte products in 11.0.  The model: a
+// turn of a pair 1 to begin with, then 0.39 a block or its finish, 4 (SwiGLU 5.8, with a
+// residual 8), whichever is longer; of a single CTA 0.48 a block (0.52) or 4.3 (3.9, 10).
 template <class TO, bool GLU>
 static void gemm_choose(const Int8Args& a, int& width, int& split) {
     const long long cols = (a.N + 127) / 128;

@@ -3,10 +3,10 @@
 // for norm, codes and product), each warp streams whole weight rows, four a
 // step, and adds up products of four bytes an instruction.
 //
-// 2 tokens of 1024 to 4096 channels 3.4 us, to 32816 10.7 (33.6 MB from device memory;
-// 6.7 from codes and L2): about 1.5 us to the first codes, the stream, and sums across a
-// warp for every row.  Rows announced to L2 four groups ahead (bulk prefetch) made it
-// 12.5, two rows a step in place of four 11.1.
+// 2 tokens of 1024 FP32 values with a norm to 4096 channels 4.6 us (weights in L2 3.4), to
+// 32816 11 (33.6 MB from device memory; 9.7 from codes, in L2 7.7): about 1.5 us to the
+// first codes, the stream, and sums across a warp for every row.  Rows announced to L2
+// four groups ahead (bulk prefetch) took 2 us more.
 #include "int8_ops.cuh"
 
 namespace skb {
@@ -145,9 +145,10 @@ __global__ void __launch_bounds__(GV_THREADS, 2) int8_gemv_kernel(const Int8Args
     }
 }
 
-// Codes made by every CTA save a launch, 1.4 us, and cost what their values take:
-// 2 tokens of 1024 to 4096 channels 3.6 us, in two launches 4.0; of 4096 to 4096 8.4
-// and 6.9.
+// Codes made by every CTA save a launch and cost what their values take: with a norm, 1
+// token of 1024 FP32 values to 4096 channels 3.9 us, in two launches 4.3, 2 tokens 4.2 and
+// 4.4, 1 of 4096 to 1024 5.2 and 5.4; 2 of 4096 to 4096 9.9 and 7.6.  Beside many
+// channels it no longer shows (2 tokens to 32816 10.6 and 10.3).
 bool int8_gemv_fuses(int T, int K) { return T <= GV_FUSED_T && T * ceil16(K) <= GV_FUSED; }
 
 // Here, or on the tensor cores; from codes, us.  Up to 4 tokens weights come in about as
@@ -175,6 +176,10 @@ static cudaError_t gemv_go(const Int8Args& a, int R, int tt, bool glu, bool earl
     return launch(Kernel, grid, dim3(GV_THREADS), (size_t)tt * ceil16(a.in.K), s, true, a, early);
 }
 
+// As many rows a warp at a time as gives every warp of 296 CTAs, two an SM, rows to take.
+// Two tokens of 1024 values by one, two and four, us: to 2048 channels 2.7, 2.8, 3.0, to
+// 4096 4.3, 3.6, 3.9, to 8192 6.3, 5.4, 5.0, to 32816 14.9, 10.8, 9.9; SwiGLU by a pair and
+// two pairs: to 2048 3.6 and 3.8, to 4096 5.2 and 4.8.
 template <class TX, int TT, bool GLU>
 static cudaError_t gemv_rows(const Int8Args& a, bool early, cudaStream_t s) {
     const long long rows = (long long)a.N * (GLU ? 2 : 1);

@@ -2,12 +2,14 @@
 // the definition).  Activations before a product, weights once.
 //
 // One pass over memory: a row stays in registers between the search for its largest
-// and its codes.  6541 rows of 1024 FP32 values with a norm 7.3 us, 4.6 TB/s; 20000
-// without 17.2, 6.0.  BF16 rows are bound by instructions, 12 a value (4096 of 4096
-// 12.0 us, 4.2 TB/s; four vectors a thread need more registers than two CTAs' worth);
-// a few rows by latency, 1.4 to 2 us.  Rows brought to shared memory by bulk copies, a
-// warp to each, were no faster: 5.4 us for the 6541 without a norm (6.2 here), 8.2 with
-// one, 18.9 for the BF16 rows.
+// and its codes.  From device memory: 6541 rows of 1024 FP32 values with a norm 7.8 us,
+// 4.3 TB/s; 20000 without 18.9, 5.4.  16-bit rows are bound by instructions, 12 a value
+// (4096 of 4096 BF16 12.1 us, 4.2 TB/s, FP16 10.1; four vectors a thread need more
+// registers than two CTAs' worth); a few rows by latency, 1.0 to 2 us.  Rows brought to
+// shared memory by bulk copies, a warp to each, were no faster: 5.4 us for the 6541 without
+// a norm where this took 6.2, 8.2 with one (7.3), 18.9 for the BF16 rows (12.0).
+// The order of a row's squares (Squares) costs rows of 64 and 128 threads up to 0.3 us
+// (6541 of 1024 FP32 values 7.0 -> 7.3 in L2), others nothing.
 #include "int8_ops.cuh"
 
 namespace skb {
@@ -158,13 +160,16 @@ static cudaError_t quantize_typed(const RowsIn& in, int8_t* q, long long ldq, fl
     const int vectors = (in.K + V - 1) / V;
     // a warp's one vector a lane (33000 rows of 256 BF16 values 8.5 us, by two a lane 10.8)
     if (vectors <= 32) return rows_launch<TX, 32, 1>(in, q, ldq, scale, s);
-    // rows that are few: as many threads as a row has vectors
+    // rows that are few: as many threads as a row has vectors (128 rows of 1024 values with
+    // a norm, FP32 1.5 us, by two vectors a thread 1.7, BF16 1.6 and 2.0; 300 rows, FP32, 1.9
+    // and 1.75)
     if (in.T <= 296) {
         if (vectors <= 256) return rows_launch<TX, 256, 1>(in, q, ldq, scale, s);
         if (vectors <= 512) return rows_launch<TX, 256, 2>(in, q, ldq, scale, s);
     }
-    // many: two vectors a thread, which leaves room for four CTAs an SM (6541 rows of
-    // 1024 with a norm 8.3 us; four vectors 9.7, one 14)
+    // many: two vectors a thread, which leaves room for four CTAs an SM (6541 rows of 1024
+    // FP32 values 6.8 us, by four vectors 6.7, by one 8.5; 5003 of 2048 BF16 8.6, 10.2
+    // and 9.3)
     if (vectors <= 64) return rows_launch<TX, 32, 2>(in, q, ldq, scale, s);
     if (vectors <= 128) return rows_launch<TX, 64, 2>(in, q, ldq, scale, s);
     if (vectors <= 256) return rows_launch<TX, 128, 2>(in, q, ldq, scale, s);

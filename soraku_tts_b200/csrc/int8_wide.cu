@@ -13,11 +13,12 @@
 // For SwiGLU a CTA's rows are 64 of the gate and the same 64 of up: the warps of a
 // gate row and of its up row hand each other half of their tokens.
 //
-// From codes: 4096 tokens of 4096 to 4096 channels (BF16 out) 48 to 50 us, 2.7 to 2.9
-// POPS, 61 % of the tensor pipe's cycles, with all-zero operands 4.3 POPS: power.  6541 of
-// 1024 to 4096 (FP32 out, 107 MB, which a fill writes in 15.5 us) 34 us: six turns of
-// 3.1 us of products beside 4 us of results, which share shared memory and issue slots.
-// 5003 of 2048 to 2 x 4096 64 to 72 us, 2.3 to 2.6 POPS.  Not faster: 8 epilogue
+// From codes: 4096 tokens of 4096 to 4096 channels (BF16 out) 48 to 50 us in bursts of a few
+// ms, 2.7 to 2.9 POPS, 61 % of the tensor pipe's cycles, 58 in a run of 20 ms and more (with
+// all-zero operands 4.3 POPS: power).  6541 of 1024 to 4096 (FP32 out, 107 MB, which a fill
+// writes in 15.5 us) 32 to 37 us: six turns of 3.1 us of products beside 4 us of results,
+// which share shared memory and issue slots.  5003 of 2048 to 2 x 4096 64 to 75 us, 2.2 to
+// 2.6 POPS.  Not faster: 8 epilogue
 // warps in place of 16, their loop unrolled with an early hand-back, tensor memory read
 // one step ahead.
 #include <cudaTypedefs.h>

@@ -9,10 +9,12 @@
 // these is one question: where does a running sum (of ones, or of weights)
 // along the order reach a target?
 //
-// Weights are whole multiples of 2^-44, formed in 64 bits, so sums are exact in
-// any order and a draw does not depend on the order of atomics; what weighs less than
-// 2^-45 of the largest weighs nothing, and all of it together (2^18 logits at most)
-// is less than the last step 2^-24 of a uniform number.  A cluster of CTAs holds
+// Weights are whole multiples of 2^-44 of the largest, so sums are exact in any order and a
+// draw does not depend on the order of atomics.  Each is within 2^-38 of its value (a table
+// and a series in 64 bits, cut off behind its third power): borders of top-p and min-p
+// are where they are to that.  What weighs less than 2^-45 of the largest weighs nothing,
+// and all of it together (2^18 logits at most) is less than the last step 2^-24 of a
+// uniform number.  A cluster of CTAs holds
 // the row in shared memory, read once from the device's.
 //
 // With a top-k of up to 1280: the k-th largest of the threads' own largest logits (four each)
@@ -35,6 +37,8 @@
 // copy's rate).  A small batch is bound by latency: code that runs once, barriers over
 // the cluster, and the first CTA putting its list in order, where phases by half of
 // its threads were no faster.  A large one by instructions a logit beside the stream.
+// All are at 64 registers a thread: those for clusters keep 632 bytes of arrays in local
+// memory and spill 176 to 260, those of short rows 132 to 156, streamed ones 72 at most.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -1106,7 +1110,9 @@ static int sample_clusters() {
 // of 151,936 15.1; by a cluster 13.2 and 31.2).  By windows each logit costs more, and
 // a cluster shares that: 1 row of 32,000 20 us, of 151,936 26, streamed 27 and 75.  But
 // few clusters run at once: 16 rows 41 and 52 us, streamed 27 and 76, 32 rows of 151,936 79
-// and 75.
+// and 75.  A top-k of each row's own is on the device, so that the call goes by the
+// windows' rule, also where the rows' are small and streaming would be faster (16 rows of
+// 151,936 by their own top-k 50 64 us, by one number 20; 32 rows 20 and 20).
 template <class TX>
 static cudaError_t sample_typed(const SampleArgs& a, cudaStream_t s) {
     if (a.V <= 8192) return sample_launch<TX, 1, 512, true>(a, s);
